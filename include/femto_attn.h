@@ -124,6 +124,29 @@ int femto_paged_attention_gemv_noalloc(
     const int32_t* kv_lens, int num_seqs, int n_heads, int max_kv_len,
     void* stream);
 
+/* Paged decode attention under a sliding window with sinks: sequence b's
+ * query, at position kv_lens[b] - 1, sees key j iff j < kv_lens[b] and
+ * (j >= kv_lens[b] - window or j < sinks).  Everything else as
+ * femto_paged_attention_gemv; pages with no visible key are not read (their
+ * table entries may be -1 or stale), and keys that are not seen have no
+ * influence, whatever they hold.  window >= 1 (any larger than the contexts:
+ * all keys), sinks >= 0.  The one-launch limit counts min(max_kv_len, window +
+ * sinks) keys, and only longer calls need the workspace (of the size below).
+ * No counterpart in the reference, whose decode always sees the whole context. */
+int femto_paged_attention_gemv_window(
+    int dtype,
+    const void* q, int64_t q_stride_head, int64_t q_stride_seq,
+    void* out, int64_t out_stride_head, int64_t out_stride_seq,
+    const void* k_pool, const void* v_pool,
+    int64_t num_blocks, int n_kv_heads, int block_size, int head_dim,
+    int64_t pool_stride_block, int64_t pool_stride_head, int64_t pool_stride_row,
+    const int32_t* kv_page_tables, int num_pages_per_seq, int64_t table_stride,
+    const int32_t* kv_lens, int num_seqs, int n_heads, int max_kv_len, int window, int sinks,
+    void* workspace, size_t workspace_bytes,
+    void* stream);
+size_t femto_paged_attention_gemv_window_workspace_size(int num_seqs, int n_heads, int max_kv_len, int window,
+                                                        int sinks);
+
 /* Paged chunked / varlen / causal prefill attention on bf16 or f16 MFMA:
  * token t of sequence b (cu_seqlens[b] <= t < cu_seqlens[b+1]) sees key j
  * iff j < kv_lens[b] and j <= positions[t].
@@ -184,6 +207,30 @@ size_t femto_paged_attention_gemm_workspace_size(int num_seqs, int num_tokens, i
  * need no initialisation).  No counterpart in the
  * reference. */
 size_t femto_paged_attention_gemm_split_bytes(void);
+
+/* femto_paged_attention_gemm under a sliding window with sinks: token t of
+ * sequence b sees key j iff j < kv_lens[b], j <= positions[t] and
+ * (j > positions[t] - window or j < sinks).  Types, head dims, strides and the
+ * optional workspace (of the size below; the same leading split bytes start
+ * zero-filled) are those of femto_paged_attention_gemm.  Pages that no token
+ * of a call sees are not read.  Keys that no token of a query tile (32, 64 or
+ * 128 tokens of a sequence) sees have no influence on it, whatever they hold;
+ * a NaN or an infinity of V in a key that some of the tile's tokens see may
+ * also reach those that do not.  No counterpart in the reference. */
+int femto_paged_attention_gemm_window(
+    int dtype,
+    const void* q, int64_t q_stride_head, int64_t q_stride_token,
+    void* out, int64_t out_stride_head, int64_t out_stride_token,
+    const void* k_pool, const void* v_pool,
+    int64_t num_blocks, int n_kv_heads, int block_size, int head_dim,
+    int64_t pool_stride_block, int64_t pool_stride_head, int64_t pool_stride_row,
+    const int32_t* cu_seqlens, int num_seqs, int num_tokens, int max_q_len, int n_heads,
+    const int32_t* kv_page_tables, int num_pages_per_seq, int64_t table_stride,
+    const int32_t* kv_lens, const int32_t* positions, int window, int sinks,
+    void* workspace, size_t workspace_bytes,
+    void* stream);
+size_t femto_paged_attention_gemm_window_workspace_size(int num_seqs, int num_tokens, int max_q_len, int n_heads,
+                                                        int n_kv_heads, int num_pages_per_seq, int window, int sinks);
 
 /* KV-cache write: scatter new K/V rows into the paged pools, bit-exact.
  * k, v: (num_tokens, n_kv_heads, head_dim), element strides per token and

@@ -12,10 +12,12 @@ instruction selection is disabled for the device pass.
 
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -25,7 +27,8 @@ OUT_DIR = os.path.join(HERE, "femtovllm", "_lib")
 LIB = os.path.join(OUT_DIR, "libfemto_attn.so")
 NATIVE = os.path.join(OUT_DIR, "femto_native.so")
 
-SOURCES = ["femto_attn_api.hip", "paged_decode.hip", "paged_prefill.hip", "kv_cache_write.hip", "qk_norm_rope.hip", "varlen_metadata.hip"]
+SOURCES = ["femto_attn_api.hip", "paged_decode.hip", "paged_prefill.hip", "kv_cache_write.hip", "qk_norm_rope.hip", "varlen_metadata.hip",
+           "window_decode.hip", "window_prefill.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
@@ -59,16 +62,7 @@ def native_command(out: str) -> list:
             *[f"-L{d}" for d in cpp_extension.library_paths()], "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip"]
 
 
-def build(verbose: bool = False) -> str:
-    os.makedirs(OUT_DIR, exist_ok=True)
-    native_tmp = NATIVE + ".tmp"
-    native_cmd = native_command(native_tmp)
-    if verbose:
-        print(" ".join(native_cmd), flush=True)
-    native = subprocess.Popen(native_cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    tmp = LIB + ".tmp"
-    cmd = [hipcc(), *HIPCC_FLAGS, "-I", INCLUDE, "-I", CSRC,
-           *[os.path.join(CSRC, s) for s in SOURCES], "-o", tmp]
+def _hipcc(cmd: list, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -80,6 +74,24 @@ def build(verbose: bool = False) -> str:
         raise RuntimeError(f"hipcc failed ({res.returncode}):\n{errs}")
     if verbose and errs.strip():
         print(errs, flush=True)
+
+
+def build(verbose: bool = False) -> str:
+    os.makedirs(OUT_DIR, exist_ok=True)
+    native_tmp = NATIVE + ".tmp"
+    native_cmd = native_command(native_tmp)
+    if verbose:
+        print(" ".join(native_cmd), flush=True)
+    native = subprocess.Popen(native_cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    tmp = LIB + ".tmp"
+    # One object per source, compiled side by side, then the link.
+    compile_flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+    with tempfile.TemporaryDirectory() as obj_dir, concurrent.futures.ThreadPoolExecutor(len(SOURCES)) as pool:
+        objects = [os.path.join(obj_dir, s + ".o") for s in SOURCES]
+        compiles = [[hipcc(), *compile_flags, "-I", INCLUDE, "-I", CSRC, "-c", os.path.join(CSRC, s), "-o", o]
+                    for s, o in zip(SOURCES, objects)]
+        list(pool.map(lambda cmd: _hipcc(cmd, verbose), compiles))
+        _hipcc([hipcc(), *HIPCC_FLAGS, *objects, "-o", tmp], verbose)
     native_out = native.communicate()[0]
     if native.returncode != 0:
         raise RuntimeError(f"g++ failed ({native.returncode}):\n{native_out}")

@@ -213,15 +213,53 @@ struct PagePV<F32> {
 
 __device__ __forceinline__ int pages_of(int kv_len) { return kv_len > 0 ? (kv_len + kPage - 1) / kPage : 0; }
 
+// Which pages of a sequence's table a decode worker walks.
+//  * kAllPages: pages 0 .. pages_of(len) - 1;
+//  * kWindowPages (a.window, a.sinks): those with a key j < len that has
+//    j >= start or j < a.sinks, i.e. the sinks' pages and then the window's;
+//  * kTailPages (a.first_page): those from page a.first_page on (the pages
+//    before it are a shared prefix, which the MFMA tiles take).
+// The pages walked are numbered without the ones left out: a slice of
+// `count` pages is cut, balanced and merged as if they were contiguous, and
+// page(i) is the table column of the i-th.
+enum PageRule { kAllPages, kWindowPages, kTailPages };
+
+template <int RULE>
+struct PageList {
+    int head = 0, gap = 0, count;  // columns 0 .. head - 1, then head + gap on
+    __device__ __forceinline__ PageList(const DecodeArgs& a, int len, int start) : count(pages_of(len)) {
+        if constexpr (RULE == kWindowPages) {
+            head = pages_of(min(a.sinks, len));
+            gap = max(0, min(start / kPage, count) - head);
+        } else if constexpr (RULE == kTailPages) {
+            gap = min(a.first_page, count);
+        }
+        count -= gap;
+    }
+    __device__ __forceinline__ int page(int i) const {
+        return RULE == kAllPages || (RULE == kWindowPages && i < head) ? i : i + gap;
+    }
+};
+
+template <int RULE>
+__device__ __forceinline__ int pages_seen(const DecodeArgs& a, int len, int start) {
+    return PageList<RULE>(a, len, start).count;
+}
+
 // Keys seen by sequence b's query and the row of q / out that holds it.  A
 // decode call: kv_lens[b] keys, row b.  Decode rows of a varlen prefill call
 // (cu_seqlens set): a sequence of exactly one token t = cu_seqlens[b] sees
 // keys j < kv_lens[b] with j <= positions[t] (the prefill kernel's causal
 // rule); every other sequence is left to the prefill kernel (no keys here).
-__device__ __forceinline__ bool decode_row_of(const DecodeArgs& a, int b, int& row, int& len) {
+// start (kWindowPages): the first key of the window that ends at the query's
+// own position, kv_lens[b] - 1 or positions[t].
+template <int RULE = kAllPages>
+__device__ __forceinline__ bool decode_row_of(const DecodeArgs& a, int b, int& row, int& len, int& start) {
+    start = 0;
     if (!a.cu_seqlens) {
         row = b;
         len = a.kv_lens[b];
+        if constexpr (RULE == kWindowPages) start = max(0, max(len, 0) - a.window);
         return true;
     }
     row = a.cu_seqlens[b];
@@ -232,11 +270,13 @@ __device__ __forceinline__ bool decode_row_of(const DecodeArgs& a, int b, int& r
     const int kvl = a.kv_lens[b];
     const int pos = a.positions[row];
     len = pos < kvl ? max(0, pos + 1) : kvl;
+    if constexpr (RULE == kWindowPages) start = max(0, max(pos, 0) - (a.window - 1));
     return true;
 }
-__device__ __forceinline__ int decode_len(const DecodeArgs& a, int b) {
+template <int RULE = kAllPages>
+__device__ __forceinline__ int decode_len(const DecodeArgs& a, int b, int& start) {
     int row, len;
-    decode_row_of(a, b, row, len);
+    decode_row_of<RULE>(a, b, row, len, start);
     return len;
 }
 
@@ -277,9 +317,15 @@ __device__ __forceinline__ void merge_dpp_rows(float (&m)[NREP], float (&l)[NREP
 //
 // FULL: head_dim == 128 (every lane reads its 8 dims); else a.head_dim < 128
 // and lanes read only the dims below it (the rest are zeros).
-template <typename E, int NREP, bool FULL = true>
-__device__ __forceinline__ void decode_segment(const DecodeArgs& a, int b, int kv_len, int lp0, int n, int qrow,
-                                               int h0, int64_t head_off, float (&m)[NREP], float (&l)[NREP],
+//
+// lp0 counts the pages that RULE walks; start is the window's first key.  A
+// page that crosses an end of what the query sees has its hidden rows'
+// scores masked and, under a window, their V zeroed (rows of the same page
+// before the window's start hold older tokens, whatever they are: a NaN or
+// an infinity there must not meet a weight of 0).
+template <typename E, int NREP, bool FULL = true, int RULE = kAllPages>
+__device__ __forceinline__ void decode_segment(const DecodeArgs& a, int b, int kv_len, int start, int lp0, int n,
+                                               int qrow, int h0, int64_t head_off, float (&m)[NREP], float (&l)[NREP],
                                                float (&acc)[NREP][8]) {
     constexpr int EB = E::kBytes;
     const int lane = threadIdx.x & 63;
@@ -305,9 +351,10 @@ __device__ __forceinline__ void decode_segment(const DecodeArgs& a, int b, int k
     }
 
     const int32_t* table = a.tables + (int64_t)b * a.table_stride;
+    const PageList<RULE> pages(a, kv_len, start);
     int tbl = -1;
     auto fetch_table = [&](int i0) {
-        const int pg = lp0 + i0 + lane;
+        const int pg = pages.page(lp0 + i0 + lane);
         tbl = (i0 + lane < n && pg < a.num_pages_per_seq) ? table[pg] : -1;
     };
     // The 8 (f32: 16) 16-byte loads of page lp0 + i.  Rows past kv_len
@@ -317,7 +364,7 @@ __device__ __forceinline__ void decode_segment(const DecodeArgs& a, int b, int k
     auto issue = [&](int i, PageRegs<E>& pr, bool& blk_ok) {
         const int blk = __builtin_amdgcn_readlane(tbl, i & 63);
         blk_ok = blk >= 0 && (int64_t)blk < a.num_blocks;
-        const int pg = lp0 + i;
+        const int pg = pages.page(lp0 + i);
         const int last_row = kv_len - 1 - pg * kPage;
         const int64_t page_off = ((int64_t)(blk_ok ? blk : 0) * a.pool_stride_block + head_off) * EB;
 #pragma unroll
@@ -342,7 +389,7 @@ __device__ __forceinline__ void decode_segment(const DecodeArgs& a, int b, int k
                 pr.v[j].zero();
             }
         }
-        const int pg = lp0 + i;
+        const int pg = pages.page(lp0 + i);
         float sc[NREP][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -356,12 +403,19 @@ __device__ __forceinline__ void decode_segment(const DecodeArgs& a, int b, int k
 #pragma unroll
             for (int r = 0; r < NREP; ++r) sc[r][j] = row16_sum(sc[r][j]);
         }
-        if (pg * kPage + kPage > kv_len) {  // wave-uniform
+        bool ragged = pg * kPage + kPage > kv_len;
+        if constexpr (RULE == kWindowPages) ragged |= pg * kPage < start && pg * kPage + kPage > a.sinks;
+        if (ragged) {  // wave-uniform
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const bool valid = (pg * kPage + rg + 4 * j) < kv_len;
+                const int key = pg * kPage + rg + 4 * j;
+                bool valid = key < kv_len;
+                if constexpr (RULE == kWindowPages) valid &= key >= start || key < a.sinks;
 #pragma unroll
                 for (int r = 0; r < NREP; ++r) sc[r][j] = valid ? sc[r][j] : -INFINITY;
+                if constexpr (RULE != kAllPages) {
+                    if (!valid) pr.v[j].zero();
+                }
             }
         }
         // Lazy rescale: the running max m (log2 units) only moves when a
@@ -547,7 +601,7 @@ __device__ __forceinline__ void publish_and_merge(const DecodeArgs& a, int b, in
 // return on its own); used by the decode kernel and by the fused prefill
 // launch, whose first workgroups are decode workers.
 // MAY_MERGE: built with the in-launch merge (used when a.merge_counters is set).
-template <typename E, int NREP, bool FULL, bool MAY_MERGE>
+template <typename E, int NREP, bool FULL, bool MAY_MERGE, int RULE = kAllPages>
 __device__ __forceinline__ void decode_waves(const DecodeArgs& a, int block) {
     const int lane = threadIdx.x & 63;
     const int gw = block * 4 + (threadIdx.x >> 6);
@@ -565,8 +619,8 @@ __device__ __forceinline__ void decode_waves(const DecodeArgs& a, int block) {
         // Rows with no visible key, which no wave below meets: 0 / 0, as the
         // merge launch writes them.
         for (int i = lane; i < B; i += kWave) {
-            int row, len;
-            if (!decode_row_of(a, i, row, len) || len > 0) continue;
+            int row, len, start;
+            if (!decode_row_of<RULE>(a, i, row, len, start) || pages_seen<RULE>(a, len, start) > 0) continue;
             for (int r = 0; r < NREP; ++r)
                 for (int d = 0; d < a.head_dim; ++d)
                     store_elem<E>(reinterpret_cast<char*>(a.out),
@@ -579,14 +633,16 @@ __device__ __forceinline__ void decode_waves(const DecodeArgs& a, int block) {
     // 64 sequences this pass already loads what pass 2 needs (6 sequences of
     // 6-8k keys 38.9 -> 38.5 us, 2 of 2-3k 15.1 -> 14.9).
     int total = 0, longest = 0;
-    int my_len = 0;
+    int my_len = 0, my_start = 0;
     if (B <= kWave) {
-        my_len = lane < B ? decode_len(a, lane) : 0;
-        total = longest = pages_of(my_len);
+        my_len = lane < B ? decode_len<RULE>(a, lane, my_start) : 0;
+        total = longest = pages_seen<RULE>(a, my_len, my_start);
     } else {
 #pragma unroll 4
         for (int i = lane; i < B; i += kWave) {
-            const int pg = pages_of(decode_len(a, i));
+            int start;
+            const int len = decode_len<RULE>(a, i, start);
+            const int pg = pages_seen<RULE>(a, len, start);
             total += pg;
             longest = max(longest, pg);
         }
@@ -606,8 +662,8 @@ __device__ __forceinline__ void decode_waves(const DecodeArgs& a, int block) {
     int base = 0, carry = 0, my_excl = 0, chunk_total = 0;
     for (;; base += kWave) {
         const int i = base + lane;
-        if (B > kWave) my_len = i < B ? decode_len(a, i) : 0;
-        const int pg = pages_of(my_len);
+        if (B > kWave) my_len = i < B ? decode_len<RULE>(a, i, my_start) : 0;
+        const int pg = pages_seen<RULE>(a, my_len, my_start);
         const int incl = wave_incl_scan_i32(pg);
         my_excl = carry + incl - pg;
         chunk_total = __builtin_amdgcn_readlane(incl, kWave - 1);
@@ -615,7 +671,7 @@ __device__ __forceinline__ void decode_waves(const DecodeArgs& a, int block) {
         carry += chunk_total;
     }
     // first sequence of the chunk whose pages end after x0 (skips empty ones)
-    const uint64_t after = __ballot(base + lane < B && my_excl + pages_of(my_len) > x0);
+    const uint64_t after = __ballot(base + lane < B && my_excl + pages_seen<RULE>(a, my_len, my_start) > x0);
     int b = base + __builtin_ctzll(after);
 
     const int64_t head_off = (int64_t)kvh * a.pool_stride_head;
@@ -627,15 +683,16 @@ __device__ __forceinline__ void decode_waves(const DecodeArgs& a, int block) {
             carry += chunk_total;
             base += kWave;
             const int i = base + lane;
-            my_len = i < B ? decode_len(a, i) : 0;
-            const int pg = pages_of(my_len);
+            my_len = i < B ? decode_len<RULE>(a, i, my_start) : 0;
+            const int pg = pages_seen<RULE>(a, my_len, my_start);
             const int incl = wave_incl_scan_i32(pg);
             my_excl = carry + incl - pg;
             chunk_total = __builtin_amdgcn_readlane(incl, kWave - 1);
         }
         const int kv_len = __builtin_amdgcn_readlane(my_len, b - base);  // b - base is wave-uniform
+        const int start = RULE == kWindowPages ? __builtin_amdgcn_readlane(my_start, b - base) : 0;
         const int S = __builtin_amdgcn_readlane(my_excl, b - base);
-        const int npg = pages_of(kv_len);
+        const int npg = pages_seen<RULE>(a, kv_len, start);
         if (npg == 0 || S + npg <= x) {
             ++b;
             continue;
@@ -646,7 +703,7 @@ __device__ __forceinline__ void decode_waves(const DecodeArgs& a, int block) {
 
         const int qrow = a.cu_seqlens ? a.cu_seqlens[b] : b;
         float m[NREP], l[NREP], acc[NREP][8];
-        decode_segment<E, NREP, FULL>(a, b, kv_len, lp0, n, qrow, h0, head_off, m, l, acc);
+        decode_segment<E, NREP, FULL, RULE>(a, b, kv_len, start, lp0, n, qrow, h0, head_off, m, l, acc);
 
         // Partial state of this segment.
         const int slot = wi - S / C;

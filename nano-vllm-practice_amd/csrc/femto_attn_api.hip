@@ -238,15 +238,30 @@ static bool capturing(hipStream_t st) {
     return true;
 }
 
-// Decode entry points: femto_paged_attention_gemv (workspace from the caller)
-// and femto_paged_attention_gemv_noalloc (workspace = this device's scratch).
+// Most keys that a decode query under a window reads, in whole pages: a
+// window of w keys touches at most (w + 14) / 16 + 1 pages.
+static int window_max_keys(int max_kv_len, int window, int sinks) {
+    const int64_t pages = ((int64_t)window + 14) / femto::kPage + 1 + ((int64_t)sinks + femto::kPage - 1) / femto::kPage;
+    return (int)std::min<int64_t>(max_kv_len, pages * femto::kPage);
+}
+
+static int check_window(const std::string& fn, int window, int sinks) {
+    if (window < 1) return fail(FEMTO_ERR_INVALID, fn + ": window must be at least 1, got " + std::to_string(window));
+    if (sinks < 0) return fail(FEMTO_ERR_INVALID, fn + ": sinks must be >= 0, got " + std::to_string(sinks));
+    return FEMTO_OK;
+}
+
+// Decode entry points: femto_paged_attention_gemv (workspace from the caller),
+// femto_paged_attention_gemv_noalloc (workspace = this device's scratch) and
+// femto_paged_attention_gemv_window (window > 0).
 static int paged_decode_entry(const char* fn_name, int dtype, const void* q, int64_t q_stride_head,
                               int64_t q_stride_seq, void* out, int64_t out_stride_head, int64_t out_stride_seq,
                               const void* k_pool, const void* v_pool, int64_t num_blocks, int n_kv_heads,
                               int block_size, int head_dim, int64_t pool_stride_block, int64_t pool_stride_head,
                               int64_t pool_stride_row, const int32_t* kv_page_tables, int num_pages_per_seq,
                               int64_t table_stride, const int32_t* kv_lens, int num_seqs, int n_heads, int max_kv_len,
-                              bool use_scratch, void* workspace, size_t workspace_bytes, void* stream) {
+                              int window, int sinks, bool use_scratch, void* workspace, size_t workspace_bytes,
+                              void* stream) {
     g_err.clear();
     const std::string fn(fn_name);
     if (dtype != FEMTO_F32 && dtype != FEMTO_F16 && dtype != FEMTO_BF16)
@@ -259,15 +274,23 @@ static int paged_decode_entry(const char* fn_name, int dtype, const void* q, int
                                 q_stride_head, q_stride_seq, kv_page_tables, num_pages_per_seq, table_stride, true);
     if (rc != FEMTO_OK) return rc;
 
+    // Under a window the call is planned for the keys that a query reads, and
+    // routed by those it sees.
+    int seen = max_kv_len;
+    if (window > 0) {
+        seen = (int)std::min<int64_t>(max_kv_len, (int64_t)window + sinks);
+        max_kv_len = window_max_keys(max_kv_len, window, sinks);
+    }
+    const auto launch = window > 0 ? femto::launch_window_decode : femto::launch_paged_decode;
     femto::DecodePlan plan = femto::plan_paged_decode(n_heads, n_kv_heads, max_kv_len, dtype);
     const int limit = g_single_max_kv.load(std::memory_order_relaxed);
-    bool single = max_kv_len <= limit;
+    bool single = seen <= limit;
     femto::DecodeRoute route{};
     if (single) {
         int cus = 0;
         rc = hip_status(femto::device_cu_count(cus), (fn + ": device query").c_str());
         if (rc != FEMTO_OK) return rc;
-        route = femto::decode_route(num_seqs, n_heads, n_kv_heads, plan.nrep_tile, max_kv_len, dtype == FEMTO_F32, cus);
+        route = femto::decode_route(num_seqs, n_heads, n_kv_heads, plan.nrep_tile, seen, dtype == FEMTO_F32, cus);
     }
     if (single && route.split && !use_scratch && limit == kSingleMaxKV) {
         // The split route, if the caller's workspace holds its partial slots:
@@ -291,8 +314,9 @@ static int paged_decode_entry(const char* fn_name, int dtype, const void* q, int
             n_kv_heads, head_dim, pool_stride_block, pool_stride_head, pool_stride_row, kv_page_tables,
             num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads, nullptr);
         a.single_waves = route.waves;
-        return hip_status(femto::launch_paged_decode(dtype, a, plan.nrep_tile, num_seqs, true,
-                                                     static_cast<hipStream_t>(stream)),
+        a.window = window;
+        a.sinks = sinks;
+        return hip_status(launch(dtype, a, plan.nrep_tile, num_seqs, true, static_cast<hipStream_t>(stream)),
                           (fn + " launch").c_str());
     }
     if (use_scratch) {
@@ -322,12 +346,13 @@ static int paged_decode_entry(const char* fn_name, int dtype, const void* q, int
                                            " bytes (256-byte aligned) required, got " +
                                            std::to_string(workspace_bytes));
 
-    const femto::DecodeArgs a = femto::decode_args(
+    femto::DecodeArgs a = femto::decode_args(
         plan, q, q_stride_head, q_stride_seq, out, out_stride_head, out_stride_seq, k_pool, v_pool, num_blocks,
         n_kv_heads, head_dim, pool_stride_block, pool_stride_head, pool_stride_row, kv_page_tables, num_pages_per_seq,
         table_stride, kv_lens, num_seqs, n_heads, workspace);
-    return hip_status(femto::launch_paged_decode(dtype, a, plan.nrep_tile, num_seqs, false,
-                                                 static_cast<hipStream_t>(stream)),
+    a.window = window;
+    a.sinks = sinks;
+    return hip_status(launch(dtype, a, plan.nrep_tile, num_seqs, false, static_cast<hipStream_t>(stream)),
                       (fn + " launch").c_str());
 }
 
@@ -343,6 +368,141 @@ static size_t gemm_decode_bytes(int num_seqs, int num_tokens, int max_q_len, int
     if (femto::decode_rows_bound(num_seqs, num_tokens, max_q_len) == 0) return 0;
     const femto::DecodePlan plan = gemm_decode_plan(n_heads, n_kv_heads, num_pages_per_seq);
     return (femto::decode_workspace_bytes(num_seqs, n_heads, plan.max_slots) + 255) & ~(size_t)255;
+}
+
+// Pages that a decode row of a prefill call may read: the table's width, or
+// under a window what it sees of it.
+static int gemm_decode_pages(int num_pages_per_seq, int window, int sinks) {
+    if (window == 0) return num_pages_per_seq;
+    const int64_t table_keys = std::min<int64_t>((int64_t)num_pages_per_seq * femto::kPage, 1 << 30);
+    return (window_max_keys((int)table_keys, window, sinks) + femto::kPage - 1) / femto::kPage;
+}
+
+// Prefill entry points: femto_paged_attention_gemm (window == 0) and
+// femto_paged_attention_gemm_window.
+static int paged_gemm_entry(const char* fn_name, int dtype, const void* q, int64_t q_stride_head, int64_t q_stride_token, void* out,
+                            int64_t out_stride_head, int64_t out_stride_token, const void* k_pool,
+                            const void* v_pool, int64_t num_blocks, int n_kv_heads, int block_size,
+                            int head_dim, int64_t pool_stride_block, int64_t pool_stride_head,
+                            int64_t pool_stride_row, const int32_t* cu_seqlens, int num_seqs, int num_tokens,
+                            int max_q_len, int n_heads, const int32_t* kv_page_tables, int num_pages_per_seq,
+                            int64_t table_stride, const int32_t* kv_lens, const int32_t* positions, int window, int sinks,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+    g_err.clear();
+    const std::string fn(fn_name);
+    if (dtype != FEMTO_F16 && dtype != FEMTO_BF16)
+        return fail(FEMTO_ERR_UNSUPPORTED, fn + ": not implemented for '" +
+                                               dtype_name(dtype) + "' (bf16 / f16 MFMA only)");
+    if (num_seqs < 0 || num_tokens < 0 || max_q_len < 0)
+        return fail(FEMTO_ERR_INVALID, fn + ": negative size");
+    if (num_seqs == 0 || num_tokens == 0) return FEMTO_OK;
+    if (!cu_seqlens || !kv_lens || !positions)
+        return fail(FEMTO_ERR_INVALID, fn + ": null cu_seqlens / kv_lens / positions");
+    int rc = check_paged_common(fn_name, dtype, q, out, k_pool, v_pool, num_blocks, n_kv_heads,
+                                block_size, head_dim, pool_stride_block, pool_stride_head, pool_stride_row, n_heads,
+                                q_stride_head, q_stride_token, kv_page_tables, num_pages_per_seq, table_stride, false);
+    if (rc != FEMTO_OK) return rc;
+    if (out_stride_head % 4 || out_stride_token % 4)
+        return fail(FEMTO_ERR_INVALID, fn + ": out strides must be multiples of 8 bytes");
+    if (pool_stride_row < 0 || pool_stride_row > (1 << 24))
+        return fail(FEMTO_ERR_INVALID, fn + ": pool row stride out of range");
+
+    femto::PrefillArgs a{};
+    a.q = q;
+    a.q_stride_batch = 0;
+    a.q_stride_head = q_stride_head;
+    a.q_stride_token = q_stride_token;
+    a.out = out;
+    a.out_stride_batch = 0;
+    a.out_stride_head = out_stride_head;
+    a.out_stride_token = out_stride_token;
+    a.k = k_pool;
+    a.v = v_pool;
+    a.k_stride0 = a.v_stride0 = pool_stride_block;
+    a.k_stride1 = a.v_stride1 = pool_stride_head;
+    a.k_stride2 = a.v_stride2 = pool_stride_row;
+    a.num_blocks = num_blocks;
+    a.cu_seqlens = cu_seqlens;
+    a.tables = kv_page_tables;
+    a.table_stride = table_stride;
+    a.num_pages_per_seq = num_pages_per_seq;
+    a.kv_lens = kv_lens;
+    a.positions = positions;
+    a.num_seqs = num_seqs;
+    a.n_heads = n_heads;
+    a.n_kv_heads = n_kv_heads;
+    a.n_rep = n_heads / n_kv_heads;
+    a.head_dim = head_dim;
+    a.scale_log2 = scale_log2(head_dim);
+    a.window = window;
+    a.sinks = sinks;
+    const int decode_pages = gemm_decode_pages(num_pages_per_seq, window, sinks);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    int decode_rows = 0;
+    if (workspace) {
+        int resident = 0;
+        rc = hip_status(femto::prefill_resident_workgroups(resident), (fn + ": device query").c_str());
+        if (rc != FEMTO_OK) return rc;
+        const size_t split_bytes = femto::prefill_workspace_bytes(resident);
+        const size_t need = split_bytes + gemm_decode_bytes(num_seqs, num_tokens, max_q_len, n_heads, n_kv_heads,
+                                                            decode_pages);
+        if (workspace_bytes < need || !aligned(workspace, 256))
+            return fail(FEMTO_ERR_INVALID, fn + ": workspace of " + std::to_string(need) +
+                                               " bytes (256-byte aligned) required, got " +
+                                               std::to_string(workspace_bytes));
+        a.counters = static_cast<int*>(workspace);
+        a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + femto::prefill_counter_bytes(resident));
+        if (need > split_bytes) {
+            // Sequences of one query token (decode rows of a mixed batch) run
+            // on the decode kernel's wave workers, which stream their pages at
+            // HBM speed (an MFMA tile would hold one valid row of 32).  When
+            // the workers take as many query heads per wave as a tile takes
+            // (every head ratio but multiples of 8) they run in the same
+            // launch as the tiles, which fill the CU slots beside them; else
+            // the decode kernel runs first.
+            const femto::DecodePlan plan = gemm_decode_plan(n_heads, n_kv_heads, decode_pages);
+            decode_rows = femto::decode_rows_bound(num_seqs, num_tokens, max_q_len);
+            // Few possible one-token sequences (often none: chunks of uneven
+            // lengths leave the bound above zero): the workers merge their
+            // partials in the launch, the last wave of each (sequence, KV
+            // head group) folding the others', so no merge launch follows.
+            // That serial tail beats the launch while the merges are at most
+            // a quarter of the ~1024 worker waves: 1024 new tokens beside
+            // 1 / 16 / 31 rows on 8 KV heads 40.5 -> 38.5, 65.3 -> 57.8,
+            // 72.9 -> 68.8 us; 4 uneven chunks without rows 51.5 -> 50.1 us;
+            // 48 rows 93.6 -> 94.0 and, beside 64 tokens, 44.5 -> 45.2 us.
+            // (Few rows of equal contexts, cut alike, all end with the fold: 4
+            // of 2000 keys beside 64 tokens 16.6 -> 17.3 us, with lengths
+            // spread over a factor of eight 15 % faster.)
+            // Groups of four heads keep the merge launch: the fold costs the
+            // tiles' kernel its registers (256, and 2x slower workers).
+            const int group = femto::prefill_group(a.n_rep);
+            const int64_t groups = n_heads / group;
+            const bool few = group <= 2 && decode_rows * groups <= resident / 2 && num_seqs * groups <= resident;
+            femto::DecodeArgs d = femto::decode_args(
+                plan, q, q_stride_head, q_stride_token, out, out_stride_head, out_stride_token, k_pool, v_pool,
+                num_blocks, n_kv_heads, head_dim, pool_stride_block, pool_stride_head, pool_stride_row,
+                kv_page_tables, num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads,
+                static_cast<char*>(workspace) + split_bytes);
+            d.cu_seqlens = cu_seqlens;
+            d.positions = positions;
+            d.window = window;
+            d.sinks = sinks;
+            if (few) d.merge_counters = a.counters + resident;
+            a.skip_decode_rows = 1;
+            if (plan.nrep_tile == group) {
+                a.decode_blocks = femto::decode_worker_blocks(d);
+                if (a.decode_blocks <= 0) return fail(FEMTO_ERR_HIP, fn + ": device query");
+                a.dec = d;
+            } else {
+                const auto launch = window > 0 ? femto::launch_window_decode : femto::launch_paged_decode;
+                rc = hip_status(launch(dtype, d, plan.nrep_tile, num_seqs, false, st),
+                                (fn + " decode-row launch").c_str());
+                if (rc != FEMTO_OK) return rc;
+            }
+        }
+    }
+    return hip_status(femto::launch_paged_prefill(dtype, a, num_tokens, decode_rows, st), (fn + " launch").c_str());
 }
 
 extern "C" {
@@ -389,8 +549,32 @@ int femto_paged_attention_gemv(int dtype, const void* q, int64_t q_stride_head, 
     return paged_decode_entry("paged_attention_gemv", dtype, q, q_stride_head, q_stride_seq, out, out_stride_head,
                               out_stride_seq, k_pool, v_pool, num_blocks, n_kv_heads, block_size, head_dim,
                               pool_stride_block, pool_stride_head, pool_stride_row, kv_page_tables,
-                              num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads, max_kv_len, false,
+                              num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads, max_kv_len, 0, 0, false,
                               workspace, workspace_bytes, stream);
+}
+
+size_t femto_paged_attention_gemv_window_workspace_size(int num_seqs, int n_heads, int max_kv_len, int window,
+                                                        int sinks) {
+    if (num_seqs <= 0 || n_heads <= 0 || window < 1 || sinks < 0) return 0;
+    return femto_paged_attention_gemv_workspace_size(num_seqs, n_heads, window_max_keys(max_kv_len, window, sinks));
+}
+
+int femto_paged_attention_gemv_window(int dtype, const void* q, int64_t q_stride_head, int64_t q_stride_seq, void* out,
+                                      int64_t out_stride_head, int64_t out_stride_seq, const void* k_pool,
+                                      const void* v_pool, int64_t num_blocks, int n_kv_heads, int block_size,
+                                      int head_dim, int64_t pool_stride_block, int64_t pool_stride_head,
+                                      int64_t pool_stride_row, const int32_t* kv_page_tables, int num_pages_per_seq,
+                                      int64_t table_stride, const int32_t* kv_lens, int num_seqs, int n_heads,
+                                      int max_kv_len, int window, int sinks, void* workspace, size_t workspace_bytes,
+                                      void* stream) {
+    g_err.clear();
+    const int rc = check_window("paged_attention_gemv_window", window, sinks);
+    if (rc != FEMTO_OK) return rc;
+    return paged_decode_entry("paged_attention_gemv_window", dtype, q, q_stride_head, q_stride_seq, out,
+                              out_stride_head, out_stride_seq, k_pool, v_pool, num_blocks, n_kv_heads, block_size,
+                              head_dim, pool_stride_block, pool_stride_head, pool_stride_row, kv_page_tables,
+                              num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads, max_kv_len, window, sinks,
+                              false, workspace, workspace_bytes, stream);
 }
 
 int femto_paged_attention_gemv_noalloc(int dtype, const void* q, int64_t q_stride_head, int64_t q_stride_seq,
@@ -404,8 +588,8 @@ int femto_paged_attention_gemv_noalloc(int dtype, const void* q, int64_t q_strid
     return paged_decode_entry("paged_attention_gemv_noalloc", dtype, q, q_stride_head, q_stride_seq, out,
                               out_stride_head, out_stride_seq, k_pool, v_pool, num_blocks, n_kv_heads, block_size,
                               head_dim, pool_stride_block, pool_stride_head, pool_stride_row, kv_page_tables,
-                              num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads, max_kv_len, true, nullptr,
-                              0, stream);
+                              num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads, max_kv_len, 0, 0, true,
+                              nullptr, 0, stream);
 }
 
 int femto_paged_attention_gemm(int dtype, const void* q, int64_t q_stride_head, int64_t q_stride_token, void* out,
@@ -416,114 +600,36 @@ int femto_paged_attention_gemm(int dtype, const void* q, int64_t q_stride_head, 
                                int max_q_len, int n_heads, const int32_t* kv_page_tables, int num_pages_per_seq,
                                int64_t table_stride, const int32_t* kv_lens, const int32_t* positions,
                                void* workspace, size_t workspace_bytes, void* stream) {
-    g_err.clear();
-    if (dtype != FEMTO_F16 && dtype != FEMTO_BF16)
-        return fail(FEMTO_ERR_UNSUPPORTED, std::string("paged_attention_gemm: not implemented for '") +
-                                               dtype_name(dtype) + "' (bf16 / f16 MFMA only)");
-    if (num_seqs < 0 || num_tokens < 0 || max_q_len < 0)
-        return fail(FEMTO_ERR_INVALID, "paged_attention_gemm: negative size");
-    if (num_seqs == 0 || num_tokens == 0) return FEMTO_OK;
-    if (!cu_seqlens || !kv_lens || !positions)
-        return fail(FEMTO_ERR_INVALID, "paged_attention_gemm: null cu_seqlens / kv_lens / positions");
-    int rc = check_paged_common("paged_attention_gemm", dtype, q, out, k_pool, v_pool, num_blocks, n_kv_heads,
-                                block_size, head_dim, pool_stride_block, pool_stride_head, pool_stride_row, n_heads,
-                                q_stride_head, q_stride_token, kv_page_tables, num_pages_per_seq, table_stride, false);
-    if (rc != FEMTO_OK) return rc;
-    if (out_stride_head % 4 || out_stride_token % 4)
-        return fail(FEMTO_ERR_INVALID, "paged_attention_gemm: out strides must be multiples of 8 bytes");
-    if (pool_stride_row < 0 || pool_stride_row > (1 << 24))
-        return fail(FEMTO_ERR_INVALID, "paged_attention_gemm: pool row stride out of range");
+    return paged_gemm_entry("paged_attention_gemm", dtype, q, q_stride_head, q_stride_token, out, out_stride_head,
+                            out_stride_token, k_pool, v_pool, num_blocks, n_kv_heads, block_size, head_dim,
+                            pool_stride_block, pool_stride_head, pool_stride_row, cu_seqlens, num_seqs, num_tokens,
+                            max_q_len, n_heads, kv_page_tables, num_pages_per_seq, table_stride, kv_lens, positions,
+                            0, 0, workspace, workspace_bytes, stream);
+}
 
-    femto::PrefillArgs a{};
-    a.q = q;
-    a.q_stride_batch = 0;
-    a.q_stride_head = q_stride_head;
-    a.q_stride_token = q_stride_token;
-    a.out = out;
-    a.out_stride_batch = 0;
-    a.out_stride_head = out_stride_head;
-    a.out_stride_token = out_stride_token;
-    a.k = k_pool;
-    a.v = v_pool;
-    a.k_stride0 = a.v_stride0 = pool_stride_block;
-    a.k_stride1 = a.v_stride1 = pool_stride_head;
-    a.k_stride2 = a.v_stride2 = pool_stride_row;
-    a.num_blocks = num_blocks;
-    a.cu_seqlens = cu_seqlens;
-    a.tables = kv_page_tables;
-    a.table_stride = table_stride;
-    a.num_pages_per_seq = num_pages_per_seq;
-    a.kv_lens = kv_lens;
-    a.positions = positions;
-    a.num_seqs = num_seqs;
-    a.n_heads = n_heads;
-    a.n_kv_heads = n_kv_heads;
-    a.n_rep = n_heads / n_kv_heads;
-    a.head_dim = head_dim;
-    a.scale_log2 = scale_log2(head_dim);
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    int decode_rows = 0;
-    if (workspace) {
-        int resident = 0;
-        rc = hip_status(femto::prefill_resident_workgroups(resident), "paged_attention_gemm: device query");
-        if (rc != FEMTO_OK) return rc;
-        const size_t split_bytes = femto::prefill_workspace_bytes(resident);
-        const size_t need = split_bytes + gemm_decode_bytes(num_seqs, num_tokens, max_q_len, n_heads, n_kv_heads,
-                                                            num_pages_per_seq);
-        if (workspace_bytes < need || !aligned(workspace, 256))
-            return fail(FEMTO_ERR_INVALID, "paged_attention_gemm: workspace of " + std::to_string(need) +
-                                               " bytes (256-byte aligned) required, got " +
-                                               std::to_string(workspace_bytes));
-        a.counters = static_cast<int*>(workspace);
-        a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + femto::prefill_counter_bytes(resident));
-        if (need > split_bytes) {
-            // Sequences of one query token (decode rows of a mixed batch) run
-            // on the decode kernel's wave workers, which stream their pages at
-            // HBM speed (an MFMA tile would hold one valid row of 32).  When
-            // the workers take as many query heads per wave as a tile takes
-            // (every head ratio but multiples of 8) they run in the same
-            // launch as the tiles, which fill the CU slots beside them; else
-            // the decode kernel runs first.
-            const femto::DecodePlan plan = gemm_decode_plan(n_heads, n_kv_heads, num_pages_per_seq);
-            decode_rows = femto::decode_rows_bound(num_seqs, num_tokens, max_q_len);
-            // Few possible one-token sequences (often none: chunks of uneven
-            // lengths leave the bound above zero): the workers merge their
-            // partials in the launch, the last wave of each (sequence, KV
-            // head group) folding the others', so no merge launch follows.
-            // That serial tail beats the launch while the merges are at most
-            // a quarter of the ~1024 worker waves: 1024 new tokens beside
-            // 1 / 16 / 31 rows on 8 KV heads 40.5 -> 38.5, 65.3 -> 57.8,
-            // 72.9 -> 68.8 us; 4 uneven chunks without rows 51.5 -> 50.1 us;
-            // 48 rows 93.6 -> 94.0 and, beside 64 tokens, 44.5 -> 45.2 us.
-            // (Few rows of equal contexts, cut alike, all end with the fold: 4
-            // of 2000 keys beside 64 tokens 16.6 -> 17.3 us, with lengths
-            // spread over a factor of eight 15 % faster.)
-            // Groups of four heads keep the merge launch: the fold costs the
-            // tiles' kernel its registers (256, and 2x slower workers).
-            const int group = femto::prefill_group(a.n_rep);
-            const int64_t groups = n_heads / group;
-            const bool few = group <= 2 && decode_rows * groups <= resident / 2 && num_seqs * groups <= resident;
-            femto::DecodeArgs d = femto::decode_args(
-                plan, q, q_stride_head, q_stride_token, out, out_stride_head, out_stride_token, k_pool, v_pool,
-                num_blocks, n_kv_heads, head_dim, pool_stride_block, pool_stride_head, pool_stride_row,
-                kv_page_tables, num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads,
-                static_cast<char*>(workspace) + split_bytes);
-            d.cu_seqlens = cu_seqlens;
-            d.positions = positions;
-            if (few) d.merge_counters = a.counters + resident;
-            a.skip_decode_rows = 1;
-            if (plan.nrep_tile == group) {
-                a.decode_blocks = femto::decode_worker_blocks(d);
-                if (a.decode_blocks <= 0) return fail(FEMTO_ERR_HIP, "paged_attention_gemm: device query");
-                a.dec = d;
-            } else {
-                rc = hip_status(femto::launch_paged_decode(dtype, d, plan.nrep_tile, num_seqs, false, st),
-                                "paged_attention_gemm decode-row launch");
-                if (rc != FEMTO_OK) return rc;
-            }
-        }
-    }
-    return hip_status(femto::launch_paged_prefill(dtype, a, num_tokens, decode_rows, st), "paged_attention_gemm launch");
+size_t femto_paged_attention_gemm_window_workspace_size(int num_seqs, int num_tokens, int max_q_len, int n_heads,
+                                                        int n_kv_heads, int num_pages_per_seq, int window, int sinks) {
+    if (window < 1 || sinks < 0) return 0;
+    return femto_paged_attention_gemm_workspace_size(num_seqs, num_tokens, max_q_len, n_heads, n_kv_heads,
+                                                     gemm_decode_pages(num_pages_per_seq, window, sinks));
+}
+
+int femto_paged_attention_gemm_window(int dtype, const void* q, int64_t q_stride_head, int64_t q_stride_token, void* out,
+                               int64_t out_stride_head, int64_t out_stride_token, const void* k_pool,
+                               const void* v_pool, int64_t num_blocks, int n_kv_heads, int block_size,
+                               int head_dim, int64_t pool_stride_block, int64_t pool_stride_head,
+                               int64_t pool_stride_row, const int32_t* cu_seqlens, int num_seqs, int num_tokens,
+                               int max_q_len, int n_heads, const int32_t* kv_page_tables, int num_pages_per_seq,
+                               int64_t table_stride, const int32_t* kv_lens, const int32_t* positions,
+                               int window, int sinks, void* workspace, size_t workspace_bytes, void* stream) {
+    g_err.clear();
+    const int rc = check_window("paged_attention_gemm_window", window, sinks);
+    if (rc != FEMTO_OK) return rc;
+    return paged_gemm_entry("paged_attention_gemm_window", dtype, q, q_stride_head, q_stride_token, out, out_stride_head,
+                            out_stride_token, k_pool, v_pool, num_blocks, n_kv_heads, block_size, head_dim,
+                            pool_stride_block, pool_stride_head, pool_stride_row, cu_seqlens, num_seqs, num_tokens,
+                            max_q_len, n_heads, kv_page_tables, num_pages_per_seq, table_stride, kv_lens, positions,
+                            window, sinks, workspace, workspace_bytes, stream);
 }
 
 int femto_kv_cache_write(int dtype, const void* k, int64_t k_stride_token, int64_t k_stride_head, const void* v,

@@ -43,6 +43,10 @@ struct DecodeArgs {
     // waves of a cut sequence merge their partials themselves and no merge
     // launch follows.  Null: partials only.
     int* merge_counters;
+    // Window calls (PageList in decode_worker.h): keys a query sees before
+    // and at its own position (>= 1), and first keys that stay visible.
+    int window, sinks;
+    int first_page;  // tail pages of a shared-prefix call start here
 };
 
 // Compute units of the current device, queried once per device (safe to call
@@ -66,6 +70,10 @@ hipError_t launch_paged_decode(int dtype, const DecodeArgs& a, int nrep_tile, in
 // a.waves_per_group; 0 on a device error), and the merge that follows.
 int decode_worker_blocks(DecodeArgs& a);
 hipError_t launch_paged_decode_merge(int dtype, const DecodeArgs& a, int num_seqs, hipStream_t st);
+// The same under a sliding window with sinks (window_decode.hip).
+hipError_t launch_window_decode(int dtype, const DecodeArgs& a, int nrep_tile, int num_seqs, bool single,
+                                hipStream_t st);
+hipError_t launch_window_decode_merge(int dtype, const DecodeArgs& a, int num_seqs, hipStream_t st);
 
 struct PrefillArgs {
     const void* q;
@@ -103,6 +111,8 @@ struct PrefillArgs {
     // sequences), the rest the MFMA tiles; 0: none.
     int decode_blocks;
     DecodeArgs dec;
+    // Sliding window with sinks (paged only; window == 0: none).
+    int window, sinks;
 };
 
 // Key split: at most kMaxPieces pieces per query tile, each leaving a
@@ -184,6 +194,9 @@ hipError_t launch_varlen_metadata(const MetadataArgs& a, int max_q_len, hipStrea
 // prefill_group(n_rep) heads each) and the merge follows on `st`.
 hipError_t launch_paged_prefill(int dtype, PrefillArgs a, int num_tokens, int decode_rows_max, hipStream_t st);
 int prefill_group(int n_rep);
+// The tile launch of a paged call with a.window > 0 (window_prefill.hip), for
+// launch_paged_prefill.
+hipError_t launch_window_tiles(int dtype, int G, const PrefillArgs& a, hipStream_t st);
 hipError_t launch_dense_attention(int dtype, PrefillArgs a, hipStream_t st);
 
 }  // namespace femto

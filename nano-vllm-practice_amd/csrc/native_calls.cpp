@@ -16,10 +16,12 @@
 #include <Python.h>
 
 #include <ATen/Functions.h>
+#include <hip/hip_runtime_api.h>
 #include <c10/hip/HIPStream.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "femto_attn.h"
@@ -33,6 +35,10 @@ decltype(&femto_paged_attention_gemm) g_gemm;
 decltype(&femto_paged_attention_gemm_workspace_size) g_gemm_ws;
 decltype(&femto_qk_norm_rope_cache_write) g_prologue;
 decltype(&femto_flash_attention) g_flash;
+decltype(&femto_paged_attention_gemv_window) g_gemv_window;
+decltype(&femto_paged_attention_gemv_window_workspace_size) g_gemv_window_ws;
+decltype(&femto_paged_attention_gemm_window) g_gemm_window;
+decltype(&femto_paged_attention_gemm_window_workspace_size) g_gemm_window_ws;
 
 // Thrown (and caught in `guarded`) where the Python path has to take over.
 struct NotHere {};
@@ -70,6 +76,20 @@ int dtype_code(const at::Tensor& t) {
 
 void* stream_of(const at::Tensor& t) {
     return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
+}
+
+// The calls below launch on the current device, and a call that is being
+// captured into a graph gets a workspace of its own: both left to the Python
+// path where they apply.
+void need_current_device(const at::Tensor& t) {
+    int dev = -1;
+    need(hipGetDevice(&dev) == hipSuccess && dev == t.device().index());
+}
+void need_not_captured(void* stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const bool known = hipStreamIsCapturing((hipStream_t)stream, &status) == hipSuccess;
+    if (!known) (void)hipGetLastError();
+    need(known && status == hipStreamCaptureStatusNone);
 }
 
 const int32_t* i32(const at::Tensor& t) { return static_cast<const int32_t*>(t.const_data_ptr()); }
@@ -122,18 +142,20 @@ void check_paged(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, 
 // The library call and its result.  The result's Python object is made first and whatever the library
 // throws is an error: nothing can decline the call once the library has been entered (the Python path
 // would make it a second time, on a q that the first may have overwritten).
-template <typename F>
+// HOLD_GIL: for calls of more than one launch over the stream's workspace, which
+// another thread's call on the stream must not come between.
+template <bool HOLD_GIL = false, typename F>
 PyObject* launch(const at::Tensor& out, F call) {
     PyObject* result = THPVariable_Wrap(out);
     need(result != nullptr);
     int rc;
-    PyThreadState* gil = PyEval_SaveThread();
+    PyThreadState* gil = HOLD_GIL ? nullptr : PyEval_SaveThread();
     try {
         rc = call();
     } catch (...) {
         rc = -1;
     }
-    PyEval_RestoreThread(gil);
+    if (!HOLD_GIL) PyEval_RestoreThread(gil);
     if (rc == 0) return result;
     Py_DECREF(result);
     PyErr_SetString(PyExc_RuntimeError, rc < 0 ? "femto_native: the library threw" : g_last_error());
@@ -176,6 +198,46 @@ PyObject* gemv(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// Whether the pools, too, are on q's device, and that device is the current one.
+void need_one_device(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v) {
+    need(k.device() == q.device() && v.device() == q.device());
+    need_current_device(q);
+}
+
+// A window or sinks argument: those past int32 see as many keys as the largest int32.
+int key_count(PyObject* o, int64_t lowest) {
+    const int64_t n = integer(o);
+    need(n >= lowest);
+    return (int)std::min<int64_t>(n, INT32_MAX);
+}
+
+// gemv_window(q, k_pool, v_pool, tables, kv_lens, max_kv_len, window, sinks, workspaces)
+PyObject* gemv_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 9, [&]() -> PyObject* {
+        need(g_gemv_window);
+        const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]), &tab = tensor(a[3]), &len = tensor(a[4]);
+        const int max_kv = int32(integer(a[5])), window = key_count(a[6], 1), sinks = key_count(a[7], 0);
+        check_paged(q, k, v, tab, len, false, 16, 1);
+        need_one_device(q, k, v);
+        const int64_t H = q.size(0), B = q.size(1);
+        need(B > 0 && B == tab.size(0) && B == len.size(0));
+        const int dt = dtype_code(q);
+        void* st = stream_of(q);
+        const size_t bytes = g_gemv_window_ws(int32(B), int32(H), max_kv, window, sinks);
+        if (bytes) need_not_captured(st);
+        const Workspace w = workspace(a[8], q, st, bytes);
+        at::Tensor out = at::empty({H, B, q.size(2)}, q.options());
+        const void *qp = q.const_data_ptr(), *kp = k.const_data_ptr(), *vp = v.const_data_ptr();
+        const int32_t *tp = i32(tab), *lp = i32(len);
+        void* op = out.data_ptr();
+        return launch<true>(out, [&] {
+            return g_gemv_window(dt, qp, q.stride(0), q.stride(1), op, out.stride(0), out.stride(1), kp, vp, k.size(0),
+                                 (int)k.size(1), (int)k.size(2), (int)k.size(3), k.stride(0), k.stride(1), k.stride(2), tp,
+                                 (int)tab.size(1), tab.stride(0), lp, (int)B, (int)H, max_kv, window, sinks, w.ptr, w.bytes, st);
+        });
+    });
+}
+
 // gemm(q, k_pool, v_pool, cu_seqlens, max_q_len, tables, kv_lens, positions, contiguous_q, workspaces)
 PyObject* gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 10, [&]() -> PyObject* {
@@ -200,6 +262,39 @@ PyObject* gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
             return g_gemm(dt, qp, q.stride(0), q.stride(1), op, out.stride(0), out.stride(1), kp, vp, k.size(0), (int)k.size(1),
                           (int)k.size(2), (int)k.size(3), k.stride(0), k.stride(1), k.stride(2), cp, (int)B, (int)T, max_q, (int)H,
                           tp, (int)tab.size(1), tab.stride(0), lp, pp, w.ptr, w.bytes, st);
+        });
+    });
+}
+
+// gemm_window(q, k_pool, v_pool, cu_seqlens, max_q_len, tables, kv_lens, positions, window, sinks, workspaces)
+PyObject* gemm_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 11, [&]() -> PyObject* {
+        need(g_gemm_window);
+        const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]), &cu = tensor(a[3]);
+        const at::Tensor &tab = tensor(a[5]), &len = tensor(a[6]), &pos = tensor(a[7]);
+        const int max_q = int32(integer(a[4])), window = key_count(a[8], 1), sinks = key_count(a[9], 0);
+        check_paged(q, k, v, tab, len, false, 1, 16);
+        need_one_device(q, k, v);
+        need(cu.scalar_type() == at::kInt && cu.is_contiguous() && cu.device() == q.device());
+        need(pos.scalar_type() == at::kInt && pos.is_contiguous() && pos.device() == q.device());
+        const int64_t H = q.size(0), T = q.size(1), B = cu.numel() - 1;
+        need(B > 0 && T > 0 && B == tab.size(0) && B == len.size(0) && T == pos.numel());
+        need(q.scalar_type() != at::kFloat);
+        const int dt = dtype_code(q);
+        void* st = stream_of(q);
+        const size_t bytes = g_gemm_window_ws(int32(B), int32(T), max_q, int32(H), (int)k.size(1), int32(tab.size(1)), window,
+                                              sinks);
+        if (bytes) need_not_captured(st);
+        const Workspace w = workspace(a[10], q, st, bytes);
+        at::Tensor out = at::empty({H, T, q.size(2)}, q.options());
+        const void *qp = q.const_data_ptr(), *kp = k.const_data_ptr(), *vp = v.const_data_ptr();
+        const int32_t *cp = i32(cu), *tp = i32(tab), *lp = i32(len), *pp = i32(pos);
+        void* op = out.data_ptr();
+        return launch<true>(out, [&] {
+            return g_gemm_window(dt, qp, q.stride(0), q.stride(1), op, out.stride(0), out.stride(1), kp, vp, k.size(0),
+                                 (int)k.size(1), (int)k.size(2), (int)k.size(3), k.stride(0), k.stride(1), k.stride(2), cp, (int)B,
+                                 (int)T, max_q, (int)H, tp, (int)tab.size(1), tab.stride(0), lp, pp, window, sinks, w.ptr, w.bytes,
+                                 st);
         });
     });
 }
@@ -298,6 +393,13 @@ PyObject* bind(PyObject*, PyObject* names) {
         !get("femto_qk_norm_rope_cache_write", g_prologue) || !get("femto_flash_attention", g_flash) ||
         !get("femto_paged_attention_gemv", g_gemv))
         return nullptr;
+    // A call whose function is not bound is declined.
+    auto optional = [&](const char* name, auto& fn) { return !PyDict_GetItemString(names, name) || get(name, fn); };
+    if (!optional("femto_paged_attention_gemv_window", g_gemv_window) ||
+        !optional("femto_paged_attention_gemv_window_workspace_size", g_gemv_window_ws) ||
+        !optional("femto_paged_attention_gemm_window", g_gemm_window) ||
+        !optional("femto_paged_attention_gemm_window_workspace_size", g_gemm_window_ws))
+        return nullptr;
     Py_RETURN_NONE;
 }
 
@@ -306,6 +408,8 @@ PyMethodDef methods[] = {
     {"bind", bind, METH_O, nullptr},
     {"gemv", FEMTO_FAST(gemv)},
     {"gemm", FEMTO_FAST(gemm)},
+    {"gemv_window", FEMTO_FAST(gemv_window)},
+    {"gemm_window", FEMTO_FAST(gemm_window)},
     {"prologue", FEMTO_FAST(prologue)},
     {"flash", FEMTO_FAST(flash)},
     {nullptr, nullptr, 0, nullptr},

@@ -31,6 +31,7 @@ from __future__ import annotations
 import ctypes
 import importlib.machinery
 import importlib.util
+import operator
 import os
 
 import torch
@@ -91,7 +92,29 @@ def _load() -> ctypes.CDLL:
     return lib
 
 
+def _declare_added(lib) -> None:
+    """Argument types of the entry points that have no counterpart in the reference's ``_C``."""
+    i, i64, p, sz = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t
+    lib.femto_paged_attention_gemv_window.restype = i
+    lib.femto_paged_attention_gemv_window.argtypes = [
+        i, p, i64, i64, p, i64, i64, p, p, i64, i, i, i, i64, i64, i64, p, i, i64, p, i, i, i, i, i, p, sz, p,
+    ]
+    lib.femto_paged_attention_gemv_window_workspace_size.restype = sz
+    lib.femto_paged_attention_gemv_window_workspace_size.argtypes = [i, i, i, i, i]
+    lib.femto_paged_attention_gemm_window.restype = i
+    lib.femto_paged_attention_gemm_window.argtypes = [
+        i, p, i64, i64, p, i64, i64, p, p, i64, i, i, i, i64, i64, i64, p, i, i, i, i, p, i, i64, p, p, i, i, p, sz, p,
+    ]
+    lib.femto_paged_attention_gemm_window_workspace_size.restype = sz
+    lib.femto_paged_attention_gemm_window_workspace_size.argtypes = [i, i, i, i, i, i, i, i]
+
+
 _lib = _load()
+_declare_added(_lib)
+# The added entry points are called with the interpreter lock held: a call may be several launches over the
+# stream's workspace, and another thread's call on the stream must not come between them.
+_lib_held = ctypes.PyDLL(_LIB_PATH)
+_declare_added(_lib_held)
 
 
 def _load_native():
@@ -108,7 +131,9 @@ def _load_native():
     loader.exec_module(module)
     names = ("femto_attn_last_error", "femto_paged_attention_gemv", "femto_paged_attention_gemv_workspace_size",
              "femto_paged_attention_gemm", "femto_paged_attention_gemm_workspace_size",
-             "femto_qk_norm_rope_cache_write", "femto_flash_attention")
+             "femto_qk_norm_rope_cache_write", "femto_flash_attention",
+             "femto_paged_attention_gemv_window", "femto_paged_attention_gemv_window_workspace_size",
+             "femto_paged_attention_gemm_window", "femto_paged_attention_gemm_window_workspace_size")
     module.bind({n: ctypes.cast(getattr(_lib, n), ctypes.c_void_p).value for n in names})
     return module
 
@@ -191,6 +216,26 @@ def _prefill_workspace(device: torch.device, num_seqs: int, num_tokens: int, max
     nbytes = int(_lib.femto_paged_attention_gemm_workspace_size(num_seqs, num_tokens, max_q_len, n_heads,
                                                                  n_kv_heads, num_pages_per_seq))
     return _cached_workspace(_prefill_workspaces, device, nbytes, zero=True)
+
+
+# Workspaces of the window calls, one per (device, stream) as above.  No captured graph holds one: a call
+# that is being captured takes its own, from the graph's memory.
+_window_workspaces: dict = {}
+_window_prefill_workspaces: dict = {}
+
+
+def _call_workspace(cache: dict, device: torch.device, nbytes: int, zero_bytes: int):
+    """(pointer, bytes, tensor) of ``nbytes``, the first ``zero_bytes`` zero-filled when it is new.  The
+    current device has to be ``device``."""
+    if nbytes == 0:
+        return None, 0, None
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
+        offset = -ws.data_ptr() % 256
+        if zero_bytes:
+            ws[offset : offset + zero_bytes].zero_()
+        return ws.data_ptr() + offset, ws.numel() - offset, ws
+    return *_cached_workspace(cache, device, nbytes, zero=zero_bytes > 0), None
 
 
 # The native calls look the workspaces up by themselves: a caller that replaces one of the functions
@@ -306,6 +351,112 @@ def _paged_attention_gemm(q, k_pool, v_pool, cu_seqlens, max_q_len, kv_page_tabl
         kv_lens.data_ptr(), positions.data_ptr(),
         ws, ws_bytes, _stream(q.device),
     )
+    _raise_on(rc)
+    return out
+
+
+_INT32_MAX = 2**31 - 1
+
+
+def _int32_arg(fn: str, name: str, value) -> int:
+    value = operator.index(value)
+    _check(-_INT32_MAX - 1 <= value <= _INT32_MAX, f"{fn}: {name} {value} is out of range")
+    return value
+
+
+def _check_window(fn: str, window, sinks):
+    """(window, sinks), those past int32 cut to it: no context is longer."""
+    window, sinks = operator.index(window), operator.index(sinks)
+    _check(window >= 1, f"{fn}: window must be at least 1, got {window}")
+    _check(sinks >= 0, f"{fn}: sinks must be >= 0, got {sinks}")
+    return min(window, _INT32_MAX), min(sinks, _INT32_MAX)
+
+
+def _check_paged_added(fn, q, k_pool, v_pool, tables, kv_lens, decode):
+    """_check_paged, and what the entry points with no counterpart in the reference check besides."""
+    for name, t in (("k_pool", k_pool), ("v_pool", v_pool)):
+        _check(t.device == q.device, f"{fn}: {name} must be on {q.device}")
+    _check(k_pool.dim() == 4 and k_pool.size(1) > 0, f"{fn}: the pools must be 4-D with at least one KV head")
+    _check_paged(fn, q, k_pool, v_pool, tables, kv_lens, False, decode=decode)
+    _check(kv_lens.dim() == 1, f"{fn}: kv_lens must be 1-D")
+
+
+def _paged_attention_gemv_window(q, k_pool, v_pool, kv_page_tables, kv_lens, max_kv_len, window, sinks=0):
+    """Decode under a sliding window with sinks; out (n_heads, num_seqs, head_dim)."""
+    out = _native.gemv_window(q, k_pool, v_pool, kv_page_tables, kv_lens, max_kv_len, window, sinks, _window_workspaces)
+    if out is not None:
+        return out
+    fn = "paged_attention_gemv_window"
+    _check_paged_added(fn, q, k_pool, v_pool, kv_page_tables, kv_lens, decode=True)
+    n_heads, num_seqs, dim = q.shape
+    _check(num_seqs == kv_page_tables.size(0), f"{fn}: q.size(1) must equal kv_page_tables.size(0)")
+    _check(num_seqs == kv_lens.size(0), f"{fn}: q.size(1) must equal kv_lens.size(0)")
+    max_kv_len = _int32_arg(fn, "max_kv_len", max_kv_len)
+    window, sinks = _check_window(fn, window, sinks)
+    dtype = _dtype_code(q, fn)
+    with torch.cuda.device(q.device):
+        out = torch.empty((n_heads, num_seqs, dim), dtype=q.dtype, device=q.device)
+        if num_seqs == 0:
+            return out
+        nbytes = _lib.femto_paged_attention_gemv_window_workspace_size(num_seqs, n_heads, max_kv_len, window, sinks)
+        ws, ws_bytes, _hold = _call_workspace(_window_workspaces, q.device, nbytes, 0)
+        rc = _lib_held.femto_paged_attention_gemv_window(
+            dtype,
+            q.data_ptr(), q.stride(0), q.stride(1),
+            out.data_ptr(), out.stride(0), out.stride(1),
+            k_pool.data_ptr(), v_pool.data_ptr(),
+            k_pool.size(0), k_pool.size(1), k_pool.size(2), k_pool.size(3),
+            k_pool.stride(0), k_pool.stride(1), k_pool.stride(2),
+            kv_page_tables.data_ptr(), kv_page_tables.size(1), kv_page_tables.stride(0),
+            kv_lens.data_ptr(), num_seqs, n_heads, max_kv_len, window, sinks,
+            ws, ws_bytes, _stream(q.device),
+        )
+    _raise_on(rc)
+    return out
+
+
+def _paged_attention_gemm_window(q, k_pool, v_pool, cu_seqlens, max_q_len, kv_page_tables, kv_lens, positions, window,
+                                 sinks=0):
+    """Varlen causal prefill under a sliding window with sinks; out (n_heads, num_tokens, head_dim)."""
+    out = _native.gemm_window(q, k_pool, v_pool, cu_seqlens, max_q_len, kv_page_tables, kv_lens, positions, window,
+                              sinks, _window_prefill_workspaces)
+    if out is not None:
+        return out
+    fn = "paged_attention_gemm_window"
+    _check_paged_added(fn, q, k_pool, v_pool, kv_page_tables, kv_lens, decode=False)
+    for name, t in (("cu_seqlens", cu_seqlens), ("positions", positions)):
+        _check(t.dtype == torch.int32, f"{fn}: {name} must be int32")
+        _check(t.is_contiguous(), f"{fn}: {name} must be contiguous")
+        _check(t.device == q.device, f"{fn}: {name} must be on {q.device}")
+    num_seqs = cu_seqlens.numel() - 1
+    _check(num_seqs == kv_page_tables.size(0), f"{fn}: cu_seqlens.numel()-1 must equal kv_page_tables.size(0)")
+    _check(num_seqs == kv_lens.size(0), f"{fn}: cu_seqlens.numel()-1 must equal kv_lens.size(0)")
+    n_heads, num_tokens, dim = q.shape
+    _check(num_tokens == positions.numel(), f"{fn}: q.size(1) must equal positions.numel()")
+    max_q_len = _int32_arg(fn, "max_q_len", max_q_len)
+    window, sinks = _check_window(fn, window, sinks)
+    _check(q.dtype != torch.float32, f'"{fn}" not implemented for \'Float\'')
+    dtype = _dtype_code(q, fn)
+    with torch.cuda.device(q.device):
+        out = torch.empty((n_heads, num_tokens, dim), dtype=q.dtype, device=q.device)
+        if num_seqs <= 0 or num_tokens == 0:
+            return out
+        nbytes = _lib.femto_paged_attention_gemm_window_workspace_size(
+            num_seqs, num_tokens, max_q_len, n_heads, k_pool.size(1), kv_page_tables.size(1), window, sinks)
+        ws, ws_bytes, _hold = _call_workspace(_window_prefill_workspaces, q.device, nbytes,
+                                              _lib.femto_paged_attention_gemm_split_bytes())
+        rc = _lib_held.femto_paged_attention_gemm_window(
+            dtype,
+            q.data_ptr(), q.stride(0), q.stride(1),
+            out.data_ptr(), out.stride(0), out.stride(1),
+            k_pool.data_ptr(), v_pool.data_ptr(),
+            k_pool.size(0), k_pool.size(1), k_pool.size(2), k_pool.size(3),
+            k_pool.stride(0), k_pool.stride(1), k_pool.stride(2),
+            cu_seqlens.data_ptr(), num_seqs, num_tokens, max_q_len, n_heads,
+            kv_page_tables.data_ptr(), kv_page_tables.size(1), kv_page_tables.stride(0),
+            kv_lens.data_ptr(), positions.data_ptr(), window, sinks,
+            ws, ws_bytes, _stream(q.device),
+        )
     _raise_on(rc)
     return out
 

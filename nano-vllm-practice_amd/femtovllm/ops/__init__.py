@@ -19,6 +19,10 @@ loops that write the new K/V into the paged pools before the attention ops
 taking the same metadata; the second also fuses the q/k RMSNorm and the
 rotary embedding that precede those loops (qwen3.py:230-238, 312-320).
 
+``paged_attention_gemv_window`` and ``paged_attention_gemm_window`` are the
+two attention operators under a sliding window whose first tokens may stay
+visible; the reference has no windowed attention.
+
 One deliberate difference: ``q`` arrives as ``q.transpose(0, 1)`` of a
 ``(tokens, n_heads, head_dim)`` tensor (femtovllm/models/qwen/qwen3.py:270,
 372).  The reference copies it with ``.contiguous()``; the HIP kernels take
@@ -141,6 +145,54 @@ def paged_attention_gemm(
         )
     else:
         raise NotImplementedError()
+
+
+def paged_attention_gemv_window(
+    q: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    kv_page_tables: torch.Tensor,
+    kv_lens: torch.Tensor,
+    max_kv_len: int,
+    window: int,
+    sinks: int = 0,
+):
+    """:func:`paged_attention_gemv` under a sliding window with sinks.
+
+    Sequence b's query, at position ``kv_lens[b] - 1``, sees key j iff
+    ``j < kv_lens[b]`` and (``j >= kv_lens[b] - window`` or ``j < sinks``).
+    ``window >= 1`` counts the query's own key; one larger than the contexts
+    sees all keys.  Blocks that hold no visible key are not read, so their
+    table entries may be -1 or handed to another sequence.  Contexts may be of
+    any length (no ``MAX_KV_LEN_NON_SPLIT`` here); an empty one gives zeros.
+    """
+    return _hip_backend._paged_attention_gemv_window(_ensure_valid_tensor(q, "q"), k_pool, v_pool, kv_page_tables,
+                                                     kv_lens, max_kv_len, window, sinks)
+
+
+def paged_attention_gemm_window(
+    q: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    max_q_len: int,
+    kv_page_tables: torch.Tensor,
+    kv_lens: torch.Tensor,
+    positions: torch.Tensor,
+    window: int,
+    sinks: int = 0,
+):
+    """:func:`paged_attention_gemm` under a sliding window with sinks.
+
+    Token t of sequence b sees key j iff ``j < kv_lens[b]``, ``j <=
+    positions[t]`` and (``j > positions[t] - window`` or ``j < sinks``).  A
+    token that sees no key gives NaN, as in ``paged_attention_gemm``.  Blocks
+    that no token of the call sees are not read.  V has to be finite in keys
+    that some token of a sequence sees: one that is not may also reach tokens
+    up to 128 away that do not see it.
+    """
+    return _hip_backend._paged_attention_gemm_window(_ensure_valid_tensor(q, "q"), k_pool, v_pool, cu_seqlens,
+                                                     max_q_len, kv_page_tables, kv_lens, positions, window, sinks)
 
 
 def kv_cache_write(
