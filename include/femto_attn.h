@@ -232,6 +232,35 @@ int femto_paged_attention_gemm_window(
 size_t femto_paged_attention_gemm_window_workspace_size(int num_seqs, int num_tokens, int max_q_len, int n_heads,
                                                         int n_kv_heads, int num_pages_per_seq, int window, int sinks);
 
+/* Paged decode attention of a batch whose sequences share their first pages
+ * (a common system prompt in the prefix tree), which are read once for all of
+ * them: femto_paged_attention_gemv with key j of sequence b in block
+ * prefix_table[j / 16] for j < 16 * prefix_pages and in kv_page_tables[b][j / 16]
+ * from there on.  kv_lens counts the prefix's keys too and may end inside it;
+ * the first prefix_pages columns of kv_page_tables are not read, nor is a block
+ * id outside the pool dereferenced (zeros).  prefix_pages may be 0.
+ * dtype: F16 or BF16 (the prefix runs on MFMA); head_dim <= 128, a multiple of 16;
+ * at most 65535 sequences.  kv_len == 0 yields a zero row.  A NaN or an infinity
+ * of V in a prefix key may also reach sequences that end before it inside the
+ * prefix.  The workspace (256-byte aligned, no initialisation; the size is
+ * that of the current device, 0 without one) is always needed; calls that may
+ * overlap must not share one.  No counterpart in the reference, whose decode
+ * reads a shared block once per sequence. */
+int femto_paged_attention_gemv_shared_prefix(
+    int dtype,
+    const void* q, int64_t q_stride_head, int64_t q_stride_seq,
+    void* out, int64_t out_stride_head, int64_t out_stride_seq,
+    const void* k_pool, const void* v_pool,
+    int64_t num_blocks, int n_kv_heads, int block_size, int head_dim,
+    int64_t pool_stride_block, int64_t pool_stride_head, int64_t pool_stride_row,
+    const int32_t* prefix_table, int prefix_pages,
+    const int32_t* kv_page_tables, int num_pages_per_seq, int64_t table_stride,
+    const int32_t* kv_lens, int num_seqs, int n_heads, int max_kv_len,
+    void* workspace, size_t workspace_bytes,
+    void* stream);
+size_t femto_paged_attention_gemv_shared_prefix_workspace_size(int num_seqs, int n_heads, int n_kv_heads,
+                                                               int prefix_pages, int max_kv_len);
+
 /* KV-cache write: scatter new K/V rows into the paged pools, bit-exact.
  * k, v: (num_tokens, n_kv_heads, head_dim), element strides per token and
  * per head (head_dim contiguous, rows 16-byte aligned).  Pools as above.
@@ -279,6 +308,32 @@ int femto_qk_norm_rope_cache_write(
     void* q_out, int64_t q_out_stride_token, int64_t q_out_stride_head,
     const void* q_weight, const void* k_weight, float eps,
     const float* cos, const float* sin, int64_t rope_stride, int rope_rows,
+    void* k_pool, void* v_pool,
+    int64_t num_blocks, int n_heads, int n_kv_heads, int block_size, int head_dim,
+    int64_t pool_stride_block, int64_t pool_stride_head, int64_t pool_stride_row,
+    const int32_t* cu_seqlens, int num_seqs, int num_tokens, int max_q_len,
+    const int32_t* positions, const int32_t* kv_page_tables, int num_pages_per_seq, int64_t table_stride,
+    void* stream);
+
+/* Rotary positions of q and k without norms, rotated q to q_out (may be q
+ * itself, or share no memory with q, k and v), rotated k and raw v into the
+ * pools by the rule of femto_kv_cache_write (same cu_seqlens / positions /
+ * table arguments).  The first rotary_dim (even) dims of a head are pairs
+ * (a, b), dims (i, i + rotary_dim / 2) or, interleaved != 0, (2i, 2i + 1);
+ * they become (a c - b s, b c + a s) with c, s = cos / sin[positions[t]][i]
+ * (fp32 tables (rope_rows, rotary_dim / 2), row stride rope_stride); dims from
+ * rotary_dim on pass through.  In fp32, each output rounded once.  A position
+ * outside the tables yields NaN in the rotated dims.  dtype: F32, F16 or BF16;
+ * head_dim <= 128 in whole 16-byte chunks.  The reference rotates whole heads
+ * in the half layout, after a norm (femtovllm/models/qwen/qwen3.py:97-138,
+ * 230-238): femto_qk_norm_rope_cache_write. */
+int femto_rope_cache_write(
+    int dtype,
+    const void* q, int64_t q_stride_token, int64_t q_stride_head,
+    const void* k, int64_t k_stride_token, int64_t k_stride_head,
+    const void* v, int64_t v_stride_token, int64_t v_stride_head,
+    void* q_out, int64_t q_out_stride_token, int64_t q_out_stride_head,
+    const float* cos, const float* sin, int64_t rope_stride, int rope_rows, int rotary_dim, int interleaved,
     void* k_pool, void* v_pool,
     int64_t num_blocks, int n_heads, int n_kv_heads, int block_size, int head_dim,
     int64_t pool_stride_block, int64_t pool_stride_head, int64_t pool_stride_row,

@@ -262,7 +262,12 @@ __device__ __forceinline__ int serpentine(int k, int n, int cus) {
 // tile sees are numbered without those between the sinks and the window
 // (tile_at gives the key tile of a number), so the loop, the key split and
 // its merge run on as over contiguous keys; tiles that cross a row's window
-// start or the sinks' end take the mask.
+// start or the sinks' end take the mask.  kTailPages is the prefix of a
+// shared-prefix decode call, whose rest the decode workers of the launch walk:
+// the "tokens" are the sequences, all of one table (a.tables), each seeing
+// the keys below min(kv_lens[t], kv_len); the prefix is cut into
+// a.dec.prefix_pieces pieces, each leaving its rows' states (m, l and the
+// unnormalised output) as partial slots of the merge launch.
 template <typename E, int G, bool PAGED, bool FUSED, bool FULLD = true, int RULE = kAllPages>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_mfma_kernel(PrefillArgs a) {
     constexpr int EB = 2;
@@ -273,7 +278,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __shared__ int s_seq, s_ltile, s_old;
     __shared__ int s_kend[4];
     __shared__ int s_kbeg[4];  // kWindowPages
-    constexpr bool WINDOW = RULE == kWindowPages;
+    constexpr bool WINDOW = RULE == kWindowPages, PREFIX = RULE == kTailPages;
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -290,7 +295,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         // the decode kernel would use for this head ratio); they are
         // dispatched first, one per CU, and the tiles fill the other slots.
         if (lin < a.decode_blocks) {
-            decode_waves<E, G, FULLD, (G <= 2), RULE>(a.dec, lin);
+            decode_waves<E, G, FULLD, (G <= 2 && !PREFIX), RULE>(a.dec, lin);
             return;
         }
         lin -= a.decode_blocks;  // a multiple of 8: the XCD of a tile is unchanged
@@ -315,7 +320,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
         return n;
     };
-    if constexpr (PAGED) {
+    if constexpr (PREFIX) {
+        // KV head groups outermost (a head's pages stay in one XCD's L2), the
+        // row tiles of a piece next to each other.
+        const int per_xcd = (a.total_work + 7) >> 3;
+        const int w = (lin & 7) * per_xcd + (lin >> 3);
+        if ((lin >> 3) >= per_xcd || w >= a.total_work) return;
+        npieces = a.dec.prefix_pieces;
+        grp = w / (a.tiles_per_group * npieces);
+        tile_lin = w - grp * (a.tiles_per_group * npieces);
+        piece = tile_lin / a.tiles_per_group;
+        tile = tile_lin - piece * a.tiles_per_group;
+        b = 0;
+        q_begin = 0;
+        q_end = a.num_seqs;
+        kv_len = a.kv_len;
+    } else if constexpr (PAGED) {
         const int groups = a.n_kv_heads * a.head_groups;
         bool split = a.part != nullptr;
         auto pieces_of = [&](int kvl, int t) {
@@ -561,7 +581,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int tb = wave / G;
     const int h = kvh * a.n_rep + hg * G + hw;
     const int t = q_begin + tile * BT + tb * 32 + l32;  // this lane's query token
-    const bool qvalid = t < q_end;
+    const bool qvalid = t < q_end && (!PREFIX || a.kv_lens[t] > 0);  // (empty slots of a decode batch)
 
     // ---- KV staging: wave w copies page w of each tile (16 keys x 256 B of
     // K and of V) with 4 + 4 direct-to-LDS loads; in load j, lane i writes
@@ -740,7 +760,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // Number of keys visible to this lane's query; under a window the first
     // of those that are no sinks.
     int lim, lo = 0;
-    if constexpr (PAGED) {
+    if constexpr (PREFIX) {
+        lim = qvalid ? min(a.kv_lens[t], kv_len) : 0;
+    } else if constexpr (PAGED) {
         const int pos = qvalid ? a.positions[t] : kv_len;
         if constexpr (WINDOW) {
             lim = pos < kv_len ? pos + 1 : kv_len;
@@ -1024,6 +1046,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         tile_loop(std::false_type{});
     }
 
+    if constexpr (PREFIX) {
+        // The piece's states, for the merge launch (it takes a row's pieces
+        // up to the row's limit only).
+        float l_lo, l_hi;
+        pair32(l_run, l_lo, l_hi);
+        if (qvalid && lim > t_lo * kKvTile) {
+            const int64_t slot = ((int64_t)t * a.n_heads + h) * slot_stride<RULE>(a.dec) + a.dec.max_slots + piece;
+            float* acc = a.dec.part_acc + slot * kDimHead;
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int d0 = 32 * dt + 8 * g + 4 * h2;
+                    if (!FULLD && d0 >= a.head_dim) continue;
+                    *reinterpret_cast<f32x4*>(acc + d0) =
+                        f32x4{oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]};
+                }
+            }
+            if (h2 == 0) {
+                a.dec.part_ml[slot * 2] = m_run;
+                a.dec.part_ml[slot * 2 + 1] = l_lo + l_hi;
+            }
+        }
+        return;
+    }
+
     if (PAGED && nne > 1) {
         // Partial of this piece, lane-major so each lane later reads back
         // exactly its own values.  f32 and f16 storage: the raw accumulators,
@@ -1237,10 +1285,11 @@ static hipError_t launch_gf(int G, const PrefillArgs& a, hipStream_t st) {
 
 template <typename E, bool PAGED, int RULE>
 static hipError_t launch_g(int G, const PrefillArgs& a, hipStream_t st) {
-    if constexpr (PAGED) {
+    if constexpr (RULE == kTailPages) return launch_gf<E, true, true, RULE>(G, a, st);
+    if constexpr (PAGED && RULE != kTailPages) {
         if (a.decode_blocks > 0) return launch_gf<E, true, true, RULE>(G, a, st);
     }
-    return launch_gf<E, PAGED, false, RULE>(G, a, st);
+    if constexpr (RULE != kTailPages) return launch_gf<E, PAGED, false, RULE>(G, a, st);
 }
 
 template <bool PAGED, int RULE>

@@ -241,6 +241,13 @@ struct PageList {
     }
 };
 
+// Partial slots from one (sequence, head) to the next: with a shared prefix
+// its pieces' slots follow the workers'.
+template <int RULE>
+__device__ __forceinline__ int slot_stride(const DecodeArgs& a) {
+    return RULE == kTailPages ? a.max_slots + a.prefix_pieces : a.max_slots;
+}
+
 template <int RULE>
 __device__ __forceinline__ int pages_seen(const DecodeArgs& a, int len, int start) {
     return PageList<RULE>(a, len, start).count;
@@ -718,7 +725,7 @@ __device__ __forceinline__ void decode_waves(const DecodeArgs& a, int block) {
         if (rg == 0) {
 #pragma unroll
             for (int r = 0; r < NREP; ++r) {
-                const int64_t sl = ((int64_t)b * H + h0 + r) * a.max_slots + slot;
+                const int64_t sl = ((int64_t)b * H + h0 + r) * slot_stride<RULE>(a) + slot;
                 float* dst = a.part_acc + sl * kDimHead;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dst[RowSlice<E>::dim(c, e)] = acc[r][e];

@@ -632,6 +632,86 @@ int femto_paged_attention_gemm_window(int dtype, const void* q, int64_t q_stride
                             window, sinks, workspace, workspace_bytes, stream);
 }
 
+size_t femto_paged_attention_gemv_shared_prefix_workspace_size(int num_seqs, int n_heads, int n_kv_heads,
+                                                               int prefix_pages, int max_kv_len) {
+    if (num_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || prefix_pages < 0) return 0;
+    int cus = 0;
+    if (femto::device_cu_count(cus) != hipSuccess) return 0;
+    const femto::SharedPrefixPlan p =
+        femto::plan_shared_prefix(num_seqs, n_heads, n_kv_heads, prefix_pages, max_kv_len, FEMTO_BF16, cus);
+    return femto::decode_workspace_bytes(num_seqs, n_heads, p.tail.max_slots + p.pieces);
+}
+
+int femto_paged_attention_gemv_shared_prefix(
+    int dtype, const void* q, int64_t q_stride_head, int64_t q_stride_seq, void* out, int64_t out_stride_head,
+    int64_t out_stride_seq, const void* k_pool, const void* v_pool, int64_t num_blocks, int n_kv_heads, int block_size,
+    int head_dim, int64_t pool_stride_block, int64_t pool_stride_head, int64_t pool_stride_row,
+    const int32_t* prefix_table, int prefix_pages, const int32_t* kv_page_tables, int num_pages_per_seq,
+    int64_t table_stride, const int32_t* kv_lens, int num_seqs, int n_heads, int max_kv_len, void* workspace,
+    size_t workspace_bytes, void* stream) {
+    g_err.clear();
+    const char* fn_name = "paged_attention_gemv_shared_prefix";
+    const std::string fn(fn_name);
+    if (dtype != FEMTO_F16 && dtype != FEMTO_BF16)
+        return fail(FEMTO_ERR_UNSUPPORTED,
+                    fn + ": not implemented for '" + dtype_name(dtype) + "' (bf16 / f16 MFMA only)");
+    if (num_seqs < 0 || max_kv_len < 0) return fail(FEMTO_ERR_INVALID, fn + ": negative size");
+    if (prefix_pages < 0 || prefix_pages > (1 << 26))
+        return fail(FEMTO_ERR_INVALID, fn + ": prefix_pages " + std::to_string(prefix_pages) + " out of range");
+    if (num_seqs > 65535) return fail(FEMTO_ERR_INVALID, fn + ": at most 65535 sequences per call");
+    if (num_seqs == 0) return FEMTO_OK;
+    if (!kv_lens || (prefix_pages > 0 && !prefix_table))
+        return fail(FEMTO_ERR_INVALID, fn + ": null kv_lens or prefix_table");
+    int rc = check_paged_common(fn_name, dtype, q, out, k_pool, v_pool, num_blocks, n_kv_heads, block_size, head_dim,
+                                pool_stride_block, pool_stride_head, pool_stride_row, n_heads, q_stride_head,
+                                q_stride_seq, kv_page_tables, num_pages_per_seq, table_stride, false);
+    if (rc != FEMTO_OK) return rc;
+    if (pool_stride_row < 0 || pool_stride_row > (1 << 24))
+        return fail(FEMTO_ERR_INVALID, fn + ": pool row stride out of range");
+    int cus = 0;
+    rc = hip_status(femto::device_cu_count(cus), (fn + ": device query").c_str());
+    if (rc != FEMTO_OK) return rc;
+    const femto::SharedPrefixPlan plan =
+        femto::plan_shared_prefix(num_seqs, n_heads, n_kv_heads, prefix_pages, max_kv_len, dtype, cus);
+    const size_t need = femto::decode_workspace_bytes(num_seqs, n_heads, plan.tail.max_slots + plan.pieces);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
+        return fail(FEMTO_ERR_INVALID, fn + ": workspace of " + std::to_string(need) +
+                                           " bytes (256-byte aligned) required, got " + std::to_string(workspace_bytes));
+
+    femto::PrefillArgs a{};
+    a.q = q;
+    a.q_stride_head = q_stride_head;
+    a.q_stride_token = q_stride_seq;
+    a.k = k_pool;
+    a.v = v_pool;
+    a.k_stride0 = a.v_stride0 = pool_stride_block;
+    a.k_stride1 = a.v_stride1 = pool_stride_head;
+    a.k_stride2 = a.v_stride2 = pool_stride_row;
+    a.num_blocks = num_blocks;
+    a.tables = prefix_table;
+    a.num_pages_per_seq = prefix_pages;
+    a.kv_lens = kv_lens;
+    a.num_seqs = num_seqs;
+    a.kv_len = prefix_pages * femto::kPage;
+    a.n_heads = n_heads;
+    a.n_kv_heads = n_kv_heads;
+    a.n_rep = n_heads / n_kv_heads;
+    a.head_dim = head_dim;
+    a.scale_log2 = scale_log2(head_dim);
+    // The workers' partial slots, with room for the prefix's behind each head's.
+    femto::DecodePlan slots = plan.tail;
+    slots.max_slots += plan.pieces;
+    a.dec = femto::decode_args(slots, q, q_stride_head, q_stride_seq, out, out_stride_head, out_stride_seq, k_pool,
+                               v_pool, num_blocks, n_kv_heads, head_dim, pool_stride_block, pool_stride_head,
+                               pool_stride_row, kv_page_tables, num_pages_per_seq, table_stride, kv_lens, num_seqs,
+                               n_heads, workspace);
+    a.dec.max_slots = plan.tail.max_slots;
+    a.dec.first_page = prefix_pages;
+    a.dec.prefix_pieces = plan.pieces;
+    a.dec.prefix_piece_keys = plan.piece_keys;
+    return hip_status(femto::launch_shared_prefix(dtype, a, static_cast<hipStream_t>(stream)), (fn + " launch").c_str());
+}
+
 int femto_kv_cache_write(int dtype, const void* k, int64_t k_stride_token, int64_t k_stride_head, const void* v,
                          int64_t v_stride_token, int64_t v_stride_head, void* k_pool, void* v_pool,
                          int64_t num_blocks, int n_kv_heads, int block_size, int head_dim,
@@ -776,6 +856,95 @@ int femto_qk_norm_rope_cache_write(int dtype, const void* q, int64_t q_stride_to
     a.n_heads = n_heads;
     return hip_status(femto::launch_qk_norm_rope(dtype, a, cu_seqlens ? max_q_len : 1, static_cast<hipStream_t>(stream)),
                       "qk_norm_rope_cache_write launch");
+}
+
+int femto_rope_cache_write(int dtype, const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k,
+                           int64_t k_stride_token, int64_t k_stride_head, const void* v, int64_t v_stride_token,
+                           int64_t v_stride_head, void* q_out, int64_t q_out_stride_token, int64_t q_out_stride_head,
+                           const float* cos, const float* sin, int64_t rope_stride, int rope_rows, int rotary_dim,
+                           int interleaved, void* k_pool, void* v_pool, int64_t num_blocks, int n_heads, int n_kv_heads,
+                           int block_size, int head_dim, int64_t pool_stride_block, int64_t pool_stride_head,
+                           int64_t pool_stride_row, const int32_t* cu_seqlens, int num_seqs, int num_tokens,
+                           int max_q_len, const int32_t* positions, const int32_t* kv_page_tables,
+                           int num_pages_per_seq, int64_t table_stride, void* stream) {
+    g_err.clear();
+    const std::string f = "rope_cache_write";
+    if (dtype != FEMTO_F32 && dtype != FEMTO_F16 && dtype != FEMTO_BF16)
+        return fail(FEMTO_ERR_UNSUPPORTED, f + ": unsupported dtype " + std::to_string(dtype));
+    const int eb = elem_bytes(dtype);
+    if (head_dim <= 0 || head_dim > femto::kDimHead || (head_dim * eb) % 16 != 0)
+        return fail(FEMTO_ERR_UNSUPPORTED, f + ": head_dim must be at most " + std::to_string(femto::kDimHead) +
+                                               " and a multiple of 16 bytes (" + std::to_string(16 / eb) +
+                                               " elements), got " + std::to_string(head_dim));
+    if (rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2 != 0)
+        return fail(FEMTO_ERR_INVALID, f + ": rotary_dim must be even and from 2 to head_dim (" +
+                                           std::to_string(head_dim) + "), got " + std::to_string(rotary_dim));
+    if (num_seqs < 0 || num_tokens < 0 || max_q_len < 0) return fail(FEMTO_ERR_INVALID, f + ": negative size");
+    if (num_seqs == 0 || num_tokens == 0) return FEMTO_OK;
+    if (!cu_seqlens && num_tokens != num_seqs)
+        return fail(FEMTO_ERR_INVALID, f + ": without cu_seqlens every sequence has one token (num_tokens == num_seqs)");
+    if (max_q_len < 1) return fail(FEMTO_ERR_INVALID, f + ": max_q_len must be >= 1");
+    if (num_seqs > 65535) return fail(FEMTO_ERR_INVALID, f + ": at most 65535 sequences per call");
+    if (block_size != femto::kPage)
+        return fail(FEMTO_ERR_INVALID, f + ": block_size must be " + std::to_string(femto::kPage) + ", got " +
+                                           std::to_string(block_size));
+    if (n_heads <= 0 || n_kv_heads <= 0) return fail(FEMTO_ERR_INVALID, f + ": head counts must be positive");
+    if (num_blocks < 1) return fail(FEMTO_ERR_INVALID, f + ": the pool needs at least one block");
+    if (!q || !k || !v || !q_out || !cos || !sin || !k_pool || !v_pool || !positions || !kv_page_tables)
+        return fail(FEMTO_ERR_INVALID, f + ": null pointer argument");
+    if (rope_rows < 1 || rope_stride < rotary_dim / 2) return fail(FEMTO_ERR_INVALID, f + ": rope tables too small");
+    if (num_pages_per_seq < 0 || table_stride < num_pages_per_seq)
+        return fail(FEMTO_ERR_INVALID, f + ": table stride smaller than its width");
+    const void* ptrs[] = {q, k, v, q_out, k_pool, v_pool};
+    for (const void* p : ptrs)
+        if (!aligned(p, 16)) return fail(FEMTO_ERR_INVALID, f + ": tensors must be 16-byte aligned");
+    if (!aligned(cos, 4) || !aligned(sin, 4)) return fail(FEMTO_ERR_INVALID, f + ": cos and sin must be 4-byte aligned");
+    const int64_t step = 16 / eb;
+    const int64_t strides[] = {q_stride_token,     q_stride_head,     k_stride_token,    k_stride_head,
+                               v_stride_token,     v_stride_head,     q_out_stride_token, q_out_stride_head,
+                               pool_stride_block,  pool_stride_head,  pool_stride_row};
+    for (int64_t s : strides)
+        if (s % step) return fail(FEMTO_ERR_INVALID, f + ": strides must be multiples of 16 bytes");
+
+    femto::RopeArgs a{};
+    femto::CacheWriteArgs& c = a.cw;
+    c.k = k;
+    c.v = v;
+    c.k_stride_token = k_stride_token;
+    c.k_stride_head = k_stride_head;
+    c.v_stride_token = v_stride_token;
+    c.v_stride_head = v_stride_head;
+    c.k_pool = k_pool;
+    c.v_pool = v_pool;
+    c.num_blocks = num_blocks;
+    c.pool_stride_block = pool_stride_block;
+    c.pool_stride_head = pool_stride_head;
+    c.pool_stride_row = pool_stride_row;
+    c.cu_seqlens = cu_seqlens;
+    c.positions = positions;
+    c.tables = kv_page_tables;
+    c.table_stride = table_stride;
+    c.num_pages_per_seq = num_pages_per_seq;
+    c.num_seqs = num_seqs;
+    c.n_kv_heads = n_kv_heads;
+    c.row_chunks = head_dim * eb / 16;
+    c.elem_bytes = eb;
+    a.q = q;
+    a.q_stride_token = q_stride_token;
+    a.q_stride_head = q_stride_head;
+    a.q_out = q_out;
+    a.q_out_stride_token = q_out_stride_token;
+    a.q_out_stride_head = q_out_stride_head;
+    a.cos = cos;
+    a.sin = sin;
+    a.rope_stride = rope_stride;
+    a.rope_rows = rope_rows;
+    a.n_heads = n_heads;
+    a.head_dim = head_dim;
+    a.rotary_dim = rotary_dim;
+    a.interleaved = interleaved != 0;
+    return hip_status(femto::launch_rope_cache_write(dtype, a, cu_seqlens ? max_q_len : 1, static_cast<hipStream_t>(stream)),
+                      "rope_cache_write launch");
 }
 
 int femto_build_varlen_metadata(int num_seqs, const int32_t* num_computed, const int32_t* num_tokens,

@@ -46,7 +46,11 @@ struct DecodeArgs {
     // Window calls (PageList in decode_worker.h): keys a query sees before
     // and at its own position (>= 1), and first keys that stay visible.
     int window, sinks;
-    int first_page;  // tail pages of a shared-prefix call start here
+    // Shared-prefix calls: the workers' pages start here; the tiles of the
+    // pages before leave prefix_pieces partials per (sequence, head), of
+    // prefix_piece_keys keys each, behind the workers' max_slots.
+    int first_page;
+    int prefix_pieces, prefix_piece_keys;
 };
 
 // Compute units of the current device, queried once per device (safe to call
@@ -125,6 +129,19 @@ hipError_t prefill_resident_workgroups(int& resident);
 size_t prefill_counter_bytes(int resident);
 size_t prefill_workspace_bytes(int resident);
 
+// Decode of a batch whose first pages are the same (shared_prefix.hip).  The
+// plan: query heads per wave and tile, pieces of the prefix (prefix_pieces of
+// prefix_piece_keys keys), and the workers' plan for the rest.
+struct SharedPrefixPlan {
+    DecodePlan tail;
+    int pieces, piece_keys;
+};
+SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, int prefix_pages, int max_kv_len,
+                                    int dtype, int cus);
+// a: q rows as tokens, kv_len = 16 * prefix pages, their table in a.tables,
+// kv_lens, and the workers' arguments in a.dec.
+hipError_t launch_shared_prefix(int dtype, PrefillArgs a, hipStream_t st);
+
 // KV-cache write (kv_cache_write.hip).
 struct CacheWriteArgs {
     const void* k;  // (tokens, n_kv_heads, head_dim), any token / head strides
@@ -170,6 +187,26 @@ struct PrologueArgs {
 };
 
 hipError_t launch_qk_norm_rope(int dtype, const PrologueArgs& a, int max_q_len, hipStream_t st);
+
+// Rotary positions + KV-cache write (rope_cache_write.hip); cw as above.
+struct RopeArgs {
+    CacheWriteArgs cw;
+    const void* q;  // (tokens, n_heads, head_dim)
+    int64_t q_stride_token, q_stride_head;
+    void* q_out;    // same shape, may be q itself
+    int64_t q_out_stride_token, q_out_stride_head;
+    const float* cos;  // (rope_rows, rotary_dim / 2) fp32
+    const float* sin;
+    int64_t rope_stride;
+    int rope_rows;
+    int n_heads, head_dim, rotary_dim;
+    int interleaved;
+    // set by the launcher: lanes per head row (a power of two), its log2, and
+    // whether table rows are 16-byte aligned
+    int row_lanes, row_shift, table_vectors;
+};
+
+hipError_t launch_rope_cache_write(int dtype, RopeArgs a, int max_q_len, hipStream_t st);
 
 // Varlen metadata build (varlen_metadata.hip).
 struct MetadataArgs {

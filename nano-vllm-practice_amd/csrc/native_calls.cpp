@@ -35,6 +35,9 @@ decltype(&femto_paged_attention_gemm) g_gemm;
 decltype(&femto_paged_attention_gemm_workspace_size) g_gemm_ws;
 decltype(&femto_qk_norm_rope_cache_write) g_prologue;
 decltype(&femto_flash_attention) g_flash;
+decltype(&femto_rope_cache_write) g_rope;
+decltype(&femto_paged_attention_gemv_shared_prefix) g_shared;
+decltype(&femto_paged_attention_gemv_shared_prefix_workspace_size) g_shared_ws;
 decltype(&femto_paged_attention_gemv_window) g_gemv_window;
 decltype(&femto_paged_attention_gemv_window_workspace_size) g_gemv_window_ws;
 decltype(&femto_paged_attention_gemm_window) g_gemm_window;
@@ -238,6 +241,37 @@ PyObject* gemv_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// gemv_shared(q, k_pool, v_pool, prefix_pages, tables, kv_lens, max_kv_len, workspaces)
+PyObject* gemv_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 8, [&]() -> PyObject* {
+        need(g_shared);
+        const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]), &pre = tensor(a[3]);
+        const at::Tensor &tab = tensor(a[4]), &len = tensor(a[5]);
+        const int max_kv = int32(integer(a[6]));
+        check_paged(q, k, v, tab, len, false, 1, 16);
+        need_one_device(q, k, v);
+        need(pre.scalar_type() == at::kInt && pre.dim() == 1 && pre.is_contiguous() && pre.device() == q.device());
+        const int64_t H = q.size(0), B = q.size(1);
+        need(B > 0 && B == tab.size(0) && B == len.size(0));
+        need(q.scalar_type() != at::kFloat);
+        const int dt = dtype_code(q), pages = int32(pre.size(0));
+        void* st = stream_of(q);
+        need_not_captured(st);
+        const size_t bytes = g_shared_ws(int32(B), int32(H), (int)k.size(1), pages, max_kv);
+        need(bytes > 0);
+        const Workspace w = workspace(a[7], q, st, bytes);
+        at::Tensor out = at::empty({H, B, q.size(2)}, q.options());
+        const void *qp = q.const_data_ptr(), *kp = k.const_data_ptr(), *vp = v.const_data_ptr();
+        const int32_t *pp = i32(pre), *tp = i32(tab), *lp = i32(len);
+        void* op = out.data_ptr();
+        return launch<true>(out, [&] {
+            return g_shared(dt, qp, q.stride(0), q.stride(1), op, out.stride(0), out.stride(1), kp, vp, k.size(0), (int)k.size(1),
+                            (int)k.size(2), (int)k.size(3), k.stride(0), k.stride(1), k.stride(2), pp, pages, tp,
+                            (int)tab.size(1), tab.stride(0), lp, (int)B, (int)H, max_kv, w.ptr, w.bytes, st);
+        });
+    });
+}
+
 // gemm(q, k_pool, v_pool, cu_seqlens, max_q_len, tables, kv_lens, positions, contiguous_q, workspaces)
 PyObject* gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 10, [&]() -> PyObject* {
@@ -355,6 +389,59 @@ PyObject* prologue(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// rope(q, k, v, cos, sin, positions, k_pool, v_pool, tables, cu_seqlens | None, max_q_len, interleaved, out | None)
+PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 13, [&]() -> PyObject* {
+        need(g_rope);
+        const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]), &cos = tensor(a[3]), &sin = tensor(a[4]);
+        const at::Tensor &pos = tensor(a[5]), &kp = tensor(a[6]), &vp = tensor(a[7]), &tab = tensor(a[8]);
+        const int max_q = int32(integer(a[10]));
+        need(PyBool_Check(a[11]));
+        const int interleaved = a[11] == Py_True;
+        need(q.is_cuda());
+        for (const at::Tensor* t : {&k, &v, &cos, &sin, &kp, &vp, &pos, &tab}) need(t->device() == q.device());
+        need_current_device(q);
+        need(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes());
+        need(q.size(0) == k.size(0) && q.size(2) == k.size(2));
+        need(q.stride(2) == 1 && k.stride(2) == 1 && v.stride(2) == 1);
+        for (const at::Tensor* t : {&k, &v, &kp, &vp}) need(t->scalar_type() == q.scalar_type());
+        need(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat);
+        need(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.strides() == sin.strides() && cos.stride(1) == 1);
+        need(kp.dim() == 4 && kp.sizes() == vp.sizes() && kp.is_contiguous() && vp.is_contiguous());
+        need(k.size(1) == kp.size(1) && kp.size(3) == q.size(2) && kp.size(2) == 16 && q.size(1) > 0 && k.size(1) > 0);
+        need(pos.scalar_type() == at::kInt && pos.is_contiguous());
+        need(tab.scalar_type() == at::kInt && tab.dim() == 2 && (tab.size(1) <= 1 || tab.stride(1) == 1));
+        need(cos.stride(0) >= cos.size(1) && tab.stride(0) >= tab.size(1));
+        const int64_t T = q.size(0), B = tab.size(0);
+        need(T > 0 && B > 0 && pos.numel() == T);
+        const int32_t* cp = nullptr;
+        if (a[9] == Py_None) {
+            need(T == B);
+        } else {
+            const at::Tensor& cu = tensor(a[9]);
+            need(cu.scalar_type() == at::kInt && cu.is_contiguous() && cu.device() == q.device() && cu.numel() - 1 == B);
+            cp = i32(cu);
+        }
+        const int dt = dtype_code(q);
+        at::Tensor out = a[12] == Py_None ? at::empty_like(q) : tensor(a[12]);
+        need(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.stride(2) == 1 && out.device() == q.device());
+        need(a[12] == Py_None || (out.const_data_ptr() == q.const_data_ptr() && out.strides() == q.strides()));
+        void* st = stream_of(q);
+        const void *qd = q.const_data_ptr(), *kd = k.const_data_ptr(), *vd = v.const_data_ptr();
+        const float* cd = static_cast<const float*>(cos.const_data_ptr());
+        const float* sd = static_cast<const float*>(sin.const_data_ptr());
+        void *od = out.data_ptr(), *kpd = kp.data_ptr(), *vpd = vp.data_ptr();
+        const int32_t *pd = i32(pos), *td = i32(tab);
+        const int H = int32(q.size(1)), rows = int32(cos.size(0)), R = int32(2 * cos.size(1)), tokens = int32(T), seqs = int32(B);
+        return launch(out, [&] {
+            return g_rope(dt, qd, q.stride(0), q.stride(1), kd, k.stride(0), k.stride(1), vd, v.stride(0), v.stride(1), od,
+                          out.stride(0), out.stride(1), cd, sd, cos.stride(0), rows, R, interleaved, kpd, vpd, kp.size(0), H,
+                          (int)kp.size(1), (int)kp.size(2), (int)kp.size(3), kp.stride(0), kp.stride(1), kp.stride(2), cp, seqs,
+                          tokens, max_q, pd, td, (int)tab.size(1), tab.stride(0), st);
+        });
+    });
+}
+
 // flash(q, k, v)
 PyObject* flash(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 3, [&]() -> PyObject* {
@@ -395,7 +482,8 @@ PyObject* bind(PyObject*, PyObject* names) {
         return nullptr;
     // A call whose function is not bound is declined.
     auto optional = [&](const char* name, auto& fn) { return !PyDict_GetItemString(names, name) || get(name, fn); };
-    if (!optional("femto_paged_attention_gemv_window", g_gemv_window) ||
+    if (!optional("femto_rope_cache_write", g_rope) || !optional("femto_paged_attention_gemv_shared_prefix", g_shared) ||
+        !optional("femto_paged_attention_gemv_shared_prefix_workspace_size", g_shared_ws) || !optional("femto_paged_attention_gemv_window", g_gemv_window) ||
         !optional("femto_paged_attention_gemv_window_workspace_size", g_gemv_window_ws) ||
         !optional("femto_paged_attention_gemm_window", g_gemm_window) ||
         !optional("femto_paged_attention_gemm_window_workspace_size", g_gemm_window_ws))
@@ -411,6 +499,8 @@ PyMethodDef methods[] = {
     {"gemv_window", FEMTO_FAST(gemv_window)},
     {"gemm_window", FEMTO_FAST(gemm_window)},
     {"prologue", FEMTO_FAST(prologue)},
+    {"gemv_shared", FEMTO_FAST(gemv_shared)},
+    {"rope", FEMTO_FAST(rope)},
     {"flash", FEMTO_FAST(flash)},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -105,6 +105,17 @@ def _declare_added(lib) -> None:
     lib.femto_paged_attention_gemm_window.argtypes = [
         i, p, i64, i64, p, i64, i64, p, p, i64, i, i, i, i64, i64, i64, p, i, i, i, i, p, i, i64, p, p, i, i, p, sz, p,
     ]
+    lib.femto_paged_attention_gemv_shared_prefix.restype = i
+    lib.femto_paged_attention_gemv_shared_prefix.argtypes = [
+        i, p, i64, i64, p, i64, i64, p, p, i64, i, i, i, i64, i64, i64, p, i, p, i, i64, p, i, i, i, p, sz, p,
+    ]
+    lib.femto_paged_attention_gemv_shared_prefix_workspace_size.restype = sz
+    lib.femto_paged_attention_gemv_shared_prefix_workspace_size.argtypes = [i, i, i, i, i]
+    lib.femto_rope_cache_write.restype = i
+    lib.femto_rope_cache_write.argtypes = [
+        i, p, i64, i64, p, i64, i64, p, i64, i64, p, i64, i64, p, p, i64, i, i, i,
+        p, p, i64, i, i, i, i, i64, i64, i64, p, i, i, i, p, p, i, i64, p,
+    ]
     lib.femto_paged_attention_gemm_window_workspace_size.restype = sz
     lib.femto_paged_attention_gemm_window_workspace_size.argtypes = [i, i, i, i, i, i, i, i]
 
@@ -132,7 +143,8 @@ def _load_native():
     names = ("femto_attn_last_error", "femto_paged_attention_gemv", "femto_paged_attention_gemv_workspace_size",
              "femto_paged_attention_gemm", "femto_paged_attention_gemm_workspace_size",
              "femto_qk_norm_rope_cache_write", "femto_flash_attention",
-             "femto_paged_attention_gemv_window", "femto_paged_attention_gemv_window_workspace_size",
+             "femto_paged_attention_gemv_shared_prefix", "femto_paged_attention_gemv_shared_prefix_workspace_size",
+             "femto_rope_cache_write", "femto_paged_attention_gemv_window", "femto_paged_attention_gemv_window_workspace_size",
              "femto_paged_attention_gemm_window", "femto_paged_attention_gemm_window_workspace_size")
     module.bind({n: ctypes.cast(getattr(_lib, n), ctypes.c_void_p).value for n in names})
     return module
@@ -218,10 +230,11 @@ def _prefill_workspace(device: torch.device, num_seqs: int, num_tokens: int, max
     return _cached_workspace(_prefill_workspaces, device, nbytes, zero=True)
 
 
-# Workspaces of the window calls, one per (device, stream) as above.  No captured graph holds one: a call
+# Workspaces of the window and shared-prefix calls, one per (device, stream) as above.  No captured graph holds one: a call
 # that is being captured takes its own, from the graph's memory.
 _window_workspaces: dict = {}
 _window_prefill_workspaces: dict = {}
+_shared_prefix_workspaces: dict = {}
 
 
 def _call_workspace(cache: dict, device: torch.device, nbytes: int, zero_bytes: int):
@@ -461,6 +474,47 @@ def _paged_attention_gemm_window(q, k_pool, v_pool, cu_seqlens, max_q_len, kv_pa
     return out
 
 
+def _paged_attention_gemv_shared_prefix(q, k_pool, v_pool, prefix_pages, kv_page_tables, kv_lens, max_kv_len):
+    """Decode of a batch on a common prefix; out (n_heads, num_seqs, head_dim)."""
+    out = _native.gemv_shared(q, k_pool, v_pool, prefix_pages, kv_page_tables, kv_lens, max_kv_len,
+                              _shared_prefix_workspaces)
+    if out is not None:
+        return out
+    fn = "paged_attention_gemv_shared_prefix"
+    _check_paged_added(fn, q, k_pool, v_pool, kv_page_tables, kv_lens, decode=False)
+    _check(prefix_pages.dtype == torch.int32, f"{fn}: prefix_pages must be int32")
+    _check(prefix_pages.dim() == 1 and prefix_pages.is_contiguous(), f"{fn}: prefix_pages must be 1-D and contiguous")
+    _check(prefix_pages.device == q.device, f"{fn}: prefix_pages must be on {q.device}")
+    n_heads, num_seqs, dim = q.shape
+    _check(num_seqs == kv_page_tables.size(0), f"{fn}: q.size(1) must equal kv_page_tables.size(0)")
+    _check(num_seqs == kv_lens.size(0), f"{fn}: q.size(1) must equal kv_lens.size(0)")
+    max_kv_len = _int32_arg(fn, "max_kv_len", max_kv_len)
+    _check(q.dtype != torch.float32, f'"{fn}" not implemented for \'Float\'')
+    dtype = _dtype_code(q, fn)
+    pages = prefix_pages.numel()
+    with torch.cuda.device(q.device):
+        out = torch.empty((n_heads, num_seqs, dim), dtype=q.dtype, device=q.device)
+        if num_seqs == 0:
+            return out
+        nbytes = _lib.femto_paged_attention_gemv_shared_prefix_workspace_size(num_seqs, n_heads, k_pool.size(1), pages,
+                                                                              max_kv_len)
+        ws, ws_bytes, _hold = _call_workspace(_shared_prefix_workspaces, q.device, nbytes, 0)
+        rc = _lib_held.femto_paged_attention_gemv_shared_prefix(
+            dtype,
+            q.data_ptr(), q.stride(0), q.stride(1),
+            out.data_ptr(), out.stride(0), out.stride(1),
+            k_pool.data_ptr(), v_pool.data_ptr(),
+            k_pool.size(0), k_pool.size(1), k_pool.size(2), k_pool.size(3),
+            k_pool.stride(0), k_pool.stride(1), k_pool.stride(2),
+            prefix_pages.data_ptr() if pages else None, pages,
+            kv_page_tables.data_ptr(), kv_page_tables.size(1), kv_page_tables.stride(0),
+            kv_lens.data_ptr(), num_seqs, n_heads, max_kv_len,
+            ws, ws_bytes, _stream(q.device),
+        )
+    _raise_on(rc)
+    return out
+
+
 def _kv_cache_write(k, v, k_pool, v_pool, positions, kv_page_tables, cu_seqlens=None, max_q_len=1):
     """Scatter k, v (tokens, n_kv_heads, head_dim) into the paged pools in place."""
     fn = "kv_cache_write"
@@ -577,6 +631,88 @@ def _qk_norm_rope_cache_write(q, k, v, q_weight, k_weight, eps, cos, sin, positi
         positions.data_ptr(), kv_page_tables.data_ptr(), kv_page_tables.size(1), kv_page_tables.stride(0),
         _stream(q.device),
     )
+    _raise_on(rc)
+    return out
+
+
+def _overlaps(a, b) -> bool:
+    """Whether the memory spans of two tensors meet (strided views: from the first to the last element)."""
+    def span(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a.numel() > 0 and b.numel() > 0 and a0 < b1 and b0 < a1
+
+
+def _rope_cache_write(q, k, v, cos, sin, positions, k_pool, v_pool, kv_page_tables, cu_seqlens=None, max_q_len=1,
+                      interleaved=False, out=None):
+    """Rotated q to ``out``, rotated k and v into the pools; returns ``out``."""
+    done = _native.rope(q, k, v, cos, sin, positions, k_pool, v_pool, kv_page_tables, cu_seqlens, max_q_len,
+                        interleaved, out)
+    if done is not None:
+        return done
+    fn = "rope_cache_write"
+    for name, t in (("q", q), ("k", k), ("v", v), ("cos", cos), ("sin", sin), ("positions", positions),
+                    ("k_pool", k_pool), ("v_pool", v_pool), ("kv_page_tables", kv_page_tables)):
+        _check(t.is_cuda, f"{fn}: {name} must be a GPU tensor")
+        _check(t.device == q.device, f"{fn}: {name} must be on {q.device}")
+    _check(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, f"{fn}: q, k, v must be 3-D (tokens, heads, head_dim)")
+    _check(tuple(k.shape) == tuple(v.shape) and q.size(0) == k.size(0) and q.size(2) == k.size(2),
+           f"{fn}: q, k, v shapes disagree")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _check(t.stride(-1) == 1, f"{fn}: {name} must be contiguous in head_dim")
+    _check(q.dtype == k.dtype == v.dtype == k_pool.dtype == v_pool.dtype, f"{fn}: q, k, v and the pools must share a dtype")
+    _check(cos.dtype == torch.float32 and sin.dtype == torch.float32, f"{fn}: cos / sin tables must be float32")
+    _check(cos.dim() == 2 and tuple(cos.shape) == tuple(sin.shape) and cos.stride() == sin.stride()
+           and (cos.size(1) <= 1 or cos.stride(1) == 1), f"{fn}: cos / sin must be (rows, rotary_dim / 2) row-major alike")
+    _check(k_pool.dim() == 4 and tuple(k_pool.shape) == tuple(v_pool.shape) and k_pool.is_contiguous()
+           and v_pool.is_contiguous(), f"{fn}: pools must be contiguous 4-D tensors of one shape")
+    _check(k.size(1) == k_pool.size(1) and k_pool.size(3) == q.size(2), f"{fn}: k heads or head_dim differ from the pools")
+    _check(k_pool.size(2) == kKVLenPerPage, f"{fn}: block_size must be {kKVLenPerPage}, got {k_pool.size(2)}")
+    _check(positions.dtype == torch.int32 and positions.is_contiguous(), f"{fn}: positions must be contiguous int32")
+    _check(kv_page_tables.dtype == torch.int32 and kv_page_tables.dim() == 2
+           and (kv_page_tables.size(1) <= 1 or kv_page_tables.stride(1) == 1), f"{fn}: kv_page_tables must be 2-D row-major int32")
+    num_tokens, num_seqs = q.size(0), kv_page_tables.size(0)
+    _check(positions.numel() == num_tokens, f"{fn}: positions.numel() must equal the number of tokens")
+    max_q_len = _int32_arg(fn, "max_q_len", max_q_len)
+    if cu_seqlens is None:
+        _check(num_tokens == num_seqs, f"{fn}: without cu_seqlens every sequence has one token")
+        cu_ptr = None
+    else:
+        _check(cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and cu_seqlens.device == q.device,
+               f"{fn}: cu_seqlens must be a contiguous int32 tensor on {q.device}")
+        _check(cu_seqlens.numel() - 1 == num_seqs, f"{fn}: cu_seqlens.numel()-1 must equal kv_page_tables.size(0)")
+        cu_ptr = cu_seqlens.data_ptr()
+    dtype = _dtype_code(q, fn)
+    if out is not None:
+        _check(tuple(out.shape) == tuple(q.shape) and out.dtype == q.dtype and out.stride(-1) == 1 and out.device == q.device,
+               f"{fn}: out must match q")
+        in_place = out.data_ptr() == q.data_ptr() and out.stride() == q.stride()
+        others = [("k", k), ("v", v)] if in_place else [("q", q), ("k", k), ("v", v)]
+        for name, t in others:
+            _check(in_place or not _overlaps(out, t), f"{fn}: out must be q itself or share no memory with {name}")
+    with torch.cuda.device(q.device):
+        if out is None:
+            out = torch.empty_like(q)
+        if num_tokens == 0 or num_seqs == 0:
+            return out
+        rc = _lib.femto_rope_cache_write(
+            dtype,
+            q.data_ptr(), q.stride(0), q.stride(1),
+            k.data_ptr(), k.stride(0), k.stride(1),
+            v.data_ptr(), v.stride(0), v.stride(1),
+            out.data_ptr(), out.stride(0), out.stride(1),
+            cos.data_ptr(), sin.data_ptr(), cos.stride(0) if cos.size(0) > 1 else max(cos.stride(0), cos.size(1)),
+            cos.size(0), 2 * cos.size(1), int(bool(interleaved)),
+            k_pool.data_ptr(), v_pool.data_ptr(),
+            k_pool.size(0), q.size(1), k_pool.size(1), k_pool.size(2), k_pool.size(3),
+            k_pool.stride(0), k_pool.stride(1), k_pool.stride(2),
+            cu_ptr, num_seqs, num_tokens, max_q_len,
+            positions.data_ptr(), kv_page_tables.data_ptr(), kv_page_tables.size(1),
+            kv_page_tables.stride(0) if num_seqs > 1 else max(kv_page_tables.stride(0), kv_page_tables.size(1)),
+            _stream(q.device),
+        )
     _raise_on(rc)
     return out
 

@@ -22,6 +22,9 @@ rotary embedding that precede those loops (qwen3.py:230-238, 312-320).
 ``paged_attention_gemv_window`` and ``paged_attention_gemm_window`` are the
 two attention operators under a sliding window whose first tokens may stay
 visible; the reference has no windowed attention.
+``paged_attention_gemv_shared_prefix`` is decode for a batch on a common
+prefix, which the reference reads once per sequence.  ``rope_cache_write`` is
+the prologue of layers without q/k norms, for every rotary layout.
 
 One deliberate difference: ``q`` arrives as ``q.transpose(0, 1)`` of a
 ``(tokens, n_heads, head_dim)`` tensor (femtovllm/models/qwen/qwen3.py:270,
@@ -195,6 +198,31 @@ def paged_attention_gemm_window(
                                                      max_q_len, kv_page_tables, kv_lens, positions, window, sinks)
 
 
+def paged_attention_gemv_shared_prefix(
+    q: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    prefix_pages: torch.Tensor,
+    kv_page_tables: torch.Tensor,
+    kv_lens: torch.Tensor,
+    max_kv_len: int,
+):
+    """:func:`paged_attention_gemv` for a batch whose sequences share their first blocks.
+
+    ``prefix_pages`` (P,) int32: the blocks of the common prefix, full ones (a
+    node of the prefix tree; ``kv_page_tables[0, :P]`` where that row holds
+    them).  Key j of sequence b is in block ``prefix_pages[j // 16]`` for
+    ``j < 16 P`` and in ``kv_page_tables[b, j // 16]`` after that; the tables'
+    first P columns are not read.  ``kv_lens`` counts the prefix too and may
+    end inside it.  The prefix is read once for the whole batch, and the call
+    costs its tails beside that.  bf16 or f16, head_dim a multiple of 16;
+    contexts of any length; an empty one gives zeros.  V of the prefix has to be
+    finite: a value that is not may also reach sequences that end before it.
+    """
+    return _hip_backend._paged_attention_gemv_shared_prefix(_ensure_valid_tensor(q, "q"), k_pool, v_pool, prefix_pages,
+                                                            kv_page_tables, kv_lens, max_kv_len)
+
+
 def kv_cache_write(
     k: torch.Tensor,
     v: torch.Tensor,
@@ -261,3 +289,38 @@ def qk_norm_rope_cache_write(
     return _hip_backend._qk_norm_rope_cache_write(q, k, v, q_norm_weight, k_norm_weight, eps, cos, sin, positions,
                                                    k_cache_pool, v_cache_pool, kv_page_tables, cu_seqlens,
                                                    max_q_len, out)
+
+
+def rope_cache_write(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    positions: torch.Tensor,
+    k_cache_pool: torch.Tensor,
+    v_cache_pool: torch.Tensor,
+    kv_page_tables: torch.Tensor,
+    cu_seqlens: torch.Tensor = None,
+    max_q_len: int = 1,
+    interleaved: bool = False,
+    out: torch.Tensor = None,
+):
+    """The prologue of layers without q/k norms in one kernel; returns the rotated q.
+
+    q (num_tokens, n_heads, head_dim), k and v (num_tokens, n_kv_heads,
+    head_dim), head_dim at most 128; ``cos`` / ``sin`` float32 tables
+    (max_seqlen, rotary_dim / 2), e.g. of ``femtovllm.rope.scaled_rope_tables``;
+    ``positions`` each token's position.  Rotates the first ``rotary_dim`` dims
+    of each q and k head, as pairs (i, i + rotary_dim / 2) or, ``interleaved``,
+    (2 i, 2 i + 1): (a, b) -> (a cos - b sin, b cos + a sin); the other dims
+    pass through.  The rotated q goes to ``out`` (new; if given, ``q`` itself
+    or memory of its own), the rotated k and v into the pools exactly as
+    :func:`kv_cache_write`.  Each output element is rounded once from fp32; a
+    position outside the tables gives NaN in the rotated dims.
+    """
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not t.is_cuda:
+            raise ValueError(f"Argument '{name}' must be a CUDA tensor. Got device={t.device}")
+    return _hip_backend._rope_cache_write(q, k, v, cos, sin, positions, k_cache_pool, v_cache_pool, kv_page_tables,
+                                          cu_seqlens, max_q_len, interleaved, out)
