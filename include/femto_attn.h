@@ -130,8 +130,12 @@ int femto_paged_attention_gemv_noalloc(
  * femto_paged_attention_gemv; pages with no visible key are not read (their
  * table entries may be -1 or stale), and keys that are not seen have no
  * influence, whatever they hold.  window >= 1 (any larger than the contexts:
- * all keys), sinks >= 0.  The one-launch limit counts min(max_kv_len, window +
- * sinks) keys, and only longer calls need the workspace (of the size below).
+ * all keys), sinks >= 0.  Calls of few keys or many sequences run as one
+ * launch without a workspace (the size below is 0 then); others need it
+ * (256-byte aligned, no initialisation), and those that may overlap must not
+ * share one.  The size is that of the current device (0 without one).
+ * femto_attn_set_decode_single_max_kv holds for min(max_kv_len, window + sinks)
+ * keys here.  Strides as there, pool rows at most 2^24 elements apart.
  * No counterpart in the reference, whose decode always sees the whole context. */
 int femto_paged_attention_gemv_window(
     int dtype,
@@ -144,8 +148,8 @@ int femto_paged_attention_gemv_window(
     const int32_t* kv_lens, int num_seqs, int n_heads, int max_kv_len, int window, int sinks,
     void* workspace, size_t workspace_bytes,
     void* stream);
-size_t femto_paged_attention_gemv_window_workspace_size(int num_seqs, int n_heads, int max_kv_len, int window,
-                                                        int sinks);
+size_t femto_paged_attention_gemv_window_workspace_size(int dtype, int num_seqs, int n_heads, int n_kv_heads,
+                                                        int max_kv_len, int window, int sinks);
 
 /* Paged chunked / varlen / causal prefill attention on bf16 or f16 MFMA:
  * token t of sequence b (cu_seqlens[b] <= t < cu_seqlens[b+1]) sees key j

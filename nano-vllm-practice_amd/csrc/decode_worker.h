@@ -604,38 +604,15 @@ __device__ __forceinline__ void publish_and_merge(const DecodeArgs& a, int b, in
 // holds at once.  A wave walks its slice sequence by sequence and leaves one
 // partial softmax state per (sequence segment, query head); the merge kernel
 // combines them.  Slice s of sequence b is partial slot s - first_wave(b).
-// The waves of workgroup `block` (4 per workgroup, no barriers: a wave may
-// return on its own); used by the decode kernel and by the fused prefill
-// launch, whose first workgroups are decode workers.
-// MAY_MERGE: built with the in-launch merge (used when a.merge_counters is set).
-template <typename E, int NREP, bool FULL, bool MAY_MERGE, int RULE = kAllPages>
-__device__ __forceinline__ void decode_waves(const DecodeArgs& a, int block) {
+//
+// walk_slice finds the slice of wave wi of its head group and calls
+// segment(b, kv_len, start, lp0, n, qrow, slot, count, last) for each of its
+// sequence segments: pages lp0 .. lp0 + n - 1 of sequence b's list, partial slot
+// `slot` of `count`, last: the sequence ends in it.
+template <int RULE, typename F>
+__device__ __forceinline__ void walk_slice(const DecodeArgs& a, int wi, F&& segment) {
     const int lane = threadIdx.x & 63;
-    const int gw = block * 4 + (threadIdx.x >> 6);
-    const int grp = gw / a.waves_per_group;
-    const int wi = gw - grp * a.waves_per_group;
-    if (grp >= a.grid_heads) return;  // waves are independent: no barriers below
-    const int kvh = grp / a.head_groups;
-    const int hg = grp - kvh * a.head_groups;
-    const int h0 = kvh * a.n_rep + hg * NREP;
-    const int rg = lane >> 4;
-    const int c = lane & 15;
     const int B = a.num_seqs;
-
-    if (MAY_MERGE && a.merge_counters && wi == 0) {
-        // Rows with no visible key, which no wave below meets: 0 / 0, as the
-        // merge launch writes them.
-        for (int i = lane; i < B; i += kWave) {
-            int row, len, start;
-            if (!decode_row_of<RULE>(a, i, row, len, start) || pages_seen<RULE>(a, len, start) > 0) continue;
-            for (int r = 0; r < NREP; ++r)
-                for (int d = 0; d < a.head_dim; ++d)
-                    store_elem<E>(reinterpret_cast<char*>(a.out),
-                                  (int64_t)(h0 + r) * a.out_stride_head + (int64_t)row * a.out_stride_seq + d,
-                                  __builtin_nanf(""));
-        }
-    }
-
     // Pass 1: total pages P and the longest sequence; slice length C.  Up to
     // 64 sequences this pass already loads what pass 2 needs (6 sequences of
     // 6-8k keys 38.9 -> 38.5 us, 2 of 2-3k 15.1 -> 14.9).
@@ -681,9 +658,6 @@ __device__ __forceinline__ void decode_waves(const DecodeArgs& a, int block) {
     const uint64_t after = __ballot(base + lane < B && my_excl + pages_seen<RULE>(a, my_len, my_start) > x0);
     int b = base + __builtin_ctzll(after);
 
-    const int64_t head_off = (int64_t)kvh * a.pool_stride_head;
-    const int H = a.n_heads;
-
     int x = x0;
     while (x < x1) {
         if (b - base >= kWave) {  // next chunk of sequences
@@ -709,18 +683,56 @@ __device__ __forceinline__ void decode_waves(const DecodeArgs& a, int block) {
         const int n = lp1 - lp0;
 
         const int qrow = a.cu_seqlens ? a.cu_seqlens[b] : b;
+        segment(b, kv_len, start, lp0, n, qrow, wi - S / C, (S + npg - 1) / C - S / C + 1, lp1 == npg);
+        x = S + lp1;
+        ++b;
+    }
+}
+
+// The waves of workgroup `block` (4 per workgroup, no barriers: a wave may
+// return on its own); used by the decode kernel and by the fused prefill
+// launch, whose first workgroups are decode workers.
+// MAY_MERGE: built with the in-launch merge (used when a.merge_counters is set).
+template <typename E, int NREP, bool FULL, bool MAY_MERGE, int RULE = kAllPages>
+__device__ __forceinline__ void decode_waves(const DecodeArgs& a, int block) {
+    const int lane = threadIdx.x & 63;
+    const int gw = block * 4 + (threadIdx.x >> 6);
+    const int grp = gw / a.waves_per_group;
+    const int wi = gw - grp * a.waves_per_group;
+    if (grp >= a.grid_heads) return;  // waves are independent: no barriers below
+    const int kvh = grp / a.head_groups;
+    const int hg = grp - kvh * a.head_groups;
+    const int h0 = kvh * a.n_rep + hg * NREP;
+    const int rg = lane >> 4;
+    const int c = lane & 15;
+    const int B = a.num_seqs;
+
+    if (MAY_MERGE && a.merge_counters && wi == 0) {
+        // Rows with no visible key, which no wave below meets: 0 / 0, as the
+        // merge launch writes them.
+        for (int i = lane; i < B; i += kWave) {
+            int row, len, start;
+            if (!decode_row_of<RULE>(a, i, row, len, start) || pages_seen<RULE>(a, len, start) > 0) continue;
+            for (int r = 0; r < NREP; ++r)
+                for (int d = 0; d < a.head_dim; ++d)
+                    store_elem<E>(reinterpret_cast<char*>(a.out),
+                                  (int64_t)(h0 + r) * a.out_stride_head + (int64_t)row * a.out_stride_seq + d,
+                                  __builtin_nanf(""));
+        }
+    }
+
+    const int64_t head_off = (int64_t)kvh * a.pool_stride_head;
+    const int H = a.n_heads;
+    walk_slice<RULE>(a, wi, [&](int b, int kv_len, int start, int lp0, int n, int qrow, int slot, int count, bool last)
+                                __attribute__((always_inline)) {
         float m[NREP], l[NREP], acc[NREP][8];
         decode_segment<E, NREP, FULL, RULE>(a, b, kv_len, start, lp0, n, qrow, h0, head_off, m, l, acc);
 
         // Partial state of this segment.
-        const int slot = wi - S / C;
         if (MAY_MERGE && a.merge_counters) {
-            const int count = (S + npg - 1) / C - S / C + 1;  // waves that hold a part of the sequence
             if (count == 1) store_rows<E, NREP, FULL>(a, qrow, h0, l, acc);
             else publish_and_merge<E, NREP, FULL>(a, b, grp, qrow, h0, slot, count, m, l, acc);
-            x = S + lp1;
-            ++b;
-            continue;
+            return;
         }
         if (rg == 0) {
 #pragma unroll
@@ -735,10 +747,8 @@ __device__ __forceinline__ void decode_waves(const DecodeArgs& a, int block) {
                 }
             }
         }
-        if (lane == 0 && grp == 0 && lp1 == npg) a.seq_slots[b] = slot + 1;  // last segment: slot count
-        x = S + lp1;
-        ++b;
-    }
+        if (lane == 0 && grp == 0 && last) a.seq_slots[b] = slot + 1;  // last segment: slot count
+    });
 }
 
 }  // namespace femto

@@ -16,6 +16,7 @@
 #include "decode_route.h"
 #include "femto_attn.h"
 #include "launch.h"
+#include "mfma_decode.h"
 
 // Scratch of femto_paged_attention_gemv_noalloc (see scratch_pointer below).
 constexpr size_t kScratchBytes = (size_t)64 << 20;  // 64 MiB per GPU
@@ -251,17 +252,15 @@ static int check_window(const std::string& fn, int window, int sinks) {
     return FEMTO_OK;
 }
 
-// Decode entry points: femto_paged_attention_gemv (workspace from the caller),
-// femto_paged_attention_gemv_noalloc (workspace = this device's scratch) and
-// femto_paged_attention_gemv_window (window > 0).
+// Decode entry points: femto_paged_attention_gemv (workspace from the caller)
+// and femto_paged_attention_gemv_noalloc (workspace = this device's scratch).
 static int paged_decode_entry(const char* fn_name, int dtype, const void* q, int64_t q_stride_head,
                               int64_t q_stride_seq, void* out, int64_t out_stride_head, int64_t out_stride_seq,
                               const void* k_pool, const void* v_pool, int64_t num_blocks, int n_kv_heads,
                               int block_size, int head_dim, int64_t pool_stride_block, int64_t pool_stride_head,
                               int64_t pool_stride_row, const int32_t* kv_page_tables, int num_pages_per_seq,
                               int64_t table_stride, const int32_t* kv_lens, int num_seqs, int n_heads, int max_kv_len,
-                              int window, int sinks, bool use_scratch, void* workspace, size_t workspace_bytes,
-                              void* stream) {
+                              bool use_scratch, void* workspace, size_t workspace_bytes, void* stream) {
     g_err.clear();
     const std::string fn(fn_name);
     if (dtype != FEMTO_F32 && dtype != FEMTO_F16 && dtype != FEMTO_BF16)
@@ -274,23 +273,15 @@ static int paged_decode_entry(const char* fn_name, int dtype, const void* q, int
                                 q_stride_head, q_stride_seq, kv_page_tables, num_pages_per_seq, table_stride, true);
     if (rc != FEMTO_OK) return rc;
 
-    // Under a window the call is planned for the keys that a query reads, and
-    // routed by those it sees.
-    int seen = max_kv_len;
-    if (window > 0) {
-        seen = (int)std::min<int64_t>(max_kv_len, (int64_t)window + sinks);
-        max_kv_len = window_max_keys(max_kv_len, window, sinks);
-    }
-    const auto launch = window > 0 ? femto::launch_window_decode : femto::launch_paged_decode;
     femto::DecodePlan plan = femto::plan_paged_decode(n_heads, n_kv_heads, max_kv_len, dtype);
     const int limit = g_single_max_kv.load(std::memory_order_relaxed);
-    bool single = seen <= limit;
+    bool single = max_kv_len <= limit;
     femto::DecodeRoute route{};
     if (single) {
         int cus = 0;
         rc = hip_status(femto::device_cu_count(cus), (fn + ": device query").c_str());
         if (rc != FEMTO_OK) return rc;
-        route = femto::decode_route(num_seqs, n_heads, n_kv_heads, plan.nrep_tile, seen, dtype == FEMTO_F32, cus);
+        route = femto::decode_route(num_seqs, n_heads, n_kv_heads, plan.nrep_tile, max_kv_len, dtype == FEMTO_F32, cus);
     }
     if (single && route.split && !use_scratch && limit == kSingleMaxKV) {
         // The split route, if the caller's workspace holds its partial slots:
@@ -314,9 +305,8 @@ static int paged_decode_entry(const char* fn_name, int dtype, const void* q, int
             n_kv_heads, head_dim, pool_stride_block, pool_stride_head, pool_stride_row, kv_page_tables,
             num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads, nullptr);
         a.single_waves = route.waves;
-        a.window = window;
-        a.sinks = sinks;
-        return hip_status(launch(dtype, a, plan.nrep_tile, num_seqs, true, static_cast<hipStream_t>(stream)),
+        return hip_status(femto::launch_paged_decode(dtype, a, plan.nrep_tile, num_seqs, true,
+                                                     static_cast<hipStream_t>(stream)),
                           (fn + " launch").c_str());
     }
     if (use_scratch) {
@@ -346,14 +336,61 @@ static int paged_decode_entry(const char* fn_name, int dtype, const void* q, int
                                            " bytes (256-byte aligned) required, got " +
                                            std::to_string(workspace_bytes));
 
-    femto::DecodeArgs a = femto::decode_args(
+    const femto::DecodeArgs a = femto::decode_args(
         plan, q, q_stride_head, q_stride_seq, out, out_stride_head, out_stride_seq, k_pool, v_pool, num_blocks,
         n_kv_heads, head_dim, pool_stride_block, pool_stride_head, pool_stride_row, kv_page_tables, num_pages_per_seq,
         table_stride, kv_lens, num_seqs, n_heads, workspace);
-    a.window = window;
-    a.sinks = sinks;
-    return hip_status(launch(dtype, a, plan.nrep_tile, num_seqs, false, static_cast<hipStream_t>(stream)),
+    return hip_status(femto::launch_paged_decode(dtype, a, plan.nrep_tile, num_seqs, false,
+                                                 static_cast<hipStream_t>(stream)),
                       (fn + " launch").c_str());
+}
+
+// A window decode call: planned for the pages that a query reads, routed by
+// the keys that it sees.
+struct WindowPlan {
+    femto::DecodePlan plan;
+    bool single;  // one launch, a workgroup per (sequence, KV head group)
+    int waves;    // ... of so many waves
+};
+
+// One launch of whole sequences needs no merge launch (~4.5 us) but leaves CUs
+// idle where it has fewer workgroups than there are.  16-bit types (us, equal
+// contexts twice the window / contexts spread over a factor of 16; split and
+// merge first; 350 shapes of 1-256 sequences, windows of 64-8192, six head shapes):
+//  * a workgroup per CU: whole sequences always.  32 sequences on 32/8 heads, window
+//    4096: 90.0 / 77.5 -> 81.6 / 70.5; 64 on 16/8, 2048: 88.9 / 76.7 -> 82.9 / 70.7;
+//    128 on 16/16, 1024: 170 / 145 -> 166 / 143;
+//  * half of that: up to 2048 keys.  16 on 32/8: 2048 29.9 / 26.7 -> 26.9 / 25.8, 4096
+//    49.9 / 42.5 and 50.2 / 47.8;
+//  * fewer: up to the one-launch limit.  4 on 32/8: 512 11.9 -> 8.7, 1024 14.5 -> 13.6,
+//    1500 15.7 and 17.9.
+// Eight waves where the walk is long (from 2048 keys: 1-2 %) or the workgroups are
+// few (1 on 32/8 heads, 512: 8.3 -> 7.0), else four (256 on 32/8, 256: 55.3 -> 45.9).
+// f32 follows decode_route as plain calls do.
+static WindowPlan window_plan(int dtype, int num_seqs, int n_heads, int n_kv_heads, int max_kv_len, int window,
+                              int sinks, int cus) {
+    WindowPlan w{};
+    w.plan = femto::plan_paged_decode(n_heads, n_kv_heads, window_max_keys(max_kv_len, window, sinks), dtype);
+    const int seen = (int)std::min<int64_t>(max_kv_len, (int64_t)window + sinks);
+    const int limit = g_single_max_kv.load(std::memory_order_relaxed);
+    w.single = seen <= limit;
+    if (dtype == FEMTO_F32) {
+        if (!w.single) return w;
+        const femto::DecodeRoute route =
+            femto::decode_route(num_seqs, n_heads, n_kv_heads, w.plan.nrep_tile, seen, true, cus);
+        if (route.split && limit == kSingleMaxKV) {
+            w.single = false;
+        } else {
+            w.plan.nrep_tile = route.nrep_tile;
+            w.waves = route.waves;
+        }
+        return w;
+    }
+    const int n_rep = n_heads / n_kv_heads;
+    const int64_t groups = (int64_t)num_seqs * n_kv_heads * ((n_rep + femto::kMfmaHeads - 1) / femto::kMfmaHeads);
+    if (limit == kSingleMaxKV) w.single = w.single || groups >= cus || (2 * groups >= cus && seen <= 2048);
+    w.waves = seen >= 2048 || groups <= cus / 8 ? 8 : 4;
+    return w;
 }
 
 // Decode-row part of a prefill call's workspace (after the key-split part):
@@ -478,7 +515,7 @@ static int paged_gemm_entry(const char* fn_name, int dtype, const void* q, int64
             // tiles' kernel its registers (256, and 2x slower workers).
             const int group = femto::prefill_group(a.n_rep);
             const int64_t groups = n_heads / group;
-            const bool few = group <= 2 && decode_rows * groups <= resident / 2 && num_seqs * groups <= resident;
+            const bool few = window == 0 && group <= 2 && decode_rows * groups <= resident / 2 && num_seqs * groups <= resident;
             femto::DecodeArgs d = femto::decode_args(
                 plan, q, q_stride_head, q_stride_token, out, out_stride_head, out_stride_token, k_pool, v_pool,
                 num_blocks, n_kv_heads, head_dim, pool_stride_block, pool_stride_head, pool_stride_row,
@@ -490,13 +527,13 @@ static int paged_gemm_entry(const char* fn_name, int dtype, const void* q, int64
             d.sinks = sinks;
             if (few) d.merge_counters = a.counters + resident;
             a.skip_decode_rows = 1;
-            if (plan.nrep_tile == group) {
+            if (window > 0) femto::set_mfma_heads(d);  // workers for any head ratio
+            if (window > 0 || plan.nrep_tile == group) {
                 a.decode_blocks = femto::decode_worker_blocks(d);
                 if (a.decode_blocks <= 0) return fail(FEMTO_ERR_HIP, fn + ": device query");
                 a.dec = d;
             } else {
-                const auto launch = window > 0 ? femto::launch_window_decode : femto::launch_paged_decode;
-                rc = hip_status(launch(dtype, d, plan.nrep_tile, num_seqs, false, st),
+                rc = hip_status(femto::launch_paged_decode(dtype, d, plan.nrep_tile, num_seqs, false, st),
                                 (fn + " decode-row launch").c_str());
                 if (rc != FEMTO_OK) return rc;
             }
@@ -549,14 +586,19 @@ int femto_paged_attention_gemv(int dtype, const void* q, int64_t q_stride_head, 
     return paged_decode_entry("paged_attention_gemv", dtype, q, q_stride_head, q_stride_seq, out, out_stride_head,
                               out_stride_seq, k_pool, v_pool, num_blocks, n_kv_heads, block_size, head_dim,
                               pool_stride_block, pool_stride_head, pool_stride_row, kv_page_tables,
-                              num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads, max_kv_len, 0, 0, false,
+                              num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads, max_kv_len, false,
                               workspace, workspace_bytes, stream);
 }
 
-size_t femto_paged_attention_gemv_window_workspace_size(int num_seqs, int n_heads, int max_kv_len, int window,
-                                                        int sinks) {
-    if (num_seqs <= 0 || n_heads <= 0 || window < 1 || sinks < 0) return 0;
-    return femto_paged_attention_gemv_workspace_size(num_seqs, n_heads, window_max_keys(max_kv_len, window, sinks));
+size_t femto_paged_attention_gemv_window_workspace_size(int dtype, int num_seqs, int n_heads, int n_kv_heads,
+                                                        int max_kv_len, int window, int sinks) {
+    if (num_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || max_kv_len < 0 || window < 1 ||
+        sinks < 0)
+        return 0;
+    int cus = 0;
+    if (femto::device_cu_count(cus) != hipSuccess) return 0;
+    const WindowPlan w = window_plan(dtype, num_seqs, n_heads, n_kv_heads, max_kv_len, window, sinks, cus);
+    return w.single ? 0 : femto::decode_workspace_bytes(num_seqs, n_heads, w.plan.max_slots);
 }
 
 int femto_paged_attention_gemv_window(int dtype, const void* q, int64_t q_stride_head, int64_t q_stride_seq, void* out,
@@ -568,13 +610,39 @@ int femto_paged_attention_gemv_window(int dtype, const void* q, int64_t q_stride
                                       int max_kv_len, int window, int sinks, void* workspace, size_t workspace_bytes,
                                       void* stream) {
     g_err.clear();
-    const int rc = check_window("paged_attention_gemv_window", window, sinks);
+    const char* fn_name = "paged_attention_gemv_window";
+    const std::string fn(fn_name);
+    if (dtype != FEMTO_F32 && dtype != FEMTO_F16 && dtype != FEMTO_BF16)
+        return fail(FEMTO_ERR_UNSUPPORTED, fn + ": dtype " + dtype_name(dtype) + " is not supported");
+    int rc = check_window(fn, window, sinks);
     if (rc != FEMTO_OK) return rc;
-    return paged_decode_entry("paged_attention_gemv_window", dtype, q, q_stride_head, q_stride_seq, out,
-                              out_stride_head, out_stride_seq, k_pool, v_pool, num_blocks, n_kv_heads, block_size,
-                              head_dim, pool_stride_block, pool_stride_head, pool_stride_row, kv_page_tables,
-                              num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads, max_kv_len, window, sinks,
-                              false, workspace, workspace_bytes, stream);
+    if (num_seqs < 0 || max_kv_len < 0) return fail(FEMTO_ERR_INVALID, fn + ": negative size");
+    if (num_seqs == 0) return FEMTO_OK;
+    if (!kv_lens) return fail(FEMTO_ERR_INVALID, fn + ": null kv_lens");
+    rc = check_paged_common(fn_name, dtype, q, out, k_pool, v_pool, num_blocks, n_kv_heads, block_size, head_dim,
+                            pool_stride_block, pool_stride_head, pool_stride_row, n_heads, q_stride_head, q_stride_seq,
+                            kv_page_tables, num_pages_per_seq, table_stride, true);
+    if (rc != FEMTO_OK) return rc;
+    if (pool_stride_row < 0 || pool_stride_row > (1 << 24))
+        return fail(FEMTO_ERR_INVALID, fn + ": pool row stride out of range");
+    int cus = 0;
+    rc = hip_status(femto::device_cu_count(cus), (fn + ": device query").c_str());
+    if (rc != FEMTO_OK) return rc;
+    const WindowPlan w = window_plan(dtype, num_seqs, n_heads, n_kv_heads, max_kv_len, window, sinks, cus);
+    const size_t need = w.single ? 0 : femto::decode_workspace_bytes(num_seqs, n_heads, w.plan.max_slots);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
+        return fail(FEMTO_ERR_INVALID, fn + ": workspace of " + std::to_string(need) +
+                                           " bytes (256-byte aligned) required, got " + std::to_string(workspace_bytes));
+    femto::DecodeArgs a = femto::decode_args(
+        w.plan, q, q_stride_head, q_stride_seq, out, out_stride_head, out_stride_seq, k_pool, v_pool, num_blocks,
+        n_kv_heads, head_dim, pool_stride_block, pool_stride_head, pool_stride_row, kv_page_tables, num_pages_per_seq,
+        table_stride, kv_lens, num_seqs, n_heads, need ? workspace : nullptr);
+    a.single_waves = w.waves;
+    a.window = window;
+    a.sinks = sinks;
+    return hip_status(femto::launch_window_decode(dtype, a, w.plan.nrep_tile, num_seqs, w.single,
+                                                  static_cast<hipStream_t>(stream)),
+                      (fn + " launch").c_str());
 }
 
 int femto_paged_attention_gemv_noalloc(int dtype, const void* q, int64_t q_stride_head, int64_t q_stride_seq,
@@ -588,8 +656,8 @@ int femto_paged_attention_gemv_noalloc(int dtype, const void* q, int64_t q_strid
     return paged_decode_entry("paged_attention_gemv_noalloc", dtype, q, q_stride_head, q_stride_seq, out,
                               out_stride_head, out_stride_seq, k_pool, v_pool, num_blocks, n_kv_heads, block_size,
                               head_dim, pool_stride_block, pool_stride_head, pool_stride_row, kv_page_tables,
-                              num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads, max_kv_len, 0, 0, true,
-                              nullptr, 0, stream);
+                              num_pages_per_seq, table_stride, kv_lens, num_seqs, n_heads, max_kv_len, true, nullptr,
+                              0, stream);
 }
 
 int femto_paged_attention_gemm(int dtype, const void* q, int64_t q_stride_head, int64_t q_stride_token, void* out,

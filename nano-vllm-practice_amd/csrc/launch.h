@@ -46,6 +46,7 @@ struct DecodeArgs {
     // Window calls (PageList in decode_worker.h): keys a query sees before
     // and at its own position (>= 1), and first keys that stay visible.
     int window, sinks;
+    int heads_per_wave;  // of the workers in mfma_decode.h (set_mfma_heads)
     // Shared-prefix calls: the workers' pages start here; the tiles of the
     // pages before leave prefix_pieces partials per (sequence, head), of
     // prefix_piece_keys keys each, behind the workers' max_slots.

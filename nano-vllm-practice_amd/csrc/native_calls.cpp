@@ -226,7 +226,7 @@ PyObject* gemv_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
         need(B > 0 && B == tab.size(0) && B == len.size(0));
         const int dt = dtype_code(q);
         void* st = stream_of(q);
-        const size_t bytes = g_gemv_window_ws(int32(B), int32(H), max_kv, window, sinks);
+        const size_t bytes = g_gemv_window_ws(dt, int32(B), int32(H), (int)k.size(1), max_kv, window, sinks);
         if (bytes) need_not_captured(st);
         const Workspace w = workspace(a[8], q, st, bytes);
         at::Tensor out = at::empty({H, B, q.size(2)}, q.options());

@@ -44,7 +44,7 @@ hipError_t launch_paged_prefill(int dtype, PrefillArgs a, int num_tokens, int de
         if (e != hipSuccess) return e;
     }
     if (a.decode_blocks > 0) {
-        if (!a.skip_decode_rows || a.dec.head_groups * G != a.n_rep) return hipErrorInvalidValue;
+        if (!a.skip_decode_rows || (a.window == 0 && a.dec.head_groups * G != a.n_rep)) return hipErrorInvalidValue;
         a.decode_blocks = (a.decode_blocks + 7) / 8 * 8;
     }
     if (a.part) {

@@ -11,43 +11,12 @@
 //    cut into pieces, one workgroup each;
 //  * tails: bound by their bytes, on the decode workers of decode_worker.h, in
 //    the same launch, one workgroup per CU beside the tiles.
+#include <cmath>
+
 #include "attention_tiles.h"
+#include "decode_merge.h"
 
 namespace femto {
-
-// One workgroup per (query head, sequence), one thread per head dim: the
-// tail's slots, then the pieces of the prefix that hold keys of the sequence.
-template <typename E>
-__global__ __launch_bounds__(kDimHead) void shared_prefix_merge_kernel(DecodeArgs a) {
-    __shared__ float s_m[kDimHead], s_l[kDimHead];
-    const int h = blockIdx.x, b = blockIdx.y, t = threadIdx.x;
-    const int kv_len = a.kv_lens[b];
-    char* out = reinterpret_cast<char*>(a.out);
-    const int64_t o = (int64_t)h * a.out_stride_head + (int64_t)b * a.out_stride_seq + t;
-    if (kv_len <= 0) {  // an empty slot: zeros, as in a plain decode call
-        if (t < a.head_dim) store_elem<E>(out, o, 0.0f);
-        return;
-    }
-    const int tail = pages_seen<kTailPages>(a, kv_len, 0) > 0 ? a.seq_slots[b] : 0;
-    const int prefix_keys = min(kv_len, a.first_page * kPage);
-    const int count = tail + (prefix_keys > 0 ? (prefix_keys + a.prefix_piece_keys - 1) / a.prefix_piece_keys : 0);
-    const int64_t sl0 = ((int64_t)b * a.n_heads + h) * slot_stride<kTailPages>(a);
-    auto slot = [&](int i) { return sl0 + (i < tail ? i : a.max_slots + (i - tail)); };
-    if (t < count) {
-        s_m[t] = a.part_ml[slot(t) * 2];
-        s_l[t] = a.part_ml[slot(t) * 2 + 1];
-    }
-    __syncthreads();
-    float M = kEmptyMax;
-    for (int i = 0; i < count; ++i) M = fmaxf(M, s_m[i]);
-    float L = 0.0f, O = 0.0f;
-    for (int i = 0; i < count; ++i) {
-        const float w = fast_exp2(s_m[i] - M);
-        L = fmaf(s_l[i], w, L);
-        if (t < a.head_dim) O = fmaf(a.part_acc[slot(i) * kDimHead + t], w, O);
-    }
-    if (t < a.head_dim) store_elem<E>(out, o, O / L);
-}
 
 SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, int prefix_pages, int max_kv_len,
                                     int dtype, int cus) {
@@ -55,11 +24,21 @@ SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, i
     const int n_rep = n_heads / n_kv_heads, G = prefill_group(n_rep), BT = 32 * (4 / G);
     const int tail = (int)std::max<int64_t>(1, (int64_t)max_kv_len - (int64_t)prefix_pages * kPage);
     p.tail = plan_paged_decode(n_heads, n_kv_heads, tail, dtype);
-    p.tail.nrep_tile = G;
     if (prefix_pages <= 0) return p;
+    // Pieces of the prefix: more of them shorten the tiles' chains (1.2 us per
+    // tile of 64 keys where a CU has one), but each writes and merges 520
+    // bytes per query row.  With T key tiles and U row tiles (per piece one
+    // workgroup each) the best of 2 .. 64 pieces was near 2 sqrt(T) / (1 + U / 24)
+    // over 160 shapes (4-256 sequences, prefixes of 256-16384 keys, five head
+    // shapes), within 8 % but for calls of 10-15 us: 16384 keys, 16 sequences on 16/8
+    // heads (T 256, U 8) 28 us with 32, 31 with 16, 45 with 8; 256 sequences on 64/8
+    // heads (U 128) 195 us with 4, 231 with 16.  Beyond one workgroup per
+    // CU beside the workers they only queue (4096 keys, 256 sequences on 16/8
+    // heads with tails of up to 512: 65 us with 4, 71 with 8, 79 with 16).
     const int tiles = (prefix_pages * kPage + kKvTile - 1) / kKvTile;
-    const int64_t units = (int64_t)(n_heads / G) * ((num_seqs + BT - 1) / BT);
-    const int pieces = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)tiles, 2 * cus / units, 64}));
+    const double units = (double)(n_heads / G) * ((num_seqs + BT - 1) / BT);
+    const double best = std::min(2.0 * std::sqrt((double)tiles) / (1.0 + units / 24.0), std::max(4.0, cus / units));
+    const int pieces = std::max(1, std::min({(int)(best + 0.5), tiles, 64}));
     const int per = (tiles + pieces - 1) / pieces;
     p.pieces = (tiles + per - 1) / per;
     p.piece_keys = per * kKvTile;
@@ -72,18 +51,13 @@ hipError_t launch_shared_prefix(int dtype, PrefillArgs a, hipStream_t st) {
     a.head_groups = a.n_rep / G;
     a.tiles_per_group = (a.num_seqs + BT - 1) / BT;
     a.total_work = a.tiles_per_group * a.n_kv_heads * a.head_groups * a.dec.prefix_pieces;
+    set_mfma_heads(a.dec);
     a.decode_blocks = decode_worker_blocks(a.dec);
     if (a.decode_blocks <= 0) return hipErrorInvalidDevice;
     a.decode_blocks = (a.decode_blocks + 7) / 8 * 8;
     hipError_t e = launch_dtype<true, kTailPages>(dtype, G, a, st);
     if (e != hipSuccess) return e;
-    const dim3 grid(a.n_heads, a.num_seqs);
-    switch (dtype) {
-        case kDtypeBF16: hipLaunchKernelGGL(shared_prefix_merge_kernel<BF16>, grid, dim3(kDimHead), 0, st, a.dec); break;
-        case kDtypeF16: hipLaunchKernelGGL(shared_prefix_merge_kernel<F16>, grid, dim3(kDimHead), 0, st, a.dec); break;
-        default: return hipErrorInvalidValue;
-    }
-    return hipGetLastError();
+    return launch_merge_rows<kTailPages>(dtype, a.dec, a.num_seqs, st);
 }
 
 }  // namespace femto

@@ -100,7 +100,7 @@ def _declare_added(lib) -> None:
         i, p, i64, i64, p, i64, i64, p, p, i64, i, i, i, i64, i64, i64, p, i, i64, p, i, i, i, i, i, p, sz, p,
     ]
     lib.femto_paged_attention_gemv_window_workspace_size.restype = sz
-    lib.femto_paged_attention_gemv_window_workspace_size.argtypes = [i, i, i, i, i]
+    lib.femto_paged_attention_gemv_window_workspace_size.argtypes = [i, i, i, i, i, i, i]
     lib.femto_paged_attention_gemm_window.restype = i
     lib.femto_paged_attention_gemm_window.argtypes = [
         i, p, i64, i64, p, i64, i64, p, p, i64, i, i, i, i64, i64, i64, p, i, i, i, i, p, i, i64, p, p, i, i, p, sz, p,
@@ -411,7 +411,8 @@ def _paged_attention_gemv_window(q, k_pool, v_pool, kv_page_tables, kv_lens, max
         out = torch.empty((n_heads, num_seqs, dim), dtype=q.dtype, device=q.device)
         if num_seqs == 0:
             return out
-        nbytes = _lib.femto_paged_attention_gemv_window_workspace_size(num_seqs, n_heads, max_kv_len, window, sinks)
+        nbytes = _lib.femto_paged_attention_gemv_window_workspace_size(dtype, num_seqs, n_heads, k_pool.size(1),
+                                                                       max_kv_len, window, sinks)
         ws, ws_bytes, _hold = _call_workspace(_window_workspaces, q.device, nbytes, 0)
         rc = _lib_held.femto_paged_attention_gemv_window(
             dtype,

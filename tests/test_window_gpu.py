@@ -87,8 +87,8 @@ def test_decode_long_contexts_and_empty_slots(ops, gpu):
 
 
 @pytest.mark.usefixtures("decode_path")
-def test_decode_whole_context_equals_the_plain_call(ops, gpu):
-    """A window past the context takes the same pages in the same order: the same bits."""
+def test_decode_whole_context_agrees_with_the_plain_call(ops, gpu):
+    """A window past the context: two kernels, each within the bounds of the exact value."""
     w = workloads.make_paged_workload("whole", [(L - 1, 1) for L in LENS], 16, 8, seed=9)
     q, meta = w.gemv_call(device=gpu)
     wd, q = w.to(gpu), q.to(gpu)
@@ -96,7 +96,7 @@ def test_decode_whole_context_equals_the_plain_call(ops, gpu):
     for window, sinks in ((1000, 0), (1 << 40, 0), (3, 1000)):
         b = ops.paged_attention_gemv_window(q, wd.k_pool, wd.v_pool, meta.block_tables, meta.kv_lens, meta.max_kv_len,
                                             window, sinks)
-        assert torch.equal(a, b)
+        assert_agree(b, a, BF16, f"window {window}")
 
 
 @pytest.mark.usefixtures("decode_path")
