@@ -130,10 +130,12 @@ int femto_paged_attention_gemv_noalloc(
  * femto_paged_attention_gemv; pages with no visible key are not read (their
  * table entries may be -1 or stale), and keys that are not seen have no
  * influence, whatever they hold.  window >= 1 (any larger than the contexts:
- * all keys), sinks >= 0.  Calls of few keys or many sequences run as one
- * launch without a workspace (the size below is 0 then); others need it
- * (256-byte aligned, no initialisation), and those that may overlap must not
- * share one.  The size is that of the current device (0 without one).
+ * all keys), sinks >= 0.  Calls of few keys or many sequences need no
+ * workspace (the size below is 0 then); others do (256-byte aligned, its first
+ * femto_paged_attention_gemv_window_zero_bytes() bytes zero-filled before the
+ * first use and left so by every call, whatever its shape), and those that may
+ * overlap must not share one.  The size is that of the current device (0
+ * without one).
  * femto_attn_set_decode_single_max_kv holds for min(max_kv_len, window + sinks)
  * keys here.  Strides as there, pool rows at most 2^24 elements apart.
  * No counterpart in the reference, whose decode always sees the whole context. */
@@ -150,6 +152,7 @@ int femto_paged_attention_gemv_window(
     void* stream);
 size_t femto_paged_attention_gemv_window_workspace_size(int dtype, int num_seqs, int n_heads, int n_kv_heads,
                                                         int max_kv_len, int window, int sinks);
+size_t femto_paged_attention_gemv_window_zero_bytes(void);
 
 /* Paged chunked / varlen / causal prefill attention on bf16 or f16 MFMA:
  * token t of sequence b (cu_seqlens[b] <= t < cu_seqlens[b+1]) sees key j

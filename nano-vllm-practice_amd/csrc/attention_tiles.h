@@ -190,14 +190,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // each XCD takes a contiguous range of the work list (KV head groups
     // outermost, so a head's pages stay in one L2).
     int lin = blockIdx.x;
-    if constexpr (FUSED) {
+    if constexpr (FUSED && WINDOW) {
+        // Decode rows under the window, short pieces of work: the first
+        // a.rows_first workgroups (one per CU), so that rows run beside tiles
+        // from the start, and those after the tiles.
+        const int tiles = (int)gridDim.x - a.decode_blocks;
+        if (lin < a.rows_first || lin >= a.rows_first + tiles) {
+            const int row = lin < a.rows_first ? lin : lin - tiles;
+            __shared__ float s_ml[4][kMfmaHeads][2];
+            static_assert(sizeof(smem) >= 4 * kWorkerLds<kStagesTiles>, "the rows' pages");
+            window_row<E, FULLD, 4, kStagesTiles>(a.dec, row, &smem[0][0][0], s_ml, &s_old);
+            return;
+        }
+        lin -= a.rows_first;  // a multiple of 8: the XCD of a tile is unchanged
+    } else if constexpr (FUSED) {
         // The first workgroups are decode workers (G query heads per wave, as
         // the decode kernel would use for this head ratio); they are
         // dispatched first, one per CU, and the tiles fill the other slots.
         if (lin < a.decode_blocks) {
             static_assert(sizeof(smem) >= 4 * kWorkerLds<kStagesTiles>, "the workers' pages");
-            if constexpr (RULE == kAllPages) decode_waves<E, G, FULLD, (G <= 2)>(a.dec, lin);
-            else mfma_waves<E, FULLD, RULE, kStagesTiles>(a.dec, lin, &smem[0][0][0]);
+            if constexpr (PREFIX) mfma_waves<E, FULLD, RULE, kStagesTiles>(a.dec, lin, &smem[0][0][0]);
+            else decode_waves<E, G, FULLD, (G <= 2)>(a.dec, lin);
             return;
         }
         lin -= a.decode_blocks;  // a multiple of 8: the XCD of a tile is unchanged
@@ -210,8 +223,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     int piece = 0, npieces = 1, sib_base = 0, sib_stride = 0;
     // Copies issued one per score MFMA pair instead of in one burst (only in
     // a launch whose decode workers have one-token sequences to run, and not
-    // beside the workers of mfma_decode.h, whose loads are as few and as wide:
-    // there a burst is faster, 1024 new tokens beside 127 window rows 126 -> 113 us).
+    // beside those of mfma_decode.h, which copy in the same way: there a burst
+    // is faster, 1024 new tokens beside 127 window rows 126 -> 113 us).
     bool spread = false;
     // Key tiles of a query tile whose last key is kvl - 1 (under a window: at
     // most, for tokens at consecutive positions).

@@ -246,6 +246,11 @@ static int window_max_keys(int max_kv_len, int window, int sinks) {
     return (int)std::min<int64_t>(max_kv_len, pages * femto::kPage);
 }
 
+// Counters at the front of a window call's workspace, one per (sequence, KV head
+// group) of a call whose rows are cut into parts.
+constexpr int kWindowCounters = 4096;
+constexpr size_t kWindowZeroBytes = kWindowCounters * sizeof(int);
+
 static int check_window(const std::string& fn, int window, int sinks) {
     if (window < 1) return fail(FEMTO_ERR_INVALID, fn + ": window must be at least 1, got " + std::to_string(window));
     if (sinks < 0) return fail(FEMTO_ERR_INVALID, fn + ": sinks must be >= 0, got " + std::to_string(sinks));
@@ -345,51 +350,64 @@ static int paged_decode_entry(const char* fn_name, int dtype, const void* q, int
                       (fn + " launch").c_str());
 }
 
-// A window decode call: planned for the pages that a query reads, routed by
-// the keys that it sees.
-struct WindowPlan {
-    femto::DecodePlan plan;
-    bool single;  // one launch, a workgroup per (sequence, KV head group)
-    int waves;    // ... of so many waves
+// Window rows (window_row in mfma_decode.h): workgroups per (sequence, KV head
+// group) and waves in each, for `rows` sequences whose queries see up to `seen`
+// keys.  Rows longer than 24 pages are cut where that still leaves each part a CU
+// of its own, into the square root of their pages (each more part shortens the
+// walk, and adds a state to the last part's merge).  One sequence of 8 KV heads
+// (32 query heads, bf16), whole and cut, us: 1024 keys 13.1 and 9.2 (6 parts),
+// 4096 39.2 and 13.1 (8), 8192 74 and 16.4 (12); 256 keys 7.0 whole, 7.3 in two.
+// Sixteen of 4096 keys (128 rows): 48.6, 43.6 in two, 47.4 in three; 24
+// (192 rows): 59.7 and 66.7.  Whole rows take 8 waves where they are long or few.
+struct WindowParts {
+    int parts, waves;
 };
+static WindowParts window_parts(int64_t rows, int n_heads, int n_kv_heads, int seen, int cus) {
+    const int n_rep = n_heads / n_kv_heads;
+    const int64_t groups = rows * n_kv_heads * ((n_rep + femto::kMfmaHeads - 1) / femto::kMfmaHeads);
+    const int limit = g_single_max_kv.load(std::memory_order_relaxed);
+    const int pages = (seen + femto::kPage - 1) / femto::kPage;
+    WindowParts w{1, 4};
+    if (limit == kSingleMaxKV && pages >= 24 && 2 * groups <= cus)
+        w.parts = std::min((int)(cus / groups), (int)(0.7 * std::sqrt((double)pages) + 0.5));
+    if (limit < 0) w.parts = 2;  // cut wherever there are pages for it
+    if (groups > kWindowCounters || pages < 2) w.parts = 1;
+    if (w.parts == 1 && (4 * groups <= cus || seen >= 2048)) w.waves = 8;
+    return w;
+}
 
-// One launch of whole sequences needs no merge launch (~4.5 us) but leaves CUs
-// idle where it has fewer workgroups than there are.  16-bit types (us, equal
-// contexts twice the window / contexts spread over a factor of 16; split and
-// merge first; 350 shapes of 1-256 sequences, windows of 64-8192, six head shapes):
-//  * a workgroup per CU: whole sequences always.  32 sequences on 32/8 heads, window
-//    4096: 90.0 / 77.5 -> 81.6 / 70.5; 64 on 16/8, 2048: 88.9 / 76.7 -> 82.9 / 70.7;
-//    128 on 16/16, 1024: 170 / 145 -> 166 / 143;
-//  * half of that: up to 2048 keys.  16 on 32/8: 2048 29.9 / 26.7 -> 26.9 / 25.8, 4096
-//    49.9 / 42.5 and 50.2 / 47.8;
-//  * fewer: up to the one-launch limit.  4 on 32/8: 512 11.9 -> 8.7, 1024 14.5 -> 13.6,
-//    1500 15.7 and 17.9.
-// Eight waves where the walk is long (from 2048 keys: 1-2 %) or the workgroups are
-// few (1 on 32/8 heads, 512: 8.3 -> 7.0), else four (256 on 32/8, 256: 55.3 -> 45.9).
-// f32 follows decode_route as plain calls do.
+// Workspace of a window decode call: the counters, then the parts' states (f32:
+// the split workers'); none where every sequence is one part.
+struct WindowPlan {
+    femto::DecodePlan plan;  // f32
+    bool single;             // f32: one launch
+    int parts, waves;
+    size_t bytes;
+};
 static WindowPlan window_plan(int dtype, int num_seqs, int n_heads, int n_kv_heads, int max_kv_len, int window,
                               int sinks, int cus) {
     WindowPlan w{};
-    w.plan = femto::plan_paged_decode(n_heads, n_kv_heads, window_max_keys(max_kv_len, window, sinks), dtype);
     const int seen = (int)std::min<int64_t>(max_kv_len, (int64_t)window + sinks);
-    const int limit = g_single_max_kv.load(std::memory_order_relaxed);
-    w.single = seen <= limit;
-    if (dtype == FEMTO_F32) {
-        if (!w.single) return w;
-        const femto::DecodeRoute route =
-            femto::decode_route(num_seqs, n_heads, n_kv_heads, w.plan.nrep_tile, seen, true, cus);
-        if (route.split && limit == kSingleMaxKV) {
-            w.single = false;
-        } else {
-            w.plan.nrep_tile = route.nrep_tile;
-            w.waves = route.waves;
-        }
+    if (dtype != FEMTO_F32) {
+        const WindowParts p = window_parts(num_seqs, n_heads, n_kv_heads, seen, cus);
+        w.plan.nrep_tile = 1;
+        w.plan.max_slots = w.parts = p.parts;
+        w.waves = p.waves;
+        w.bytes = p.parts > 1 ? kWindowZeroBytes + femto::decode_workspace_bytes(num_seqs, n_heads, p.parts) : 0;
         return w;
     }
-    const int n_rep = n_heads / n_kv_heads;
-    const int64_t groups = (int64_t)num_seqs * n_kv_heads * ((n_rep + femto::kMfmaHeads - 1) / femto::kMfmaHeads);
-    if (limit == kSingleMaxKV) w.single = w.single || groups >= cus || (2 * groups >= cus && seen <= 2048);
-    w.waves = seen >= 2048 || groups <= cus / 8 ? 8 : 4;
+    // as plain calls: decode_route
+    w.plan = femto::plan_paged_decode(n_heads, n_kv_heads, window_max_keys(max_kv_len, window, sinks), dtype);
+    const int limit = g_single_max_kv.load(std::memory_order_relaxed);
+    w.single = seen <= limit;
+    if (w.single) {
+        const femto::DecodeRoute route =
+            femto::decode_route(num_seqs, n_heads, n_kv_heads, w.plan.nrep_tile, seen, true, cus);
+        w.single = !route.split || limit != kSingleMaxKV;
+        if (w.single) w.plan.nrep_tile = route.nrep_tile;
+        w.waves = route.waves;
+    }
+    w.bytes = w.single ? 0 : kWindowZeroBytes + femto::decode_workspace_bytes(num_seqs, n_heads, w.plan.max_slots);
     return w;
 }
 
@@ -407,12 +425,21 @@ static size_t gemm_decode_bytes(int num_seqs, int num_tokens, int max_q_len, int
     return (femto::decode_workspace_bytes(num_seqs, n_heads, plan.max_slots) + 255) & ~(size_t)255;
 }
 
-// Pages that a decode row of a prefill call may read: the table's width, or
-// under a window what it sees of it.
-static int gemm_decode_pages(int num_pages_per_seq, int window, int sinks) {
-    if (window == 0) return num_pages_per_seq;
+// Decode-row part of a windowed prefill call: parts of its rows (at most one
+// counter each of the key split's second half), and their states.
+static WindowParts gemm_window_parts(int num_seqs, int num_tokens, int max_q_len, int n_heads, int n_kv_heads,
+                                     int num_pages_per_seq, int window, int sinks, int resident) {
+    const int rows = femto::decode_rows_bound(num_seqs, num_tokens, max_q_len);
     const int64_t table_keys = std::min<int64_t>((int64_t)num_pages_per_seq * femto::kPage, 1 << 30);
-    return (window_max_keys((int)table_keys, window, sinks) + femto::kPage - 1) / femto::kPage;
+    const int seen = (int)std::min<int64_t>(table_keys, (int64_t)window + sinks);
+    if (rows == 0) return {0, 0};
+    WindowParts p = window_parts(rows, n_heads, n_kv_heads, seen, resident / 2);
+    const int n_rep = n_heads / n_kv_heads;
+    if ((int64_t)num_seqs * n_kv_heads * ((n_rep + femto::kMfmaHeads - 1) / femto::kMfmaHeads) > resident) p.parts = 1;
+    return p;
+}
+static size_t gemm_window_bytes(int num_seqs, int n_heads, const WindowParts& p) {
+    return p.parts > 1 ? (femto::decode_workspace_bytes(num_seqs, n_heads, p.parts) + 255) & ~(size_t)255 : 0;
 }
 
 // Prefill entry points: femto_paged_attention_gemm (window == 0) and
@@ -473,16 +500,57 @@ static int paged_gemm_entry(const char* fn_name, int dtype, const void* q, int64
     a.scale_log2 = scale_log2(head_dim);
     a.window = window;
     a.sinks = sinks;
-    const int decode_pages = gemm_decode_pages(num_pages_per_seq, window, sinks);
     hipStream_t st = static_cast<hipStream_t>(stream);
     int decode_rows = 0;
-    if (workspace) {
+    if (window > 0) {
+        int resident = 0;
+        rc = hip_status(femto::prefill_resident_workgroups(resident), (fn + ": device query").c_str());
+        if (rc != FEMTO_OK) return rc;
+        WindowParts p = gemm_window_parts(num_seqs, num_tokens, max_q_len, n_heads, n_kv_heads, num_pages_per_seq,
+                                          window, sinks, resident);
+        const size_t split_bytes = femto::prefill_workspace_bytes(resident);
+        const size_t need = split_bytes + gemm_window_bytes(num_seqs, n_heads, p);
+        if (workspace && (workspace_bytes < need || !aligned(workspace, 256)))
+            return fail(FEMTO_ERR_INVALID, fn + ": workspace of " + std::to_string(need) +
+                                               " bytes (256-byte aligned) required, got " +
+                                               std::to_string(workspace_bytes));
+        if (workspace) {
+            a.counters = static_cast<int*>(workspace);
+            a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + femto::prefill_counter_bytes(resident));
+        } else {
+            p.parts = std::min(p.parts, 1);  // whole rows need no memory
+        }
+        if (p.parts > 0) {
+            // Sequences of one query token run as whole rows in the tiles'
+            // launch (an MFMA tile would hold one valid row of 32).
+            decode_rows = femto::decode_rows_bound(num_seqs, num_tokens, max_q_len);
+            femto::DecodePlan plan{};
+            plan.nrep_tile = 1;
+            plan.max_slots = p.parts;
+            a.dec = femto::decode_args(plan, q, q_stride_head, q_stride_token, out, out_stride_head, out_stride_token,
+                                       k_pool, v_pool, num_blocks, n_kv_heads, head_dim, pool_stride_block,
+                                       pool_stride_head, pool_stride_row, kv_page_tables, num_pages_per_seq,
+                                       table_stride, kv_lens, num_seqs, n_heads,
+                                       workspace ? static_cast<char*>(workspace) + split_bytes : nullptr);
+            femto::set_mfma_heads(a.dec);
+            a.dec.cu_seqlens = cu_seqlens;
+            a.dec.positions = positions;
+            a.dec.window = window;
+            a.dec.sinks = sinks;
+            a.dec.parts = p.parts;
+            a.dec.merge_counters = p.parts > 1 ? a.counters + resident : nullptr;
+            a.skip_decode_rows = 1;
+            const int64_t blocks = (int64_t)num_seqs * a.dec.grid_heads * p.parts;
+            if (blocks > (1 << 30)) return fail(FEMTO_ERR_INVALID, fn + ": too many sequences");
+            a.decode_blocks = (int)blocks;
+        }
+    } else if (workspace) {
         int resident = 0;
         rc = hip_status(femto::prefill_resident_workgroups(resident), (fn + ": device query").c_str());
         if (rc != FEMTO_OK) return rc;
         const size_t split_bytes = femto::prefill_workspace_bytes(resident);
         const size_t need = split_bytes + gemm_decode_bytes(num_seqs, num_tokens, max_q_len, n_heads, n_kv_heads,
-                                                            decode_pages);
+                                                            num_pages_per_seq);
         if (workspace_bytes < need || !aligned(workspace, 256))
             return fail(FEMTO_ERR_INVALID, fn + ": workspace of " + std::to_string(need) +
                                                " bytes (256-byte aligned) required, got " +
@@ -497,7 +565,7 @@ static int paged_gemm_entry(const char* fn_name, int dtype, const void* q, int64
             // (every head ratio but multiples of 8) they run in the same
             // launch as the tiles, which fill the CU slots beside them; else
             // the decode kernel runs first.
-            const femto::DecodePlan plan = gemm_decode_plan(n_heads, n_kv_heads, decode_pages);
+            const femto::DecodePlan plan = gemm_decode_plan(n_heads, n_kv_heads, num_pages_per_seq);
             decode_rows = femto::decode_rows_bound(num_seqs, num_tokens, max_q_len);
             // Few possible one-token sequences (often none: chunks of uneven
             // lengths leave the bound above zero): the workers merge their
@@ -515,7 +583,7 @@ static int paged_gemm_entry(const char* fn_name, int dtype, const void* q, int64
             // tiles' kernel its registers (256, and 2x slower workers).
             const int group = femto::prefill_group(a.n_rep);
             const int64_t groups = n_heads / group;
-            const bool few = window == 0 && group <= 2 && decode_rows * groups <= resident / 2 && num_seqs * groups <= resident;
+            const bool few = group <= 2 && decode_rows * groups <= resident / 2 && num_seqs * groups <= resident;
             femto::DecodeArgs d = femto::decode_args(
                 plan, q, q_stride_head, q_stride_token, out, out_stride_head, out_stride_token, k_pool, v_pool,
                 num_blocks, n_kv_heads, head_dim, pool_stride_block, pool_stride_head, pool_stride_row,
@@ -523,12 +591,9 @@ static int paged_gemm_entry(const char* fn_name, int dtype, const void* q, int64
                 static_cast<char*>(workspace) + split_bytes);
             d.cu_seqlens = cu_seqlens;
             d.positions = positions;
-            d.window = window;
-            d.sinks = sinks;
             if (few) d.merge_counters = a.counters + resident;
             a.skip_decode_rows = 1;
-            if (window > 0) femto::set_mfma_heads(d);  // workers for any head ratio
-            if (window > 0 || plan.nrep_tile == group) {
+            if (plan.nrep_tile == group) {
                 a.decode_blocks = femto::decode_worker_blocks(d);
                 if (a.decode_blocks <= 0) return fail(FEMTO_ERR_HIP, fn + ": device query");
                 a.dec = d;
@@ -598,8 +663,10 @@ size_t femto_paged_attention_gemv_window_workspace_size(int dtype, int num_seqs,
     int cus = 0;
     if (femto::device_cu_count(cus) != hipSuccess) return 0;
     const WindowPlan w = window_plan(dtype, num_seqs, n_heads, n_kv_heads, max_kv_len, window, sinks, cus);
-    return w.single ? 0 : femto::decode_workspace_bytes(num_seqs, n_heads, w.plan.max_slots);
+    return w.bytes;
 }
+
+size_t femto_paged_attention_gemv_window_zero_bytes(void) { return kWindowZeroBytes; }
 
 int femto_paged_attention_gemv_window(int dtype, const void* q, int64_t q_stride_head, int64_t q_stride_seq, void* out,
                                       int64_t out_stride_head, int64_t out_stride_seq, const void* k_pool,
@@ -629,14 +696,16 @@ int femto_paged_attention_gemv_window(int dtype, const void* q, int64_t q_stride
     rc = hip_status(femto::device_cu_count(cus), (fn + ": device query").c_str());
     if (rc != FEMTO_OK) return rc;
     const WindowPlan w = window_plan(dtype, num_seqs, n_heads, n_kv_heads, max_kv_len, window, sinks, cus);
-    const size_t need = w.single ? 0 : femto::decode_workspace_bytes(num_seqs, n_heads, w.plan.max_slots);
+    const size_t need = w.bytes;
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
         return fail(FEMTO_ERR_INVALID, fn + ": workspace of " + std::to_string(need) +
                                            " bytes (256-byte aligned) required, got " + std::to_string(workspace_bytes));
     femto::DecodeArgs a = femto::decode_args(
         w.plan, q, q_stride_head, q_stride_seq, out, out_stride_head, out_stride_seq, k_pool, v_pool, num_blocks,
         n_kv_heads, head_dim, pool_stride_block, pool_stride_head, pool_stride_row, kv_page_tables, num_pages_per_seq,
-        table_stride, kv_lens, num_seqs, n_heads, need ? workspace : nullptr);
+        table_stride, kv_lens, num_seqs, n_heads, need ? static_cast<char*>(workspace) + kWindowZeroBytes : nullptr);
+    a.merge_counters = need && dtype != FEMTO_F32 ? static_cast<int*>(workspace) : nullptr;
+    a.parts = w.parts;
     a.single_waves = w.waves;
     a.window = window;
     a.sinks = sinks;
@@ -677,9 +746,14 @@ int femto_paged_attention_gemm(int dtype, const void* q, int64_t q_stride_head, 
 
 size_t femto_paged_attention_gemm_window_workspace_size(int num_seqs, int num_tokens, int max_q_len, int n_heads,
                                                         int n_kv_heads, int num_pages_per_seq, int window, int sinks) {
-    if (window < 1 || sinks < 0) return 0;
-    return femto_paged_attention_gemm_workspace_size(num_seqs, num_tokens, max_q_len, n_heads, n_kv_heads,
-                                                     gemm_decode_pages(num_pages_per_seq, window, sinks));
+    if (num_seqs <= 0 || num_tokens <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || window < 1 ||
+        sinks < 0)
+        return 0;
+    int resident = 0;
+    if (femto::prefill_resident_workgroups(resident) != hipSuccess) return 0;
+    return femto::prefill_workspace_bytes(resident) +
+           gemm_window_bytes(num_seqs, n_heads, gemm_window_parts(num_seqs, num_tokens, max_q_len, n_heads, n_kv_heads,
+                                                                  num_pages_per_seq, window, sinks, resident));
 }
 
 int femto_paged_attention_gemm_window(int dtype, const void* q, int64_t q_stride_head, int64_t q_stride_token, void* out,

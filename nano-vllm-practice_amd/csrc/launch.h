@@ -47,6 +47,7 @@ struct DecodeArgs {
     // and at its own position (>= 1), and first keys that stay visible.
     int window, sinks;
     int heads_per_wave;  // of the workers in mfma_decode.h (set_mfma_heads)
+    int parts;           // window rows: workgroups per (sequence, KV head group); above one they use merge_counters
     // Shared-prefix calls: the workers' pages start here; the tiles of the
     // pages before leave prefix_pieces partials per (sequence, head), of
     // prefix_piece_keys keys each, behind the workers' max_slots.
@@ -75,10 +76,11 @@ hipError_t launch_paged_decode(int dtype, const DecodeArgs& a, int nrep_tile, in
 // a.waves_per_group; 0 on a device error), and the merge that follows.
 int decode_worker_blocks(DecodeArgs& a);
 hipError_t launch_paged_decode_merge(int dtype, const DecodeArgs& a, int num_seqs, hipStream_t st);
-// The same under a sliding window with sinks (window_decode.hip).
+// The same under a sliding window with sinks (window_decode.hip).  16-bit types
+// are one launch of a.parts workgroups of a.single_waves waves per (sequence,
+// KV head group) (nrep_tile and single are f32's).
 hipError_t launch_window_decode(int dtype, const DecodeArgs& a, int nrep_tile, int num_seqs, bool single,
                                 hipStream_t st);
-hipError_t launch_window_decode_merge(int dtype, const DecodeArgs& a, int num_seqs, hipStream_t st);
 
 struct PrefillArgs {
     const void* q;
@@ -113,8 +115,10 @@ struct PrefillArgs {
     int skip_decode_rows; // sequences of one query token are left to the decode workers
     // Decode workers in the same launch (paged only): the first decode_blocks
     // workgroups run the decode kernel's waves over `dec` (one-token
-    // sequences), the rest the MFMA tiles; 0: none.
+    // sequences), the rest the MFMA tiles; 0: none.  Under a window they run
+    // rows: the first rows_first, and those behind the tiles.
     int decode_blocks;
+    int rows_first;
     DecodeArgs dec;
     // Sliding window with sinks (paged only; window == 0: none).
     int window, sinks;

@@ -1,6 +1,7 @@
-// Decode wave workers on MFMA, for the calls that read a part of each
-// context: window decode (window_decode.hip), the decode rows of a windowed
-// prefill call and the tails of a shared-prefix call (attention_tiles.h).
+// Decode on MFMA, for the calls that read a part of each context: window
+// decode (window_decode.hip) and the decode rows of a windowed prefill call
+// (attention_tiles.h) as whole rows, window_row; the tails of a shared-prefix
+// call (attention_tiles.h) as slices, mfma_waves.
 //
 // Same work as decode_worker.h: one query token per sequence, slices of pages
 // per wave, bound by the bytes of K and V.  There a lane forms four scores per
@@ -235,17 +236,125 @@ __device__ __forceinline__ void store_partial(const DecodeArgs& a, int64_t sl, i
     if (g == 0) *reinterpret_cast<float2*>(a.part_ml + sl * 2) = make_float2(s.m, s.l);
 }
 
-// Normalised row of head c.
-template <typename E>
-__device__ __forceinline__ void store_head(const DecodeArgs& a, int row, int h, int g, const HeadState& s) {
-    char* out = reinterpret_cast<char*>(a.out) + ((int64_t)h * a.out_stride_head + (int64_t)row * a.out_stride_seq) * 2;
+// Window rows: workgroup `block` of W waves takes part (block % a.parts) of the
+// pages that one KV head group's query heads of one sequence see; wave w the
+// w-th of W contiguous shares of it.  The waves fold their states through LDS
+// (each over its own, done, pages).  A sequence in one part is written at once.
+// Else the part's state goes to its slot with system-scope stores (written
+// through to memory) and the workgroup counts itself in; the one that comes
+// last reads all slots (system-scope loads, in part order: the result does not
+// depend on who was last), writes the rows and leaves the counter zero.
+// lds: W * kWorkerLds<STAGES> bytes, s_ml: [W][kMfmaHeads][2].
+template <typename E, bool FULL, int W, int STAGES>
+__device__ __forceinline__ void window_row(const DecodeArgs& a, int block, uint8_t* lds, float (*s_ml)[kMfmaHeads][2],
+                                           int* s_old) {
+    constexpr int kWaveLds = kWorkerLds<STAGES>;
+    static_assert(kWaveLds >= kMfmaHeads * kDimHead * 4, "a wave's outputs");
+    const int P = a.parts;
+    const int part = block % P, bg = block / P;
+    const int b = bg / a.grid_heads, grp = bg - b * a.grid_heads;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kvh = grp / a.head_groups, hg = grp - kvh * a.head_groups;
+    const int h0 = kvh * a.n_rep + hg * a.heads_per_wave;
+    const int nh = min(a.heads_per_wave, a.n_rep - hg * a.heads_per_wave);
+    int row, kv_len, start;
+    if (b >= a.num_seqs || !decode_row_of<kWindowPages>(a, b, row, kv_len, start)) return;  // a chunk's tiles
+    const int npg = pages_seen<kWindowPages>(a, kv_len, start);
+    const int per_part = (npg + P - 1) / P;
+    const int first = part * per_part, mine = min(npg - first, per_part);
+    const int parts = npg > 0 ? (npg + per_part - 1) / per_part : 1;  // with pages
+    if (part >= parts) return;
+    const int per = (mine + W - 1) / W;
+    const int lp0 = min(mine, wave * per), n = min(mine, lp0 + per) - lp0;
+    uint8_t* own = lds + wave * kWaveLds;
+    HeadState s;
+    if (n > 0) {
+        mfma_segment<E, FULL, kWindowPages, STAGES>(a, b, kv_len, start, first + lp0, n, row, h0, nh,
+                                                    (int64_t)kvh * a.pool_stride_head, own, s);
+    } else {
+        s.clear();
+    }
+    if (c < nh) {
+        float* acc = reinterpret_cast<float*>(own) + c * kDimHead + 4 * g;
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) {
+        for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(acc + 16 * dt) = s.o[dt];
+        if (g == 0) {
+            s_ml[wave][c][0] = s.m;
+            s_ml[wave][c][1] = s.l;
+        }
+    }
+    __syncthreads();
+    // Thread i holds dims 4 (i % 32) .. of head i / 32 (and so on).
+    char* out = reinterpret_cast<char*>(a.out);
+    auto write = [&](int r, int d, f32x4 o, float l) __attribute__((always_inline)) {
+        const int64_t at = (int64_t)(h0 + r) * a.out_stride_head + (int64_t)row * a.out_stride_seq + d;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            const int d = 16 * dt + 4 * g + x;
-            if (d < a.head_dim) store_elem<E>(out, d, s.o[dt][x] / s.l);
+            // no key: zeros in a decode call, 0 / 0 in a row of a prefill call
+            const float v = npg > 0 ? o[x] / l : a.cu_seqlens ? __builtin_nanf("") : 0.0f;
+            if (FULL || d + x < a.head_dim) store_elem<E>(out, at + x, v);
         }
+    };
+    const int64_t slot0 = ((int64_t)b * a.n_heads + h0) * P;
+    const auto ra = __builtin_amdgcn_make_buffer_rsrc(a.part_acc + slot0 * kDimHead, (short)0, nh * P * kDimHead * 4, 0x00020000);
+    const auto rm = __builtin_amdgcn_make_buffer_rsrc(a.part_ml + slot0 * 2, (short)0, nh * P * 8, 0x00020000);
+    for (int i = threadIdx.x; i < nh * (kDimHead / 4); i += 64 * W) {
+        const int r = i / (kDimHead / 4), d = 4 * (i % (kDimHead / 4));
+        float M = kEmptyMax;
+#pragma unroll
+        for (int w = 0; w < W; ++w) M = fmaxf(M, s_ml[w][r][0]);
+        float L = 0.0f;
+        f32x4 O = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float f = fast_exp2(s_ml[w][r][0] - M);
+            L = fmaf(s_ml[w][r][1], f, L);
+            O += *reinterpret_cast<const f32x4*>(lds + w * kWaveLds + (r * kDimHead + d) * 4) * f;
+        }
+        if (parts == 1) {
+            write(r, d, O, L);
+        } else {
+            const int sl = r * P + part;
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, O), ra, (sl * kDimHead + d) * 4, 0, 0x11);
+            if (d == 0)
+                __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, rm, sl * 8, 0, 0x11);
+        }
+    }
+    if (parts == 1) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share is in memory
+    __syncthreads();                                    // ... and every wave's, before the count goes up
+    int* counter = a.merge_counters + bg;
+    if (threadIdx.x == 0) *s_old = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (*s_old != parts - 1) return;  // another part merges
+    if (threadIdx.x == 0) __hip_atomic_exchange(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("" ::: "memory");
+    constexpr int kAhead = 8;  // slots in flight
+    for (int i = threadIdx.x; i < nh * (kDimHead / 4); i += 64 * W) {
+        const int r = i / (kDimHead / 4), d = 4 * (i % (kDimHead / 4));
+        float M = kEmptyMax, L = 0.0f;
+        f32x4 O = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int p0 = 0; p0 < parts; p0 += kAhead) {
+            u32x2 ml[kAhead];
+            u32x4 v[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int sl = r * P + min(p0 + u, parts - 1);  // past the end: the last slot again, left out below
+                ml[u] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rm, sl * 8, 0, 0x11));
+                v[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(ra, (sl * kDimHead + d) * 4, 0, 0x11));
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (p0 + u >= parts) break;
+                const float mu = __uint_as_float(ml[u][0]), mn = fmaxf(M, mu);
+                const float f0 = fast_exp2(M - mn), f1 = fast_exp2(mu - mn);
+                L = L * f0 + __uint_as_float(ml[u][1]) * f1;
+                O = O * f0 + __builtin_bit_cast(f32x4, v[u]) * f1;
+                M = mn;
+            }
+        }
+        write(r, d, O, L);
     }
 }
 

@@ -43,13 +43,21 @@ hipError_t launch_paged_prefill(int dtype, PrefillArgs a, int num_tokens, int de
         hipError_t e = prefill_resident_workgroups(a.resident);
         if (e != hipSuccess) return e;
     }
-    if (a.decode_blocks > 0) {
-        if (!a.skip_decode_rows || (a.window == 0 && a.dec.head_groups * G != a.n_rep)) return hipErrorInvalidValue;
-        a.decode_blocks = (a.decode_blocks + 7) / 8 * 8;
-    }
+    if (a.decode_blocks > 0 && !a.skip_decode_rows) return hipErrorInvalidValue;
+    if (a.decode_blocks > 0 && a.window == 0 && a.dec.head_groups * G != a.n_rep) return hipErrorInvalidValue;
+    a.decode_blocks = (a.decode_blocks + 7) / 8 * 8;
+    // Rows under the window in the same launch: the tiles are cut for one slot
+    // of every CU, and rows run in the other from the start, half a slot's worth
+    // of them ahead of the tiles (rows_first), the rest behind them; rows load
+    // while tiles compute.  Rows seeing 1028 keys (32 query heads on 8) beside
+    // 1024 new tokens behind 4096, us: 127 rows 131 with tiles cut for both
+    // slots and ahead of all rows, 114 with all rows ahead of them, 100 so; 33
+    // rows 68, 57 and 46; 4 rows 43, 38 and 38.  Beside 2000 new tokens (tiles
+    // for both slots anyway) all rows ahead is better, 129 and 136 at 127 rows;
+    // every second or third workgroup a row: 100-125 and 125-137.
+    const int slots = a.resident;
+    if (a.window > 0 && a.decode_blocks > 0) a.resident /= 2;
     if (a.part) {
-        hipError_t e = prefill_resident_workgroups(a.resident);
-        if (e != hipSuccess) return e;
         // A split needs all pieces in the resident slots at once, and a call
         // has at least ceil(num_tokens / BT) query tiles per KV head group
         // (not counting sequences of one token when the decode workers take
@@ -65,10 +73,12 @@ hipError_t launch_paged_prefill(int dtype, PrefillArgs a, int num_tokens, int de
             a.total_work = a.total_work > a.resident ? a.total_work : a.resident;
         }
     }
-    hipError_t e = a.window > 0 ? launch_window_tiles(dtype, G, a, st) : launch_dtype<true, kAllPages>(dtype, G, a, st);
-    if (e == hipSuccess && a.decode_blocks > 0 && !a.dec.merge_counters)
-        e = a.window > 0 ? launch_window_decode_merge(dtype, a.dec, a.num_seqs, st)
-                         : launch_paged_decode_merge(dtype, a.dec, a.num_seqs, st);
+    if (a.window > 0) {
+        a.rows_first = std::min(a.decode_blocks, slots / 4) / 8 * 8;
+        return launch_window_tiles(dtype, G, a, st);
+    }
+    hipError_t e = launch_dtype<true, kAllPages>(dtype, G, a, st);
+    if (e == hipSuccess && a.decode_blocks > 0 && !a.dec.merge_counters) e = launch_paged_decode_merge(dtype, a.dec, a.num_seqs, st);
     return e;
 }
 

@@ -101,6 +101,8 @@ def _declare_added(lib) -> None:
     ]
     lib.femto_paged_attention_gemv_window_workspace_size.restype = sz
     lib.femto_paged_attention_gemv_window_workspace_size.argtypes = [i, i, i, i, i, i, i]
+    lib.femto_paged_attention_gemv_window_zero_bytes.restype = sz
+    lib.femto_paged_attention_gemv_window_zero_bytes.argtypes = []
     lib.femto_paged_attention_gemm_window.restype = i
     lib.femto_paged_attention_gemm_window.argtypes = [
         i, p, i64, i64, p, i64, i64, p, p, i64, i, i, i, i64, i64, i64, p, i, i, i, i, p, i, i64, p, p, i, i, p, sz, p,
@@ -413,7 +415,8 @@ def _paged_attention_gemv_window(q, k_pool, v_pool, kv_page_tables, kv_lens, max
             return out
         nbytes = _lib.femto_paged_attention_gemv_window_workspace_size(dtype, num_seqs, n_heads, k_pool.size(1),
                                                                        max_kv_len, window, sinks)
-        ws, ws_bytes, _hold = _call_workspace(_window_workspaces, q.device, nbytes, 0)
+        ws, ws_bytes, _hold = _call_workspace(_window_workspaces, q.device, nbytes,
+                                              _lib.femto_paged_attention_gemv_window_zero_bytes())
         rc = _lib_held.femto_paged_attention_gemv_window(
             dtype,
             q.data_ptr(), q.stride(0), q.stride(1),
