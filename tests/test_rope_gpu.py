@@ -165,6 +165,25 @@ def test_rows_behind_the_last_sequence_stay(ops, gpu):
     assert not torch.isnan(wd.k_pool).any()
 
 
+def test_pools_past_4_gib(ops, gpu):
+    """The same blocks in a compact pool and at the end of one of 4.3 GiB: equal rows written."""
+    w, q, k, v = step(CHUNKS, 16, 8, 128, BF16, seed=31)
+    blocks, n, written = 140_000, w.k_pool.size(0), []
+    tables = [t.to(gpu) for t in scaled_rope_tables(300, 128, base=1000.0)]
+    _, meta = w.gemm_call(device=gpu)
+    for base in (0, blocks - n):
+        pools = [torch.zeros((base + n, 8, 16, 128), dtype=BF16, device=gpu) for _ in range(2)]
+        cols = torch.where(meta.block_tables >= 0, meta.block_tables + base, meta.block_tables)
+        out = ops.rope_cache_write(q.to(gpu), k.to(gpu), v.to(gpu), *tables, meta.positions, *pools, cols,
+                                   cu_seqlens=meta.cu_seqlens, max_q_len=meta.max_q_len)
+        torch.cuda.synchronize()
+        assert not any(pool[:base].any() for pool in pools)
+        written.append([out] + [pool[base:].clone() for pool in pools])
+        del pools
+    for a, b in zip(*written):
+        assert torch.equal(a, b)
+
+
 def test_captured_and_replayed(ops, gpu):
     w, q, k, v = step(CHUNKS, 8, 4, 128, BF16, seed=7)
     _, meta = w.gemm_call(device=gpu)

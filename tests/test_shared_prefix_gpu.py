@@ -75,6 +75,13 @@ def test_batches(ops, gpu, seqs):
     assert_close(out, want, BF16, f"{seqs} sequences")
 
 
+@pytest.mark.parametrize("heads", [(17, 1), (48, 2), (40, 1)])
+def test_more_query_heads_than_a_wave_holds(ops, gpu, heads):
+    w, pages = batch(336, [100, 0, 45, -20], *heads, seed=sum(heads))
+    out, want, _ = run(ops, gpu, w, pages)
+    assert_close(out, want, BF16, f"heads {heads}")
+
+
 def test_no_key_past_the_prefix(ops, gpu):
     """Every context ends inside the prefix, and the largest one is understated to the call."""
     w, pages = batch(640, [-1, -100, -320, -639, -64, -63], 8, 4, seed=2)
@@ -122,6 +129,27 @@ def test_one_dominant_key_is_exact(ops, gpu):
         out, _, _ = run(ops, gpu, w, pages)
         for h in range(4):
             assert torch.equal(out[h].cpu(), w.v_pool[tables[0][j // 16], h // 2, j % 16].expand(84, -1))
+
+
+def test_pools_past_4_gib(ops, gpu):
+    """The same blocks in a compact pool and at the end of one of 4.3 GiB: equal bits."""
+    w, pages = batch(512, [100, 3, 900], 16, 8, seed=31)
+    for pool in (w.k_pool, w.v_pool):
+        pool.nan_to_num_(nan=0.5)
+    blocks, n, outs = 140_000, w.k_pool.size(0), []
+    q, meta = w.gemv_call(device=gpu)
+    for base in (0, blocks - n):
+        pools = []
+        for pool in (w.k_pool, w.v_pool):
+            big = torch.empty((base + n,) + tuple(pool.shape[1:]), dtype=BF16, device=gpu)
+            big[base:] = pool.to(gpu)
+            pools.append(big)
+        tables = torch.where(meta.block_tables >= 0, meta.block_tables + base, meta.block_tables)
+        outs.append(ops.paged_attention_gemv_shared_prefix(q.to(gpu), *pools, (pages + base).to(gpu), tables, meta.kv_lens,
+                                                           meta.max_kv_len))
+        torch.cuda.synchronize()
+        del pools
+    assert torch.equal(*outs)
 
 
 def test_captured_calls_and_other_streams(ops, gpu):

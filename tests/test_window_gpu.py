@@ -4,6 +4,8 @@ Bounds: those of the operators without a window (helpers.assert_close).  The ker
 fewer keys: P rounds to the storage type (at most eps / 2 relative per weight), the output once more.
 """
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -203,6 +205,110 @@ def test_long_prompt(ops, gpu):
     out, want = run_prefill(ops, free_hidden_blocks(w, 4096, 4), gpu, 4096, 4, rows=rows)
     idx = sorted(rows)
     assert_close(out[:, idx], want[:, idx], BF16, "32k prompt")
+
+
+@pytest.mark.usefixtures("decode_path")
+@pytest.mark.parametrize("heads", [(17, 1), (48, 2), (40, 1)])
+def test_decode_more_query_heads_than_a_wave_holds(ops, gpu, heads):
+    """Ratios above 16: a KV head's query heads in two or three groups, the last one smaller."""
+    w = workloads.make_paged_workload("ratio", [(L - 1, 1) for L in (900, 33, 1)], *heads, seed=sum(heads))
+    out, want = run_decode(ops, free_hidden_blocks(w, 420, 3), gpu, 420, 3)
+    assert_close(out, want, BF16, f"heads {heads}")
+    w = workloads.make_paged_workload("ratio", [(300, 40), (899, 1), (0, 1)], *heads, seed=sum(heads) + 1)
+    out, want = run_prefill(ops, free_hidden_blocks(w, 420, 3), gpu, 420, 3)
+    assert_close(out, want, BF16, f"prefill, heads {heads}")
+
+
+@pytest.mark.parametrize("window", [385, 4000, 20000])
+@pytest.mark.parametrize("lens", [[30000], [21000, 700], [5000, 5001, 1, 16]])
+def test_decode_rows_in_parts(ops, gpu, lens, window):
+    """Few rows over many pages: parts of a row in several workgroups, ends anywhere in a part, sequences shorter than
+    the parts; the same bits every time, whichever part ends last."""
+    w = workloads.make_paged_workload("parts", [(L - 1, 1) for L in lens], 8, 2, dtype=F16, seed=len(lens) + window)
+    free_hidden_blocks(w, window, 5)
+    out, want = run_decode(ops, w, gpu, window, 5)
+    assert_close(out, want, F16, f"window {window} lens {lens}")
+    again, _ = run_decode(ops, w, gpu, window, 5)
+    assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("chunk", [(2000, 100), (0, 5)])
+def test_mixed_batch_rows_in_parts(ops, gpu, chunk):
+    """Two rows of many pages beside a chunk: the rows are cut too."""
+    w = workloads.make_paged_workload("parts", [(9000, 1), chunk, (4500, 1)], 8, 2, seed=chunk[1])
+    free_hidden_blocks(w, 6000, 20)
+    first, want = run_prefill(ops, w, gpu, 6000, 20)
+    assert_close(first, want, BF16, f"rows in parts beside {chunk}")
+    again, _ = run_prefill(ops, w, gpu, 6000, 20)
+    assert torch.equal(again, first)
+
+
+def test_rows_behind_the_last_sequence_stay(ops, gpu):
+    """Queries past cu_seqlens[-1] (a padded batch): no kernel writes their rows, whatever they hold."""
+    w = workloads.make_paged_workload("pad", [(300, 50), (700, 1), (0, 9)], 8, 4, seed=30)
+    q, meta = w.gemm_call(device=gpu)
+    wd = w.to(gpu)
+    n = q.size(1)
+    padded = torch.full((8, n + 20, 128), float("nan"), dtype=BF16, device=gpu)
+    padded[:, :n] = q.to(gpu)
+    pos = torch.full((n + 20,), -7, dtype=torch.int32, device=gpu)
+    pos[:n] = meta.positions
+    out = ops.paged_attention_gemm_window(padded, wd.k_pool, wd.v_pool, meta.cu_seqlens, meta.max_q_len, meta.block_tables,
+                                          meta.kv_lens, pos, 100, 2)
+    want = oa.window_prefill(np64(q), np32(w.k_pool), np32(w.v_pool), meta.cu_seqlens.tolist(), np_tables(meta),
+                             meta.kv_lens.tolist(), meta.positions.cpu().numpy(), 100, 2)
+    assert out.shape == padded.shape
+    assert_close(out[:, :n], want, BF16, "padded batch")
+
+
+def test_pools_past_4_gib(ops, gpu):
+    """The same blocks in a compact pool and at the end of one of 4.3 GiB: equal bits, decode and prefill."""
+    w = workloads.make_paged_workload("big", [(2048, 1), (4000, 1), (900, 200), (30, 1)], 16, 8, seed=31, poison=False)
+    blocks, n = 140_000, w.k_pool.size(0)
+    outs = []
+    for base in (0, blocks - n):
+        pools = []
+        for pool in (w.k_pool, w.v_pool):
+            big = torch.empty((base + n,) + tuple(pool.shape[1:]), dtype=BF16, device=gpu)
+            big[base:] = pool.to(gpu)
+            pools.append(big)
+        q, meta = w.gemm_call(device=gpu)
+        q, tables = q.to(gpu), torch.where(meta.block_tables >= 0, meta.block_tables + base, meta.block_tables)
+        outs.append([ops.paged_attention_gemm_window(q, *pools, meta.cu_seqlens, meta.max_q_len, tables, meta.kv_lens,
+                                                     meta.positions, 700, 16),
+                     ops.paged_attention_gemv_window(q[:, :4].contiguous(), *pools, tables, meta.kv_lens, 4001, 700, 16)])
+        torch.cuda.synchronize()
+        del pools
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_calls_of_two_threads(ops, gpu):
+    """Two host threads, a stream each, calls whose rows are cut into parts: every result is the one alone."""
+    calls, want = [], []
+    for i, lens in enumerate(([20000], [9000, 12000])):
+        w = workloads.make_paged_workload("threads", [(L - 1, 1) for L in lens], 8, 4, seed=40 + i)
+        q, meta = w.gemv_call(device=gpu)
+        wd, q = w.to(gpu), q.to(gpu)
+        calls.append(lambda q=q, wd=wd, m=meta: ops.paged_attention_gemv_window(q, wd.k_pool, wd.v_pool, m.block_tables,
+                                                                                m.kv_lens, m.max_kv_len, 8000, 4))
+        want.append(calls[-1]())
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i].append(calls[i]())
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert len(got[i]) == 20 and all(torch.equal(x, want[i]) for x in got[i])
 
 
 def test_strided_and_other_stream(ops, gpu):
