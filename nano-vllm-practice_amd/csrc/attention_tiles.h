@@ -192,8 +192,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     int lin = blockIdx.x;
     if constexpr (FUSED && WINDOW) {
         // Decode rows under the window, short pieces of work: the first
-        // a.rows_first workgroups (one per CU), so that rows run beside tiles
-        // from the start, and those after the tiles.
+        // a.rows_first workgroups, so that rows run beside tiles from the
+        // start, and those after the tiles.
         const int tiles = (int)gridDim.x - a.decode_blocks;
         if (lin < a.rows_first || lin >= a.rows_first + tiles) {
             const int row = lin < a.rows_first ? lin : lin - tiles;
@@ -209,11 +209,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         // dispatched first, one per CU, and the tiles fill the other slots.
         if (lin < a.decode_blocks) {
             static_assert(sizeof(smem) >= 4 * kWorkerLds<kStagesTiles>, "the workers' pages");
-            if constexpr (PREFIX) mfma_waves<E, FULLD, RULE, kStagesTiles>(a.dec, lin, &smem[0][0][0]);
+            if constexpr (PREFIX) mfma_waves<E, FULLD, kStagesTiles>(a.dec, lin, &smem[0][0][0]);
             else decode_waves<E, G, FULLD, (G <= 2)>(a.dec, lin);
             return;
         }
         lin -= a.decode_blocks;  // a multiple of 8: the XCD of a tile is unchanged
+        if (PREFIX && a.dec.prefix_longest) __builtin_amdgcn_s_setprio(1);  // throughout
     }
     int grp, tile_lin;
     int b, tile, q_begin, q_end, kv_len;
@@ -934,7 +935,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             __builtin_amdgcn_s_setprio(1);
             if (((next - tbase) & ~63) != 0) fetch_table(next);
             issue_tile(next, STAGE ^ 1);  // in flight during this tile's math
-            __builtin_amdgcn_s_setprio(0);
+            if (!PREFIX || !a.dec.prefix_longest) __builtin_amdgcn_s_setprio(0);
         }
         const int kb = kt * kKvTile;
         // some row of the wave sees a key of the tile

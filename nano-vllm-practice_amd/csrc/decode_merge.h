@@ -1,5 +1,5 @@
-// Merge launch of the decode workers' partial softmax states, for the calls of
-// window_decode.hip and shared_prefix.hip.
+// Merge launch of a shared-prefix call's partial softmax states
+// (shared_prefix.hip).
 #pragma once
 
 #include "decode_worker.h"
@@ -7,45 +7,36 @@
 namespace femto {
 
 // One wave per (sequence, query head), lane t holding dims 2t and 2t + 1: the
-// workers' slots, then (kTailPages) the pieces of the prefix that hold keys of
-// the sequence.  Lane i keeps slot i's maximum and sum, so the weights of 64
+// workers' slots, then the pieces of the prefix that hold keys of the sequence.  Lane i keeps slot i's maximum and sum, so the weights of 64
 // slots at a time cost one exponential and two wave reductions; the slots'
 // outputs are loaded kMergeAhead at a time, before their weights are known.
 // Slots are added in order: the result does not depend on which wave wrote last.
 constexpr int kMergeRows = 4;    // waves per workgroup
 constexpr int kMergeAhead = 12;  // slots in flight
 
-template <typename E, int RULE>
+template <typename E>
 __global__ __launch_bounds__(64 * kMergeRows) void merge_rows_kernel(DecodeArgs a) {
     const int lane = threadIdx.x & 63;
     const int64_t i = (int64_t)blockIdx.x * kMergeRows + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (i >= (int64_t)a.num_seqs * a.n_heads) return;  // no barriers below
     const int b = (int)(i / a.n_heads), h = (int)(i - (int64_t)b * a.n_heads);
-    int row, kv_len, start;
     const int worker_slots = a.seq_slots[b];  // stale where no worker met the sequence
-    if (!decode_row_of<RULE>(a, b, row, kv_len, start)) return;  // a chunk of a prefill call
-    int count = pages_seen<RULE>(a, kv_len, start) > 0 ? worker_slots : 0;
-    const int workers = count;
-    if constexpr (RULE == kTailPages) {
-        const int prefix_keys = min(kv_len, a.first_page * kPage);
-        if (prefix_keys > 0) count += (prefix_keys + a.prefix_piece_keys - 1) / a.prefix_piece_keys;
-    }
+    const int kv_len = a.kv_lens[b];
+    const int workers = pages_seen<kTailPages>(a, kv_len, 0) > 0 ? worker_slots : 0;
+    const int prefix_keys = min(kv_len, a.first_page * kPage);
+    const int count = workers + (prefix_keys > 0 ? (prefix_keys + a.prefix_piece_keys - 1) / a.prefix_piece_keys : 0);
     char* out = reinterpret_cast<char*>(a.out);
-    const int64_t o = (int64_t)h * a.out_stride_head + (int64_t)row * a.out_stride_seq + 2 * lane;
+    const int64_t o = (int64_t)h * a.out_stride_head + (int64_t)b * a.out_stride_seq + 2 * lane;
     auto store = [&](float x, float y) __attribute__((always_inline)) {
         if (2 * lane < a.head_dim) {
             store_elem<E>(out, o, x);
             store_elem<E>(out, o + 1, y);
         }
     };
-    if (count == 0) {  // no key: zeros in a decode call, 0 / 0 in a row of a prefill call
-        const float none = a.cu_seqlens ? __builtin_nanf("") : 0.0f;
-        store(none, none);
-        return;
-    }
-    const int64_t sl0 = i * slot_stride<RULE>(a);
+    if (count == 0) return store(0.0f, 0.0f);  // no key
+    const int64_t sl0 = i * slot_stride<kTailPages>(a);
     auto slot = [&](int k) __attribute__((always_inline)) {
-        return sl0 + (RULE != kTailPages || k < workers ? k : a.max_slots + (k - workers));
+        return sl0 + (k < workers ? k : a.max_slots + (k - workers));
     };
     float M = kEmptyMax, L = 0.0f, o0 = 0.0f, o1 = 0.0f;
     for (int base = 0; base < count; base += kWave) {
@@ -80,13 +71,11 @@ __global__ __launch_bounds__(64 * kMergeRows) void merge_rows_kernel(DecodeArgs 
     store(o0 / L, o1 / L);
 }
 
-template <int RULE>
 static hipError_t launch_merge_rows(int dtype, const DecodeArgs& a, int num_seqs, hipStream_t st) {
     const dim3 grid((unsigned)(((int64_t)num_seqs * a.n_heads + kMergeRows - 1) / kMergeRows)), block(64 * kMergeRows);
     switch (dtype) {
-        case kDtypeBF16: hipLaunchKernelGGL((merge_rows_kernel<BF16, RULE>), grid, block, 0, st, a); break;
-        case kDtypeF16: hipLaunchKernelGGL((merge_rows_kernel<F16, RULE>), grid, block, 0, st, a); break;
-        case kDtypeF32: hipLaunchKernelGGL((merge_rows_kernel<F32, RULE>), grid, block, 0, st, a); break;
+        case kDtypeBF16: hipLaunchKernelGGL(merge_rows_kernel<BF16>, grid, block, 0, st, a); break;
+        case kDtypeF16: hipLaunchKernelGGL(merge_rows_kernel<F16>, grid, block, 0, st, a); break;
         default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

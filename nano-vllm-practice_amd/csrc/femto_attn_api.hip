@@ -851,6 +851,7 @@ int femto_paged_attention_gemv_shared_prefix(
     a.dec.first_page = prefix_pages;
     a.dec.prefix_pieces = plan.pieces;
     a.dec.prefix_piece_keys = plan.piece_keys;
+    a.dec.prefix_longest = plan.longest;
     return hip_status(femto::launch_shared_prefix(dtype, a, static_cast<hipStream_t>(stream)), (fn + " launch").c_str());
 }
 

@@ -53,6 +53,7 @@ struct DecodeArgs {
     // prefix_piece_keys keys each, behind the workers' max_slots.
     int first_page;
     int prefix_pieces, prefix_piece_keys;
+    int prefix_longest;  // the prefix's tiles are the call's longest work (plan_shared_prefix)
 };
 
 // Compute units of the current device, queried once per device (safe to call
@@ -140,6 +141,7 @@ size_t prefill_workspace_bytes(int resident);
 struct SharedPrefixPlan {
     DecodePlan tail;
     int pieces, piece_keys;
+    bool longest;  // the tiles outlast the tails
 };
 SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, int prefix_pages, int max_kv_len,
                                     int dtype, int cus);

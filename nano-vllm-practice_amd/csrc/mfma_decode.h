@@ -358,11 +358,11 @@ __device__ __forceinline__ void window_row(const DecodeArgs& a, int block, uint8
     }
 }
 
-// The waves of workgroup `block`, as decode_waves: slices and partial slots are
-// the same; a.heads_per_wave (at most 16) query heads per wave,
-// the last wave of a KV head's groups maybe fewer.  lds: the workgroup's
-// 4 * kWorkerLds<STAGES> bytes.
-template <typename E, bool FULL, int RULE, int STAGES>
+// Tails of a shared-prefix call: the waves of workgroup `block`, as
+// decode_waves: slices and partial slots are the same; a.heads_per_wave (at
+// most 16) query heads per wave, the last wave of a KV head's groups maybe
+// fewer.  lds: the workgroup's 4 * kWorkerLds<STAGES> bytes.
+template <typename E, bool FULL, int STAGES>
 __device__ __forceinline__ void mfma_waves(const DecodeArgs& a, int block, uint8_t* lds) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -376,11 +376,11 @@ __device__ __forceinline__ void mfma_waves(const DecodeArgs& a, int block, uint8
     const int nh = min(a.heads_per_wave, a.n_rep - hg * a.heads_per_wave);
     const int c = lane & 15, g = lane >> 4;
     const int64_t head_off = (int64_t)kvh * a.pool_stride_head;
-    walk_slice<RULE>(a, wi, [&](int b, int kv_len, int start, int lp0, int n, int qrow, int slot, int count, bool last)
+    walk_slice<kTailPages>(a, wi, [&](int b, int kv_len, int start, int lp0, int n, int qrow, int slot, int count, bool last)
                                 __attribute__((always_inline)) {
         HeadState s;
-        mfma_segment<E, FULL, RULE, STAGES>(a, b, kv_len, start, lp0, n, qrow, h0, nh, head_off, lds + wave * kWorkerLds<STAGES>, s);
-        if (c < nh) store_partial(a, ((int64_t)b * a.n_heads + h0 + c) * slot_stride<RULE>(a) + slot, g, s);
+        mfma_segment<E, FULL, kTailPages, STAGES>(a, b, kv_len, start, lp0, n, qrow, h0, nh, head_off, lds + wave * kWorkerLds<STAGES>, s);
+        if (c < nh) store_partial(a, ((int64_t)b * a.n_heads + h0 + c) * slot_stride<kTailPages>(a) + slot, g, s);
         if (lane == 0 && grp == 0 && last) a.seq_slots[b] = slot + 1;  // last segment: slot count
     });
 }

@@ -9,7 +9,7 @@
 //    attention_tiles.h, read from HBM once and not once per sequence.  It has
 //    few query tiles (one per 32-128 sequences and KV head), so its keys are
 //    cut into pieces, one workgroup each;
-//  * tails: bound by their bytes, on the decode workers of decode_worker.h, in
+//  * tails: bound by their bytes, on the MFMA workers of mfma_decode.h, in
 //    the same launch, one workgroup per CU beside the tiles.
 #include <cmath>
 
@@ -42,6 +42,12 @@ SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, i
     const int per = (tiles + pieces - 1) / pieces;
     p.pieces = (tiles + per - 1) / per;
     p.piece_keys = per * kKvTile;
+    // Long pieces beside short tails: their waves issue before the workers' on
+    // the same SIMD.  32/8 heads, prefix of 16384 keys, tails of up to 1024, us
+    // without and with: 256 sequences 141 and 135, 128 sequences 85 and 79, 64
+    // 51.7 and 50.9; where the tails take as long, or pieces are short, it costs:
+    // 8192 keys 115 and 118; 1024 keys, 64 sequences on 16/8 heads, tails of up to 64 17.1 and 18.9.
+    p.longest = per >= 16 && prefix_pages * (int64_t)kPage >= 16 * (int64_t)tail;
     return p;
 }
 
@@ -57,7 +63,7 @@ hipError_t launch_shared_prefix(int dtype, PrefillArgs a, hipStream_t st) {
     a.decode_blocks = (a.decode_blocks + 7) / 8 * 8;
     hipError_t e = launch_dtype<true, kTailPages>(dtype, G, a, st);
     if (e != hipSuccess) return e;
-    return launch_merge_rows<kTailPages>(dtype, a.dec, a.num_seqs, st);
+    return launch_merge_rows(dtype, a.dec, a.num_seqs, st);
 }
 
 }  // namespace femto
