@@ -27,19 +27,19 @@ SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, i
     if (prefix_pages <= 0) return p;
     // Pieces of the prefix: more of them shorten the tiles' chains (1.2 us per
     // tile of 64 keys where a CU has one), but each writes and merges 520
-    // bytes per query row.  With T key tiles and U row tiles (per piece one
-    // workgroup each) the best of 2 .. 64 pieces was near 2 sqrt(T) / (1 + U / 24)
-    // over 160 shapes (4-256 sequences, prefixes of 256-16384 keys, five head
-    // shapes), within 8 % but for calls of 10-15 us: 16384 keys, 16 sequences on 16/8
-    // heads (T 256, U 8) 28 us with 32, 31 with 16, 45 with 8; 256 sequences on 64/8
-    // heads (U 128) 195 us with 4, 231 with 16.  Beyond one workgroup per
-    // CU beside the workers they only queue (4096 keys, 256 sequences on 16/8
-    // heads with tails of up to 512: 65 us with 4, 71 with 8, 79 with 16).
+    // bytes per query row.  With T key tiles and R query rows the best of 2 .. 64
+    // pieces was near 2 sqrt(T) / (1 + R / 24 / 128) over 160 shapes (3-256
+    // sequences, prefixes of 256-16384 keys, five head shapes): 16384 keys, 16
+    // sequences on 16/8 heads 28 us with 32, 31 with 16, 45 with 8; 256 on 64/8
+    // heads 195 us with 4, 231 with 16; 4096 keys, 8 on 16/8 heads 15.2 with 16,
+    // 16.6 with 12, 18.9 with 8.  Beyond one workgroup per CU beside the workers
+    // (U row tiles, one workgroup each per piece) they only queue (4096 keys,
+    // 256 sequences on 16/8 heads with tails of up to 512: 65 us with 4, 71 with
+    // 8, 79 with 16).
     const int tiles = (prefix_pages * kPage + kKvTile - 1) / kKvTile;
-    const double units = (double)(n_heads / G) * ((num_seqs + BT - 1) / BT);
-    const double best = std::min(2.0 * std::sqrt((double)tiles) / (1.0 + units / 24.0), std::max(4.0, cus / units));
-    const int pieces = std::max(1, std::min({(int)(best + 0.5), tiles, 64}));
-    const int per = (tiles + pieces - 1) / pieces;
+    const double units = (double)(n_heads / G) * ((num_seqs + BT - 1) / BT), rows = (double)num_seqs * n_heads;
+    const double best = std::min(2.0 * std::sqrt((double)tiles) / (1.0 + rows / (24.0 * 128)), std::max(4.0, cus / units));
+    const int per = std::max({1, (tiles + 63) / 64, (int)(tiles / best + 0.5)});
     p.pieces = (tiles + per - 1) / per;
     p.piece_keys = per * kKvTile;
     // Long pieces beside short tails: their waves issue before the workers' on
