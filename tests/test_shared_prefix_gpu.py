@@ -82,6 +82,20 @@ def test_more_query_heads_than_a_wave_holds(ops, gpu, heads):
     assert_close(out, want, BF16, f"heads {heads}")
 
 
+def test_bad_blocks_read_as_zeros(ops, gpu):
+    """Blocks that are -1 or past the pool, in the prefix and in the tails; a table that ends inside a tail."""
+    w, pages = batch(336, [100, 3, 45, 64], 8, 4, seed=9)
+    pages[2], pages[20], pages[7] = -1, 10**6, -(2**31)
+    w.raw_block_tables[0][22], w.raw_block_tables[0][26], w.raw_block_tables[2][21] = -1, 2**31 - 1, -5
+    out, want, args = run(ops, gpu, w, pages)
+    assert_close(out, want, BF16, "bad blocks")
+    narrow = args[4][:, :24].contiguous()
+    out = ops.paged_attention_gemv_shared_prefix(*args[:4], narrow, *args[5:])
+    want = added.shared_prefix_decode(np64(args[0]), np32(w.k_pool), np32(w.v_pool), pages.tolist(), narrow.cpu().numpy(),
+                                      args[5].tolist())
+    assert_close(out, want, BF16, "narrow table")
+
+
 def test_no_key_past_the_prefix(ops, gpu):
     """Every context ends inside the prefix, and the largest one is understated to the call."""
     w, pages = batch(640, [-1, -100, -320, -639, -64, -63], 8, 4, seed=2)

@@ -330,19 +330,64 @@ def test_strided_and_other_stream(ops, gpu):
     assert_close(out, want, BF16, "strides")
 
 
-@pytest.mark.parametrize("entry", ["decode", "prefill"])
+@pytest.mark.usefixtures("decode_path")
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_bad_blocks_of_seen_pages_read_as_zeros(ops, gpu, dtype):
+    """Table entries that are -1, past the pool or past a narrow table, in pages that queries see."""
+    w = workloads.make_paged_workload("bad", [(L - 1, 1) for L in (400, 77, 33, 250)], 8, 4, dtype=dtype, seed=17)
+    for b, c, x in ((0, 24, -1), (0, 20, 10**6), (0, 0, 2**31 - 1), (1, 4, -7), (2, 2, -(2**31))):
+        w.raw_block_tables[b][c] = x
+    out, want = run_decode(ops, w, gpu, 90, 5)
+    assert_close(out, want, dtype, "bad blocks")
+    q, meta = w.gemv_call(device=gpu)
+    wd, narrow = w.to(gpu), meta.block_tables[:, :14].contiguous()
+    out = ops.paged_attention_gemv_window(q.to(gpu), wd.k_pool, wd.v_pool, narrow, meta.kv_lens, meta.max_kv_len, 90, 5)
+    want = oa.window_decode(np64(q), np32(w.k_pool), np32(w.v_pool), narrow.cpu().numpy(), meta.kv_lens.tolist(), 90, 5)
+    assert_close(out, want, dtype, "narrow table")
+    if dtype == F32:
+        return
+    w = workloads.make_paged_workload("bad", [(300, 100), (76, 1), (0, 33), (240, 10)], 8, 4, dtype=dtype, seed=18)
+    for b, c, x in ((0, 24, -1), (0, 20, 10**6), (0, 0, 2**31 - 1), (1, 4, -7), (2, 2, -(2**31))):
+        w.raw_block_tables[b][c] = x
+    out, want = run_prefill(ops, w, gpu, 90, 5)
+    assert_close(out, want, dtype, "bad blocks, prefill")
+
+
+@pytest.mark.parametrize("window", [1, 70, 2**31 - 1])
+def test_prefill_negative_positions(ops, gpu, window):
+    """A token before the sequence's start sees nothing, in a chunk and as a decode row: NaN; its neighbours as always."""
+    w = workloads.make_paged_workload("neg", [(100, 40), (50, 1), (60, 1)], 4, 2, seed=15)
+    _, meta = w.gemm_call(device=gpu)
+    pos = meta.positions.cpu().numpy().copy()
+    pos[[3, 20]] = [-1, -(2**31)]
+    pos[40] = -9
+    meta.positions = torch.from_numpy(pos).to(gpu)
+    out, want = run_prefill(ops, w, gpu, window, 5, meta=meta)
+    assert torch.isnan(out[:, [3, 20, 40]]).all()
+    assert_close(out, want, BF16, f"negative positions, window {window}")
+
+
+def test_decode_many_sequences(ops, gpu):
+    """More (sequence, KV head) pairs than a call has counters: whole rows, whatever their length."""
+    rng = np.random.default_rng(16)
+    w = workloads.make_paged_workload("many", [(int(x), 1) for x in rng.integers(0, 60, size=2100)], 4, 2, dtype=F16, seed=16)
+    out, want = run_decode(ops, free_hidden_blocks(w, 25, 3), gpu, 25, 3)
+    assert_close(out, want, F16, "2100 sequences")
+
+
+@pytest.mark.parametrize("entry", ["decode", "decode_f32", "prefill"])
 def test_captured_calls_share_no_workspace(ops, gpu, entry):
     """Two graphs captured on one stream and eager calls of other sizes between their replays, also on two streams
     at once: every replay gives its eager result, with new inputs too."""
-    chunks = {"decode": [[(2999, 1), (1700, 1)], [(5000, 1)] * 3], "prefill": [[(3000, 40), (300, 1)], [(5000, 60), (20, 1), (77, 1)]]}
+    chunks = {"decode": [[(2999, 1), (1700, 1)], [(5000, 1)] * 3], "decode_f32": [[(2999, 1)], [(5000, 1)] * 2], "prefill": [[(3000, 40), (300, 1)], [(5000, 60), (20, 1), (77, 1)]]}
     window, sinks = 1500, 4
     calls, graphs = [], []
     side = torch.cuda.Stream()
     for i, c in enumerate(chunks[entry]):
-        w = workloads.make_paged_workload("graph", c, 8, 4, seed=20 + i)
+        w = workloads.make_paged_workload("graph", c, 8, 4, dtype=F32 if entry == "decode_f32" else BF16, seed=20 + i)
         q, meta = w.gemm_call(device=gpu)
         wd, q = w.to(gpu), q.to(gpu)
-        if entry == "decode":
+        if entry != "prefill":
             f = lambda q=q, wd=wd, m=meta: ops.paged_attention_gemv_window(q, wd.k_pool, wd.v_pool, m.block_tables, m.kv_lens,
                                                                            m.max_kv_len, window, sinks)
         else:
