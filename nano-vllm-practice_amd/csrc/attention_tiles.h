@@ -641,8 +641,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         gap = max(0, min(beg / kKvTile, n) - head);
         return n - gap;
     };
-    // Tiles of a piece: all pieces of a query tile find the same number.
+    // Tiles of a piece: all pieces of a query tile find the same number.  Those
+    // of a shared prefix are the plan's, by which the merge counts them.
     auto piece_tiles = [&](int ntiles) __attribute__((always_inline)) {
+        if constexpr (PREFIX) return a.dec.prefix_piece_keys / kKvTile;
         return (max(WINDOW ? ntiles : 0, tiles_bound(kv_len)) + npieces - 1) / npieces;
     };
 
@@ -664,10 +666,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         first_issued = i0 < n;
         t_first = tile_at(i0);
     } else {
-        if (PAGED && npieces > 1) {
-            const int ub = (kv_len + kKvTile - 1) / kKvTile;
-            t_first = piece * ((ub + npieces - 1) / npieces);
-        }
+        if (PAGED && npieces > 1) t_first = piece * piece_tiles(0);  // tiles_bound: of all kv_len keys
         first_issued = t_first * kKvTile < kv_len;
     }
     if (first_issued) {

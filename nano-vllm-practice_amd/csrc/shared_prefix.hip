@@ -15,12 +15,13 @@
 // both, the tails' 509 MB (92 us alone) and the tiles, 64 in series (104 alone);
 // 64 on 4096, tails of up to 512, f16 16/8 heads 27.5 us; 8 on 1024 11.9 us, two
 // launches and their round trips.
-#include <cmath>
-
 #include "attention_tiles.h"
 #include "decode_merge.h"
+#include "prefix_plan.h"
 
 namespace femto {
+
+static_assert(kPrefixTile == kKvTile, "the prefix is cut between key tiles");
 
 SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, int prefix_pages, int max_kv_len,
                                     int dtype, int cus) {
@@ -28,30 +29,10 @@ SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, i
     const int n_rep = n_heads / n_kv_heads, G = prefill_group(n_rep), BT = 32 * (4 / G);
     const int tail = (int)std::max<int64_t>(1, (int64_t)max_kv_len - (int64_t)prefix_pages * kPage);
     p.tail = plan_paged_decode(n_heads, n_kv_heads, tail, dtype);
-    if (prefix_pages <= 0) return p;
-    // Pieces of the prefix: more of them shorten the tiles' chains (1.2 us per
-    // tile of 64 keys where a CU has one), but each writes and merges 520
-    // bytes per query row.  With T key tiles and R query rows the best of 2 .. 64
-    // pieces was near 2 sqrt(T) / (1 + R / 24 / 128) over 160 shapes (3-256
-    // sequences, prefixes of 256-16384 keys, five head shapes): 16384 keys, 16
-    // sequences on 16/8 heads 28 us with 32, 31 with 16, 45 with 8; 256 on 64/8
-    // heads 195 us with 4, 231 with 16; 4096 keys, 8 on 16/8 heads 15.2 with 16,
-    // 16.6 with 12, 18.9 with 8.  Beyond one workgroup per CU beside the workers
-    // (U row tiles, one workgroup each per piece) they only queue (4096 keys,
-    // 256 sequences on 16/8 heads with tails of up to 512: 65 us with 4, 71 with
-    // 8, 79 with 16).
-    const int tiles = (prefix_pages * kPage + kKvTile - 1) / kKvTile;
-    const double units = (double)(n_heads / G) * ((num_seqs + BT - 1) / BT), rows = (double)num_seqs * n_heads;
-    const double best = std::min(2.0 * std::sqrt((double)tiles) / (1.0 + rows / (24.0 * 128)), std::max(4.0, cus / units));
-    const int per = std::max({1, (tiles + 63) / 64, (int)(tiles / best + 0.5)});
-    p.pieces = (tiles + per - 1) / per;
-    p.piece_keys = per * kKvTile;
-    // Long pieces beside short tails: their waves issue before the workers' on
-    // the same SIMD.  32/8 heads, prefix of 16384 keys, tails of up to 1024, us
-    // without and with: 256 sequences 141 and 135, 128 sequences 85 and 79, 64
-    // 51.7 and 50.9; where the tails take as long, or pieces are short, it costs:
-    // 8192 keys 115 and 118; 1024 keys, 64 sequences on 16/8 heads, tails of up to 64 17.1 and 18.9.
-    p.longest = per >= 16 && prefix_pages * (int64_t)kPage >= 16 * (int64_t)tail;
+    const PrefixPieces c = prefix_pieces(num_seqs, n_heads, G, BT, prefix_pages * kPage, tail, cus);
+    p.pieces = c.pieces;
+    p.piece_keys = c.piece_keys;
+    p.longest = c.longest;
     return p;
 }
 
