@@ -322,8 +322,8 @@ int femto_qk_norm_rope_cache_write(
     const int32_t* positions, const int32_t* kv_page_tables, int num_pages_per_seq, int64_t table_stride,
     void* stream);
 
-/* Rotary positions of q and k without norms, rotated q to q_out (may be q
- * itself, or share no memory with q, k and v), rotated k and raw v into the
+/* Rotary positions of q and k without norms, rotated q to q_out (q itself, or
+ * no element of q; none of k and v either way), rotated k and raw v into the
  * pools by the rule of femto_kv_cache_write (same cu_seqlens / positions /
  * table arguments).  The first rotary_dim (even) dims of a head are pairs
  * (a, b), dims (i, i + rotary_dim / 2) or, interleaved != 0, (2i, 2i + 1);

@@ -389,6 +389,20 @@ PyObject* prologue(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// Whether two (tokens, heads, dim) tensors contiguous in dim plainly have no element in common: their spans do not
+// meet, or they are columns of one array of token rows.  (The Python path looks at every row.)
+bool plainly_apart(const at::Tensor& a, const at::Tensor& b) {
+    const int64_t size = a.element_size();
+    const int64_t row_a = (a.size(1) - 1) * a.stride(1) + a.size(2), row_b = (b.size(1) - 1) * b.stride(1) + b.size(2);
+    const int64_t pa = (int64_t)(uintptr_t)a.const_data_ptr(), pb = (int64_t)(uintptr_t)b.const_data_ptr();
+    if (pa + size * ((a.size(0) - 1) * a.stride(0) + row_a) <= pb || pb + size * ((b.size(0) - 1) * b.stride(0) + row_b) <= pa)
+        return true;
+    const int64_t step = a.stride(0);
+    if (step <= 0 || step != b.stride(0) || (pb - pa) % size) return false;
+    const int64_t at = ((pb - pa) / size % step + step) % step;  // b's first column
+    return row_a <= at && at + row_b <= step;
+}
+
 // rope(q, k, v, cos, sin, positions, k_pool, v_pool, tables, cu_seqlens | None, max_q_len, interleaved, out | None)
 PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 13, [&]() -> PyObject* {
@@ -425,7 +439,10 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int dt = dtype_code(q);
         at::Tensor out = a[12] == Py_None ? at::empty_like(q) : tensor(a[12]);
         need(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.stride(2) == 1 && out.device() == q.device());
-        need(a[12] == Py_None || (out.const_data_ptr() == q.const_data_ptr() && out.strides() == q.strides()));
+        if (a[12] != Py_None) {
+            need(out.const_data_ptr() == q.const_data_ptr() && out.strides() == q.strides());
+            need(plainly_apart(out, k) && plainly_apart(out, v));
+        }
         void* st = stream_of(q);
         const void *qd = q.const_data_ptr(), *kd = k.const_data_ptr(), *vd = v.const_data_ptr();
         const float* cd = static_cast<const float*>(cos.const_data_ptr());

@@ -649,6 +649,23 @@ def _overlaps(a, b) -> bool:
     return a.numel() > 0 and b.numel() > 0 and a0 < b1 and b0 < a1
 
 
+def _row_starts(t):
+    """Addresses of the rows of a (tokens, heads, dim) tensor, ascending."""
+    tokens, heads = (torch.arange(n, device="cpu") * s for n, s in zip(t.shape[:2], t.stride()))
+    return (t.data_ptr() + t.element_size() * (tokens[:, None] + heads[None, :])).flatten().sort().values
+
+
+def _share_elements(a, b) -> bool:
+    """Whether two (tokens, heads, dim) tensors of one dim and dtype, contiguous in it, have an element in common."""
+    if not _overlaps(a, b):
+        return False
+    rows, others, nbytes = _row_starts(a), _row_starts(b), a.size(2) * a.element_size()
+    after = torch.searchsorted(others, rows)  # the first of b's rows at or past each of a's, and the one before it
+    ends = torch.cat((others.new_tensor([0]), others + nbytes))[after]
+    starts = torch.cat((others, others.new_tensor([2**63 - 1])))[after]
+    return bool(((ends > rows) | (starts < rows + nbytes)).any())
+
+
 def _rope_cache_write(q, k, v, cos, sin, positions, k_pool, v_pool, kv_page_tables, cu_seqlens=None, max_q_len=1,
                       interleaved=False, out=None):
     """Rotated q to ``out``, rotated k and v into the pools; returns ``out``."""
@@ -693,9 +710,10 @@ def _rope_cache_write(q, k, v, cos, sin, positions, k_pool, v_pool, kv_page_tabl
         _check(tuple(out.shape) == tuple(q.shape) and out.dtype == q.dtype and out.stride(-1) == 1 and out.device == q.device,
                f"{fn}: out must match q")
         in_place = out.data_ptr() == q.data_ptr() and out.stride() == q.stride()
-        others = [("k", k), ("v", v)] if in_place else [("q", q), ("k", k), ("v", v)]
-        for name, t in others:
-            _check(in_place or not _overlaps(out, t), f"{fn}: out must be q itself or share no memory with {name}")
+        # (k and v, too, where out is q: a token's k would be read after its q was written)
+        _check(in_place or not _share_elements(out, q), f"{fn}: out must be q itself or share no memory with q")
+        for name, t in (("k", k), ("v", v)):
+            _check(not _share_elements(out, t), f"{fn}: out must share no memory with {name}")
     with torch.cuda.device(q.device):
         if out is None:
             out = torch.empty_like(q)

@@ -315,9 +315,10 @@ def rope_cache_write(
     of each q and k head, as pairs (i, i + rotary_dim / 2) or, ``interleaved``,
     (2 i, 2 i + 1): (a, b) -> (a cos - b sin, b cos + a sin); the other dims
     pass through.  The rotated q goes to ``out`` (new; if given, ``q`` itself
-    or memory of its own), the rotated k and v into the pools exactly as
-    :func:`kv_cache_write`.  Each output element is rounded once from fp32; a
-    position outside the tables gives NaN in the rotated dims.
+    or no element of ``q``; none of ``k`` and ``v`` either way), the rotated k and
+    v into the pools exactly as :func:`kv_cache_write`.  Each output element is
+    rounded once from fp32; a position outside the tables gives NaN in the rotated
+    dims.
     """
     for name, t in (("q", q), ("k", k), ("v", v)):
         if not t.is_cuda:
