@@ -442,6 +442,8 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (a[12] != Py_None) {
             need(out.const_data_ptr() == q.const_data_ptr() && out.strides() == q.strides());
             need(plainly_apart(out, k) && plainly_apart(out, v));
+            need(out.stride(1) >= out.size(2) || out.size(1) == 1);  // its rows, head by head and token by token
+            need(out.stride(0) >= (out.size(1) - 1) * out.stride(1) + out.size(2) || out.size(0) == 1);
         }
         void* st = stream_of(q);
         const void *qd = q.const_data_ptr(), *kd = k.const_data_ptr(), *vd = v.const_data_ptr();

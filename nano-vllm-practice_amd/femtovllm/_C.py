@@ -666,6 +666,12 @@ def _share_elements(a, b) -> bool:
     return bool(((ends > rows) | (starts < rows + nbytes)).any())
 
 
+def _rows_meet(t) -> bool:
+    """Whether rows of a (tokens, heads, dim) tensor, contiguous in dim, have an element in common."""
+    rows = _row_starts(t)
+    return bool((rows.diff() < t.size(2) * t.element_size()).any())
+
+
 def _rope_cache_write(q, k, v, cos, sin, positions, k_pool, v_pool, kv_page_tables, cu_seqlens=None, max_q_len=1,
                       interleaved=False, out=None):
     """Rotated q to ``out``, rotated k and v into the pools; returns ``out``."""
@@ -709,6 +715,7 @@ def _rope_cache_write(q, k, v, cos, sin, positions, k_pool, v_pool, kv_page_tabl
     if out is not None:
         _check(tuple(out.shape) == tuple(q.shape) and out.dtype == q.dtype and out.stride(-1) == 1 and out.device == q.device,
                f"{fn}: out must match q")
+        _check(not _rows_meet(out), f"{fn}: rows of out share memory")
         in_place = out.data_ptr() == q.data_ptr() and out.stride() == q.stride()
         # (k and v, too, where out is q: a token's k would be read after its q was written)
         _check(in_place or not _share_elements(out, q), f"{fn}: out must be q itself or share no memory with q")

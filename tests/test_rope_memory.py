@@ -74,3 +74,27 @@ def test_native_call_in_place(native, case, taken):  # noqa: F811
     before = counts.get(FUNCTIONS[3], 0)
     out = module.rope(q, k, v, tab, tab, i32(3), pool, pool, i32(3, 2), None, 1, False, q)
     assert (out is not None) == taken and counts.get(FUNCTIONS[3], 0) == before + taken
+
+
+def test_rows_meet(C):
+    q, k, v = packed(5, 4, 2, 2)
+    x = torch.zeros(400)
+    assert not C._rows_meet(q) and not C._rows_meet(k[:1]) and not C._rows_meet(q[:0])
+    assert not C._rows_meet(torch.zeros(4, 5, 8).transpose(0, 1))
+    assert C._rows_meet(q[:1].expand(5, -1, -1)) and C._rows_meet(q[:, :1].expand(-1, 4, -1))
+    assert not C._rows_meet(q[:1, :1].expand(1, 1, -1))
+    assert C._rows_meet(x.as_strided((3, 2, 8), (15, 8, 1))) and not C._rows_meet(x.as_strided((3, 2, 8), (16, 8, 1)))
+
+
+@pytest.mark.parametrize("strides,taken", [((512, 128), True), ((0, 128), False), ((512, 0), False), ((511, 128), False),
+                                           ((640, 128), True), ((128, 384), False)])
+def test_native_call_with_rows_that_meet(native, strides, taken):  # noqa: F811
+    """In place, q's rows plainly apart; the others, the heads ahead of the tokens among them, go to the Python path."""
+    module, counts = native[:2]
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)
+    b16 = lambda *s: torch.zeros(s, dtype=torch.bfloat16)
+    pool, tab = b16(4, 2, 16, 128), torch.zeros(64, 64)
+    q = b16(4000).as_strided((3, 4, 128), (*strides, 1))
+    before = counts.get(FUNCTIONS[3], 0)
+    out = module.rope(q, b16(3, 2, 128), b16(3, 2, 128), tab, tab, i32(3), pool, pool, i32(3, 2), None, 1, False, q)
+    assert (out is not None) == taken and counts.get(FUNCTIONS[3], 0) == before + taken

@@ -44,3 +44,27 @@ def test_out_on_k_or_v_is_refused(ops, gpu):
             run(ops, gpu, w, *args, tables, False, out=args[0])
     with pytest.raises(RuntimeError, match="out must share no memory with v"):
         run(ops, gpu, w, q, k, long[:8, 2:], tables, False, out=long[:8])
+
+
+def test_out_whose_rows_meet_is_refused(ops, gpu):
+    w, q, k, v = step([(0, 8)], 4, 2, 64, BF16, seed=9)
+    q, k, v = q.to(gpu), k.to(gpu), v.to(gpu)
+    tables = scaled_rope_tables(64, 32)
+    row = torch.zeros(1, 4, 64, dtype=BF16, device=gpu).expand(8, -1, -1)
+    for args in ((q, k, v, row), (row, k, v, row)):
+        with pytest.raises(RuntimeError, match="rows of out share memory"):
+            run(ops, gpu, w, *args[:3], tables, False, out=args[3])
+    got, _, meta = run(ops, gpu, w, row, k, v, tables, False)  # as an input they may
+    check_rotated(got, row, *(t.numpy() for t in tables), meta.positions.cpu().numpy(), False, "one row for all tokens")
+
+
+def test_heads_ahead_of_tokens(ops, gpu):
+    """out and q as (heads, tokens, dim) arrays seen token by token."""
+    w, q, k, v = step([(0, 8), (17, 3)], 4, 2, 64, BF16, seed=10)
+    tables = scaled_rope_tables(64, 64)
+    qd = q.transpose(0, 1).contiguous().to(gpu).transpose(0, 1)
+    out = torch.empty(4, 11, 64, dtype=BF16, device=gpu).transpose(0, 1)
+    got, _, meta = run(ops, gpu, w, qd, k.to(gpu), v.to(gpu), tables, True, out=out)
+    check_rotated(got, q, *(t.numpy() for t in tables), meta.positions.cpu().numpy(), True, "out")
+    run(ops, gpu, w, qd, k.to(gpu), v.to(gpu), tables, True, out=qd)
+    assert torch.equal(qd, got)
