@@ -31,8 +31,8 @@ struct PrefixPieces {
 // Beyond one workgroup per CU beside the workers (a row tile is one workgroup
 // per piece) they only queue (4096 keys, 256 sequences on 16/8 heads with tails
 // of up to 512: 65 us with 4, 71 with 8, 79 with 16).
-inline PrefixPieces prefix_pieces(int num_seqs, int n_heads, int group, int rows_per_tile, int prefix_keys, int tail,
-                                  int cus) {
+inline PrefixPieces prefix_pieces(int num_seqs, int n_heads, int n_kv_heads, int group, int rows_per_tile,
+                                  int prefix_keys, int tail, int cus) {
     PrefixPieces p{0, 0, false};
     if (prefix_keys <= 0) return p;
     const int tiles = (prefix_keys + kPrefixTile - 1) / kPrefixTile;
@@ -43,12 +43,20 @@ inline PrefixPieces prefix_pieces(int num_seqs, int n_heads, int group, int rows
     p.pieces = (tiles + at_least - 1) / at_least;
     const int per = (tiles + p.pieces - 1) / p.pieces;  // as even as that many pieces can be
     p.piece_keys = per * kPrefixTile;
-    // Long pieces beside short tails: their waves issue before the workers' on
-    // the same SIMD.  32/8 heads, prefix of 16384 keys, tails of up to 1024, us
-    // without and with: 256 sequences 141 and 135, 128 sequences 85 and 79, 64
-    // 51.7 and 50.9; where the tails take as long, or pieces are short, it costs:
-    // 8192 keys 115 and 118; 1024 keys, 64 sequences on 16/8 heads, tails of up to 64 17.1 and 18.9.
-    p.longest = per >= 16 && prefix_keys >= 16 * (int64_t)tail;
+    // Where the tiles outlast the tails their waves issue before the workers' on
+    // the same SIMD: from one tile of 64 keys for 11 pages of the tails on (it takes
+    // ~1.2 us of a CU, a page of a KV head, 8 KB, 1.4 ns of HBM time; the host knows
+    // the longest tail only, which is about twice the mean), and where a workgroup's
+    // chain is 5 tiles or more (of 1-4 it cost 2.5-6 % on average).
+    // Measured with and without over 2,051 shapes (4-256 sequences, prefixes of
+    // 256-16384 keys, longest tails of 1/64 to 1/2 of them, six head shapes): where it
+    // is taken 1.9 % faster on average, and over all shapes 0.3 % behind the better of
+    // the two, 8 % at worst (never ahead 1.0 and 15, always 2.7 and 17).  16384 keys,
+    // 256 sequences, longest tails of 1638, 1365 and 1024 keys, us: 32/8 heads 175 and
+    // 181, 164 and 158, 153 and 141; 16/8 heads (half the tiles), 1024, 819 and 512:
+    // 113 and 120, 97 and 105, 84 and 82; 64/8 heads, 4096, 2048: 399 and 405, 294 and 267.
+    const double tail_pages = (double)num_seqs * n_kv_heads * (tail / 16.0);
+    p.longest = per >= 5 && 11 * units * tiles >= tail_pages;
     return p;
 }
 

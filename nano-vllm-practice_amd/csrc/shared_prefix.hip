@@ -29,7 +29,7 @@ SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, i
     const int n_rep = n_heads / n_kv_heads, G = prefill_group(n_rep), BT = 32 * (4 / G);
     const int tail = (int)std::max<int64_t>(1, (int64_t)max_kv_len - (int64_t)prefix_pages * kPage);
     p.tail = plan_paged_decode(n_heads, n_kv_heads, tail, dtype);
-    const PrefixPieces c = prefix_pieces(num_seqs, n_heads, G, BT, prefix_pages * kPage, tail, cus);
+    const PrefixPieces c = prefix_pieces(num_seqs, n_heads, n_kv_heads, G, BT, prefix_pages * kPage, tail, cus);
     p.pieces = c.pieces;
     p.piece_keys = c.piece_keys;
     p.longest = c.longest;
