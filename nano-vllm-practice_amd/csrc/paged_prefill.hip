@@ -52,9 +52,14 @@ hipError_t launch_paged_prefill(int dtype, PrefillArgs a, int num_tokens, int de
     // while tiles compute.  Rows seeing 1028 keys (32 query heads on 8) beside
     // 1024 new tokens behind 4096, us: 127 rows 131 with tiles cut for both
     // slots and ahead of all rows, 114 with all rows ahead of them, 100 so; 33
-    // rows 68, 57 and 46; 4 rows 43, 38 and 38.  Beside 2000 new tokens (tiles
-    // for both slots anyway) all rows ahead is better, 129 and 136 at 127 rows;
-    // every second or third workgroup a row: 100-125 and 125-137.
+    // rows 68, 57 and 46; 4 rows 43, 38 and 38.  Every second or third
+    // workgroup a row: 100-125.  Over 192 shapes (16-200 rows, 512-4000 new tokens,
+    // windows of 1024 and 4096, 64/8, 32/8 and 16/8 heads) all rows ahead is 4 %
+    // slower at the median and up to 53 % (64 rows seeing 4100 keys beside 1024
+    // tokens 157 and 242).  It is 0-7 % faster where the tiles about fill whole rounds of
+    // both slots (2000 tokens beside 127 rows 136 and 129), 20-38 % slower where they
+    // are a few more (1100 beside 64 rows of 16/8 heads 52 and 72): the host, which
+    // knows a lower bound of their number only, cannot tell these apart.
     const int slots = a.resident;
     if (a.window > 0 && a.decode_blocks > 0) a.resident /= 2;
     if (a.part) {
