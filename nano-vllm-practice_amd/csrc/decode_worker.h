@@ -6,6 +6,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "decode_slice.h"
 #include "launch.h"
 
 namespace femto {
@@ -637,9 +638,8 @@ __device__ __forceinline__ void walk_slice(const DecodeArgs& a, int wi, F&& segm
     C = max(C, a.min_chunk_pages);
     C = max(C, (longest + a.max_slots - 2) / (a.max_slots - 1));  // at most max_slots slots per sequence
     C = max(C, 1);
-    const int x0 = wi * C;
-    if (x0 >= total) return;
-    const int x1 = min(total, x0 + C);
+    int x0, x1;
+    if (!slice_pages(wi, C, total, x0, x1)) return;
 
     // Pass 2: the sequence holding page x0.  Lane i of the current 64-wide
     // chunk keeps kv_len and the exclusive page prefix of sequence base + i.

@@ -157,7 +157,7 @@ DecodePlan plan_paged_decode(int n_heads, int n_kv_heads, int max_kv_len, int dt
     const int n_rep = (n_kv_heads > 0) ? n_heads / n_kv_heads : 1;
     // f32 pages take twice the registers: at most 4 query heads per wave
     p.nrep_tile = (n_rep % 8 == 0 && dtype != kDtypeF32) ? 8 : (n_rep % 4 == 0) ? 4 : (n_rep % 2 == 0) ? 2 : 1;
-    const int max_pages = max_kv_len > 0 ? (max_kv_len + kPage - 1) / kPage : 1;
+    const int max_pages = max_kv_len > 0 ? (max_kv_len - 1) / kPage + 1 : 1;
     // A wave's slice is at least min_chunk_pages long, so a sequence is cut
     // into at most max_slots - 1 slices (+1 for a slice straddling its start).
     p.min_chunk_pages = std::max(4, (max_pages + 31) / 32);
@@ -327,7 +327,7 @@ static int paged_decode_entry(const char* fn_name, int dtype, const void* q, int
                             " exceeds the scratch limit of " + std::to_string(kScratchMaxSeqHeads) +
                             " (sequences x query heads); use femto_paged_attention_gemv with a workspace");
         if ((size_t)plan.max_slots > fit) {
-            const int max_pages = max_kv_len > 0 ? (max_kv_len + femto::kPage - 1) / femto::kPage : 1;
+            const int max_pages = max_kv_len > 0 ? (max_kv_len - 1) / femto::kPage + 1 : 1;
             plan.max_slots = (int)fit;
             plan.min_chunk_pages = std::max(plan.min_chunk_pages, (max_pages + plan.max_slots - 2) / (plan.max_slots - 1));
         }
@@ -366,7 +366,7 @@ static WindowParts window_parts(int64_t rows, int n_heads, int n_kv_heads, int s
     const int n_rep = n_heads / n_kv_heads;
     const int64_t groups = rows * n_kv_heads * ((n_rep + femto::kMfmaHeads - 1) / femto::kMfmaHeads);
     const int limit = g_single_max_kv.load(std::memory_order_relaxed);
-    const int pages = (seen + femto::kPage - 1) / femto::kPage;
+    const int pages = seen > 0 ? (seen - 1) / femto::kPage + 1 : 0;
     WindowParts w{1, 4};
     if (limit == kSingleMaxKV && pages >= 24 && 2 * groups <= cus)
         w.parts = std::min((int)(cus / groups), (int)(0.7 * std::sqrt((double)pages) + 0.5));
