@@ -197,9 +197,14 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, int b, int kv_
             pw[x] = pack2(E{}, fast_exp2(fmaf(sc[2 * x], scale, -s.m)), fast_exp2(fmaf(sc[2 * x + 1], scale, -s.m)));
             s.l = sum2(E{}, pw[x], s.l);
         }
+        // Every block of 16 dims, also those past head_dim (not stored): with an
+        // exit after the last one the compiler left out the wait between a
+        // block's MFMA and the copy of its result at the exit's target, and
+        // four-wave calls of 64 dims lost a page in dims 50, 51, 54, 55, ..  (61
+        // sequences, window 2048: 64 dims 44.3 us either way, 112 69.7 and 68.4,
+        // 16 30.3 and 31.0.)
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
-            if (!FULL && 16 * dt >= D) break;
             const int dim = 16 * dt + v_dim;
             const int off = v_key * 256 + ((((dim >> 3) ^ swz_v(v_key)) << 4) | ((dim & 4) << 1));
             const u32x2 vt = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vs + off)));
