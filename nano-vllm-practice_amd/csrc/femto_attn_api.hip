@@ -1086,7 +1086,9 @@ int femto_rope_cache_write(int dtype, const void* q, int64_t q_stride_token, int
     a.head_dim = head_dim;
     a.rotary_dim = rotary_dim;
     a.interleaved = interleaved != 0;
-    return hip_status(femto::launch_rope_cache_write(dtype, a, cu_seqlens ? max_q_len : 1, static_cast<hipStream_t>(stream)),
+    // (no sequence has more tokens than the call)
+    return hip_status(femto::launch_rope_cache_write(dtype, a, cu_seqlens ? std::min(max_q_len, num_tokens) : 1,
+                                                     static_cast<hipStream_t>(stream)),
                       "rope_cache_write launch");
 }
 

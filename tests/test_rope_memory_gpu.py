@@ -1,4 +1,5 @@
-"""rope_cache_write with an ``out`` that lies beside q, k and v in their buffer, or on them."""
+"""rope_cache_write with an ``out`` that lies beside q, k and v in their buffer, or on them; with a max_q_len far above
+the sequences' lengths."""
 
 import pytest
 import torch
@@ -68,3 +69,13 @@ def test_heads_ahead_of_tokens(ops, gpu):
     check_rotated(got, q, *(t.numpy() for t in tables), meta.positions.cpu().numpy(), True, "out")
     run(ops, gpu, w, qd, k.to(gpu), v.to(gpu), tables, True, out=qd)
     assert torch.equal(qd, got)
+
+
+@pytest.mark.parametrize("bound", [100, 1 << 24, 2**31 - 1])
+def test_overstated_max_q_len(ops, gpu, bound):
+    w, q, k, v = step([(0, 37), (15, 1), (100, 60)], 6, 2, 64, BF16, seed=11)
+    q, k, v = q.to(gpu), k.to(gpu), v.to(gpu)
+    tables = scaled_rope_tables(300, 64)
+    want, pools, _ = run(ops, gpu, w, q, k, v, tables, False)
+    got, wd, _ = run(ops, gpu, w, q, k, v, tables, False, max_q_len=bound)
+    assert torch.equal(got, want) and torch.equal(wd.k_pool, pools.k_pool) and torch.equal(wd.v_pool, pools.v_pool)
