@@ -103,7 +103,8 @@ class Timer:
 
 # Sources of the decode kernels: the committed PMC summary's traffic figure is
 # used only while these files are the ones it measured.
-DECODE_SOURCES = ("csrc/paged_decode.hip", "csrc/decode_worker.h", "csrc/common.h", "csrc/launch.h")
+DECODE_SOURCES = ("csrc/paged_decode.hip", "csrc/decode_kernels.h", "csrc/decode_worker.h", "csrc/decode_slice.h",
+                  "csrc/common.h", "csrc/launch.h")
 
 
 def sources_sha16(rel_paths):
