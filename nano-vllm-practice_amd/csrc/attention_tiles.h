@@ -666,7 +666,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         first_issued = i0 < n;
         t_first = tile_at(i0);
     } else {
-        if (PAGED && npieces > 1) t_first = piece * piece_tiles(0);  // tiles_bound: of all kv_len keys
+        if constexpr (PREFIX) {
+            t_first = piece * piece_tiles(0);
+        } else if (PAGED && npieces > 1) {
+            const int ub = (kv_len + kKvTile - 1) / kKvTile;
+            t_first = piece * ((ub + npieces - 1) / npieces);
+        }
         first_issued = t_first * kKvTile < kv_len;
     }
     if (first_issued) {
