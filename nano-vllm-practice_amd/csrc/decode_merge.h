@@ -12,7 +12,7 @@ namespace femto {
 // outputs are loaded kMergeAhead at a time, before their weights are known.
 // Slots are added in order: the result does not depend on which wave wrote last.
 constexpr int kMergeRows = 4;    // waves per workgroup
-constexpr int kMergeAhead = 16;  // slots in flight (12: 64 sequences on 4096 keys 27.1 us, now 26.4; 256 on 16384 +0.7)
+constexpr int kMergeAhead = 16;  // slots in flight (12: 64 sequences on 4096 keys 2.6 % slower, 256 on 16384 0.5 %)
 
 template <typename E>
 __global__ __launch_bounds__(64 * kMergeRows) void merge_rows_kernel(DecodeArgs a) {

@@ -23,12 +23,16 @@
 // from memory, which the wave has read before it stores the row (the output may
 // be q itself).
 //
-// Bound by its bytes: 8 x 512 tokens of 32/8 bf16 heads (103 MB) take 20.7 us a
-// call, 4.97 TB/s, a plain copy's rate.  Stores are non-temporal: the launch
+// Bound by its bytes: 8 x 512 tokens of 32/8 bf16 heads (103 MB) take 20.5 us a
+// call, 5.02 TB/s, a plain copy's rate.  Stores are non-temporal: the launch
 // does not end with dirty lines to write back (24.5 us with ordinary ones;
 // non-temporal loads besides 21.8).  Followed by the attention that reads q
-// and the pages the two take as long either way.  64 tokens: 5.7 us, the launch
-// and three dependent round trips.
+// and the pages the two take as long either way.  64 tokens: 5.6 us, the launch
+// and three dependent round trips.  Where an item's two chunks are neighbours a
+// store writes every other 16 bytes of a line, and the L2 passes some on by halves
+// (79 MB written to HBM for 50): the same tokens interleaved 31.6 us, with R = 32
+// 29.4, with R = 24 (and partners one by one) 35.9.  1024 tokens beside
+// 127 of one token each: 30.6 us, 7.8 without them, for workgroups without a token.
 #include "common.h"
 #include "launch.h"
 

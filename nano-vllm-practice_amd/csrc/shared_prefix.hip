@@ -11,9 +11,9 @@
 //    cut into pieces, one workgroup each;
 //  * tails: bound by their bytes, on the MFMA workers of mfma_decode.h, in
 //    the same launch, one workgroup per CU beside the tiles.
-// 256 sequences on 16384 keys, tails of up to 1024, 32/8 heads: 132 us, bound by
+// 256 sequences on 16384 keys, tails of up to 1024, 32/8 heads: 132-135 us, bound by
 // both, the tails' 509 MB (92 us alone) and the tiles, 64 in series (104 alone);
-// 64 on 4096, tails of up to 512, f16 16/8 heads 27.5 us; 8 on 1024 11.9 us, two
+// 64 on 4096, tails of up to 512, f16 16/8 heads 27.5 us; 8 on 1024 11.7 us, two
 // launches and their round trips.
 #include "attention_tiles.h"
 #include "decode_merge.h"
