@@ -19,7 +19,7 @@ bits 0-2 the index in that list.  With R the token's row in the page and P = 256
 
 * K, block b, dims 32 b + 2 i (low half of the byte) and + 1 (high): byte 256 b + 16 R + i;
 * V, dims 8 c + 2 i and + 1: byte P + (R // 4) * 64 N + 16 c + 4 (R % 4) + i;
-* K's scale of block b: byte 2 P + 16 b + R; V's: byte 2 P + 64 + 16 (R // 4) + 4 b + R % 4;
+* K's scale of block b: byte 2 P + 4 R + b; V's: byte 2 P + 64 + 16 (R // 4) + 4 b + R % 4;
 * page_bytes = 2 P + 128.
 
 The scale is the smallest power of two for which the block's largest magnitude is at most 7 of it (so that none is more
@@ -232,7 +232,7 @@ def _spoil(st, pool):
     n, r = torch.nonzero(row[None, :] > (last[has] % PAGE)[:, None], as_tuple=True)
     scales = pool.size(2) - 128
     for b in range(4):
-        pool[block[n], :, scales + 16 * b + r] = 255
+        pool[block[n], :, scales + 4 * r + b] = 255
         pool[block[n], :, scales + 64 + 16 * (r // 4) + 4 * b + r % 4] = 255
 
 
@@ -311,7 +311,7 @@ def _store(pool, block, row, k, v):
     i = torch.arange(16 * n, device=dev)
     pool[at, h, 256 * (i // 16) + 16 * r + i % 16] = pair(ck).reshape(T, KVH, 16 * n)
     pool[at, h, 256 * n + 64 * n * (r // 4) + 16 * (i // 4) + 4 * (r % 4) + i % 4] = pair(cv).reshape(T, KVH, 16 * n)
-    pool[at, h, 512 * n + 16 * b + r] = sk
+    pool[at, h, 512 * n + 4 * r + b] = sk
     pool[at, h, 512 * n + 64 + 16 * (r // 4) + 4 * b + r % 4] = sv
 
 
@@ -327,7 +327,7 @@ def _load(pool, dim):
 
     kc = pool[..., : 256 * n].reshape(*lead, n, 16, 16).transpose(-3, -2)
     vc = pool[..., 256 * n : 512 * n].reshape(*lead, 4, 4 * n, 4, 4).transpose(-3, -2).reshape(*lead, 16, n, 16)
-    ks = pool[..., 512 * n : 512 * n + 64].reshape(*lead, 4, 16).transpose(-2, -1)[..., :n]
+    ks = pool[..., 512 * n : 512 * n + 64].reshape(*lead, 16, 4)[..., :n]
     vs = pool[..., 512 * n + 64 :].reshape(*lead, 4, 4, 4).transpose(-2, -1).reshape(*lead, 16, 4)[..., :n]
     return values(kc, ks), values(vc, vs)
 
@@ -468,7 +468,7 @@ def _exact_rows(pool, blocks, head, length, dim):
     for b in range(n):
         i = torch.arange(16, device=pool.device)
         data = page[p[:, None], 256 * b + 16 * r[:, None] + i]
-        k.append(_exact_values(data, page[p, 512 * n + 16 * b + r]))
+        k.append(_exact_values(data, page[p, 512 * n + 4 * r + b]))
         data = page[p[:, None], 256 * n + (r // 4 * 64 * n)[:, None] + 16 * (4 * b + i // 4) + 4 * (r % 4)[:, None] + i % 4]
         v.append(_exact_values(data, page[p, 512 * n + 64 + 16 * (r // 4) + 4 * b + r % 4]))
     return torch.cat(k, -1)[:, :dim], torch.cat(v, -1)[:, :dim]
