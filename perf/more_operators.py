@@ -23,7 +23,7 @@ bits 0-2 the index in that list.  With R the token's row in the page and P = 256
 * page_bytes = 2 P + 128.
 
 The scale is the smallest power of two for which the block's largest magnitude is at most 7 of it (so that none is more
-than half a step off), at least 2^-119; values round to the nearest of the list, ties to the even index, magnitudes
+than half a step off), from 2^-119 to 2^125; values round to the nearest of the list, ties to the even index, magnitudes
 past 6 to 6; a block that holds an infinity or a NaN has the scale byte 255 and zeros, and stands for NaN.
 
 A paged batch is ``chunks`` (text, "cached+new ..."), or ``seqs`` chunks (``new_min..new_max`` tokens after
@@ -290,7 +290,7 @@ def _quantize(x):
     bad = ~torch.isfinite(x).all(-1)
     f, e = torch.frexp(torch.where(bad, torch.ones_like(top), top))  # top = f 2^e, f in [0.5, 1)
     e = torch.where(top == 0, torch.full_like(e, -1000), e - 3 + (f > 0.875))  # 7 = 0.875 * 2^3
-    e = e.clamp(min=-119)
+    e = e.clamp(-119, 125)
     y = x * _power(-e)[..., None]
     a = y.abs()
     code = ((a > 0.25).to(torch.uint8) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0)
@@ -507,6 +507,7 @@ def _exact_nearest(x):
     top = x.abs().amax(-1, keepdim=True)
     step = torch.pow(2.0, torch.ceil(torch.log2(top / 7)).clamp(min=-119))
     step = torch.where(top > 7 * step, 2 * step, torch.where((top <= 3.5 * step) & (step > 2.0 ** -119), step / 2, step))
+    step = step.clamp(max=2.0**125)
     level = torch.tensor([0.0, 1.0, 2.0, 4.0, 0.5, 1.5, 3.0, 6.0], dtype=torch.float64, device=x.device)  # even indices first
     near = level[((x / step).abs()[..., None] - level).abs().argmin(-1)]
     return (near * step * torch.sign(x)).flatten(-2)[..., :dim]
