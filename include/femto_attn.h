@@ -348,6 +348,69 @@ int femto_rope_cache_write(
     const int32_t* positions, const int32_t* kv_page_tables, int num_pages_per_seq, int64_t table_stride,
     void* stream);
 
+/* ---- KV cache held in 4 bits ----------------------------------------------
+ *
+ * kv_pool (num_blocks, n_kv_heads, page_bytes) bytes, contiguous and 16-byte
+ * aligned; a page is 16 tokens of K and V of one KV head, page_bytes =
+ * femto_fp4_page_bytes(head_dim).  head_dim <= 128, a multiple of 16.  Dims are
+ * in N = ceil(head_dim / 32) blocks of 32 (the last may be half full, zeros
+ * behind it).  A (token, block) is one scale 2^(byte - 127) and 32 values of
+ * {0, 0.5, 1, 1.5, 2, 3, 4, 6} times it, 4 bits each: bit 3 the sign, bits 0-2
+ * the index in that list.  With r the token's row in the page and P = 256 N:
+ *   K, dims 32 b + 2 i (low half of the byte) and + 1 (high): byte 256 b + 16 r + i
+ *   V, dims 8 c + 2 i and + 1: byte P + 64 N (r / 4) + 16 c + 4 (r % 4) + i
+ *   scale of K's block b: byte 2 P + 4 r + b; V's: 2 P + 64 + 16 (r / 4) + 4 b + r % 4
+ * Writes take the smallest power of two as scale for which no magnitude of the
+ * block is more than 7 of it (from 2^-119 to 2^125) and round to the nearest, ties to
+ * the even index, magnitudes past 6 to 6.  A block that holds an infinity or a
+ * NaN gets the byte 255, which stands for NaN in all of it.  Scale bytes of
+ * other writers are 1 to 254, or 255.
+ * q, k, v and outputs are F16 or BF16; the cache does not say which wrote it.
+ * Attention and reads take V and values as their own type: those past f16's
+ * range are infinities to an f16 call.  No counterpart in the reference. */
+size_t femto_fp4_page_bytes(int head_dim); /* 512 N + 128; 0: head_dim not supported */
+
+/* femto_kv_cache_write into a 4-bit cache, and the reverse: the rows of the
+ * tokens at positions[cu_seqlens[b]] + 0, 1, .. of each sequence into k_out and
+ * v_out (num_tokens, n_kv_heads, head_dim), contiguous; zeros where a write
+ * would have stopped (a table column that is -1, past the table or outside the
+ * pool).  cu_seqlens == NULL: one token per sequence.  max_q_len only sizes the
+ * launch: longer sequences are taken whole.  At most 65535 sequences. */
+int femto_kv_cache_write_fp4(
+    int dtype,
+    const void* k, int64_t k_stride_token, int64_t k_stride_head,
+    const void* v, int64_t v_stride_token, int64_t v_stride_head,
+    void* kv_pool, int64_t num_blocks, int n_kv_heads, int head_dim,
+    const int32_t* cu_seqlens, int num_seqs, int num_tokens, int max_q_len,
+    const int32_t* positions, const int32_t* kv_page_tables, int num_pages_per_seq, int64_t table_stride,
+    void* stream);
+int femto_kv_cache_read_fp4(
+    int dtype,
+    const void* kv_pool, int64_t num_blocks, int n_kv_heads, int head_dim,
+    void* k_out, void* v_out,
+    const int32_t* cu_seqlens, int num_seqs, int num_tokens, int max_q_len,
+    const int32_t* positions, const int32_t* kv_page_tables, int num_pages_per_seq, int64_t table_stride,
+    void* stream);
+
+/* The attention prologue over a 4-bit cache: femto_rope_cache_write's rotation
+ * (same layouts, tables and rules for q_out), after per-head RMSNorms of q and
+ * k where q_weight and k_weight (head_dim elements each, both or neither) are
+ * given: x w / sqrt(mean(x^2) + eps).  The norm is formed in 64 bits and rounded
+ * to fp32, the rotation in fp32 with every product and sum rounded by itself;
+ * then q rounds to its type and k to 4 bits, v as it is. */
+int femto_rope_cache_write_fp4(
+    int dtype,
+    const void* q, int64_t q_stride_token, int64_t q_stride_head,
+    const void* k, int64_t k_stride_token, int64_t k_stride_head,
+    const void* v, int64_t v_stride_token, int64_t v_stride_head,
+    void* q_out, int64_t q_out_stride_token, int64_t q_out_stride_head,
+    const void* q_weight, const void* k_weight, double eps,
+    const float* cos, const float* sin, int64_t rope_stride, int rope_rows, int rotary_dim, int interleaved,
+    void* kv_pool, int64_t num_blocks, int n_heads, int n_kv_heads, int head_dim,
+    const int32_t* cu_seqlens, int num_seqs, int num_tokens, int max_q_len,
+    const int32_t* positions, const int32_t* kv_page_tables, int num_pages_per_seq, int64_t table_stride,
+    void* stream);
+
 /* Varlen attention metadata built on the device, by the rules of the
  * reference's ModelRunner (femtovllm/engine/model_runner.py:187-202 prefill,
  * 283-293 decode, 46-72 block-table padding), which builds them with Python

@@ -15,6 +15,7 @@
 #include "common.h"
 #include "decode_route.h"
 #include "femto_attn.h"
+#include "fp4.h"
 #include "launch.h"
 #include "mfma_decode.h"
 
@@ -607,6 +608,57 @@ static int paged_gemm_entry(const char* fn_name, int dtype, const void* q, int64
     return hip_status(femto::launch_paged_prefill(dtype, a, num_tokens, decode_rows, st), (fn + " launch").c_str());
 }
 
+// Checks that the writes to and reads of a 4-bit cache share, and the arguments
+// that they fill in.
+static int fp4_cache_args(const std::string& f, int dtype, const void* kv_pool, int64_t num_blocks, int n_kv_heads,
+                          int head_dim, const int32_t* cu_seqlens, int num_seqs, int num_tokens, int max_q_len,
+                          const int32_t* positions, const int32_t* kv_page_tables, int num_pages_per_seq,
+                          int64_t table_stride, femto::Fp4CacheArgs& a) {
+    if (dtype != FEMTO_F16 && dtype != FEMTO_BF16)
+        return fail(FEMTO_ERR_UNSUPPORTED, f + ": not implemented for '" + dtype_name(dtype) + "' (bf16 / f16 only)");
+    if (head_dim <= 0 || head_dim > femto::kDimHead || head_dim % 16 != 0)
+        return fail(FEMTO_ERR_UNSUPPORTED, f + ": head_dim must be at most " + std::to_string(femto::kDimHead) +
+                                               " and a multiple of 16, got " + std::to_string(head_dim));
+    if (num_seqs < 0 || num_tokens < 0) return fail(FEMTO_ERR_INVALID, f + ": negative size");
+    if (num_seqs == 0 || num_tokens == 0) return FEMTO_OK;
+    if (!cu_seqlens && num_tokens != num_seqs)
+        return fail(FEMTO_ERR_INVALID, f + ": without cu_seqlens every sequence has one token (num_tokens == num_seqs)");
+    if (max_q_len < 1) return fail(FEMTO_ERR_INVALID, f + ": max_q_len must be >= 1");
+    if (num_seqs > 65535) return fail(FEMTO_ERR_INVALID, f + ": at most 65535 sequences per call");
+    if (n_kv_heads <= 0) return fail(FEMTO_ERR_INVALID, f + ": head counts must be positive");
+    if (num_blocks < 1) return fail(FEMTO_ERR_INVALID, f + ": the pool needs at least one block");
+    if (!kv_pool || !positions || (num_pages_per_seq > 0 && !kv_page_tables))
+        return fail(FEMTO_ERR_INVALID, f + ": null pointer argument");
+    if (num_pages_per_seq < 0 || table_stride < num_pages_per_seq)
+        return fail(FEMTO_ERR_INVALID, f + ": table stride smaller than its width");
+    if (!aligned(kv_pool, 16)) return fail(FEMTO_ERR_INVALID, f + ": kv_pool must be 16-byte aligned");
+    a.pool = static_cast<uint8_t*>(const_cast<void*>(kv_pool));
+    a.num_blocks = num_blocks;
+    a.n_kv_heads = n_kv_heads;
+    a.head_dim = head_dim;
+    a.cu_seqlens = cu_seqlens;
+    a.positions = positions;
+    a.tables = kv_page_tables;
+    a.table_stride = table_stride;
+    a.num_pages_per_seq = num_pages_per_seq;
+    a.num_seqs = num_seqs;
+    return FEMTO_OK;
+}
+static int fp4_source(const std::string& f, const void* k, int64_t k_stride_token, int64_t k_stride_head, const void* v,
+                      int64_t v_stride_token, int64_t v_stride_head, femto::Fp4CacheArgs& a) {
+    if (!k || !v) return fail(FEMTO_ERR_INVALID, f + ": null pointer argument");
+    if (!aligned(k, 16) || !aligned(v, 16)) return fail(FEMTO_ERR_INVALID, f + ": k and v must be 16-byte aligned");
+    if (k_stride_token % 8 || k_stride_head % 8 || v_stride_token % 8 || v_stride_head % 8)
+        return fail(FEMTO_ERR_INVALID, f + ": strides must be multiples of 16 bytes");
+    a.k = k;
+    a.k_stride_token = k_stride_token;
+    a.k_stride_head = k_stride_head;
+    a.v = v;
+    a.v_stride_token = v_stride_token;
+    a.v_stride_head = v_stride_head;
+    return FEMTO_OK;
+}
+
 extern "C" {
 
 const char* femto_attn_last_error(void) { return g_err.c_str(); }
@@ -1090,6 +1142,101 @@ int femto_rope_cache_write(int dtype, const void* q, int64_t q_stride_token, int
     return hip_status(femto::launch_rope_cache_write(dtype, a, cu_seqlens ? std::min(max_q_len, num_tokens) : 1,
                                                      static_cast<hipStream_t>(stream)),
                       "rope_cache_write launch");
+}
+
+size_t femto_fp4_page_bytes(int head_dim) {
+    return head_dim > 0 && head_dim <= femto::kDimHead && head_dim % 16 == 0 ? (size_t)femto::fp4_page_bytes(head_dim) : 0;
+}
+
+int femto_kv_cache_write_fp4(int dtype, const void* k, int64_t k_stride_token, int64_t k_stride_head, const void* v,
+                             int64_t v_stride_token, int64_t v_stride_head, void* kv_pool, int64_t num_blocks,
+                             int n_kv_heads, int head_dim, const int32_t* cu_seqlens, int num_seqs, int num_tokens,
+                             int max_q_len, const int32_t* positions, const int32_t* kv_page_tables,
+                             int num_pages_per_seq, int64_t table_stride, void* stream) {
+    g_err.clear();
+    const std::string f = "kv_cache_write_fp4";
+    femto::Fp4CacheArgs a{};
+    int rc = fp4_cache_args(f, dtype, kv_pool, num_blocks, n_kv_heads, head_dim, cu_seqlens, num_seqs, num_tokens,
+                            max_q_len, positions, kv_page_tables, num_pages_per_seq, table_stride, a);
+    if (rc != FEMTO_OK || num_seqs == 0 || num_tokens == 0) return rc;
+    rc = fp4_source(f, k, k_stride_token, k_stride_head, v, v_stride_token, v_stride_head, a);
+    if (rc != FEMTO_OK) return rc;
+    return hip_status(femto::launch_fp4_cache(dtype, femto::kFp4Write, a, cu_seqlens ? std::min(max_q_len, num_tokens) : 1,
+                                              static_cast<hipStream_t>(stream)),
+                      "kv_cache_write_fp4 launch");
+}
+
+int femto_kv_cache_read_fp4(int dtype, const void* kv_pool, int64_t num_blocks, int n_kv_heads, int head_dim, void* k_out,
+                            void* v_out, const int32_t* cu_seqlens, int num_seqs, int num_tokens, int max_q_len,
+                            const int32_t* positions, const int32_t* kv_page_tables, int num_pages_per_seq,
+                            int64_t table_stride, void* stream) {
+    g_err.clear();
+    const std::string f = "kv_cache_read_fp4";
+    femto::Fp4CacheArgs a{};
+    const int rc = fp4_cache_args(f, dtype, kv_pool, num_blocks, n_kv_heads, head_dim, cu_seqlens, num_seqs, num_tokens,
+                                  max_q_len, positions, kv_page_tables, num_pages_per_seq, table_stride, a);
+    if (rc != FEMTO_OK || num_seqs == 0 || num_tokens == 0) return rc;
+    if (!k_out || !v_out) return fail(FEMTO_ERR_INVALID, f + ": null pointer argument");
+    if (!aligned(k_out, 16) || !aligned(v_out, 16))
+        return fail(FEMTO_ERR_INVALID, f + ": k_out and v_out must be 16-byte aligned");
+    a.k_out = k_out;
+    a.v_out = v_out;
+    return hip_status(femto::launch_fp4_cache(dtype, femto::kFp4Read, a, cu_seqlens ? std::min(max_q_len, num_tokens) : 1,
+                                              static_cast<hipStream_t>(stream)),
+                      "kv_cache_read_fp4 launch");
+}
+
+int femto_rope_cache_write_fp4(int dtype, const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* k,
+                               int64_t k_stride_token, int64_t k_stride_head, const void* v, int64_t v_stride_token,
+                               int64_t v_stride_head, void* q_out, int64_t q_out_stride_token, int64_t q_out_stride_head,
+                               const void* q_weight, const void* k_weight, double eps, const float* cos, const float* sin,
+                               int64_t rope_stride, int rope_rows, int rotary_dim, int interleaved, void* kv_pool,
+                               int64_t num_blocks, int n_heads, int n_kv_heads, int head_dim, const int32_t* cu_seqlens,
+                               int num_seqs, int num_tokens, int max_q_len, const int32_t* positions,
+                               const int32_t* kv_page_tables, int num_pages_per_seq, int64_t table_stride, void* stream) {
+    g_err.clear();
+    const std::string f = "rope_cache_write_fp4";
+    femto::Fp4CacheArgs a{};
+    int rc = fp4_cache_args(f, dtype, kv_pool, num_blocks, n_kv_heads, head_dim, cu_seqlens, num_seqs, num_tokens,
+                            max_q_len, positions, kv_page_tables, num_pages_per_seq, table_stride, a);
+    if (rc != FEMTO_OK) return rc;
+    if (rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2 != 0)
+        return fail(FEMTO_ERR_INVALID, f + ": rotary_dim must be even and from 2 to head_dim (" +
+                                           std::to_string(head_dim) + "), got " + std::to_string(rotary_dim));
+    if (n_heads <= 0) return fail(FEMTO_ERR_INVALID, f + ": head counts must be positive");
+    if (!q_weight != !k_weight) return fail(FEMTO_ERR_INVALID, f + ": q_weight and k_weight are given both or not at all");
+    if (q_weight && !(eps >= 0.0)) return fail(FEMTO_ERR_INVALID, f + ": eps must be >= 0");
+    if (num_seqs == 0 || num_tokens == 0) return FEMTO_OK;
+    rc = fp4_source(f, k, k_stride_token, k_stride_head, v, v_stride_token, v_stride_head, a);
+    if (rc != FEMTO_OK) return rc;
+    if (!q || !q_out || !cos || !sin) return fail(FEMTO_ERR_INVALID, f + ": null pointer argument");
+    if (rope_rows < 1 || rope_stride < rotary_dim / 2) return fail(FEMTO_ERR_INVALID, f + ": rope tables too small");
+    const void* ptrs[] = {q, q_out, q_weight, k_weight};
+    for (const void* p : ptrs)
+        if (!aligned(p, 16)) return fail(FEMTO_ERR_INVALID, f + ": tensors must be 16-byte aligned");
+    if (!aligned(cos, 4) || !aligned(sin, 4)) return fail(FEMTO_ERR_INVALID, f + ": cos and sin must be 4-byte aligned");
+    if (q_stride_token % 8 || q_stride_head % 8 || q_out_stride_token % 8 || q_out_stride_head % 8)
+        return fail(FEMTO_ERR_INVALID, f + ": strides must be multiples of 16 bytes");
+    a.q = q;
+    a.q_stride_token = q_stride_token;
+    a.q_stride_head = q_stride_head;
+    a.q_out = q_out;
+    a.q_out_stride_token = q_out_stride_token;
+    a.q_out_stride_head = q_out_stride_head;
+    a.n_heads = n_heads;
+    a.q_weight = q_weight;
+    a.k_weight = k_weight;
+    a.eps = eps;
+    a.cos = cos;
+    a.sin = sin;
+    a.rope_stride = rope_stride;
+    a.rope_rows = rope_rows;
+    a.rotary_dim = rotary_dim;
+    a.interleaved = interleaved != 0;
+    return hip_status(femto::launch_fp4_cache(dtype, femto::kFp4Prologue, a,
+                                              cu_seqlens ? std::min(max_q_len, num_tokens) : 1,
+                                              static_cast<hipStream_t>(stream)),
+                      "rope_cache_write_fp4 launch");
 }
 
 int femto_build_varlen_metadata(int num_seqs, const int32_t* num_computed, const int32_t* num_tokens,

@@ -1,0 +1,302 @@
+// Writes to a KV cache held in 4 bits (layout and rounding: fp4.h), and reads
+// of its tokens.
+//
+// Placement is kv_cache_write.hip's: sequence b's tokens go to positions
+// positions[q_begin] + 0, 1, ..., until the first table column that is -1, past the
+// table or outside the pool.  A read gives zeros where a write would have
+// stopped.
+//
+// The prologue also norms (optional) and rotates q and k on the way:
+//   y = x w / sqrt(mean(x^2) + eps), per head;
+//   (a, b) -> (a cos - b sin, b cos + a sin) for pairs as rope_cache_write.hip.
+// A value next to a border of the 4-bit list falls on one side by its last
+// bit.  So that what is cached does not hang on the order of a sum or on
+// contraction, the norm is formed in 64 bits and rounded to 32, and each product
+// and sum of the rotation is rounded by itself; k rounds to 4 bits from there, q
+// to its type.
+//
+// Work: one wave per token, four head rows at a time, 16 lanes of 8 dims each; a
+// block of 32 dims is a quad of lanes, and its largest magnitude two DPP steps.
+// Rows move in batches of loads; the placement is looked up by the whole wave
+// while the first batch is on its way.
+#include <type_traits>
+
+#include "fp4.h"
+#include "launch.h"
+
+namespace femto {
+
+constexpr int kFp4Tokens = 4;  // waves (tokens) per workgroup
+constexpr int kFp4Batch = 4;   // passes of four rows whose loads are in flight
+
+enum Fp4Pairs { kFp4NoPairs, kFp4Interleaved, kFp4HalfChunks, kFp4HalfAny };
+
+// Block of the cache row that the token i after position p0 has, -1 where the
+// walk ends before it (whole wave, uniform).
+__device__ __forceinline__ int fp4_block_of(const Fp4CacheArgs& a, const int32_t* table, int p0, int i) {
+    const int lane = threadIdx.x & 63;
+    const int pc = (int)((uint32_t)p0 + (uint32_t)i);
+    if (p0 < 0 || pc < 0) return -1;  // (wraps past 2^31: not in the cache)
+    const int col = pc / kPage;
+    int blk = -1;
+    uint64_t ends = 0;
+    for (int c = p0 / kPage; c <= col; c += 64) {
+        const int id = c + lane <= col && c + lane < a.num_pages_per_seq ? table[c + lane] : -1;
+        ends |= __ballot(c + lane <= col && (id < 0 || (int64_t)id >= a.num_blocks));
+        if (c + 64 > col) blk = __builtin_amdgcn_readlane(id, col - c);
+    }
+    return ends ? -1 : blk;
+}
+
+template <typename E>
+__device__ __forceinline__ float elem_at(const char* p);
+template <>
+__device__ __forceinline__ float elem_at<BF16>(const char* p) { return (float)*reinterpret_cast<const __bf16*>(p); }
+template <>
+__device__ __forceinline__ float elem_at<F16>(const char* p) { return (float)*reinterpret_cast<const _Float16*>(p); }
+
+template <int kCtrl>
+__device__ __forceinline__ double dpp_f64(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = dpp_i32<kCtrl>((int)(uint32_t)b), hi = dpp_i32<kCtrl>((int)(uint32_t)(b >> 32));
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double row16_sum_f64(double x) {
+    x += dpp_f64<0x128>(x);  // row_ror:8
+    x += dpp_f64<0x124>(x);  // row_ror:4
+    x += dpp_f64<0x4E>(x);   // quad_perm [2,3,0,1]
+    x += dpp_f64<0xB1>(x);   // quad_perm [1,0,3,2]
+    return x;
+}
+
+template <typename E, int PAIRS, bool NORM>
+__global__ __launch_bounds__(64 * kFp4Tokens) void fp4_cache_write_kernel(Fp4CacheArgs a) {
+#pragma clang fp contract(off)
+    constexpr bool ROPE = PAIRS != kFp4NoPairs;
+    const int lane = threadIdx.x & 63, c = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.y;
+    const int q_begin = a.cu_seqlens ? a.cu_seqlens[b] : b;
+    const int q_end = a.cu_seqlens ? a.cu_seqlens[b + 1] : b + 1;
+    const int D = a.head_dim, N = fp4_blocks(D), R = a.rotary_dim, half = R / 2;
+    const int H = ROPE ? a.n_heads : 0, KVH = a.n_kv_heads, rows = H + 2 * KVH;
+    const bool has = 8 * c < D;       // dims of the row
+    const bool held = 8 * c < 32 * N;  // and those that pad its last block
+    const bool turned = ROPE && 8 * c < R;
+    // The chunk that holds the other ends of the lane's pairs.
+    const int other = PAIRS == kFp4HalfChunks && turned ? (8 * c < half ? c + half / 8 : c - half / 8) : c;
+    const int32_t* table = a.tables + (int64_t)b * a.table_stride;
+
+    // max_q_len only sizes the grid: longer sequences take more rounds.
+    for (int t = q_begin + (int)blockIdx.x * kFp4Tokens + wave; t < q_end; t += (int)gridDim.x * kFp4Tokens) {
+        const char* src[3] = {ROPE ? static_cast<const char*>(a.q) + (int64_t)t * a.q_stride_token * 2 : nullptr,
+                              static_cast<const char*>(a.k) + (int64_t)t * a.k_stride_token * 2,
+                              static_cast<const char*>(a.v) + (int64_t)t * a.v_stride_token * 2};
+        auto row_ptr = [&](int r) __attribute__((always_inline)) {
+            const int s = r < H ? 0 : r < H + KVH ? 1 : 2;
+            const int64_t hs = s == 0 ? a.q_stride_head : s == 1 ? a.k_stride_head : a.v_stride_head;
+            const char* base = s == 0 ? src[0] : s == 1 ? src[1] : src[2];
+            return base + (int64_t)(s == 0 ? r : s == 1 ? r - H : r - H - KVH) * hs * 2;
+        };
+        u32x4 w0[kFp4Batch], w1[kFp4Batch];
+        auto load = [&](int base) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < kFp4Batch; ++u) {
+                const int r = base + 4 * u + (lane >> 4);
+                w0[u] = w1[u] = u32x4{0, 0, 0, 0};
+                if (r < rows && has) {
+                    const char* p = row_ptr(r);
+                    w0[u] = ld16(p + 16 * c);
+                    if (PAIRS == kFp4HalfChunks && turned && r < H + KVH) w1[u] = ld16(p + 16 * other);
+                }
+            }
+        };
+        load(0);
+
+        const int p0 = a.positions[q_begin];
+        const int blk = fp4_block_of(a, table, p0, t - q_begin);
+        const int row = (int)((uint32_t)p0 + (uint32_t)(t - q_begin)) & (kPage - 1);
+
+        // The lane's table fragment and weights.
+        float cs[8], sn[8];
+        float wq[8], wk[8], xq[8], xk[8];  // xq, xk: of the other chunk
+        if constexpr (ROPE) {
+            const int pos = a.positions[t];
+            const bool in_tables = pos >= 0 && pos < a.rope_rows;
+            const float* ct = a.cos + (int64_t)(in_tables ? pos : 0) * a.rope_stride;
+            const float* st = a.sin + (int64_t)(in_tables ? pos : 0) * a.rope_stride;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                // pair of dim 8 c + e
+                const int d = 8 * c + e;
+                const int j = PAIRS == kFp4Interleaved ? d / 2 : d < half ? d : d - half;
+                const bool in = d < R;
+                cs[e] = in ? ct[j] : 1.0f;
+                sn[e] = in ? st[j] : 0.0f;
+                if (!in_tables) cs[e] = sn[e] = __builtin_nanf("");
+            }
+            if constexpr (NORM) {
+                auto weights = [&](const void* p, int chunk, float (&f)[8]) __attribute__((always_inline)) {
+                    u32x4 w{0, 0, 0, 0};
+                    if (has) w = ld16(static_cast<const char*>(p) + 16 * chunk);
+                    unpack8(E{}, w, f);
+                };
+                weights(a.q_weight, c, wq);
+                weights(a.k_weight, c, wk);
+                if constexpr (PAIRS == kFp4HalfChunks) {
+                    weights(a.q_weight, other, xq);
+                    weights(a.k_weight, other, xk);
+                }
+            }
+        }
+
+        for (int base = 0; base < rows; base += 4 * kFp4Batch) {
+            if (base) load(base);
+#pragma unroll
+            for (int u = 0; u < kFp4Batch; ++u) {
+                const int r = base + 4 * u + (lane >> 4);
+                float x[8];
+                unpack8(E{}, w0[u], x);
+                if constexpr (ROPE) {
+                    double inv = 1.0;
+                    if constexpr (NORM) {
+                        double s = 0.0;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) s += (double)x[e] * (double)x[e];
+                        s = row16_sum_f64(s);
+                        inv = 1.0 / sqrt(s / (double)D + (double)a.eps);
+                    }
+                    if (r < H + KVH) {
+                        auto normed = [&](float v, float w) __attribute__((always_inline)) {
+                            return NORM ? (float)((double)v * inv * (double)w) : v;
+                        };
+                        auto weight = [&](int e) __attribute__((always_inline)) { return NORM ? (r < H ? wq[e] : wk[e]) : 1.0f; };
+                        float y[8];  // the other ends
+                        if constexpr (PAIRS == kFp4HalfChunks) {
+                            unpack8(E{}, w1[u], y);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) y[e] = normed(y[e], NORM ? (r < H ? xq[e] : xk[e]) : 1.0f);
+                        } else if constexpr (PAIRS == kFp4HalfAny) {
+                            const char* p = row_ptr(min(r, rows - 1));
+                            const char* w = static_cast<const char*>(r < H ? a.q_weight : a.k_weight);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const int d = 8 * c + e, o = d < half ? d + half : d - half;
+                                y[e] = d < R ? normed(elem_at<E>(p + 2 * o), NORM ? elem_at<E>(w + 2 * o) : 1.0f) : 0.0f;
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = normed(x[e], weight(e));
+                        if constexpr (PAIRS == kFp4Interleaved) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) y[e] = x[e ^ 1];
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int d = 8 * c + e;
+                            const bool first = PAIRS == kFp4Interleaved ? (e & 1) == 0 : d < half;
+                            const float p = x[e] * cs[e], q = y[e] * sn[e];
+                            if (d < R) x[e] = first ? p - q : p + q;
+                        }
+                    }
+                }
+                if (ROPE && r < H) {
+                    if (has)
+                        st16_nt(static_cast<char*>(a.q_out) + ((int64_t)t * a.q_out_stride_token + (int64_t)r * a.q_out_stride_head) * 2 + 16 * c,
+                                pack8(E{}, x));
+                    continue;
+                }
+                // The block's largest magnitude: this lane's and its quad's.
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+                top = max(top, (uint32_t)dpp_i32<0xB1>((int)top));
+                top = max(top, (uint32_t)dpp_i32<0x4E>((int)top));
+                if (r >= rows || blk < 0 || !held) continue;
+                const int byte = fp4_scale_byte(top);
+                const uint32_t word = byte == kFp4NanScale ? 0u : fp4_pack8(x, fp4_scale(byte));
+                const bool is_k = r < H + KVH;
+                const int h = is_k ? r - H : r - H - KVH;
+                uint8_t* page = a.pool + ((int64_t)blk * KVH + h) * fp4_page_bytes(D);
+                *reinterpret_cast<uint32_t*>(page + (is_k ? fp4_k_at(row, c) : fp4_v_at(N, row, c))) = word;
+                if ((c & 3) == 0) page[is_k ? fp4_k_scale_at(N, row, c >> 2) : fp4_v_scale_at(N, row, c >> 2)] = (uint8_t)byte;
+            }
+        }
+    }
+}
+
+// Rows of the tokens at positions[q_begin] + 0, 1, .. of each sequence, as E.
+template <typename E>
+__global__ __launch_bounds__(64 * kFp4Tokens) void fp4_cache_read_kernel(Fp4CacheArgs a) {
+    const int lane = threadIdx.x & 63, c = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.y;
+    const int q_begin = a.cu_seqlens ? a.cu_seqlens[b] : b;
+    const int q_end = a.cu_seqlens ? a.cu_seqlens[b + 1] : b + 1;
+    const int D = a.head_dim, N = fp4_blocks(D), KVH = a.n_kv_heads;
+    const int32_t* table = a.tables + (int64_t)b * a.table_stride;
+    for (int t = q_begin + (int)blockIdx.x * kFp4Tokens + wave; t < q_end; t += (int)gridDim.x * kFp4Tokens) {
+        const int p0 = a.positions[q_begin];
+        const int blk = fp4_block_of(a, table, p0, t - q_begin);
+        const int row = (int)((uint32_t)p0 + (uint32_t)(t - q_begin)) & (kPage - 1);
+        for (int base = 0; base < 2 * KVH; base += 4 * kFp4Batch) {
+            uint32_t word[kFp4Batch];
+            int byte[kFp4Batch];
+#pragma unroll
+            for (int u = 0; u < kFp4Batch; ++u) {
+                const int r = base + 4 * u + (lane >> 4);
+                word[u] = 0;
+                byte[u] = kFp4MinScale;
+                if (r < 2 * KVH && blk >= 0 && 8 * c < D) {
+                    const bool is_k = r < KVH;
+                    const uint8_t* page = a.pool + ((int64_t)blk * KVH + (is_k ? r : r - KVH)) * fp4_page_bytes(D);
+                    word[u] = *reinterpret_cast<const uint32_t*>(page + (is_k ? fp4_k_at(row, c) : fp4_v_at(N, row, c)));
+                    byte[u] = page[is_k ? fp4_k_scale_at(N, row, c >> 2) : fp4_v_scale_at(N, row, c >> 2)];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kFp4Batch; ++u) {
+                const int r = base + 4 * u + (lane >> 4);
+                if (r >= 2 * KVH || 8 * c >= D) continue;
+                const bool is_k = r < KVH;
+                char* out = static_cast<char*>(is_k ? a.k_out : a.v_out) +
+                            ((int64_t)t * KVH + (is_k ? r : r - KVH)) * D * 2 + 16 * c;
+                st16_nt(out, fp4_unpack8(E{}, word[u], fp4_scale(byte[u])));
+            }
+        }
+    }
+}
+
+template <typename E, int PAIRS>
+static void launch_write(const Fp4CacheArgs& a, dim3 grid, hipStream_t st) {
+    const dim3 block(64 * kFp4Tokens);
+    if constexpr (PAIRS != kFp4NoPairs) {
+        if (a.q_weight) {
+            hipLaunchKernelGGL((fp4_cache_write_kernel<E, PAIRS, true>), grid, block, 0, st, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((fp4_cache_write_kernel<E, PAIRS, false>), grid, block, 0, st, a);
+}
+
+template <typename E>
+static hipError_t launch_cache(Fp4CacheOp op, const Fp4CacheArgs& a, dim3 grid, hipStream_t st) {
+    if (op == kFp4Read) hipLaunchKernelGGL(fp4_cache_read_kernel<E>, grid, dim3(64 * kFp4Tokens), 0, st, a);
+    else if (op == kFp4Write) launch_write<E, kFp4NoPairs>(a, grid, st);
+    else if (a.interleaved) launch_write<E, kFp4Interleaved>(a, grid, st);
+    else if (a.rotary_dim % 16 == 0) launch_write<E, kFp4HalfChunks>(a, grid, st);
+    else launch_write<E, kFp4HalfAny>(a, grid, st);
+    return hipGetLastError();
+}
+
+hipError_t launch_fp4_cache(int dtype, Fp4CacheOp op, const Fp4CacheArgs& a, int max_q_len, hipStream_t st) {
+    if (a.num_seqs <= 0 || max_q_len <= 0) return hipSuccess;
+    const dim3 grid((max_q_len - 1) / kFp4Tokens + 1, a.num_seqs);
+    switch (dtype) {
+        case kDtypeBF16: return launch_cache<BF16>(op, a, grid, st);
+        case kDtypeF16: return launch_cache<F16>(op, a, grid, st);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace femto

@@ -215,6 +215,40 @@ struct RopeArgs {
 
 hipError_t launch_rope_cache_write(int dtype, RopeArgs a, int max_q_len, hipStream_t st);
 
+// Writes to and reads of a KV cache held in 4 bits (fp4_cache.hip); k, v, q and
+// their outputs are bf16 or f16, tables and placement as for kv_cache_write.
+struct Fp4CacheArgs {
+    uint8_t* pool;  // (num_blocks, n_kv_heads, fp4_page_bytes(head_dim))
+    int64_t num_blocks;
+    int n_kv_heads, head_dim;
+    const int32_t* cu_seqlens;  // null: one token per sequence (decode)
+    const int32_t* positions;   // first token of each sequence at positions[q_begin]; rotary positions of all
+    const int32_t* tables;
+    int64_t table_stride;
+    int num_pages_per_seq, num_seqs;
+    const void* k;  // writes: (tokens, n_kv_heads, head_dim)
+    const void* v;
+    int64_t k_stride_token, k_stride_head, v_stride_token, v_stride_head;
+    void* k_out;  // reads: the same, contiguous
+    void* v_out;
+    // Prologue: q in and out (tokens, n_heads, head_dim), norm weights (or
+    // null) and eps, rotary tables.
+    const void* q;
+    int64_t q_stride_token, q_stride_head;
+    void* q_out;
+    int64_t q_out_stride_token, q_out_stride_head;
+    int n_heads;
+    const void* q_weight;
+    const void* k_weight;
+    double eps;
+    const float* cos;  // (rope_rows, rotary_dim / 2) fp32
+    const float* sin;
+    int64_t rope_stride;
+    int rope_rows, rotary_dim, interleaved;
+};
+enum Fp4CacheOp { kFp4Write, kFp4Prologue, kFp4Read };
+hipError_t launch_fp4_cache(int dtype, Fp4CacheOp op, const Fp4CacheArgs& a, int max_q_len, hipStream_t st);
+
 // Varlen metadata build (varlen_metadata.hip).
 struct MetadataArgs {
     const int32_t* num_computed;   // (num_seqs,)

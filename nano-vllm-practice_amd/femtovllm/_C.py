@@ -118,6 +118,19 @@ def _declare_added(lib) -> None:
         i, p, i64, i64, p, i64, i64, p, i64, i64, p, i64, i64, p, p, i64, i, i, i,
         p, p, i64, i, i, i, i, i64, i64, i64, p, i, i, i, p, p, i, i64, p,
     ]
+    lib.femto_fp4_page_bytes.restype = sz
+    lib.femto_fp4_page_bytes.argtypes = [i]
+    lib.femto_kv_cache_write_fp4.restype = i
+    lib.femto_kv_cache_write_fp4.argtypes = [
+        i, p, i64, i64, p, i64, i64, p, i64, i, i, p, i, i, i, p, p, i, i64, p,
+    ]
+    lib.femto_kv_cache_read_fp4.restype = i
+    lib.femto_kv_cache_read_fp4.argtypes = [i, p, i64, i, i, p, p, p, i, i, i, p, p, i, i64, p]
+    lib.femto_rope_cache_write_fp4.restype = i
+    lib.femto_rope_cache_write_fp4.argtypes = [
+        i, p, i64, i64, p, i64, i64, p, i64, i64, p, i64, i64, p, p, ctypes.c_double, p, p, i64, i, i, i,
+        p, i64, i, i, i, p, i, i, i, p, p, i, i64, p,
+    ]
     lib.femto_paged_attention_gemm_window_workspace_size.restype = sz
     lib.femto_paged_attention_gemm_window_workspace_size.argtypes = [i, i, i, i, i, i, i, i]
 
@@ -741,6 +754,143 @@ def _rope_cache_write(q, k, v, cos, sin, positions, k_pool, v_pool, kv_page_tabl
             positions.data_ptr(), kv_page_tables.data_ptr(), kv_page_tables.size(1),
             kv_page_tables.stride(0) if num_seqs > 1 else max(kv_page_tables.stride(0), kv_page_tables.size(1)),
             _stream(q.device),
+        )
+    _raise_on(rc)
+    return out
+
+
+def _check_fp4_pool(fn, kv_pool, head_dim, device):
+    """The pool of a 4-bit cache for heads of ``head_dim``."""
+    _check(kv_pool.is_cuda and kv_pool.device == device, f"{fn}: kv_pool must be on {device}")
+    _check(head_dim > 0 and head_dim <= kDimHead and head_dim % 16 == 0,
+           f"{fn}: head_dim must be at most {kDimHead} and a multiple of 16, got {head_dim}")
+    page = int(_lib.femto_fp4_page_bytes(head_dim))
+    _check(kv_pool.dtype == torch.uint8, f"{fn}: kv_pool must be uint8")
+    _check(kv_pool.dim() == 3 and kv_pool.size(1) > 0 and kv_pool.size(2) == page and kv_pool.is_contiguous(),
+           f"{fn}: kv_pool must be contiguous (num_blocks, n_kv_heads, {page}) for head_dim {head_dim}")
+
+
+def _check_placement(fn, positions, kv_page_tables, cu_seqlens, num_tokens, device):
+    """Positions, tables and (unless each sequence has one token) cu_seqlens of a cache write; the tables' row
+    stride (of one row: its width, whatever the tensor says) and the pointer of cu_seqlens."""
+    _check(positions.dtype == torch.int32 and positions.is_contiguous() and positions.device == device,
+           f"{fn}: positions must be a contiguous int32 tensor on {device}")
+    _check(kv_page_tables.dtype == torch.int32 and kv_page_tables.dim() == 2 and kv_page_tables.device == device
+           and (kv_page_tables.size(1) <= 1 or kv_page_tables.stride(1) == 1),
+           f"{fn}: kv_page_tables must be 2-D row-major int32 on {device}")
+    num_seqs = kv_page_tables.size(0)
+    _check(positions.numel() == num_tokens, f"{fn}: positions.numel() must equal the number of tokens")
+    stride = kv_page_tables.stride(0) if num_seqs > 1 else max(kv_page_tables.stride(0), kv_page_tables.size(1))
+    if cu_seqlens is None:
+        _check(num_tokens == num_seqs, f"{fn}: without cu_seqlens every sequence has one token")
+        return stride, None
+    _check(cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and cu_seqlens.device == device,
+           f"{fn}: cu_seqlens must be a contiguous int32 tensor on {device}")
+    _check(cu_seqlens.numel() - 1 == num_seqs, f"{fn}: cu_seqlens.numel()-1 must equal kv_page_tables.size(0)")
+    return stride, cu_seqlens.data_ptr()
+
+
+def _check_kv_source(fn, k, v, kv_pool):
+    _check(k.dim() == 3 and v.dim() == 3 and tuple(k.shape) == tuple(v.shape),
+           f"{fn}: k and v must be 3-D (tokens, n_kv_heads, head_dim) of one shape")
+    _check(k.is_cuda and v.device == k.device, f"{fn}: k and v must be on one GPU")
+    _check(k.stride(-1) == 1 and v.stride(-1) == 1, f"{fn}: k and v must be contiguous in head_dim")
+    _check(k.dtype == v.dtype, f"{fn}: k and v must share a dtype")
+    _check_fp4_pool(fn, kv_pool, k.size(2), k.device)
+    _check(k.size(1) == kv_pool.size(1), f"{fn}: k heads differ from the pool's")
+    _check(k.dtype != torch.float32, f'"{fn}" not implemented for \'Float\'')
+    return _dtype_code(k, fn)
+
+
+def _kv_cache_write_fp4(k, v, kv_pool, positions, kv_page_tables, cu_seqlens=None, max_q_len=1):
+    """Round k, v (tokens, n_kv_heads, head_dim) to 4 bits, into the paged pool in place."""
+    fn = "kv_cache_write_fp4"
+    dtype = _check_kv_source(fn, k, v, kv_pool)
+    stride, cu_ptr = _check_placement(fn, positions, kv_page_tables, cu_seqlens, k.size(0), k.device)
+    max_q_len = _int32_arg(fn, "max_q_len", max_q_len)
+    if k.size(0) == 0 or kv_page_tables.size(0) == 0:
+        return
+    with torch.cuda.device(k.device):
+        rc = _lib.femto_kv_cache_write_fp4(
+            dtype,
+            k.data_ptr(), k.stride(0), k.stride(1),
+            v.data_ptr(), v.stride(0), v.stride(1),
+            kv_pool.data_ptr(), kv_pool.size(0), kv_pool.size(1), k.size(2),
+            cu_ptr, kv_page_tables.size(0), k.size(0), max_q_len,
+            positions.data_ptr(), kv_page_tables.data_ptr(), kv_page_tables.size(1), stride, _stream(k.device),
+        )
+    _raise_on(rc)
+
+
+def _kv_cache_read_fp4(kv_pool, head_dim, dtype, positions, kv_page_tables, cu_seqlens=None, max_q_len=1):
+    """(k, v) of the tokens, (tokens, n_kv_heads, head_dim) of ``dtype``."""
+    fn = "kv_cache_read_fp4"
+    head_dim = operator.index(head_dim)
+    _check_fp4_pool(fn, kv_pool, head_dim, kv_pool.device)
+    _check(dtype in (torch.bfloat16, torch.float16), f"{fn}: dtype must be bfloat16 or float16, got {dtype}")
+    tokens = positions.numel()
+    stride, cu_ptr = _check_placement(fn, positions, kv_page_tables, cu_seqlens, tokens, kv_pool.device)
+    max_q_len = _int32_arg(fn, "max_q_len", max_q_len)
+    with torch.cuda.device(kv_pool.device):
+        k, v = (torch.empty((tokens, kv_pool.size(1), head_dim), dtype=dtype, device=kv_pool.device) for _ in range(2))
+        if tokens == 0 or kv_page_tables.size(0) == 0:
+            return k, v
+        rc = _lib.femto_kv_cache_read_fp4(
+            _DTYPE[dtype], kv_pool.data_ptr(), kv_pool.size(0), kv_pool.size(1), head_dim, k.data_ptr(), v.data_ptr(),
+            cu_ptr, kv_page_tables.size(0), tokens, max_q_len,
+            positions.data_ptr(), kv_page_tables.data_ptr(), kv_page_tables.size(1), stride, _stream(kv_pool.device),
+        )
+    _raise_on(rc)
+    return k, v
+
+
+def _rope_cache_write_fp4(q, k, v, cos, sin, positions, kv_pool, kv_page_tables, cu_seqlens=None, max_q_len=1,
+                          interleaved=False, q_weight=None, k_weight=None, eps=1e-6, out=None):
+    """Normed (with weights) and rotated q to ``out``, rotated k and v in 4 bits into the pool; returns ``out``."""
+    fn = "rope_cache_write_fp4"
+    dtype = _check_kv_source(fn, k, v, kv_pool)
+    for name, t in (("q", q), ("cos", cos), ("sin", sin)):
+        _check(t.device == k.device, f"{fn}: {name} must be on {k.device}")
+    _check(q.dim() == 3 and q.size(0) == k.size(0) and q.size(2) == k.size(2) and q.size(1) > 0,
+           f"{fn}: q must be 3-D (tokens, heads, head_dim) like k and v")
+    _check(q.stride(-1) == 1, f"{fn}: q must be contiguous in head_dim")
+    _check(q.dtype == k.dtype, f"{fn}: q, k and v must share a dtype")
+    _check(cos.dtype == torch.float32 and sin.dtype == torch.float32, f"{fn}: cos / sin tables must be float32")
+    _check(cos.dim() == 2 and tuple(cos.shape) == tuple(sin.shape) and cos.stride() == sin.stride()
+           and (cos.size(1) <= 1 or cos.stride(1) == 1), f"{fn}: cos / sin must be (rows, rotary_dim / 2) row-major alike")
+    _check((q_weight is None) == (k_weight is None), f"{fn}: q_norm_weight and k_norm_weight are given both or not at all")
+    for name, t in (("q_norm_weight", q_weight), ("k_norm_weight", k_weight)):
+        _check(t is None or (t.device == q.device and t.dtype == q.dtype and t.is_contiguous()
+                             and tuple(t.shape) == (q.size(2),)),
+               f"{fn}: {name} must be a contiguous ({q.size(2)},) tensor of q's dtype on {q.device}")
+    stride, cu_ptr = _check_placement(fn, positions, kv_page_tables, cu_seqlens, k.size(0), k.device)
+    max_q_len = _int32_arg(fn, "max_q_len", max_q_len)
+    if out is not None:
+        _check(tuple(out.shape) == tuple(q.shape) and out.dtype == q.dtype and out.stride(-1) == 1 and out.device == q.device,
+               f"{fn}: out must match q")
+        _check(not _rows_meet(out), f"{fn}: rows of out share memory")
+        in_place = out.data_ptr() == q.data_ptr() and out.stride() == q.stride()
+        # (k and v, too, where out is q: a token's k would be read after its q was written)
+        _check(in_place or not _share_elements(out, q), f"{fn}: out must be q itself or share no memory with q")
+        for name, t in (("k", k), ("v", v)):
+            _check(not _share_elements(out, t), f"{fn}: out must share no memory with {name}")
+    with torch.cuda.device(q.device):
+        if out is None:
+            out = torch.empty_like(q)
+        if q.size(0) == 0 or kv_page_tables.size(0) == 0:
+            return out
+        rc = _lib.femto_rope_cache_write_fp4(
+            dtype,
+            q.data_ptr(), q.stride(0), q.stride(1),
+            k.data_ptr(), k.stride(0), k.stride(1),
+            v.data_ptr(), v.stride(0), v.stride(1),
+            out.data_ptr(), out.stride(0), out.stride(1),
+            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), float(eps),
+            cos.data_ptr(), sin.data_ptr(), cos.stride(0) if cos.size(0) > 1 else max(cos.stride(0), cos.size(1)),
+            cos.size(0), 2 * cos.size(1), int(bool(interleaved)),
+            kv_pool.data_ptr(), kv_pool.size(0), q.size(1), kv_pool.size(1), q.size(2),
+            cu_ptr, kv_page_tables.size(0), q.size(0), max_q_len,
+            positions.data_ptr(), kv_page_tables.data_ptr(), kv_page_tables.size(1), stride, _stream(q.device),
         )
     _raise_on(rc)
     return out

@@ -26,6 +26,11 @@ visible; the reference has no windowed attention.
 prefix, which the reference reads once per sequence.  ``rope_cache_write`` is
 the prologue of layers without q/k norms, for every rotary layout.
 
+The operators whose names end in ``_fp4`` work on a KV cache held in 4 bits
+(:mod:`femtovllm.fp4`): the write of new tokens, the prologue with norms and
+rotation, a read of tokens, and both attention operators.  The reference's
+cache is 16 bits wide.
+
 One deliberate difference: ``q`` arrives as ``q.transpose(0, 1)`` of a
 ``(tokens, n_heads, head_dim)`` tensor (femtovllm/models/qwen/qwen3.py:270,
 372).  The reference copies it with ``.contiguous()``; the HIP kernels take
@@ -325,3 +330,84 @@ def rope_cache_write(
             raise ValueError(f"Argument '{name}' must be a CUDA tensor. Got device={t.device}")
     return _hip_backend._rope_cache_write(q, k, v, cos, sin, positions, k_cache_pool, v_cache_pool, kv_page_tables,
                                           cu_seqlens, max_q_len, interleaved, out)
+
+
+def kv_cache_write_fp4(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    kv_pool: torch.Tensor,
+    positions: torch.Tensor,
+    kv_page_tables: torch.Tensor,
+    cu_seqlens: torch.Tensor = None,
+    max_q_len: int = 1,
+):
+    """:func:`kv_cache_write` into a cache held in 4 bits (in place).
+
+    ``kv_pool`` is a pool of :func:`femtovllm.fp4.new_pool`; k and v (bf16 or
+    f16, head_dim a multiple of 16 up to 128), ``positions``, the tables and
+    ``cu_seqlens`` are those of :func:`kv_cache_write`.  Each 32 dims of a row are
+    rounded to the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} times their scale, the
+    smallest power of two of which no magnitude is more than 7 (from 2^-119 to 2^125);
+    32 dims that hold an infinity or a NaN become NaN.  ``max_q_len`` only sizes
+    the launch: longer sequences are written whole.
+    """
+    for name, t in (("k", k), ("v", v)):
+        if not t.is_cuda:
+            raise ValueError(f"Argument '{name}' must be a CUDA tensor. Got device={t.device}")
+    k = k if k.stride(-1) == 1 else k.contiguous()
+    v = v if v.stride(-1) == 1 else v.contiguous()
+    _hip_backend._kv_cache_write_fp4(k, v, kv_pool, positions, kv_page_tables, cu_seqlens, max_q_len)
+
+
+def kv_cache_read_fp4(
+    kv_pool: torch.Tensor,
+    head_dim: int,
+    dtype: torch.dtype,
+    positions: torch.Tensor,
+    kv_page_tables: torch.Tensor,
+    cu_seqlens: torch.Tensor = None,
+    max_q_len: int = 1,
+):
+    """(k, v), each (num_tokens, n_kv_heads, head_dim) of ``dtype`` (bf16 or f16), of tokens in a 4-bit cache.
+
+    The tokens are those that :func:`kv_cache_write_fp4` would write with the
+    same arguments, e.g. a whole prefix that moves to 16-bit pools; zeros where
+    that would have stopped.  bf16 holds every value exactly; f16 rounds, and
+    values past its range are infinities.
+    """
+    if not kv_pool.is_cuda:
+        raise ValueError(f"Argument 'kv_pool' must be a CUDA tensor. Got device={kv_pool.device}")
+    return _hip_backend._kv_cache_read_fp4(kv_pool, head_dim, dtype, positions, kv_page_tables, cu_seqlens, max_q_len)
+
+
+def rope_cache_write_fp4(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    positions: torch.Tensor,
+    kv_pool: torch.Tensor,
+    kv_page_tables: torch.Tensor,
+    cu_seqlens: torch.Tensor = None,
+    max_q_len: int = 1,
+    interleaved: bool = False,
+    q_norm_weight: torch.Tensor = None,
+    k_norm_weight: torch.Tensor = None,
+    eps: float = 1e-6,
+    out: torch.Tensor = None,
+):
+    """The attention layer's prologue over a 4-bit cache in one kernel; returns the rotated q.
+
+    :func:`rope_cache_write` (same layouts, tables, positions and rules for
+    ``out``) with k and v rounded to 4 bits as :func:`kv_cache_write_fp4` does.
+    With ``q_norm_weight`` and ``k_norm_weight`` ((head_dim,) of q's dtype, both or
+    neither) and ``eps``, q and k first pass the layer's RMSNorms, as in
+    :func:`qk_norm_rope_cache_write`.  bf16 or f16.  k is rounded once, from
+    float32.
+    """
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not t.is_cuda:
+            raise ValueError(f"Argument '{name}' must be a CUDA tensor. Got device={t.device}")
+    return _hip_backend._rope_cache_write_fp4(q, k, v, cos, sin, positions, kv_pool, kv_page_tables, cu_seqlens,
+                                              max_q_len, interleaved, q_norm_weight, k_norm_weight, eps, out)
