@@ -411,6 +411,27 @@ int femto_rope_cache_write_fp4(
     const int32_t* positions, const int32_t* kv_page_tables, int num_pages_per_seq, int64_t table_stride,
     void* stream);
 
+/* femto_paged_attention_gemv over a 4-bit cache: sequence b's query sees the
+ * keys j < kv_lens[b], of any number.  A block id outside the pool, or a column
+ * past the table, reads as zeros; kv_len == 0 yields a zero row.  Rows of the last
+ * page past kv_len may hold anything.  P rounds to q's type for the second
+ * product, everything else is 32-bit or exact but q, which is taken to 2^-14 of
+ * the largest magnitude of its 32 dims.  The workspace (256-byte aligned;
+ * workspace_size 0: none; it is that of the current device) has to be zero in
+ * its first femto_paged_attention_gemv_fp4_zero_bytes() bytes before its first
+ * use and is left so; calls that may overlap must not share one. */
+int femto_paged_attention_gemv_fp4(
+    int dtype,
+    const void* q, int64_t q_stride_head, int64_t q_stride_seq,
+    void* out, int64_t out_stride_head, int64_t out_stride_seq,
+    const void* kv_pool, int64_t num_blocks, int n_kv_heads, int head_dim,
+    const int32_t* kv_page_tables, int num_pages_per_seq, int64_t table_stride,
+    const int32_t* kv_lens, int num_seqs, int n_heads, int max_kv_len,
+    void* workspace, size_t workspace_bytes,
+    void* stream);
+size_t femto_paged_attention_gemv_fp4_workspace_size(int num_seqs, int n_heads, int n_kv_heads, int max_kv_len);
+size_t femto_paged_attention_gemv_fp4_zero_bytes(void);
+
 /* Varlen attention metadata built on the device, by the rules of the
  * reference's ModelRunner (femtovllm/engine/model_runner.py:187-202 prefill,
  * 283-293 decode, 46-72 block-table padding), which builds them with Python

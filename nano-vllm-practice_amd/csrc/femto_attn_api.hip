@@ -659,6 +659,42 @@ static int fp4_source(const std::string& f, const void* k, int64_t k_stride_toke
     return FEMTO_OK;
 }
 
+// Workgroups per row and waves in each of a decode call over a 4-bit cache, and
+// its workspace: counters, then the parts' states; none where every row is one part.
+struct Fp4DecodePlan {
+    WindowParts rows;
+    size_t bytes;
+};
+static Fp4DecodePlan fp4_decode_plan(int num_seqs, int n_heads, int n_kv_heads, int max_kv_len, int cus) {
+    Fp4DecodePlan p;
+    p.rows = window_parts(num_seqs, n_heads, n_kv_heads, max_kv_len, cus);
+    p.bytes = p.rows.parts > 1 ? kWindowZeroBytes + femto::decode_workspace_bytes(num_seqs, n_heads, p.rows.parts) : 0;
+    return p;
+}
+
+// Checks that attention calls over a 4-bit cache share.
+static int check_fp4_attention(const std::string& f, int dtype, const void* q, int64_t q_s0, int64_t q_s1, const void* out,
+                               const void* kv_pool, int64_t num_blocks, int n_kv_heads, int head_dim, int n_heads,
+                               const int32_t* tables, int num_pages_per_seq, int64_t table_stride) {
+    if (dtype != FEMTO_F16 && dtype != FEMTO_BF16)
+        return fail(FEMTO_ERR_UNSUPPORTED, f + ": not implemented for '" + dtype_name(dtype) + "' (bf16 / f16 only)");
+    if (head_dim <= 0 || head_dim > femto::kDimHead || head_dim % 16 != 0)
+        return fail(FEMTO_ERR_UNSUPPORTED, f + ": head_dim must be at most " + std::to_string(femto::kDimHead) +
+                                               " and a multiple of 16, got " + std::to_string(head_dim));
+    if (n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads != 0)
+        return fail(FEMTO_ERR_INVALID, f + ": n_heads (" + std::to_string(n_heads) +
+                                           ") must be a positive multiple of n_kv_heads (" +
+                                           std::to_string(n_kv_heads) + ")");
+    if (num_blocks < 1 || num_pages_per_seq < 0 || table_stride < 0)
+        return fail(FEMTO_ERR_INVALID, f + ": the pool needs at least one block and table sizes must be >= 0");
+    if (!q || !out || !kv_pool || (num_pages_per_seq > 0 && !tables))
+        return fail(FEMTO_ERR_INVALID, f + ": null pointer argument");
+    if (!aligned(q, 16) || !aligned(kv_pool, 16) || !aligned(out, 8))
+        return fail(FEMTO_ERR_INVALID, f + ": q and kv_pool must be 16-byte aligned, out 8-byte aligned");
+    if (q_s0 % 8 || q_s1 % 8) return fail(FEMTO_ERR_INVALID, f + ": q strides must be multiples of 16 bytes");
+    return FEMTO_OK;
+}
+
 extern "C" {
 
 const char* femto_attn_last_error(void) { return g_err.c_str(); }
@@ -1237,6 +1273,49 @@ int femto_rope_cache_write_fp4(int dtype, const void* q, int64_t q_stride_token,
                                               cu_seqlens ? std::min(max_q_len, num_tokens) : 1,
                                               static_cast<hipStream_t>(stream)),
                       "rope_cache_write_fp4 launch");
+}
+
+size_t femto_paged_attention_gemv_fp4_workspace_size(int num_seqs, int n_heads, int n_kv_heads, int max_kv_len) {
+    if (num_seqs <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || max_kv_len < 0) return 0;
+    int cus = 0;
+    if (femto::device_cu_count(cus) != hipSuccess) return 0;
+    return fp4_decode_plan(num_seqs, n_heads, n_kv_heads, max_kv_len, cus).bytes;
+}
+
+size_t femto_paged_attention_gemv_fp4_zero_bytes(void) { return kWindowZeroBytes; }
+
+int femto_paged_attention_gemv_fp4(int dtype, const void* q, int64_t q_stride_head, int64_t q_stride_seq, void* out,
+                                   int64_t out_stride_head, int64_t out_stride_seq, const void* kv_pool, int64_t num_blocks,
+                                   int n_kv_heads, int head_dim, const int32_t* kv_page_tables, int num_pages_per_seq,
+                                   int64_t table_stride, const int32_t* kv_lens, int num_seqs, int n_heads, int max_kv_len,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+    g_err.clear();
+    const std::string fn = "paged_attention_gemv_fp4";
+    if (num_seqs < 0 || max_kv_len < 0) return fail(FEMTO_ERR_INVALID, fn + ": negative size");
+    if (num_seqs == 0) return FEMTO_OK;
+    int rc = check_fp4_attention(fn, dtype, q, q_stride_head, q_stride_seq, out, kv_pool, num_blocks, n_kv_heads, head_dim,
+                                 n_heads, kv_page_tables, num_pages_per_seq, table_stride);
+    if (rc != FEMTO_OK) return rc;
+    if (!kv_lens) return fail(FEMTO_ERR_INVALID, fn + ": null kv_lens");
+    int cus = 0;
+    rc = hip_status(femto::device_cu_count(cus), (fn + ": device query").c_str());
+    if (rc != FEMTO_OK) return rc;
+    const Fp4DecodePlan w = fp4_decode_plan(num_seqs, n_heads, n_kv_heads, max_kv_len, cus);
+    if (w.bytes && (!workspace || workspace_bytes < w.bytes || !aligned(workspace, 256)))
+        return fail(FEMTO_ERR_INVALID, fn + ": workspace of " + std::to_string(w.bytes) +
+                                           " bytes (256-byte aligned) required, got " + std::to_string(workspace_bytes));
+    const int page = femto::fp4_page_bytes(head_dim);
+    femto::DecodePlan plan{};
+    plan.nrep_tile = 1;
+    plan.max_slots = w.rows.parts;
+    femto::DecodeArgs a = femto::decode_args(
+        plan, q, q_stride_head, q_stride_seq, out, out_stride_head, out_stride_seq, kv_pool, nullptr, num_blocks, n_kv_heads,
+        head_dim, (int64_t)n_kv_heads * page, page, 0, kv_page_tables, num_pages_per_seq, table_stride, kv_lens, num_seqs,
+        n_heads, w.bytes ? static_cast<char*>(workspace) + kWindowZeroBytes : nullptr);
+    a.merge_counters = w.bytes ? static_cast<int*>(workspace) : nullptr;
+    a.parts = w.rows.parts;
+    a.single_waves = w.rows.waves;
+    return hip_status(femto::launch_fp4_decode(dtype, a, num_seqs, static_cast<hipStream_t>(stream)), (fn + " launch").c_str());
 }
 
 int femto_build_varlen_metadata(int num_seqs, const int32_t* num_computed, const int32_t* num_tokens,

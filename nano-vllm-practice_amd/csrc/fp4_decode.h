@@ -1,0 +1,295 @@
+// Decode over a KV cache held in 4 bits (layout: fp4.h): one query token per
+// sequence, for decode calls (fp4_decode.hip) and the decode rows of a prefill
+// call.
+//
+// Formula: out[h] = sum_j w_j v_j / sum_j w_j, w_j = exp(q[h] . k_j / sqrt(D)), over
+// the keys j < kv_len, as paged_decode.hip; k and v are the values that the cache
+// stands for.
+//
+// As in mfma_decode.h up to 16 query heads of a KV head are the columns of two
+// matrix products, here over two pages (32 keys) at a time:
+//   S^T (16 keys x 16 heads) = K . Q^T, v_mfma_scale_f32_16x16x128, K straight from
+//     memory: the lane of key r and block b holds 32 4-bit dims and their scale,
+//     which is the operand that the instruction takes.
+//   O^T (128 dims x 16 heads) += V^T . P^T, 8 x v_mfma_f32_16x16x32.
+// The first product reads K without converting it.  Its other operand may have
+// 6 bits at the same rate (8 bits halve it): q is split into three terms of 6 bits,
+// each with a scale for 32 dims, which leave out at most 2^-14 of the largest of
+// those dims (fp4_query), a quarter of f16's rounding there; products are exact
+// and sums 32-bit.
+// V is wanted by dims, its values convert to 16 bits two dims at a time
+// (v_cvt_scalef32_pk, exact in bf16), and a permute per two values pairs keys: a
+// 16-byte load holds 8 dims of four keys, so no V passes through LDS.  Row 4 g + i
+// of the O^T tile dt is dim 8 (4 g + i) + dt.
+// P rounds to q's type, and the row sum adds the rounded P.
+#pragma once
+
+#include "fp4.h"
+#include "lds_copy.h"
+#include "mfma_decode.h"
+
+namespace femto {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
+typedef float f32x32 __attribute__((ext_vector_type(32)));
+
+constexpr int kFp4Terms = 3;
+constexpr int kFormatFp6 = 2, kFormatFp4 = 4;  // operand formats of the scaled matrix instructions
+
+// 32 dims of a query as kFp4Terms terms of 6 bits (a sign, 0 to 7.5); byte i of
+// `scales` is the scale byte of term i.
+struct Fp4Query {
+    u32x6 term[kFp4Terms];
+    uint32_t scales;
+};
+
+// x: dims 0 .. 31.  With the first scale s no |x / s| is past 7.75, so the first
+// term leaves at most s / 4; of the second's scale, s / 16, that is at most 4, and at
+// most an eighth of it is left; of the third's, s / 512, again at most 4 and an
+// eighth: 2^-12 s, and the largest magnitude is above 3.875 s.  A block with an
+// infinity or a NaN has NaN scales: its scores are NaN.
+__device__ __forceinline__ Fp4Query fp4_query(const float (&x)[32]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    const int byte = top >= 0x7f800000u ? kFp4NanScale : max(10, (int)((top + 0x7ffffu) >> 23) - 2);
+    constexpr int kDown[kFp4Terms] = {0, 4, 9};
+    Fp4Query q;
+    q.scales = 0;
+    f32x16 even, odd;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        even[i] = x[2 * i];
+        odd[i] = x[2 * i + 1];
+    }
+#pragma unroll
+    for (int t = 0; t < kFp4Terms; ++t) {
+        const int b = byte == kFp4NanScale ? byte : byte - kDown[t];
+        const float s = fp4_scale(byte == kFp4NanScale ? 127 : b);
+        q.scales |= (uint32_t)b << (8 * t);
+        q.term[t] = __builtin_bit_cast(u32x6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, s));
+        if (t + 1 < kFp4Terms) {
+            const f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(
+                __builtin_bit_cast(decltype(__builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, s)), q.term[t]), s);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                even[i] -= back[2 * i];
+                odd[i] -= back[2 * i + 1];
+            }
+        }
+    }
+    return q;
+}
+
+// The same of dims 32 b .. of a row of 16-bit values; dims from D on are zeros.
+template <typename E>
+__device__ __forceinline__ Fp4Query fp4_query_row(const char* row, int b, int D, bool valid) {
+    float x[32];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int d = 32 * b + 8 * i;
+        const u32x4 w = valid && d < D ? ld16(row + 2 * d) : u32x4{0, 0, 0, 0};
+        unpack8(E{}, w, *reinterpret_cast<float(*)[8]>(x + 8 * i));
+    }
+    return fp4_query(x);
+}
+
+__device__ __forceinline__ i32x8 fp4_operand(u32x4 w) {
+    return i32x8{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+}
+__device__ __forceinline__ i32x8 fp4_operand(u32x6 w) {
+    return i32x8{(int)w[0], (int)w[1], (int)w[2], (int)w[3], (int)w[4], (int)w[5], 0, 0};
+}
+// c + K . q over 128 dims: K's 16 keys x 4 blocks with the scale in byte 0 of ks;
+// the smallest term first.
+__device__ __forceinline__ f32x4 fp4_scores16(u32x4 k, uint32_t ks, const Fp4Query& q) {
+    f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(k), fp4_operand(q.term[2]), c, kFormatFp4, kFormatFp6,
+                                                         0, (int)ks, 2, (int)q.scales);
+    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(k), fp4_operand(q.term[1]), c, kFormatFp4, kFormatFp6,
+                                                         0, (int)ks, 1, (int)q.scales);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(k), fp4_operand(q.term[0]), c, kFormatFp4,
+                                                            kFormatFp6, 0, (int)ks, 0, (int)q.scales);
+}
+
+// A page in registers: the lane of key (or dims) c = lane % 16 and block (or four
+// keys) g = lane / 16.
+struct Fp4Page {
+    u32x4 k, v;       // dims 32 g .. of key c; dims 8 c .. of keys 4 g ..
+    uint32_t ks, vs;  // scale of k; of v's four keys, a byte each
+};
+
+// Heads h0 .. h0 + nh - 1 of sequence b over pages [lp0, lp0 + n) of its kv_len
+// keys.  FULL: head_dim 128.  Else lanes of dims past the row's blocks read block
+// 0 (q is zero there, and those output dims are not stored).
+template <typename E, bool FULL, int STAGES>
+__device__ __forceinline__ void fp4_segment(const DecodeArgs& a, int b, int kv_len, int lp0, int n, int qrow, int h0, int nh,
+                                            int kvh, HeadState& s) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int D = FULL ? kDimHead : a.head_dim, N = fp4_blocks(D);
+    s.clear();
+    const Fp4Query q = fp4_query_row<E>(static_cast<const char*>(a.q) + ((int64_t)(h0 + c) * a.q_stride_head + (int64_t)qrow * a.q_stride_seq) * 2,
+                                        g, D, c < nh);
+    const int kb = FULL || g < N ? g : 0, vc = FULL || c < 4 * N ? c : 0;
+    const uint32_t k_at = 256 * kb + 16 * c, v_at = 256 * N + 64 * N * g + 16 * vc;
+    const uint32_t ks_at = 512 * N + 4 * c + kb, vs_at = 512 * N + 64 + 16 * g + 4 * (vc >> 2);
+    const uint8_t* pool = static_cast<const uint8_t*>(a.k_pool) + (int64_t)kvh * a.pool_stride_head;
+    const uint8_t* zero = reinterpret_cast<const uint8_t*>(g_zero_page);
+    const int32_t* table = a.tables + (int64_t)b * a.table_stride;
+    int tbl = -1;
+    // Every page's loads go out, whether it is there or not (past the segment and
+    // for a block outside the pool those of a page of zeros): the waits
+    // count them.
+    auto issue = [&](int i, Fp4Page& p) __attribute__((always_inline)) {
+        if ((i & 63) == 0) {
+            const int pg = lp0 + i + lane;
+            tbl = i + lane < n && pg < a.num_pages_per_seq ? table[pg] : -1;
+            asm volatile("" : "+v"(tbl));  // waited for here, once per 64 pages
+        }
+        const int blk = __builtin_amdgcn_readlane(tbl, i & 63);
+        const bool ok = blk >= 0 && (int64_t)blk < a.num_blocks;
+        const uint8_t* page = ok ? pool + (int64_t)blk * a.pool_stride_block : zero;
+        p.k = ld16_nt(page + k_at);
+        p.v = ld16_nt(page + v_at);
+        p.ks = __builtin_nontemporal_load(page + ks_at);
+        p.vs = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(page + vs_at));
+    };
+    const float scale = a.scale_log2;
+    auto consume = [&](int i, Fp4Page (&p)[2]) __attribute__((always_inline)) {
+        float sc[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const f32x4 x = fp4_scores16(p[h].k, p[h].ks, q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[4 * h + j] = x[j];
+        }
+        // Keys past the segment or the context: no weight, and V of zeros (0
+        // times a NaN would not be 0).
+        const int key0 = (lp0 + i) * kPage, end = min(kv_len, (lp0 + n) * kPage);
+        if (key0 + 2 * kPage > end) {  // wave-uniform
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const int h = x >> 2, j = x & 3;
+                const bool seen = key0 + kPage * h + 4 * g + j < end;
+                sc[x] = seen ? sc[x] : -INFINITY;
+                p[h].v[j] = seen ? p[h].v[j] : 0;
+                p[h].vs = seen ? p[h].vs : p[h].vs & ~(0xffu << (8 * j));
+            }
+        }
+        float mx = fmaxf(sc[0], sc[1]);
+#pragma unroll
+        for (int x = 2; x < 8; ++x) mx = fmaxf(mx, sc[x]);
+        mx *= scale;
+        if (__ballot(mx > s.m + kLazyMax)) {
+            const float mn = fmaxf(s.m, head_max(mx));
+            const float al = fast_exp2(s.m - mn);
+            s.l *= al;
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) s.o[dt] *= al;
+            s.m = mn;
+        }
+        u32x4 pw;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            pw[x] = pack2(E{}, fast_exp2(fmaf(sc[2 * x], scale, -s.m)), fast_exp2(fmaf(sc[2 * x + 1], scale, -s.m)));
+            s.l = sum2(E{}, pw[x], s.l);
+        }
+        float vsc[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t w = p[h].vs;
+            vsc[4 * h] = __uint_as_float((w << 23) & 0x7f800000u);
+            vsc[4 * h + 1] = __uint_as_float((w << 15) & 0x7f800000u);
+            vsc[4 * h + 2] = __uint_as_float((w << 7) & 0x7f800000u);
+            vsc[4 * h + 3] = __uint_as_float((w >> 1) & 0x7f800000u);
+        }
+        auto dims = [&](auto pair) __attribute__((always_inline)) {  // 2 pair and 2 pair + 1 of the lane's 8
+            constexpr int I = decltype(pair)::value;
+            uint32_t w[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) w[x] = fp4_pair<I>(E{}, p[x >> 2].v[x & 3], vsc[x]);
+            u32x4 lo, hi;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                lo[x] = __builtin_amdgcn_perm(w[2 * x + 1], w[2 * x], 0x05040100u);
+                hi[x] = __builtin_amdgcn_perm(w[2 * x + 1], w[2 * x], 0x07060302u);
+            }
+            s.o[2 * I] = mfma16x16x32(E{}, lo, pw, s.o[2 * I]);
+            s.o[2 * I + 1] = mfma16x16x32(E{}, hi, pw, s.o[2 * I + 1]);
+        };
+        dims(std::integral_constant<int, 0>{});
+        dims(std::integral_constant<int, 1>{});
+        dims(std::integral_constant<int, 2>{});
+        dims(std::integral_constant<int, 3>{});
+    };
+
+    // STAGES - 1 pairs of pages are on their way during a pair's math.
+    Fp4Page p[STAGES][2];
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+        issue(2 * i, p[i][0]);
+        issue(2 * i + 1, p[i][1]);
+    }
+    for (int i0 = 0; i0 < n; i0 += 2 * STAGES) {
+#pragma unroll
+        for (int x = 0; x < STAGES; ++x) {
+            const int i = i0 + 2 * x;
+            if (i >= n) break;
+            const int next = i + 2 * (STAGES - 1);
+            issue(next, p[(x + STAGES - 1) % STAGES][0]);
+            issue(next + 1, p[(x + STAGES - 1) % STAGES][1]);
+            consume(i, p[x]);
+        }
+    }
+    s.l = head_sum(s.l);
+}
+
+// The lane's share of head c's outputs: dims 32 g + 8 i + dt, o[dt][i].
+__device__ __forceinline__ void fp4_put_outputs(float* row, int g, const HeadState& s) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        *reinterpret_cast<f32x4*>(row + 32 * g + 8 * i) = f32x4{s.o[0][i], s.o[1][i], s.o[2][i], s.o[3][i]};
+        *reinterpret_cast<f32x4*>(row + 32 * g + 8 * i + 4) = f32x4{s.o[4][i], s.o[5][i], s.o[6][i], s.o[7][i]};
+    }
+}
+
+// Workgroup `block` of W waves takes part (block % a.parts) of the pages of one
+// sequence for one KV head group's query heads, wave w the w-th of W contiguous
+// shares of it; finish_row (mfma_decode.h) folds the waves' states and writes the
+// row.  lds: W * kFp4WaveLds bytes, s_ml: [W][kMfmaHeads][2].
+constexpr int kFp4WaveLds = kMfmaHeads * kDimHead * 4;
+template <typename E, bool FULL, int W, int STAGES>
+__device__ __forceinline__ void fp4_row(const DecodeArgs& a, int block, uint8_t* lds, float (*s_ml)[kMfmaHeads][2], int* s_old) {
+    const int P = a.parts;
+    const int part = block % P, bg = block / P;
+    const int b = bg / a.grid_heads, grp = bg - b * a.grid_heads;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kvh = grp / a.head_groups, hg = grp - kvh * a.head_groups;
+    const int h0 = kvh * a.n_rep + hg * a.heads_per_wave;
+    const int nh = min(a.heads_per_wave, a.n_rep - hg * a.heads_per_wave);
+    int row, kv_len, start;
+    if (b >= a.num_seqs || !decode_row_of<kAllPages>(a, b, row, kv_len, start)) return;  // a chunk's tiles
+    const int npg = pages_of(kv_len);
+    const int per_part = (npg + P - 1) / P;
+    const int first = part * per_part, mine = min(npg - first, per_part);
+    const int parts = npg > 0 ? (npg + per_part - 1) / per_part : 1;  // with pages
+    if (part >= parts) return;
+    const int per = (mine + W - 1) / W;
+    const int lp0 = min(mine, wave * per), n = min(mine, lp0 + per) - lp0;
+    HeadState s;
+    if (n > 0) fp4_segment<E, FULL, STAGES>(a, b, kv_len, first + lp0, n, row, h0, nh, kvh, s);
+    else s.clear();
+    if (c < nh) {
+        fp4_put_outputs(reinterpret_cast<float*>(lds + wave * kFp4WaveLds) + c * kDimHead, g, s);
+        if (g == 0) {
+            s_ml[wave][c][0] = s.m;
+            s_ml[wave][c][1] = s.l;
+        }
+    }
+    __syncthreads();
+    finish_row<E, FULL, W, kFp4WaveLds>(a, b, bg, h0, nh, row, npg, part, parts, lds, s_ml, s_old);
+}
+
+}  // namespace femto

@@ -83,6 +83,11 @@ hipError_t launch_paged_decode_merge(int dtype, const DecodeArgs& a, int num_seq
 hipError_t launch_window_decode(int dtype, const DecodeArgs& a, int nrep_tile, int num_seqs, bool single,
                                 hipStream_t st);
 
+// Over a KV cache held in 4 bits (fp4_decode.hip; bf16 and f16 q): one launch of
+// a.parts workgroups of a.single_waves waves per (sequence, KV head group).  The
+// pool is a.k_pool, its block and head strides in bytes.
+hipError_t launch_fp4_decode(int dtype, DecodeArgs a, int num_seqs, hipStream_t st);
+
 struct PrefillArgs {
     const void* q;
     int64_t q_stride_batch, q_stride_head, q_stride_token;

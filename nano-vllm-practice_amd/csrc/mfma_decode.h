@@ -241,55 +241,17 @@ __device__ __forceinline__ void store_partial(const DecodeArgs& a, int64_t sl, i
     if (g == 0) *reinterpret_cast<float2*>(a.part_ml + sl * 2) = make_float2(s.m, s.l);
 }
 
-// Window rows: workgroup `block` of W waves takes part (block % a.parts) of the
-// pages that one KV head group's query heads of one sequence see; wave w the
-// w-th of W contiguous shares of it.  The waves fold their states through LDS
-// (each over its own, done, pages).  A sequence in one part is written at once.
+// What a row's workgroup (W waves) does once its waves' states are in LDS: wave
+// w's outputs of head r at lds + w WAVE_LDS + 512 r, m and l in s_ml.  A sequence
+// in one part is written at once.
 // Else the part's state goes to its slot with system-scope stores (written
 // through to memory) and the workgroup counts itself in; the one that comes
 // last reads all slots (system-scope loads, in part order: the result does not
 // depend on who was last), writes the rows and leaves the counter zero.
-// lds: W * kWorkerLds<STAGES> bytes, s_ml: [W][kMfmaHeads][2].
-template <typename E, bool FULL, int W, int STAGES>
-__device__ __forceinline__ void window_row(const DecodeArgs& a, int block, uint8_t* lds, float (*s_ml)[kMfmaHeads][2],
-                                           int* s_old) {
-    constexpr int kWaveLds = kWorkerLds<STAGES>;
-    static_assert(kWaveLds >= kMfmaHeads * kDimHead * 4, "a wave's outputs");
+template <typename E, bool FULL, int W, int WAVE_LDS>
+__device__ __forceinline__ void finish_row(const DecodeArgs& a, int b, int bg, int h0, int nh, int row, int npg, int part,
+                                           int parts, const uint8_t* lds, const float (*s_ml)[kMfmaHeads][2], int* s_old) {
     const int P = a.parts;
-    const int part = block % P, bg = block / P;
-    const int b = bg / a.grid_heads, grp = bg - b * a.grid_heads;
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kvh = grp / a.head_groups, hg = grp - kvh * a.head_groups;
-    const int h0 = kvh * a.n_rep + hg * a.heads_per_wave;
-    const int nh = min(a.heads_per_wave, a.n_rep - hg * a.heads_per_wave);
-    int row, kv_len, start;
-    if (b >= a.num_seqs || !decode_row_of<kWindowPages>(a, b, row, kv_len, start)) return;  // a chunk's tiles
-    const int npg = pages_seen<kWindowPages>(a, kv_len, start);
-    const int per_part = (npg + P - 1) / P;
-    const int first = part * per_part, mine = min(npg - first, per_part);
-    const int parts = npg > 0 ? (npg + per_part - 1) / per_part : 1;  // with pages
-    if (part >= parts) return;
-    const int per = (mine + W - 1) / W;
-    const int lp0 = min(mine, wave * per), n = min(mine, lp0 + per) - lp0;
-    uint8_t* own = lds + wave * kWaveLds;
-    HeadState s;
-    if (n > 0) {
-        mfma_segment<E, FULL, kWindowPages, STAGES>(a, b, kv_len, start, first + lp0, n, row, h0, nh,
-                                                    (int64_t)kvh * a.pool_stride_head, own, s);
-    } else {
-        s.clear();
-    }
-    if (c < nh) {
-        float* acc = reinterpret_cast<float*>(own) + c * kDimHead + 4 * g;
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(acc + 16 * dt) = s.o[dt];
-        if (g == 0) {
-            s_ml[wave][c][0] = s.m;
-            s_ml[wave][c][1] = s.l;
-        }
-    }
-    __syncthreads();
     // Thread i holds dims 4 (i % 32) .. of head i / 32 (and so on).
     char* out = reinterpret_cast<char*>(a.out);
     auto write = [&](int r, int d, f32x4 o, float l) __attribute__((always_inline)) {
@@ -315,7 +277,7 @@ __device__ __forceinline__ void window_row(const DecodeArgs& a, int block, uint8
         for (int w = 0; w < W; ++w) {
             const float f = fast_exp2(s_ml[w][r][0] - M);
             L = fmaf(s_ml[w][r][1], f, L);
-            O += *reinterpret_cast<const f32x4*>(lds + w * kWaveLds + (r * kDimHead + d) * 4) * f;
+            O += *reinterpret_cast<const f32x4*>(lds + w * WAVE_LDS + (r * kDimHead + d) * 4) * f;
         }
         if (parts == 1) {
             write(r, d, O, L);
@@ -361,6 +323,54 @@ __device__ __forceinline__ void window_row(const DecodeArgs& a, int block, uint8
         }
         write(r, d, O, L);
     }
+}
+
+// Window rows: workgroup `block` of W waves takes part (block % a.parts) of the
+// pages that one KV head group's query heads of one sequence see; wave w the
+// w-th of W contiguous shares of it.  The waves fold their states through LDS
+// (each over its own, done, pages), and finish_row writes or publishes the row.
+// lds: W * kWorkerLds<STAGES> bytes, s_ml: [W][kMfmaHeads][2].
+template <typename E, bool FULL, int W, int STAGES>
+__device__ __forceinline__ void window_row(const DecodeArgs& a, int block, uint8_t* lds, float (*s_ml)[kMfmaHeads][2],
+                                           int* s_old) {
+    constexpr int kWaveLds = kWorkerLds<STAGES>;
+    static_assert(kWaveLds >= kMfmaHeads * kDimHead * 4, "a wave's outputs");
+    const int P = a.parts;
+    const int part = block % P, bg = block / P;
+    const int b = bg / a.grid_heads, grp = bg - b * a.grid_heads;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kvh = grp / a.head_groups, hg = grp - kvh * a.head_groups;
+    const int h0 = kvh * a.n_rep + hg * a.heads_per_wave;
+    const int nh = min(a.heads_per_wave, a.n_rep - hg * a.heads_per_wave);
+    int row, kv_len, start;
+    if (b >= a.num_seqs || !decode_row_of<kWindowPages>(a, b, row, kv_len, start)) return;  // a chunk's tiles
+    const int npg = pages_seen<kWindowPages>(a, kv_len, start);
+    const int per_part = (npg + P - 1) / P;
+    const int first = part * per_part, mine = min(npg - first, per_part);
+    const int parts = npg > 0 ? (npg + per_part - 1) / per_part : 1;  // with pages
+    if (part >= parts) return;
+    const int per = (mine + W - 1) / W;
+    const int lp0 = min(mine, wave * per), n = min(mine, lp0 + per) - lp0;
+    uint8_t* own = lds + wave * kWaveLds;
+    HeadState s;
+    if (n > 0) {
+        mfma_segment<E, FULL, kWindowPages, STAGES>(a, b, kv_len, start, first + lp0, n, row, h0, nh,
+                                                    (int64_t)kvh * a.pool_stride_head, own, s);
+    } else {
+        s.clear();
+    }
+    if (c < nh) {
+        float* acc = reinterpret_cast<float*>(own) + c * kDimHead + 4 * g;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(acc + 16 * dt) = s.o[dt];
+        if (g == 0) {
+            s_ml[wave][c][0] = s.m;
+            s_ml[wave][c][1] = s.l;
+        }
+    }
+    __syncthreads();
+    finish_row<E, FULL, W, kWaveLds>(a, b, bg, h0, nh, row, npg, part, parts, lds, s_ml, s_old);
 }
 
 // Tails of a shared-prefix call: the waves of workgroup `block`, as

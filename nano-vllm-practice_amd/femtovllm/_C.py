@@ -118,6 +118,14 @@ def _declare_added(lib) -> None:
         i, p, i64, i64, p, i64, i64, p, i64, i64, p, i64, i64, p, p, i64, i, i, i,
         p, p, i64, i, i, i, i, i64, i64, i64, p, i, i, i, p, p, i, i64, p,
     ]
+    lib.femto_paged_attention_gemv_fp4.restype = i
+    lib.femto_paged_attention_gemv_fp4.argtypes = [
+        i, p, i64, i64, p, i64, i64, p, i64, i, i, p, i, i64, p, i, i, i, p, sz, p,
+    ]
+    lib.femto_paged_attention_gemv_fp4_workspace_size.restype = sz
+    lib.femto_paged_attention_gemv_fp4_workspace_size.argtypes = [i, i, i, i]
+    lib.femto_paged_attention_gemv_fp4_zero_bytes.restype = sz
+    lib.femto_paged_attention_gemv_fp4_zero_bytes.argtypes = []
     lib.femto_fp4_page_bytes.restype = sz
     lib.femto_fp4_page_bytes.argtypes = [i]
     lib.femto_kv_cache_write_fp4.restype = i
@@ -245,11 +253,12 @@ def _prefill_workspace(device: torch.device, num_seqs: int, num_tokens: int, max
     return _cached_workspace(_prefill_workspaces, device, nbytes, zero=True)
 
 
-# Workspaces of the window and shared-prefix calls, one per (device, stream) as above.  No captured graph holds one: a call
+# Workspaces of the window, shared-prefix and 4-bit-cache calls, one per (device, stream) as above.  No captured graph holds one: a call
 # that is being captured takes its own, from the graph's memory.
 _window_workspaces: dict = {}
 _window_prefill_workspaces: dict = {}
 _shared_prefix_workspaces: dict = {}
+_fp4_workspaces: dict = {}
 
 
 def _call_workspace(cache: dict, device: torch.device, nbytes: int, zero_bytes: int):
@@ -891,6 +900,48 @@ def _rope_cache_write_fp4(q, k, v, cos, sin, positions, kv_pool, kv_page_tables,
             kv_pool.data_ptr(), kv_pool.size(0), q.size(1), kv_pool.size(1), q.size(2),
             cu_ptr, kv_page_tables.size(0), q.size(0), max_q_len,
             positions.data_ptr(), kv_page_tables.data_ptr(), kv_page_tables.size(1), stride, _stream(q.device),
+        )
+    _raise_on(rc)
+    return out
+
+
+def _check_fp4_attention(fn, q, kv_pool, tables, kv_lens):
+    _check(q.is_cuda, f"{fn}: q must be a GPU tensor")
+    _check(q.dim() == 3, f"{fn}: q must be 3-D (n_heads, tokens, head_dim), got {q.dim()}-D")
+    _check(q.stride(-1) == 1, f"{fn}: q must be contiguous in head_dim")
+    _check(q.dtype != torch.float32, f'"{fn}" not implemented for \'Float\'')
+    _check_fp4_pool(fn, kv_pool, q.size(2), q.device)
+    _check(q.size(0) > 0 and q.size(0) % kv_pool.size(1) == 0, f"{fn}: n_heads must be a multiple of n_kv_heads")
+    _check(tables.dtype == torch.int32 and tables.dim() == 2 and tables.device == q.device
+           and (tables.size(1) <= 1 or tables.stride(1) == 1), f"{fn}: kv_page_tables must be 2-D row-major int32 on {q.device}")
+    _check(kv_lens.dtype == torch.int32 and kv_lens.dim() == 1 and kv_lens.is_contiguous() and kv_lens.device == q.device,
+           f"{fn}: kv_lens must be a contiguous 1-D int32 tensor on {q.device}")
+    return _dtype_code(q, fn)
+
+
+def _paged_attention_gemv_fp4(q, kv_pool, kv_page_tables, kv_lens, max_kv_len):
+    """Decode over a 4-bit cache; out (n_heads, num_seqs, head_dim)."""
+    fn = "paged_attention_gemv_fp4"
+    dtype = _check_fp4_attention(fn, q, kv_pool, kv_page_tables, kv_lens)
+    n_heads, num_seqs, dim = q.shape
+    _check(num_seqs == kv_page_tables.size(0), f"{fn}: q.size(1) must equal kv_page_tables.size(0)")
+    _check(num_seqs == kv_lens.size(0), f"{fn}: q.size(1) must equal kv_lens.size(0)")
+    max_kv_len = _int32_arg(fn, "max_kv_len", max_kv_len)
+    with torch.cuda.device(q.device):
+        out = torch.empty((n_heads, num_seqs, dim), dtype=q.dtype, device=q.device)
+        if num_seqs == 0:
+            return out
+        nbytes = _lib.femto_paged_attention_gemv_fp4_workspace_size(num_seqs, n_heads, kv_pool.size(1), max_kv_len)
+        ws, ws_bytes, _hold = _call_workspace(_fp4_workspaces, q.device, nbytes,
+                                              _lib.femto_paged_attention_gemv_fp4_zero_bytes())
+        rc = _lib_held.femto_paged_attention_gemv_fp4(
+            dtype,
+            q.data_ptr(), q.stride(0), q.stride(1),
+            out.data_ptr(), out.stride(0), out.stride(1),
+            kv_pool.data_ptr(), kv_pool.size(0), kv_pool.size(1), dim,
+            kv_page_tables.data_ptr(), kv_page_tables.size(1), kv_page_tables.stride(0),
+            kv_lens.data_ptr(), num_seqs, n_heads, max_kv_len,
+            ws, ws_bytes, _stream(q.device),
         )
     _raise_on(rc)
     return out

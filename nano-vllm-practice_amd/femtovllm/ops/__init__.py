@@ -411,3 +411,21 @@ def rope_cache_write_fp4(
             raise ValueError(f"Argument '{name}' must be a CUDA tensor. Got device={t.device}")
     return _hip_backend._rope_cache_write_fp4(q, k, v, cos, sin, positions, kv_pool, kv_page_tables, cu_seqlens,
                                               max_q_len, interleaved, q_norm_weight, k_norm_weight, eps, out)
+
+
+def paged_attention_gemv_fp4(
+    q: torch.Tensor,
+    kv_pool: torch.Tensor,
+    kv_page_tables: torch.Tensor,
+    kv_lens: torch.Tensor,
+    max_kv_len: int,
+):
+    """:func:`paged_attention_gemv` over a KV cache held in 4 bits.
+
+    q (n_heads, num_seqs, head_dim) bf16 or f16, head_dim a multiple of 16 up to
+    128; ``kv_pool`` (num_blocks, n_kv_heads, page bytes) as written by
+    :func:`kv_cache_write_fp4`.  Contexts of any length; an empty one gives zeros.
+    Keys and values are what the cache stands for (f16: V past its range is an
+    infinity); rows behind a context may hold anything.
+    """
+    return _hip_backend._paged_attention_gemv_fp4(_ensure_valid_tensor(q, "q"), kv_pool, kv_page_tables, kv_lens, max_kv_len)
