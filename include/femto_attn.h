@@ -432,6 +432,27 @@ int femto_paged_attention_gemv_fp4(
 size_t femto_paged_attention_gemv_fp4_workspace_size(int num_seqs, int n_heads, int n_kv_heads, int max_kv_len);
 size_t femto_paged_attention_gemv_fp4_zero_bytes(void);
 
+/* femto_paged_attention_gemm over a 4-bit cache: token t of sequence b sees the
+ * keys j < kv_lens[b] with j <= positions[t]; a token that sees none gives NaN.
+ * Sequences of one token are taken as decode rows.  A block of V that is NaN has
+ * to be at a position that no token of its sequence's chunk sees past: one in
+ * a key j < kv_lens[b] may also reach tokens of the chunk before it.  The
+ * workspace (256-byte aligned, always needed) has to be zero in its first
+ * femto_paged_attention_gemm_split_bytes() bytes before its first use and is
+ * left so; calls that may overlap must not share one. */
+int femto_paged_attention_gemm_fp4(
+    int dtype,
+    const void* q, int64_t q_stride_head, int64_t q_stride_token,
+    void* out, int64_t out_stride_head, int64_t out_stride_token,
+    const void* kv_pool, int64_t num_blocks, int n_kv_heads, int head_dim,
+    const int32_t* cu_seqlens, int num_seqs, int num_tokens, int max_q_len, int n_heads,
+    const int32_t* kv_page_tables, int num_pages_per_seq, int64_t table_stride,
+    const int32_t* kv_lens, const int32_t* positions,
+    void* workspace, size_t workspace_bytes,
+    void* stream);
+size_t femto_paged_attention_gemm_fp4_workspace_size(int num_seqs, int num_tokens, int max_q_len, int n_heads,
+                                                     int n_kv_heads, int num_pages_per_seq);
+
 /* Varlen attention metadata built on the device, by the rules of the
  * reference's ModelRunner (femtovllm/engine/model_runner.py:187-202 prefill,
  * 283-293 decode, 46-72 block-table padding), which builds them with Python

@@ -28,7 +28,7 @@ LIB = os.path.join(OUT_DIR, "libfemto_attn.so")
 NATIVE = os.path.join(OUT_DIR, "femto_native.so")
 
 SOURCES = ["femto_attn_api.hip", "paged_decode.hip", "paged_prefill.hip", "kv_cache_write.hip", "qk_norm_rope.hip", "varlen_metadata.hip",
-           "window_decode.hip", "window_prefill.hip", "rope_cache_write.hip", "shared_prefix.hip", "fp4_cache.hip", "fp4_decode.hip"]
+           "window_decode.hip", "window_prefill.hip", "rope_cache_write.hip", "shared_prefix.hip", "fp4_cache.hip", "fp4_decode.hip", "fp4_prefill.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -71,6 +71,7 @@
 
 #include "common.h"
 #include "decode_worker.h"
+#include "fp4_decode.h"
 #include "lds_copy.h"
 #include "mfma_decode.h"
 #include "launch.h"
@@ -167,7 +168,13 @@ __device__ __forceinline__ int serpentine(int k, int n, int cus) {
 // the "tokens" are the sequences, all of one table (a.tables), each seeing
 // the keys below min(kv_lens[t], kv_len); the prefix is cut into
 // a.dec.prefix_pieces pieces, each leaving its rows' states (m, l and the
-// unnormalised output) as partial slots of the merge launch.
+// unnormalised output) as partial slots of the merge launch.  kFp4Pages is the
+// causal rule over a cache held in 4 bits (fp4.h; a.k the pool, a.k_stride0 and
+// a.k_stride1 bytes from block to block and head to head): K's codes are copied
+// into LDS as they are and multiplied by scaled matrix instructions with q in
+// three terms of 6 bits (fp4_decode.h); V's are loaded into registers a tile
+// ahead, and converted into LDS rows of the storage type after the tile's math,
+// once for all of the tile's query rows.
 template <typename E, int G, bool PAGED, bool FUSED, bool FULLD = true, int RULE = kAllPages>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_mfma_kernel(PrefillArgs a) {
     constexpr int EB = 2;
@@ -178,7 +185,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __shared__ int s_seq, s_ltile, s_old;
     __shared__ int s_kend[4];
     __shared__ int s_kbeg[4];  // kWindowPages
-    constexpr bool WINDOW = RULE == kWindowPages, PREFIX = RULE == kTailPages;
+    constexpr bool WINDOW = RULE == kWindowPages, PREFIX = RULE == kTailPages, FP4 = RULE == kFp4Pages;
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -550,7 +557,55 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // Others are not read: their values, a NaN or an infinity of V among
     // them, would meet weights of 0.
     int seen_beg = 0, seen_end = kv_len;
+    // kFp4Pages: this lane's part of the next tile's V, four keys (4 (lane / 16) ..)
+    // of 8 dims with a scale each, and K's scales of row lane % 16.
+    const int fp4_n = fp4_blocks(FULLD ? kDimHead : a.head_dim);
+    u32x4 v4 = {0, 0, 0, 0};
+    uint32_t v4_scale = 0, k4_scale = 0;
+    auto issue_fp4 = [&](int it, int stage) __attribute__((always_inline)) {
+        const int key0 = it * kKvTile + 16 * wave;
+        const int blk = key0 < kv_len ? __builtin_amdgcn_readlane(tbl, it - tbase) : -1;
+        const bool ok = blk >= 0 && (int64_t)blk < a.num_blocks;
+        const char* page = ok ? kbase_p + (int64_t)blk * a.k_stride0 + (int64_t)kvh * a.k_stride1
+                              : reinterpret_cast<const char*>(g_zero_page);
+        // Lanes of dims past the row's blocks take block 0's (q is zero there, and
+        // those output dims are not stored).
+        const int vc = FULLD || lpos < 4 * fp4_n ? lpos : 0;
+        lds_dma_one((uint64_t)(uintptr_t)page, FULLD || lane < 16 * fp4_n ? 16 * lane : 0,
+                    lds_addr(&smem[stage][0][1024 * wave]));
+        v4 = ld16(page + 256 * fp4_n + 64 * fp4_n * lrow + 16 * vc);
+        v4_scale = *reinterpret_cast<const uint32_t*>(page + 512 * fp4_n + 64 + 16 * lrow + 4 * (vc >> 2));
+        k4_scale = *reinterpret_cast<const uint32_t*>(page + 512 * fp4_n + 4 * lpos);
+    };
+    // ... and into LDS: V as rows of the storage type, zeros past kv_len (their
+    // weights are 0, and 0 times a NaN would not be); K's scales behind its codes,
+    // those of blocks past the row's 1.
+    auto store_fp4 = [&](int it, int stage) __attribute__((always_inline)) {
+        const int key0 = it * kKvTile + 16 * wave + 4 * lrow;
+        if (it * kKvTile + kKvTile > kv_len) {  // wave-uniform
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v4[j] = key0 + j < kv_len ? v4[j] : 0;
+                v4_scale = key0 + j < kv_len ? v4_scale : v4_scale & ~(0xffu << (8 * j));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int row = 16 * wave + 4 * lrow + j;
+            const float s = __uint_as_float((j == 3 ? v4_scale >> 1 : v4_scale << (23 - 8 * j)) & 0x7f800000u);
+            *reinterpret_cast<u32x4*>(&smem[stage][1][row * kRowBytes + ((lpos ^ swz_v(row)) << 4)]) = fp4_unpack8(E{}, v4[j], s);
+        }
+        if (lane < 16) {
+            uint32_t ks = k4_scale;
+            if constexpr (!FULLD) {
+                const uint32_t keep = fp4_n < 4 ? (1u << (8 * fp4_n)) - 1u : ~0u;
+                ks = (ks & keep) | (0x7f7f7f7fu & ~keep);
+            }
+            *reinterpret_cast<uint32_t*>(&smem[stage][0][4 * 1024 + 4 * (16 * wave + lane)]) = ks;
+        }
+    };
     auto issue_tile = [&](int it, int stage) __attribute__((always_inline)) {
+        if constexpr (FP4) return issue_fp4(it, stage);
         const int key0 = it * kKvTile + 16 * wave;  // first key of this wave's page
         // Keys past the last one seen (kv_len; under a window seen_end) read
         // its row (finite data, masked later); pages wholly past it read that
@@ -736,7 +791,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
     // Q rows in registers: the B operand of S^T = K . Q^T.
     u32x4 qreg[8];
-    {
+    Fp4Query q4[2];  // kFp4Pages: of dims 32 h2 .. and 64 + 32 h2 ..
+    if constexpr (FP4) {
+        const char* qrow = reinterpret_cast<const char*>(a.q) + ((int64_t)h * a.q_stride_head + (int64_t)t * a.q_stride_token) * EB;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) q4[kk] = fp4_query_row<E>(qrow, 2 * kk + h2, FULLD ? kDimHead : a.head_dim, qvalid);
+    } else {
         const char* qrow = reinterpret_cast<const char*>(a.q) +
                            ((int64_t)b * a.q_stride_batch + (int64_t)h * a.q_stride_head + (int64_t)t * a.q_stride_token) * EB;
 #pragma unroll
@@ -877,6 +937,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             }
             l_run = sum;
         };
+        // kFp4Pages: operand and scales of K's keys 32 block + l32, dims 64 kk + 32 h2 ..
+        auto k4frag = [&](int block, int kk) __attribute__((always_inline)) {
+            return *reinterpret_cast<const u32x4*>(ks + 1024 * (l32 >> 4) + 256 * h2 + 16 * (l32 & 15) + 2048 * block + 512 * kk);
+        };
+        // (the word's bytes 0 and 2: those of kk = 0 and 1)
+        auto k4scale = [&](int block) __attribute__((always_inline)) {
+            return *reinterpret_cast<const uint32_t*>(ks + 4 * 1024 + 4 * (32 * block + l32)) >> (8 * h2);
+        };
         constexpr int kAhead = 4;  // fragments read ahead of their MFMA (3: 1 % slower on long context)
         u32x4 p0[2], p1[2];
         float sum0 = l_run;
@@ -884,6 +952,51 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         // Each MFMA is fenced into one bundle with the fragment read ahead of
         // it and its share of the other block's softmax: the compiler's own
         // order puts the exponentials after the MFMAs (4-6 % slower).
+        if constexpr (FP4) {
+            u32x4 k4[2][2];
+            uint32_t ks4[2];
+#pragma unroll
+            for (int block = 0; block < 2; ++block) {
+                ks4[block] = k4scale(block);
+                k4[block][0] = k4frag(block, 0);
+                k4[block][1] = k4frag(block, 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            // MFMA m of a block: term 2 - m / 2 (the smallest first), half m % 2 of the dims.
+            auto score = [&](f32x16& s, int block, auto m_c) __attribute__((always_inline)) {
+                constexpr int m = decltype(m_c)::value, kk = m & 1, term = 2 - (m >> 1);
+                s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(k4[block][kk]), fp4_operand(q4[kk].term[term]), s,
+                                                                    kFormatFp4, kFormatFp6, 2 * kk, (int)ks4[block], term,
+                                                                    (int)q4[kk].scales);
+            };
+            auto bundle0 = [&](auto m_c) __attribute__((always_inline)) {
+                score(s0, 0, m_c);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            auto bundle1 = [&](auto m_c) __attribute__((always_inline)) {
+                constexpr int m = decltype(m_c)::value;
+                if constexpr (m >= 2) vf[m - 2] = vfrag(m - 2);
+                score(s1, 1, m_c);
+                if constexpr (m > 0 && m < 5) soft(s0, m - 1, p0, sum0);
+                if constexpr (m == 5) {
+#pragma unroll
+                    for (int i = 4; i < 8; ++i) soft(s0, i, p0, sum0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            bundle0(std::integral_constant<int, 0>{});
+            bundle0(std::integral_constant<int, 1>{});
+            bundle0(std::integral_constant<int, 2>{});
+            bundle0(std::integral_constant<int, 3>{});
+            bundle0(std::integral_constant<int, 4>{});
+            bundle0(std::integral_constant<int, 5>{});
+            bundle1(std::integral_constant<int, 0>{});
+            bundle1(std::integral_constant<int, 1>{});
+            bundle1(std::integral_constant<int, 2>{});
+            bundle1(std::integral_constant<int, 3>{});
+            bundle1(std::integral_constant<int, 4>{});
+            bundle1(std::integral_constant<int, 5>{});
+        } else {
 #pragma unroll
         for (int n = 0; n < kAhead; ++n) kf[n] = kfrag(n);
         __builtin_amdgcn_sched_barrier(0);
@@ -907,6 +1020,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             if (n > 8) soft(s0, n - 9, p0, sum0);
             if (n == 15) soft(s0, 7, p0, sum0);
             __builtin_amdgcn_sched_barrier(0);
+        }
         }
         // (keeps the exponentials above from being sunk below settle's branches)
         asm volatile("" : "+v"(p0[0]), "+v"(p0[1]), "+v"(sum0));
@@ -970,7 +1084,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         } else {
             if (any) tile_math(kb, STAGE == 0 && it == t_lo, stage_c, std::false_type{});
         }
+        if constexpr (FP4) {
+            if (more) store_fp4(next, STAGE ^ 1);
+        }
     };
+    if constexpr (FP4) {
+        if (t_hi > t_lo) store_fp4(t_lo, 0);  // (t_first: the piece's first tile does not depend on the positions)
+    }
     auto tile_loop = [&](auto spread_c) __attribute__((always_inline)) {
         for (int it = t_lo; it < t_hi; it += 2) {
             step(it, std::integral_constant<int, 0>{}, spread_c);
@@ -1085,12 +1205,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         // reads its last one again and gives the copies weight 0.
         constexpr int kR = kHalf ? 4 : 2;
         constexpr int kLoads = kHalf ? 8 : 16;
-        // Under a window the piece's own partial is read back too, and all are
+        // Under a window and over a 4-bit cache the piece's own partial is read back too, and all are
         // merged in piece order, so that the result does not depend on which
         // piece came last.
-        const int pc = __builtin_amdgcn_readfirstlane(WINDOW ? nne : piece);
-        const int n_o = __builtin_amdgcn_readfirstlane(nne) - (WINDOW ? 0 : 1);
-        if constexpr (WINDOW) {
+        const int pc = __builtin_amdgcn_readfirstlane(WINDOW || FP4 ? nne : piece);
+        const int n_o = __builtin_amdgcn_readfirstlane(nne) - (WINDOW || FP4 ? 0 : 1);
+        if constexpr (WINDOW || FP4) {
             m_run = kEmptyMaxP;
             l_run = 0.0f;
 #pragma unroll
@@ -1224,7 +1344,7 @@ static hipError_t launch_gf(int G, const PrefillArgs& a, hipStream_t st) {
 template <typename E, bool PAGED, int RULE>
 static hipError_t launch_g(int G, const PrefillArgs& a, hipStream_t st) {
     if constexpr (RULE == kTailPages) return launch_gf<E, true, true, RULE>(G, a, st);
-    if constexpr (PAGED && RULE != kTailPages) {
+    if constexpr (PAGED && RULE != kTailPages && RULE != kFp4Pages) {
         if (a.decode_blocks > 0) return launch_gf<E, true, true, RULE>(G, a, st);
     }
     if constexpr (RULE != kTailPages) return launch_gf<E, PAGED, false, RULE>(G, a, st);

@@ -220,10 +220,11 @@ __device__ __forceinline__ int pages_of(int kv_len) { return kv_len > 0 ? (kv_le
 //    j >= start or j < a.sinks, i.e. the sinks' pages and then the window's;
 //  * kTailPages (a.first_page): those from page a.first_page on (the pages
 //    before it are a shared prefix, which the MFMA tiles take).
+// (kFp4Pages: as kAllPages, over a cache held in 4 bits, for the tiles only.)
 // The pages walked are numbered without the ones left out: a slice of
 // `count` pages is cut, balanced and merged as if they were contiguous, and
 // page(i) is the table column of the i-th.
-enum PageRule { kAllPages, kWindowPages, kTailPages };
+enum PageRule { kAllPages, kWindowPages, kTailPages, kFp4Pages };
 
 template <int RULE>
 struct PageList {

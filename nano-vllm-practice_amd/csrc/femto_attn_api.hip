@@ -672,6 +672,19 @@ static Fp4DecodePlan fp4_decode_plan(int num_seqs, int n_heads, int n_kv_heads, 
     return p;
 }
 
+// The decode rows of a prefill call over a 4-bit cache: parts of its rows (one
+// counter each of the key split's second half), and the bytes of their states.
+static WindowParts gemm_fp4_parts(int num_seqs, int num_tokens, int max_q_len, int n_heads, int n_kv_heads,
+                                  int num_pages_per_seq, int resident) {
+    const int rows = femto::decode_rows_bound(num_seqs, num_tokens, max_q_len);
+    if (rows == 0) return {0, 0};
+    const int table_keys = (int)std::min<int64_t>((int64_t)num_pages_per_seq * femto::kPage, 1 << 30);
+    WindowParts p = window_parts(rows, n_heads, n_kv_heads, table_keys, resident / 2);
+    const int n_rep = n_heads / n_kv_heads;
+    if ((int64_t)num_seqs * n_kv_heads * ((n_rep + femto::kMfmaHeads - 1) / femto::kMfmaHeads) > resident) p.parts = 1;
+    return p;
+}
+
 // Checks that attention calls over a 4-bit cache share.
 static int check_fp4_attention(const std::string& f, int dtype, const void* q, int64_t q_s0, int64_t q_s1, const void* out,
                                const void* kv_pool, int64_t num_blocks, int n_kv_heads, int head_dim, int n_heads,
@@ -1316,6 +1329,94 @@ int femto_paged_attention_gemv_fp4(int dtype, const void* q, int64_t q_stride_he
     a.parts = w.rows.parts;
     a.single_waves = w.rows.waves;
     return hip_status(femto::launch_fp4_decode(dtype, a, num_seqs, static_cast<hipStream_t>(stream)), (fn + " launch").c_str());
+}
+
+size_t femto_paged_attention_gemm_fp4_workspace_size(int num_seqs, int num_tokens, int max_q_len, int n_heads,
+                                                     int n_kv_heads, int num_pages_per_seq) {
+    if (num_seqs <= 0 || num_tokens <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads) return 0;
+    int resident = 0;
+    if (femto::prefill_resident_workgroups(resident) != hipSuccess) return 0;
+    return femto::prefill_workspace_bytes(resident) +
+           gemm_window_bytes(num_seqs, n_heads, gemm_fp4_parts(num_seqs, num_tokens, max_q_len, n_heads, n_kv_heads,
+                                                               num_pages_per_seq, resident));
+}
+
+int femto_paged_attention_gemm_fp4(int dtype, const void* q, int64_t q_stride_head, int64_t q_stride_token, void* out,
+                                   int64_t out_stride_head, int64_t out_stride_token, const void* kv_pool,
+                                   int64_t num_blocks, int n_kv_heads, int head_dim, const int32_t* cu_seqlens,
+                                   int num_seqs, int num_tokens, int max_q_len, int n_heads, const int32_t* kv_page_tables,
+                                   int num_pages_per_seq, int64_t table_stride, const int32_t* kv_lens,
+                                   const int32_t* positions, void* workspace, size_t workspace_bytes, void* stream) {
+    g_err.clear();
+    const std::string fn = "paged_attention_gemm_fp4";
+    if (num_seqs < 0 || num_tokens < 0 || max_q_len < 0) return fail(FEMTO_ERR_INVALID, fn + ": negative size");
+    if (num_seqs == 0 || num_tokens == 0) return FEMTO_OK;
+    int rc = check_fp4_attention(fn, dtype, q, q_stride_head, q_stride_token, out, kv_pool, num_blocks, n_kv_heads, head_dim,
+                                 n_heads, kv_page_tables, num_pages_per_seq, table_stride);
+    if (rc != FEMTO_OK) return rc;
+    if (!cu_seqlens || !kv_lens || !positions)
+        return fail(FEMTO_ERR_INVALID, fn + ": null cu_seqlens / kv_lens / positions");
+    if (out_stride_head % 4 || out_stride_token % 4)
+        return fail(FEMTO_ERR_INVALID, fn + ": out strides must be multiples of 8 bytes");
+    int resident = 0;
+    rc = hip_status(femto::prefill_resident_workgroups(resident), (fn + ": device query").c_str());
+    if (rc != FEMTO_OK) return rc;
+    const WindowParts p = gemm_fp4_parts(num_seqs, num_tokens, max_q_len, n_heads, n_kv_heads, num_pages_per_seq, resident);
+    const size_t split_bytes = femto::prefill_workspace_bytes(resident);
+    const size_t need = split_bytes + gemm_window_bytes(num_seqs, n_heads, p);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
+        return fail(FEMTO_ERR_INVALID, fn + ": workspace of " + std::to_string(need) +
+                                           " bytes (256-byte aligned) required, got " + std::to_string(workspace_bytes));
+    const int page = femto::fp4_page_bytes(head_dim);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    femto::PrefillArgs a{};
+    a.q = q;
+    a.q_stride_head = q_stride_head;
+    a.q_stride_token = q_stride_token;
+    a.out = out;
+    a.out_stride_head = out_stride_head;
+    a.out_stride_token = out_stride_token;
+    a.k = a.v = kv_pool;
+    a.k_stride0 = a.v_stride0 = (int64_t)n_kv_heads * page;
+    a.k_stride1 = a.v_stride1 = page;
+    a.num_blocks = num_blocks;
+    a.cu_seqlens = cu_seqlens;
+    a.tables = kv_page_tables;
+    a.table_stride = table_stride;
+    a.num_pages_per_seq = num_pages_per_seq;
+    a.kv_lens = kv_lens;
+    a.positions = positions;
+    a.num_seqs = num_seqs;
+    a.n_heads = n_heads;
+    a.n_kv_heads = n_kv_heads;
+    a.n_rep = n_heads / n_kv_heads;
+    a.head_dim = head_dim;
+    a.scale_log2 = scale_log2(head_dim);
+    a.fp4 = 1;
+    a.counters = static_cast<int*>(workspace);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + femto::prefill_counter_bytes(resident));
+    int decode_rows = 0;
+    if (p.parts > 0) {
+        // Sequences of one query token run as rows (an MFMA tile would hold one
+        // valid row of 32).
+        decode_rows = femto::decode_rows_bound(num_seqs, num_tokens, max_q_len);
+        femto::DecodePlan plan{};
+        plan.nrep_tile = 1;
+        plan.max_slots = p.parts;
+        femto::DecodeArgs d = femto::decode_args(
+            plan, q, q_stride_head, q_stride_token, out, out_stride_head, out_stride_token, kv_pool, nullptr, num_blocks,
+            n_kv_heads, head_dim, a.k_stride0, a.k_stride1, 0, kv_page_tables, num_pages_per_seq, table_stride, kv_lens,
+            num_seqs, n_heads, static_cast<char*>(workspace) + split_bytes);
+        d.cu_seqlens = cu_seqlens;
+        d.positions = positions;
+        d.parts = p.parts;
+        d.single_waves = p.waves;
+        d.merge_counters = p.parts > 1 ? a.counters + resident : nullptr;
+        a.skip_decode_rows = 1;
+        rc = hip_status(femto::launch_fp4_decode(dtype, d, num_seqs, st), (fn + " decode-row launch").c_str());
+        if (rc != FEMTO_OK) return rc;
+    }
+    return hip_status(femto::launch_paged_prefill(dtype, a, num_tokens, decode_rows, st), (fn + " launch").c_str());
 }
 
 int femto_build_varlen_metadata(int num_seqs, const int32_t* num_computed, const int32_t* num_tokens,

@@ -128,6 +128,7 @@ struct PrefillArgs {
     DecodeArgs dec;
     // Sliding window with sinks (paged only; window == 0: none).
     int window, sinks;
+    int fp4;  // a cache held in 4 bits: k the pool, k_stride0 and k_stride1 in bytes
 };
 
 // Key split: at most kMaxPieces pieces per query tile, each leaving a
@@ -280,6 +281,8 @@ int prefill_group(int n_rep);
 // The tile launch of a paged call with a.window > 0 (window_prefill.hip), for
 // launch_paged_prefill.
 hipError_t launch_window_tiles(int dtype, int G, const PrefillArgs& a, hipStream_t st);
+// ... and of one over a 4-bit cache (fp4_prefill.hip).
+hipError_t launch_fp4_tiles(int dtype, int G, const PrefillArgs& a, hipStream_t st);
 hipError_t launch_dense_attention(int dtype, PrefillArgs a, hipStream_t st);
 
 }  // namespace femto

@@ -82,6 +82,7 @@ hipError_t launch_paged_prefill(int dtype, PrefillArgs a, int num_tokens, int de
         a.rows_first = std::min(a.decode_blocks, slots / 4) / 8 * 8;
         return launch_window_tiles(dtype, G, a, st);
     }
+    if (a.fp4) return launch_fp4_tiles(dtype, G, a, st);
     hipError_t e = launch_dtype<true, kAllPages>(dtype, G, a, st);
     if (e == hipSuccess && a.decode_blocks > 0 && !a.dec.merge_counters) e = launch_paged_decode_merge(dtype, a.dec, a.num_seqs, st);
     return e;

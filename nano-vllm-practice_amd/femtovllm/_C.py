@@ -126,6 +126,12 @@ def _declare_added(lib) -> None:
     lib.femto_paged_attention_gemv_fp4_workspace_size.argtypes = [i, i, i, i]
     lib.femto_paged_attention_gemv_fp4_zero_bytes.restype = sz
     lib.femto_paged_attention_gemv_fp4_zero_bytes.argtypes = []
+    lib.femto_paged_attention_gemm_fp4.restype = i
+    lib.femto_paged_attention_gemm_fp4.argtypes = [
+        i, p, i64, i64, p, i64, i64, p, i64, i, i, p, i, i, i, i, p, i, i64, p, p, p, sz, p,
+    ]
+    lib.femto_paged_attention_gemm_fp4_workspace_size.restype = sz
+    lib.femto_paged_attention_gemm_fp4_workspace_size.argtypes = [i, i, i, i, i, i]
     lib.femto_fp4_page_bytes.restype = sz
     lib.femto_fp4_page_bytes.argtypes = [i]
     lib.femto_kv_cache_write_fp4.restype = i
@@ -259,6 +265,7 @@ _window_workspaces: dict = {}
 _window_prefill_workspaces: dict = {}
 _shared_prefix_workspaces: dict = {}
 _fp4_workspaces: dict = {}
+_fp4_prefill_workspaces: dict = {}
 
 
 def _call_workspace(cache: dict, device: torch.device, nbytes: int, zero_bytes: int):
@@ -941,6 +948,41 @@ def _paged_attention_gemv_fp4(q, kv_pool, kv_page_tables, kv_lens, max_kv_len):
             kv_pool.data_ptr(), kv_pool.size(0), kv_pool.size(1), dim,
             kv_page_tables.data_ptr(), kv_page_tables.size(1), kv_page_tables.stride(0),
             kv_lens.data_ptr(), num_seqs, n_heads, max_kv_len,
+            ws, ws_bytes, _stream(q.device),
+        )
+    _raise_on(rc)
+    return out
+
+
+def _paged_attention_gemm_fp4(q, kv_pool, cu_seqlens, max_q_len, kv_page_tables, kv_lens, positions):
+    """Varlen causal prefill over a 4-bit cache; out (n_heads, num_tokens, head_dim)."""
+    fn = "paged_attention_gemm_fp4"
+    dtype = _check_fp4_attention(fn, q, kv_pool, kv_page_tables, kv_lens)
+    for name, t in (("cu_seqlens", cu_seqlens), ("positions", positions)):
+        _check(t.dtype == torch.int32 and t.is_contiguous() and t.device == q.device,
+               f"{fn}: {name} must be a contiguous int32 tensor on {q.device}")
+    num_seqs = cu_seqlens.numel() - 1
+    _check(num_seqs == kv_page_tables.size(0), f"{fn}: cu_seqlens.numel()-1 must equal kv_page_tables.size(0)")
+    _check(num_seqs == kv_lens.size(0), f"{fn}: cu_seqlens.numel()-1 must equal kv_lens.size(0)")
+    n_heads, num_tokens, dim = q.shape
+    _check(num_tokens == positions.numel(), f"{fn}: q.size(1) must equal positions.numel()")
+    max_q_len = _int32_arg(fn, "max_q_len", max_q_len)
+    with torch.cuda.device(q.device):
+        out = torch.empty((n_heads, num_tokens, dim), dtype=q.dtype, device=q.device)
+        if num_seqs <= 0 or num_tokens == 0:
+            return out
+        nbytes = _lib.femto_paged_attention_gemm_fp4_workspace_size(num_seqs, num_tokens, max_q_len, n_heads,
+                                                                    kv_pool.size(1), kv_page_tables.size(1))
+        ws, ws_bytes, _hold = _call_workspace(_fp4_prefill_workspaces, q.device, nbytes,
+                                              _lib.femto_paged_attention_gemm_split_bytes())
+        rc = _lib_held.femto_paged_attention_gemm_fp4(
+            dtype,
+            q.data_ptr(), q.stride(0), q.stride(1),
+            out.data_ptr(), out.stride(0), out.stride(1),
+            kv_pool.data_ptr(), kv_pool.size(0), kv_pool.size(1), dim,
+            cu_seqlens.data_ptr(), num_seqs, num_tokens, max_q_len, n_heads,
+            kv_page_tables.data_ptr(), kv_page_tables.size(1), kv_page_tables.stride(0),
+            kv_lens.data_ptr(), positions.data_ptr(),
             ws, ws_bytes, _stream(q.device),
         )
     _raise_on(rc)

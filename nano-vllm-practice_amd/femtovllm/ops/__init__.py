@@ -429,3 +429,24 @@ def paged_attention_gemv_fp4(
     infinity); rows behind a context may hold anything.
     """
     return _hip_backend._paged_attention_gemv_fp4(_ensure_valid_tensor(q, "q"), kv_pool, kv_page_tables, kv_lens, max_kv_len)
+
+
+def paged_attention_gemm_fp4(
+    q: torch.Tensor,
+    kv_pool: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    max_q_len: int,
+    kv_page_tables: torch.Tensor,
+    kv_lens: torch.Tensor,
+    positions: torch.Tensor,
+):
+    """:func:`paged_attention_gemm` over a KV cache held in 4 bits.
+
+    Token t of sequence b sees key j iff ``j < kv_lens[b]`` and ``j <=
+    positions[t]``; a token that sees no key gives NaN.  Types, dims and the
+    pool as :func:`paged_attention_gemv_fp4`; chunks and single tokens may share a
+    call.  V that is NaN or, to f16, infinite in a key below ``kv_lens[b]`` may
+    also reach tokens of the sequence's chunk that do not see it.
+    """
+    return _hip_backend._paged_attention_gemm_fp4(_ensure_valid_tensor(q, "q"), kv_pool, cu_seqlens, max_q_len,
+                                                  kv_page_tables, kv_lens, positions)
