@@ -42,6 +42,14 @@ decltype(&femto_paged_attention_gemv_window) g_gemv_window;
 decltype(&femto_paged_attention_gemv_window_workspace_size) g_gemv_window_ws;
 decltype(&femto_paged_attention_gemm_window) g_gemm_window;
 decltype(&femto_paged_attention_gemm_window_workspace_size) g_gemm_window_ws;
+decltype(&femto_fp4_page_bytes) g_fp4_page;
+decltype(&femto_kv_cache_write_fp4) g_write_fp4;
+decltype(&femto_kv_cache_read_fp4) g_read_fp4;
+decltype(&femto_rope_cache_write_fp4) g_rope_fp4;
+decltype(&femto_paged_attention_gemv_fp4) g_gemv_fp4;
+decltype(&femto_paged_attention_gemv_fp4_workspace_size) g_gemv_fp4_ws;
+decltype(&femto_paged_attention_gemm_fp4) g_gemm_fp4;
+decltype(&femto_paged_attention_gemm_fp4_workspace_size) g_gemm_fp4_ws;
 
 // Thrown (and caught in `guarded`) where the Python path has to take over.
 struct NotHere {};
@@ -148,9 +156,7 @@ void check_paged(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, 
 // HOLD_GIL: for calls of more than one launch over the stream's workspace, which
 // another thread's call on the stream must not come between.
 template <bool HOLD_GIL = false, typename F>
-PyObject* launch(const at::Tensor& out, F call) {
-    PyObject* result = THPVariable_Wrap(out);
-    need(result != nullptr);
+PyObject* launch_for(PyObject* result, F call) {
     int rc;
     PyThreadState* gil = HOLD_GIL ? nullptr : PyEval_SaveThread();
     try {
@@ -163,6 +169,13 @@ PyObject* launch(const at::Tensor& out, F call) {
     Py_DECREF(result);
     PyErr_SetString(PyExc_RuntimeError, rc < 0 ? "femto_native: the library threw" : g_last_error());
     return nullptr;
+}
+
+template <bool HOLD_GIL = false, typename F>
+PyObject* launch(const at::Tensor& out, F call) {
+    PyObject* result = THPVariable_Wrap(out);
+    need(result != nullptr);
+    return launch_for<HOLD_GIL>(result, call);
 }
 
 template <typename F>
@@ -461,6 +474,211 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// ---- calls over a KV cache held in 4 bits (the checks of _C.py) ----
+
+void check_fp4_pool(const at::Tensor& pool, int64_t dim, const at::Device& dev) {
+    need(pool.is_cuda() && pool.device() == dev && pool.scalar_type() == at::kByte && pool.dim() == 3 && pool.is_contiguous());
+    need(dim > 0 && dim <= 128 && dim % 16 == 0 && pool.size(1) > 0 && pool.size(2) == (int64_t)g_fp4_page((int)dim));
+}
+
+// Positions, tables and cu_seqlens (or None) of a cache write of T > 0 tokens.
+struct Placement {
+    const int32_t *cu = nullptr, *positions, *tables;
+    int seqs, tokens, width;
+    int64_t stride;
+};
+Placement placement(PyObject* pos_o, PyObject* tab_o, PyObject* cu_o, int64_t T, const at::Device& dev) {
+    const at::Tensor &pos = tensor(pos_o), &tab = tensor(tab_o);
+    need(pos.scalar_type() == at::kInt && pos.is_contiguous() && pos.device() == dev && pos.numel() == T);
+    need(tab.scalar_type() == at::kInt && tab.dim() == 2 && tab.device() == dev && (tab.size(1) <= 1 || tab.stride(1) == 1));
+    Placement p;
+    p.seqs = int32(tab.size(0));
+    p.tokens = int32(T);
+    p.width = int32(tab.size(1));
+    need(p.seqs > 0 && T > 0);
+    p.stride = p.seqs > 1 ? tab.stride(0) : std::max(tab.stride(0), tab.size(1));
+    if (cu_o == Py_None) {
+        need(T == p.seqs);
+    } else {
+        const at::Tensor& cu = tensor(cu_o);
+        need(cu.scalar_type() == at::kInt && cu.is_contiguous() && cu.device() == dev && cu.numel() - 1 == p.seqs);
+        p.cu = i32(cu);
+    }
+    p.positions = i32(pos);
+    p.tables = i32(tab);
+    return p;
+}
+
+int check_kv_source(const at::Tensor& k, const at::Tensor& v, const at::Tensor& pool) {
+    need(k.is_cuda() && v.device() == k.device() && k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes());
+    need(k.stride(2) == 1 && v.stride(2) == 1 && k.scalar_type() == v.scalar_type() && k.scalar_type() != at::kFloat);
+    check_fp4_pool(pool, k.size(2), k.device());
+    need(k.size(1) == pool.size(1));
+    need_current_device(k);
+    return dtype_code(k);
+}
+
+// write_fp4(k, v, kv_pool, positions, tables, cu_seqlens | None, max_q_len): True where it was made
+PyObject* write_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 7, [&]() -> PyObject* {
+        need(g_write_fp4 && g_fp4_page);
+        const at::Tensor &k = tensor(a[0]), &v = tensor(a[1]), &pool = tensor(a[2]);
+        const int max_q = int32(integer(a[6]));
+        const int dt = check_kv_source(k, v, pool);
+        const Placement p = placement(a[3], a[4], a[5], k.size(0), k.device());
+        void *st = stream_of(k), *pp = pool.data_ptr();
+        const void *kd = k.const_data_ptr(), *vd = v.const_data_ptr();
+        Py_INCREF(Py_True);
+        return launch_for(Py_True, [&] {
+            return g_write_fp4(dt, kd, k.stride(0), k.stride(1), vd, v.stride(0), v.stride(1), pp, pool.size(0), (int)pool.size(1),
+                               (int)k.size(2), p.cu, p.seqs, p.tokens, max_q, p.positions, p.tables, p.width, p.stride, st);
+        });
+    });
+}
+
+// read_fp4(kv_pool, head_dim, bf16, positions, tables, cu_seqlens | None, max_q_len): (k, v)
+PyObject* read_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 7, [&]() -> PyObject* {
+        need(g_read_fp4 && g_fp4_page);
+        const at::Tensor& pool = tensor(a[0]);
+        const int64_t dim = integer(a[1]), T = tensor(a[3]).numel();
+        need(PyBool_Check(a[2]));
+        const bool bf16 = a[2] == Py_True;
+        const int max_q = int32(integer(a[6]));
+        check_fp4_pool(pool, dim, pool.device());
+        need_current_device(pool);
+        const Placement p = placement(a[3], a[4], a[5], T, pool.device());
+        const auto options = pool.options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
+        at::Tensor k = at::empty({T, pool.size(1), dim}, options), v = at::empty({T, pool.size(1), dim}, options);
+        PyObject *ko = THPVariable_Wrap(k), *vo = ko ? THPVariable_Wrap(v) : nullptr;
+        PyObject* both = vo ? PyTuple_Pack(2, ko, vo) : nullptr;
+        Py_XDECREF(ko);
+        Py_XDECREF(vo);
+        need(both != nullptr);
+        void *st = stream_of(pool), *kd = k.data_ptr(), *vd = v.data_ptr();
+        const void* pp = pool.const_data_ptr();
+        return launch_for(both, [&] {
+            return g_read_fp4(bf16 ? FEMTO_BF16 : FEMTO_F16, pp, pool.size(0), (int)pool.size(1), (int)dim, kd, vd, p.cu, p.seqs,
+                              p.tokens, max_q, p.positions, p.tables, p.width, p.stride, st);
+        });
+    });
+}
+
+// rope_fp4(q, k, v, cos, sin, positions, kv_pool, tables, cu_seqlens | None, max_q_len, interleaved, q_weight | None,
+//          k_weight | None, eps, out | None)
+PyObject* rope_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 15, [&]() -> PyObject* {
+        need(g_rope_fp4 && g_fp4_page);
+        const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]), &cos = tensor(a[3]), &sin = tensor(a[4]);
+        const at::Tensor& pool = tensor(a[6]);
+        const int max_q = int32(integer(a[9]));
+        need(PyBool_Check(a[10]) && PyFloat_CheckExact(a[13]));
+        const int interleaved = a[10] == Py_True;
+        const double eps = PyFloat_AS_DOUBLE(a[13]);
+        const int dt = check_kv_source(k, v, pool);
+        for (const at::Tensor* t : {&q, &cos, &sin}) need(t->device() == k.device());
+        need(q.dim() == 3 && q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.size(1) > 0 && q.stride(2) == 1);
+        need(q.scalar_type() == k.scalar_type());
+        need(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat);
+        need(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.strides() == sin.strides() && cos.stride(1) == 1);
+        need(cos.stride(0) >= cos.size(1));
+        const void *wq = nullptr, *wk = nullptr;
+        need((a[11] == Py_None) == (a[12] == Py_None));
+        if (a[11] != Py_None) {
+            const at::Tensor &x = tensor(a[11]), &y = tensor(a[12]);
+            for (const at::Tensor* t : {&x, &y})
+                need(t->device() == q.device() && t->scalar_type() == q.scalar_type() && t->dim() == 1 && t->is_contiguous() &&
+                     t->size(0) == q.size(2));
+            wq = x.const_data_ptr();
+            wk = y.const_data_ptr();
+        }
+        const Placement p = placement(a[5], a[7], a[8], k.size(0), k.device());
+        at::Tensor out = a[14] == Py_None ? at::empty_like(q) : tensor(a[14]);
+        need(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.stride(2) == 1 && out.device() == q.device());
+        if (a[14] != Py_None) {
+            need(out.const_data_ptr() == q.const_data_ptr() && out.strides() == q.strides());
+            need(plainly_apart(out, k) && plainly_apart(out, v));
+            need(out.stride(1) >= out.size(2) || out.size(1) == 1);  // its rows, head by head and token by token
+            need(out.stride(0) >= (out.size(1) - 1) * out.stride(1) + out.size(2) || out.size(0) == 1);
+        }
+        void *st = stream_of(q), *od = out.data_ptr(), *pp = pool.data_ptr();
+        const void *qd = q.const_data_ptr(), *kd = k.const_data_ptr(), *vd = v.const_data_ptr();
+        const float* cd = static_cast<const float*>(cos.const_data_ptr());
+        const float* sd = static_cast<const float*>(sin.const_data_ptr());
+        const int H = int32(q.size(1)), rows = int32(cos.size(0)), R = int32(2 * cos.size(1));
+        return launch(out, [&] {
+            return g_rope_fp4(dt, qd, q.stride(0), q.stride(1), kd, k.stride(0), k.stride(1), vd, v.stride(0), v.stride(1), od,
+                              out.stride(0), out.stride(1), wq, wk, eps, cd, sd, cos.stride(0), rows, R, interleaved, pp,
+                              pool.size(0), H, (int)pool.size(1), (int)q.size(2), p.cu, p.seqs, p.tokens, max_q, p.positions,
+                              p.tables, p.width, p.stride, st);
+        });
+    });
+}
+
+int check_fp4_attention(const at::Tensor& q, const at::Tensor& pool, const at::Tensor& tab, const at::Tensor& len) {
+    need(q.is_cuda() && q.dim() == 3 && q.stride(2) == 1 && q.scalar_type() != at::kFloat);
+    check_fp4_pool(pool, q.size(2), q.device());
+    need(q.size(0) > 0 && q.size(0) % pool.size(1) == 0);
+    need(tab.scalar_type() == at::kInt && tab.dim() == 2 && tab.device() == q.device() && (tab.size(1) <= 1 || tab.stride(1) == 1));
+    need(len.scalar_type() == at::kInt && len.dim() == 1 && len.is_contiguous() && len.device() == q.device());
+    need_current_device(q);
+    return dtype_code(q);
+}
+
+// gemv_fp4(q, kv_pool, tables, kv_lens, max_kv_len, workspaces)
+PyObject* gemv_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 6, [&]() -> PyObject* {
+        need(g_gemv_fp4 && g_gemv_fp4_ws && g_fp4_page);
+        const at::Tensor &q = tensor(a[0]), &pool = tensor(a[1]), &tab = tensor(a[2]), &len = tensor(a[3]);
+        const int max_kv = int32(integer(a[4]));
+        const int dt = check_fp4_attention(q, pool, tab, len);
+        const int64_t H = q.size(0), B = q.size(1);
+        need(B > 0 && B == tab.size(0) && B == len.size(0));
+        void* st = stream_of(q);
+        const size_t bytes = g_gemv_fp4_ws(int32(B), int32(H), (int)pool.size(1), max_kv);
+        if (bytes) need_not_captured(st);
+        const Workspace w = workspace(a[5], q, st, bytes);
+        at::Tensor out = at::empty({H, B, q.size(2)}, q.options());
+        const void *qp = q.const_data_ptr(), *pp = pool.const_data_ptr();
+        const int32_t *tp = i32(tab), *lp = i32(len);
+        void* op = out.data_ptr();
+        return launch<true>(out, [&] {
+            return g_gemv_fp4(dt, qp, q.stride(0), q.stride(1), op, out.stride(0), out.stride(1), pp, pool.size(0),
+                              (int)pool.size(1), (int)q.size(2), tp, (int)tab.size(1), tab.stride(0), lp, (int)B, (int)H, max_kv,
+                              w.ptr, w.bytes, st);
+        });
+    });
+}
+
+// gemm_fp4(q, kv_pool, cu_seqlens, max_q_len, tables, kv_lens, positions, workspaces)
+PyObject* gemm_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 8, [&]() -> PyObject* {
+        need(g_gemm_fp4 && g_gemm_fp4_ws && g_fp4_page);
+        const at::Tensor &q = tensor(a[0]), &pool = tensor(a[1]), &cu = tensor(a[2]), &tab = tensor(a[4]), &len = tensor(a[5]);
+        const at::Tensor& pos = tensor(a[6]);
+        const int max_q = int32(integer(a[3]));
+        const int dt = check_fp4_attention(q, pool, tab, len);
+        need(cu.scalar_type() == at::kInt && cu.is_contiguous() && cu.device() == q.device());
+        need(pos.scalar_type() == at::kInt && pos.is_contiguous() && pos.device() == q.device());
+        const int64_t H = q.size(0), T = q.size(1), B = cu.numel() - 1;
+        need(B > 0 && T > 0 && B == tab.size(0) && B == len.size(0) && T == pos.numel());
+        void* st = stream_of(q);
+        need_not_captured(st);
+        const Workspace w = workspace(a[7], q, st, g_gemm_fp4_ws(int32(B), int32(T), max_q, int32(H), (int)pool.size(1),
+                                                                 int32(tab.size(1))));
+        need(w.ptr != nullptr);
+        at::Tensor out = at::empty({H, T, q.size(2)}, q.options());
+        const void *qp = q.const_data_ptr(), *pp = pool.const_data_ptr();
+        const int32_t *cp = i32(cu), *tp = i32(tab), *lp = i32(len), *sp = i32(pos);
+        void* op = out.data_ptr();
+        return launch<true>(out, [&] {
+            return g_gemm_fp4(dt, qp, q.stride(0), q.stride(1), op, out.stride(0), out.stride(1), pp, pool.size(0),
+                              (int)pool.size(1), (int)q.size(2), cp, (int)B, (int)T, max_q, (int)H, tp, (int)tab.size(1),
+                              tab.stride(0), lp, sp, w.ptr, w.bytes, st);
+        });
+    });
+}
+
 // flash(q, k, v)
 PyObject* flash(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 3, [&]() -> PyObject* {
@@ -505,7 +723,13 @@ PyObject* bind(PyObject*, PyObject* names) {
         !optional("femto_paged_attention_gemv_shared_prefix_workspace_size", g_shared_ws) || !optional("femto_paged_attention_gemv_window", g_gemv_window) ||
         !optional("femto_paged_attention_gemv_window_workspace_size", g_gemv_window_ws) ||
         !optional("femto_paged_attention_gemm_window", g_gemm_window) ||
-        !optional("femto_paged_attention_gemm_window_workspace_size", g_gemm_window_ws))
+        !optional("femto_paged_attention_gemm_window_workspace_size", g_gemm_window_ws) ||
+        !optional("femto_fp4_page_bytes", g_fp4_page) || !optional("femto_kv_cache_write_fp4", g_write_fp4) ||
+        !optional("femto_kv_cache_read_fp4", g_read_fp4) || !optional("femto_rope_cache_write_fp4", g_rope_fp4) ||
+        !optional("femto_paged_attention_gemv_fp4", g_gemv_fp4) ||
+        !optional("femto_paged_attention_gemv_fp4_workspace_size", g_gemv_fp4_ws) ||
+        !optional("femto_paged_attention_gemm_fp4", g_gemm_fp4) ||
+        !optional("femto_paged_attention_gemm_fp4_workspace_size", g_gemm_fp4_ws))
         return nullptr;
     Py_RETURN_NONE;
 }
@@ -520,6 +744,11 @@ PyMethodDef methods[] = {
     {"prologue", FEMTO_FAST(prologue)},
     {"gemv_shared", FEMTO_FAST(gemv_shared)},
     {"rope", FEMTO_FAST(rope)},
+    {"write_fp4", FEMTO_FAST(write_fp4)},
+    {"read_fp4", FEMTO_FAST(read_fp4)},
+    {"rope_fp4", FEMTO_FAST(rope_fp4)},
+    {"gemv_fp4", FEMTO_FAST(gemv_fp4)},
+    {"gemm_fp4", FEMTO_FAST(gemm_fp4)},
     {"flash", FEMTO_FAST(flash)},
     {nullptr, nullptr, 0, nullptr},
 };

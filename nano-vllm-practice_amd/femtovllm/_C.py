@@ -174,7 +174,10 @@ def _load_native():
              "femto_qk_norm_rope_cache_write", "femto_flash_attention",
              "femto_paged_attention_gemv_shared_prefix", "femto_paged_attention_gemv_shared_prefix_workspace_size",
              "femto_rope_cache_write", "femto_paged_attention_gemv_window", "femto_paged_attention_gemv_window_workspace_size",
-             "femto_paged_attention_gemm_window", "femto_paged_attention_gemm_window_workspace_size")
+             "femto_paged_attention_gemm_window", "femto_paged_attention_gemm_window_workspace_size",
+             "femto_fp4_page_bytes", "femto_kv_cache_write_fp4", "femto_kv_cache_read_fp4", "femto_rope_cache_write_fp4",
+             "femto_paged_attention_gemv_fp4", "femto_paged_attention_gemv_fp4_workspace_size",
+             "femto_paged_attention_gemm_fp4", "femto_paged_attention_gemm_fp4_workspace_size")
     module.bind({n: ctypes.cast(getattr(_lib, n), ctypes.c_void_p).value for n in names})
     return module
 
@@ -820,6 +823,8 @@ def _check_kv_source(fn, k, v, kv_pool):
 
 def _kv_cache_write_fp4(k, v, kv_pool, positions, kv_page_tables, cu_seqlens=None, max_q_len=1):
     """Round k, v (tokens, n_kv_heads, head_dim) to 4 bits, into the paged pool in place."""
+    if _native.write_fp4(k, v, kv_pool, positions, kv_page_tables, cu_seqlens, max_q_len):
+        return
     fn = "kv_cache_write_fp4"
     dtype = _check_kv_source(fn, k, v, kv_pool)
     stride, cu_ptr = _check_placement(fn, positions, kv_page_tables, cu_seqlens, k.size(0), k.device)
@@ -840,6 +845,10 @@ def _kv_cache_write_fp4(k, v, kv_pool, positions, kv_page_tables, cu_seqlens=Non
 
 def _kv_cache_read_fp4(kv_pool, head_dim, dtype, positions, kv_page_tables, cu_seqlens=None, max_q_len=1):
     """(k, v) of the tokens, (tokens, n_kv_heads, head_dim) of ``dtype``."""
+    if dtype in (torch.bfloat16, torch.float16):
+        both = _native.read_fp4(kv_pool, head_dim, dtype is torch.bfloat16, positions, kv_page_tables, cu_seqlens, max_q_len)
+        if both is not None:
+            return both
     fn = "kv_cache_read_fp4"
     head_dim = operator.index(head_dim)
     _check_fp4_pool(fn, kv_pool, head_dim, kv_pool.device)
@@ -863,6 +872,10 @@ def _kv_cache_read_fp4(kv_pool, head_dim, dtype, positions, kv_page_tables, cu_s
 def _rope_cache_write_fp4(q, k, v, cos, sin, positions, kv_pool, kv_page_tables, cu_seqlens=None, max_q_len=1,
                           interleaved=False, q_weight=None, k_weight=None, eps=1e-6, out=None):
     """Normed (with weights) and rotated q to ``out``, rotated k and v in 4 bits into the pool; returns ``out``."""
+    done = _native.rope_fp4(q, k, v, cos, sin, positions, kv_pool, kv_page_tables, cu_seqlens, max_q_len, interleaved,
+                            q_weight, k_weight, eps, out)
+    if done is not None:
+        return done
     fn = "rope_cache_write_fp4"
     dtype = _check_kv_source(fn, k, v, kv_pool)
     for name, t in (("q", q), ("cos", cos), ("sin", sin)):
@@ -928,6 +941,9 @@ def _check_fp4_attention(fn, q, kv_pool, tables, kv_lens):
 
 def _paged_attention_gemv_fp4(q, kv_pool, kv_page_tables, kv_lens, max_kv_len):
     """Decode over a 4-bit cache; out (n_heads, num_seqs, head_dim)."""
+    out = _native.gemv_fp4(q, kv_pool, kv_page_tables, kv_lens, max_kv_len, _fp4_workspaces)
+    if out is not None:
+        return out
     fn = "paged_attention_gemv_fp4"
     dtype = _check_fp4_attention(fn, q, kv_pool, kv_page_tables, kv_lens)
     n_heads, num_seqs, dim = q.shape
@@ -956,6 +972,9 @@ def _paged_attention_gemv_fp4(q, kv_pool, kv_page_tables, kv_lens, max_kv_len):
 
 def _paged_attention_gemm_fp4(q, kv_pool, cu_seqlens, max_q_len, kv_page_tables, kv_lens, positions):
     """Varlen causal prefill over a 4-bit cache; out (n_heads, num_tokens, head_dim)."""
+    out = _native.gemm_fp4(q, kv_pool, cu_seqlens, max_q_len, kv_page_tables, kv_lens, positions, _fp4_prefill_workspaces)
+    if out is not None:
+        return out
     fn = "paged_attention_gemm_fp4"
     dtype = _check_fp4_attention(fn, q, kv_pool, kv_page_tables, kv_lens)
     for name, t in (("cu_seqlens", cu_seqlens), ("positions", positions)):
