@@ -659,16 +659,58 @@ static int fp4_source(const std::string& f, const void* k, int64_t k_stride_toke
     return FEMTO_OK;
 }
 
-// Workgroups per row and waves in each of a decode call over a 4-bit cache, and
-// its workspace: counters, then the parts' states; none where every row is one part.
+// Decode calls over a 4-bit cache.  A row (a sequence's query heads of one KV
+// head, up to kMfmaHeads) is a workgroup, or a few where there are fewer rows
+// than CUs, or all rows are cut into equal slices for split workers.  Measured
+// (bf16, 32/8 heads unless said, us; equal contexts / drawn from a sixteenth on):
+//  * parts of a row: about a third of the root of its pages, as far as each has a
+//    CU of its own.  One sequence (8 rows) of 2048 keys 11.1 whole, 9.6 in two,
+//    8.6 in four, 9.4 in eight; 32768: 22.3 in eight, 19.2 in 16.  Sixteen of 8192:
+//    33.3 whole, 26.5 in two, 31.1 in four.  1024 keys: 8.1 whole, 8.0 in four;
+//  * waves of a workgroup: eight where there is at most a row per CU (32 sequences
+//    of 2048 keys 14.4, with four 16.9) or rows of 8192 keys and more in a few
+//    rounds (128 of 8192: 173 / 110, with four 182 / 120); else four (128 of 1024:
+//    30.8 / 19.5, with eight 33.0 / 26.8; 256 of 8192: 339 / 203 and 344 / 205);
+//  * split workers, which do not care how uneven contexts are, but cost a merge
+//    launch: with a row per CU or more past 12288 keys (64 of 16384: 171 / 113, as
+//    rows 169 / 123; 32 of 8192: 51.0 / 37.5, as rows 46.4 / 34.3), with half as
+//    many past 24576 (16 of 32768: 93.3 / 60.4, as rows 88.4 / 67.5; of 16384
+//    51.7 / 37.7 and 47.7 / 37.5).
 struct Fp4DecodePlan {
+    bool split;
     WindowParts rows;
-    size_t bytes;
+    femto::DecodePlan slots;
+    size_t bytes;  // workspace: counters, then the parts' or slices' states; none for rows in one part
 };
+static WindowParts fp4_rows(int64_t rows, int n_heads, int n_kv_heads, int max_kv_len, int cus) {
+    const int n_rep = n_heads / n_kv_heads;
+    const int64_t groups = rows * n_kv_heads * ((n_rep + femto::kMfmaHeads - 1) / femto::kMfmaHeads);
+    const int pages = max_kv_len > 0 ? (max_kv_len - 1) / femto::kPage + 1 : 0;
+    WindowParts w{1, 4};
+    if (pages >= 96 && 2 * groups <= cus)
+        w.parts = std::min((int)(cus / groups), (int)(0.354 * std::sqrt((double)pages) + 0.5));
+    if ((groups <= cus && pages >= 32) || (groups <= 4 * cus && pages >= 512)) w.waves = 8;
+    return w;
+}
 static Fp4DecodePlan fp4_decode_plan(int num_seqs, int n_heads, int n_kv_heads, int max_kv_len, int cus) {
-    Fp4DecodePlan p;
-    p.rows = window_parts(num_seqs, n_heads, n_kv_heads, max_kv_len, cus);
-    p.bytes = p.rows.parts > 1 ? kWindowZeroBytes + femto::decode_workspace_bytes(num_seqs, n_heads, p.rows.parts) : 0;
+    Fp4DecodePlan p{};
+    const int limit = g_single_max_kv.load(std::memory_order_relaxed);
+    p.rows = fp4_rows(num_seqs, n_heads, n_kv_heads, max_kv_len, cus);
+    if (limit == kSingleMaxKV) {
+        const int n_rep = n_heads / n_kv_heads;
+        const int64_t groups = (int64_t)num_seqs * n_kv_heads * ((n_rep + femto::kMfmaHeads - 1) / femto::kMfmaHeads);
+        p.split = (max_kv_len > 12288 && groups >= cus) || (max_kv_len > 24576 && 2 * groups >= cus);
+    } else {
+        p.split = max_kv_len > limit;
+        p.rows.parts = 1;
+    }
+    if (p.split) {
+        p.slots = femto::plan_paged_decode(n_heads, 1, max_kv_len, femto::kDtypeBF16);  // slots only
+        p.bytes = kWindowZeroBytes + femto::decode_workspace_bytes(num_seqs, n_heads, p.slots.max_slots);
+    } else {
+        p.slots.max_slots = p.rows.parts;
+        p.bytes = p.rows.parts > 1 ? kWindowZeroBytes + femto::decode_workspace_bytes(num_seqs, n_heads, p.rows.parts) : 0;
+    }
     return p;
 }
 
@@ -679,7 +721,7 @@ static WindowParts gemm_fp4_parts(int num_seqs, int num_tokens, int max_q_len, i
     const int rows = femto::decode_rows_bound(num_seqs, num_tokens, max_q_len);
     if (rows == 0) return {0, 0};
     const int table_keys = (int)std::min<int64_t>((int64_t)num_pages_per_seq * femto::kPage, 1 << 30);
-    WindowParts p = window_parts(rows, n_heads, n_kv_heads, table_keys, resident / 2);
+    WindowParts p = fp4_rows(rows, n_heads, n_kv_heads, table_keys, resident / 2);
     const int n_rep = n_heads / n_kv_heads;
     if ((int64_t)num_seqs * n_kv_heads * ((n_rep + femto::kMfmaHeads - 1) / femto::kMfmaHeads) > resident) p.parts = 1;
     return p;
@@ -1318,13 +1360,14 @@ int femto_paged_attention_gemv_fp4(int dtype, const void* q, int64_t q_stride_he
         return fail(FEMTO_ERR_INVALID, fn + ": workspace of " + std::to_string(w.bytes) +
                                            " bytes (256-byte aligned) required, got " + std::to_string(workspace_bytes));
     const int page = femto::fp4_page_bytes(head_dim);
-    femto::DecodePlan plan{};
+    femto::DecodePlan plan = w.slots;
     plan.nrep_tile = 1;
-    plan.max_slots = w.rows.parts;
     femto::DecodeArgs a = femto::decode_args(
         plan, q, q_stride_head, q_stride_seq, out, out_stride_head, out_stride_seq, kv_pool, nullptr, num_blocks, n_kv_heads,
         head_dim, (int64_t)n_kv_heads * page, page, 0, kv_page_tables, num_pages_per_seq, table_stride, kv_lens, num_seqs,
         n_heads, w.bytes ? static_cast<char*>(workspace) + kWindowZeroBytes : nullptr);
+    if (w.split)
+        return hip_status(femto::launch_fp4_split(dtype, a, num_seqs, static_cast<hipStream_t>(stream)), (fn + " launch").c_str());
     a.merge_counters = w.bytes ? static_cast<int*>(workspace) : nullptr;
     a.parts = w.rows.parts;
     a.single_waves = w.rows.waves;

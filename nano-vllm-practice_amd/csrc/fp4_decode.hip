@@ -1,10 +1,16 @@
 // Decode over a KV cache held in 4 bits: the kernel of fp4_decode.h and its
 // launches.
+#include <algorithm>
+
 #include "fp4_decode.h"
 
 namespace femto {
 
-constexpr int kFp4Stages = 3;  // pairs of pages in registers, one of them computed
+// Pairs of pages in registers, one of them computed (three: 0-3 % slower, but 3-8 %
+// faster for calls of four waves a row and equal contexts).
+constexpr int kFp4Stages = 2;
+// Split workers: waves per CU (4 or 6: 3-14 % slower, 10 or more 3-8 %).
+constexpr int kFp4SplitWaves = 8;
 
 template <typename E, bool FULL, int W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) void fp4_decode_kernel(DecodeArgs a) {
@@ -21,6 +27,35 @@ static hipError_t launch_rows(const DecodeArgs& a, int num_seqs, hipStream_t st)
     if (a.single_waves == 8) hipLaunchKernelGGL((fp4_decode_kernel<E, FULL, 8>), dim3((unsigned)grid), dim3(512), 0, st, a);
     else hipLaunchKernelGGL((fp4_decode_kernel<E, FULL, 4>), dim3((unsigned)grid), dim3(256), 0, st, a);
     return hipGetLastError();
+}
+
+template <typename E, bool FULL>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void fp4_split_kernel(DecodeArgs a) {
+    fp4_waves<E, FULL, kFp4Stages>(a, blockIdx.x);
+}
+
+template <typename E, bool FULL>
+static hipError_t launch_split(int dtype, DecodeArgs a, int num_seqs, hipStream_t st) {
+    int cus = 0;
+    hipError_t e = device_cu_count(cus);
+    if (e != hipSuccess) return e;
+    a.waves_per_group = std::max(1, cus * kFp4SplitWaves / a.grid_heads);
+    const int grid = (a.waves_per_group * a.grid_heads + 3) / 4;
+    hipLaunchKernelGGL((fp4_split_kernel<E, FULL>), dim3(grid), dim3(256), 0, st, a);
+    e = hipGetLastError();
+    return e == hipSuccess ? launch_paged_decode_merge(dtype, a, num_seqs, st) : e;
+}
+
+hipError_t launch_fp4_split(int dtype, DecodeArgs a, int num_seqs, hipStream_t st) {
+    if (num_seqs <= 0 || a.n_heads <= 0) return hipSuccess;
+    if (a.head_dim <= 0 || a.head_dim > kDimHead || a.head_dim % 16) return hipErrorInvalidValue;
+    set_mfma_heads(a);
+    const bool full = a.head_dim == kDimHead;
+    switch (dtype) {
+        case kDtypeBF16: return full ? launch_split<BF16, true>(dtype, a, num_seqs, st) : launch_split<BF16, false>(dtype, a, num_seqs, st);
+        case kDtypeF16: return full ? launch_split<F16, true>(dtype, a, num_seqs, st) : launch_split<F16, false>(dtype, a, num_seqs, st);
+        default: return hipErrorInvalidValue;
+    }
 }
 
 hipError_t launch_fp4_decode(int dtype, DecodeArgs a, int num_seqs, hipStream_t st) {

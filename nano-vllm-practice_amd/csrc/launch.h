@@ -87,6 +87,8 @@ hipError_t launch_window_decode(int dtype, const DecodeArgs& a, int nrep_tile, i
 // a.parts workgroups of a.single_waves waves per (sequence, KV head group).  The
 // pool is a.k_pool, its block and head strides in bytes.
 hipError_t launch_fp4_decode(int dtype, DecodeArgs a, int num_seqs, hipStream_t st);
+// ... or split workers and the merge launch (a.max_slots, a.min_chunk_pages).
+hipError_t launch_fp4_split(int dtype, DecodeArgs a, int num_seqs, hipStream_t st);
 
 struct PrefillArgs {
     const void* q;

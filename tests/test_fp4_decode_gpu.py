@@ -69,6 +69,15 @@ def test_max_kv_len_only_plans(ops, gpu, max_kv_len):
     check(ops, gpu, w, f"max_kv_len {max_kv_len}", max_kv_len=max_kv_len)
 
 
+@pytest.mark.parametrize("lens", [[3000], [16384, 20, 17], [500, 1, 0, 2047], [33000] + [40] * 15, [17000] + [300] * 31])
+def test_rows_in_parts_and_split_calls(ops, gpu, lens):
+    """Few long rows are cut into parts (short ones among them into fewer), many of the longest contexts run split."""
+    w = Batch([(max(n - 1, 0), min(n, 1)) for n in lens], 16, 8, 128, BF16, sum(lens), decode=True)
+    a = check(ops, gpu, w, f"lens {lens[:3]}")
+    for _ in range(5):  # parts are merged in order, whoever comes last
+        assert torch.equal(run(ops, gpu, w), a)
+
+
 @pytest.mark.usefixtures("decode_path")
 def test_blocks_outside_the_pool_and_short_tables(ops, gpu):
     """A block id outside the pool and a column past the table read as zeros, with their weight."""
