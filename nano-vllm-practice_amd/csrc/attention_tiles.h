@@ -197,16 +197,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // each XCD takes a contiguous range of the work list (KV head groups
     // outermost, so a head's pages stay in one L2).
     int lin = blockIdx.x;
-    if constexpr (FUSED && WINDOW) {
-        // Decode rows under the window, short pieces of work: the first
+    if constexpr (FUSED && (WINDOW || FP4)) {
+        // Decode rows under the window or over a 4-bit cache: the first
         // a.rows_first workgroups, so that rows run beside tiles from the
         // start, and those after the tiles.
         const int tiles = (int)gridDim.x - a.decode_blocks;
         if (lin < a.rows_first || lin >= a.rows_first + tiles) {
             const int row = lin < a.rows_first ? lin : lin - tiles;
             __shared__ float s_ml[4][kMfmaHeads][2];
-            static_assert(sizeof(smem) >= 4 * kWorkerLds<kStagesTiles>, "the rows' pages");
-            window_row<E, FULLD, 4, kStagesTiles>(a.dec, row, &smem[0][0][0], s_ml, &s_old);
+            if constexpr (FP4) {
+                static_assert(sizeof(smem) >= 4 * kFp4WaveLds, "the waves' outputs");
+                fp4_row<E, FULLD, 4, 4>(a.dec, row, &smem[0][0][0], s_ml, &s_old);
+            } else {
+                static_assert(sizeof(smem) >= 4 * kWorkerLds<kStagesTiles>, "the rows' pages");
+                window_row<E, FULLD, 4, kStagesTiles>(a.dec, row, &smem[0][0][0], s_ml, &s_old);
+            }
             return;
         }
         lin -= a.rows_first;  // a multiple of 8: the XCD of a tile is unchanged
@@ -291,7 +296,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 dec = a.skip_decode_rows && ql == 1;
                 if (dec) ql = 0;  // run by the decode workers
             }
-            if constexpr (FUSED && !WINDOW) spread = __ballot(dec) != 0;
+            if constexpr (FUSED && !WINDOW && !FP4) spread = __ballot(dec) != 0;
             const int nt = ql > 0 ? (ql + BT - 1) / BT : 0;
             int pp = 1, total = wave_sum_i32(nt);
             if (split) {
@@ -377,7 +382,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 // the work total and each sequence's first query tile.
                 const int nt = tid < a.num_seqs && my_ql > 0 ? (my_ql + BT - 1) / BT : 0;
                 // beside decode workers with one-token sequences the copies are spread
-                if constexpr (FUSED && !WINDOW) spread = __syncthreads_or(my_dec) != 0;
+                if constexpr (FUSED && !WINDOW && !FP4) spread = __syncthreads_or(my_dec) != 0;
                 int total;
                 const int incl = block_incl_scan(nt, s_red, total);
                 const int work = groups * total;
@@ -420,7 +425,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
                     for (int k = 0; k <= kSplitTries + 1; ++k) cnt[k] += c[k];
                 }
-                if constexpr (FUSED && !WINDOW) spread = __builtin_amdgcn_readfirstlane(cnt[kSplitTries + 1]) > 0;
+                if constexpr (FUSED && !WINDOW && !FP4) spread = __builtin_amdgcn_readfirstlane(cnt[kSplitTries + 1]) > 0;
                 int T = 0, total = cnt[kSplitTries];
                 if (split) {
 #pragma unroll
@@ -562,25 +567,35 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int fp4_n = fp4_blocks(FULLD ? kDimHead : a.head_dim);
     u32x4 v4 = {0, 0, 0, 0};
     uint32_t v4_scale = 0, k4_scale = 0;
-    auto issue_fp4 = [&](int it, int stage) __attribute__((always_inline)) {
+    uint64_t page4 = 0;  // the wave's page of the tile that v4 is of
+    uint64_t zero4 = 0;
+    const uint32_t blocks4 = (uint32_t)min(a.num_blocks, (int64_t)0x7fffffff);  // (an id below 0 is past it, too)
+    if constexpr (FP4) {
+        zero4 = (uint64_t)(uintptr_t)g_zero_page;
+        asm volatile("" : "+s"(zero4));  // (else its address is loaded, and waited for, in every tile)
+    }
+    auto load_fp4 = [&](int it) __attribute__((always_inline)) {
         const int key0 = it * kKvTile + 16 * wave;
         const int blk = key0 < kv_len ? __builtin_amdgcn_readlane(tbl, it - tbase) : -1;
-        const bool ok = blk >= 0 && (int64_t)blk < a.num_blocks;
-        const char* page = ok ? kbase_p + (int64_t)blk * a.k_stride0 + (int64_t)kvh * a.k_stride1
-                              : reinterpret_cast<const char*>(g_zero_page);
+        const bool ok = (uint32_t)blk < blocks4;
+        const GlobalBytes page = ok ? as_global(kbase_p) + (int64_t)blk * a.k_stride0 + (int64_t)kvh * a.k_stride1
+                                    : (GlobalBytes)(uintptr_t)zero4;
+        page4 = (uint64_t)(uintptr_t)page;
         // Lanes of dims past the row's blocks take block 0's (q is zero there, and
         // those output dims are not stored).
         const int vc = FULLD || lpos < 4 * fp4_n ? lpos : 0;
-        lds_dma_one((uint64_t)(uintptr_t)page, FULLD || lane < 16 * fp4_n ? 16 * lane : 0,
+        v4 = load_global<u32x4>(page + 256 * fp4_n + 64 * fp4_n * lrow + 16 * vc);
+        v4_scale = load_global<uint32_t>(page + 512 * fp4_n + 64 + 16 * lrow + 4 * (vc >> 2));
+        k4_scale = load_global<uint32_t>(page + 512 * fp4_n + 4 * lpos);
+    };
+    auto copy_fp4 = [&](int stage) __attribute__((always_inline)) {
+        lds_dma_one(page4, FULLD || lane < 16 * fp4_n ? 16 * lane : 0,
                     lds_addr(&smem[stage][0][1024 * wave]));
-        v4 = ld16(page + 256 * fp4_n + 64 * fp4_n * lrow + 16 * vc);
-        v4_scale = *reinterpret_cast<const uint32_t*>(page + 512 * fp4_n + 64 + 16 * lrow + 4 * (vc >> 2));
-        k4_scale = *reinterpret_cast<const uint32_t*>(page + 512 * fp4_n + 4 * lpos);
     };
     // ... and into LDS: V as rows of the storage type, zeros past kv_len (their
     // weights are 0, and 0 times a NaN would not be); K's scales behind its codes,
     // those of blocks past the row's 1.
-    auto store_fp4 = [&](int it, int stage) __attribute__((always_inline)) {
+    auto mask_fp4 = [&](int it) __attribute__((always_inline)) {
         const int key0 = it * kKvTile + 16 * wave + 4 * lrow;
         if (it * kKvTile + kKvTile > kv_len) {  // wave-uniform
 #pragma unroll
@@ -589,12 +604,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 v4_scale = key0 + j < kv_len ? v4_scale : v4_scale & ~(0xffu << (8 * j));
             }
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int row = 16 * wave + 4 * lrow + j;
-            const float s = __uint_as_float((j == 3 ? v4_scale >> 1 : v4_scale << (23 - 8 * j)) & 0x7f800000u);
-            *reinterpret_cast<u32x4*>(&smem[stage][1][row * kRowBytes + ((lpos ^ swz_v(row)) << 4)]) = fp4_unpack8(E{}, v4[j], s);
-        }
+    };
+    auto store_row_fp4 = [&](int j, int stage) __attribute__((always_inline)) {
+        const int row = 16 * wave + 4 * lrow + j;
+        const float s = __uint_as_float((j == 3 ? v4_scale >> 1 : v4_scale << (23 - 8 * j)) & 0x7f800000u);
+        *reinterpret_cast<u32x4*>(&smem[stage][1][row * kRowBytes + ((lpos ^ swz_v(row)) << 4)]) = fp4_unpack8(E{}, v4[j], s);
+    };
+    auto store_scales_fp4 = [&](int stage) __attribute__((always_inline)) {
         if (lane < 16) {
             uint32_t ks = k4_scale;
             if constexpr (!FULLD) {
@@ -605,7 +621,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
     };
     auto issue_tile = [&](int it, int stage) __attribute__((always_inline)) {
-        if constexpr (FP4) return issue_fp4(it, stage);
+        if constexpr (FP4) {
+            load_fp4(it);
+            copy_fp4(stage);
+            return;
+        }
         const int key0 = it * kKvTile + 16 * wave;  // first key of this wave's page
         // Keys past the last one seen (kv_len; under a window seen_end) read
         // its row (finite data, masked later); pages wholly past it read that
@@ -795,7 +815,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if constexpr (FP4) {
         const char* qrow = reinterpret_cast<const char*>(a.q) + ((int64_t)h * a.q_stride_head + (int64_t)t * a.q_stride_token) * EB;
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) q4[kk] = fp4_query_row<E>(qrow, 2 * kk + h2, FULLD ? kDimHead : a.head_dim, qvalid);
+        for (int kk = 0; kk < 2; ++kk) q4[kk] = fp4_query_row<E>(qrow, 2 * kk + h2, FULLD ? kDimHead : a.head_dim, qvalid, a.scale_log2);
     } else {
         const char* qrow = reinterpret_cast<const char*>(a.q) +
                            ((int64_t)b * a.q_stride_batch + (int64_t)h * a.q_stride_head + (int64_t)t * a.q_stride_token) * EB;
@@ -817,8 +837,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     f32x16 oacc[4];
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) oacc[dt] = f32x16{};
-    float m_run = kEmptyMaxP;
+    float m_run = FP4 ? 0.0f : kEmptyMaxP;
     float l_run = 0.0f;
+    // kFp4Pages: q holds the scale, and the scores start from minus the running max
+    // (0 before the first tile, which sets it), so the exponentials take them as
+    // they are; m_late is what the max moved by since block 1's scores started.
+    f32x16 neg_m16 = f32x16{};
+    float m_late = 0.0f;
+    auto set_max = [&](float m) __attribute__((always_inline)) {
+        m_run = m;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) neg_m16[x] = -m;
+    };
     const float scale = a.scale_log2;
 
     // One 64-key tile from LDS stage STAGE (a compile-time constant, so the
@@ -861,7 +891,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             float e[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                e[j] = fast_exp2(fmaf(sv[2 * i + j], scale, neg_m));
+                e[j] = fast_exp2(FP4 ? sv[2 * i + j] : fmaf(sv[2 * i + j], scale, neg_m));
             }
             const uint32_t w = pack2(E{}, e[0], e[1]);
             pw[i >> 2][i & 3] = w;
@@ -912,22 +942,49 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 for (int x = 0; x < 16; ++x) mx = fmaxf(mx, fmaxf(sv[x], seen(32 + 8 * (x >> 2) + (x & 3)) ? s1[x] : -INFINITY));
                 float m_lo, m_hi;  // the row's two lane halves (keys 4*h2 + ...)
                 pair32(mx, m_lo, m_hi);
-                m_run = fmaxf(m_run, fmaxf(m_lo, m_hi) * scale);
-                neg_m = -m_run;
+                if constexpr (FP4) {
+                    const float m = fmaxf(m_lo, m_hi);
+                    m_late = m > -INFINITY ? m : 0.0f;  // (a row of a later piece that sees no key of it)
+                    set_max(m_late);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) sv[x] -= m_late;
+                } else {
+                    m_run = fmaxf(m_run, fmaxf(m_lo, m_hi) * scale);
+                    neg_m = -m_run;
+                }
                 sum = l_run;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) soft(sv, i, pw, sum);
             }
-            if (__builtin_expect(__ballot(sum - l_run > kMaxBlockSum) != 0, 0)) {
+            bool moved = sum - l_run > kMaxBlockSum;
+            if constexpr (FP4) moved |= kb2 == 1 && m_late != 0.0f;
+            if (__builtin_expect(__ballot(moved) != 0, 0)) {
+                if constexpr (FP4) {
+                    if (kb2 == 1) {
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) sv[x] -= m_late;
+                        m_late = 0.0f;
+                    }
+                }
                 float mx = sv[0];
 #pragma unroll
                 for (int x = 1; x < 16; ++x) mx = fmaxf(mx, sv[x]);
                 float m_lo, m_hi;
                 pair32(mx, m_lo, m_hi);
-                const float m_new = fmaxf(m_run, fmaxf(m_lo, m_hi) * scale);
-                const float alpha = fast_exp2(m_run - m_new);
-                m_run = m_new;
-                neg_m = -m_new;
+                float alpha;
+                if constexpr (FP4) {
+                    const float up = fmaxf(0.0f, fmaxf(m_lo, m_hi));
+                    alpha = fast_exp2(-up);
+                    set_max(m_run + up);
+                    if (kb2 == 0) m_late += up;
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) sv[x] -= up;
+                } else {
+                    const float m_new = fmaxf(m_run, fmaxf(m_lo, m_hi) * scale);
+                    alpha = fast_exp2(m_run - m_new);
+                    m_run = m_new;
+                    neg_m = -m_new;
+                }
                 l_run *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < 4; ++dt) oacc[dt] *= alpha;
@@ -965,7 +1022,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             // MFMA m of a block: term 2 - m / 2 (the smallest first), half m % 2 of the dims.
             auto score = [&](f32x16& s, int block, auto m_c) __attribute__((always_inline)) {
                 constexpr int m = decltype(m_c)::value, kk = m & 1, term = 2 - (m >> 1);
-                s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(k4[block][kk]), fp4_operand(q4[kk].term[term]), s,
+                s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(k4[block][kk]), fp4_operand(q4[kk].term[term]),
+                                                                    m == 0 ? neg_m16 : s,
                                                                     kFormatFp4, kFormatFp6, 2 * kk, (int)ks4[block], term,
                                                                     (int)q4[kk].scales);
             };
@@ -996,6 +1054,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             bundle1(std::integral_constant<int, 3>{});
             bundle1(std::integral_constant<int, 4>{});
             bundle1(std::integral_constant<int, 5>{});
+            asm volatile("" ::"v"(s1));  // (keeps its MFMAs from being sunk below settle's branches)
         } else {
 #pragma unroll
         for (int n = 0; n < kAhead; ++n) kf[n] = kfrag(n);
@@ -1036,10 +1095,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
         asm volatile("" : "+v"(p1[0]), "+v"(p1[1]), "+v"(sum1));
         settle(s1, 1, p1, sum1);
+        if constexpr (FP4) mask_fp4(kb / kKvTile + 1);
 #pragma unroll
         for (int n = 8; n < 16; ++n) {
             if (n + kAhead < 16) vf[(n + kAhead) % (kAhead + 1)] = vfrag(n + kAhead);
             oacc[n & 3] = mfma32x32x16(E{}, vf[n % (kAhead + 1)], p1[(n >> 2) - 2], oacc[n & 3]);
+            if constexpr (FP4) {  // beside them the next tile's V is converted
+                if (n % 2 == 0) store_row_fp4(n / 2 - 4, STAGE ^ 1);
+                if (n == 15) store_scales_fp4(STAGE ^ 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
 
@@ -1082,14 +1147,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 for (int j = 0; j < 8; ++j) copy_one(j);
             }
         } else {
-            if (any) tile_math(kb, STAGE == 0 && it == t_lo, stage_c, std::false_type{});
-        }
-        if constexpr (FP4) {
-            if (more) store_fp4(next, STAGE ^ 1);
+            if constexpr (FP4) {
+                // (after the last tile: whatever the registers hold, into the stage that nothing reads)
+                if (any) {
+                    tile_math(kb, STAGE == 0 && it == t_lo, stage_c, std::false_type{});
+                } else {
+                    mask_fp4(next);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) store_row_fp4(j, STAGE ^ 1);
+                    store_scales_fp4(STAGE ^ 1);
+                }
+            } else {
+                if (any) tile_math(kb, STAGE == 0 && it == t_lo, stage_c, std::false_type{});
+            }
         }
     };
     if constexpr (FP4) {
-        if (t_hi > t_lo) store_fp4(t_lo, 0);  // (t_first: the piece's first tile does not depend on the positions)
+        if (t_hi > t_lo) {  // (t_lo is t_first: the piece's first tile does not depend on the positions)
+            mask_fp4(t_lo);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) store_row_fp4(j, 0);
+            store_scales_fp4(0);
+        }
     }
     auto tile_loop = [&](auto spread_c) __attribute__((always_inline)) {
         for (int it = t_lo; it < t_hi; it += 2) {
@@ -1153,6 +1232,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         {
             const auto r = slot_rsrc(slot_of(piece));
             float l_pub = l_run;
+            if constexpr (FP4) {  // a row that saw no key of the piece has no maximum
+                float l_lo, l_hi;
+                pair32(l_run, l_lo, l_hi);
+                if (l_lo + l_hi == 0.0f) m_run = kEmptyMaxP;
+            }
             if constexpr (kHalf) {
                 float l_lo, l_hi;
                 pair32(l_run, l_lo, l_hi);
@@ -1344,7 +1428,7 @@ static hipError_t launch_gf(int G, const PrefillArgs& a, hipStream_t st) {
 template <typename E, bool PAGED, int RULE>
 static hipError_t launch_g(int G, const PrefillArgs& a, hipStream_t st) {
     if constexpr (RULE == kTailPages) return launch_gf<E, true, true, RULE>(G, a, st);
-    if constexpr (PAGED && RULE != kTailPages && RULE != kFp4Pages) {
+    if constexpr (PAGED && RULE != kTailPages) {
         if (a.decode_blocks > 0) return launch_gf<E, true, true, RULE>(G, a, st);
     }
     if constexpr (RULE != kTailPages) return launch_gf<E, PAGED, false, RULE>(G, a, st);

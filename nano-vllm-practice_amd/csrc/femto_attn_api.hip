@@ -664,18 +664,18 @@ static int fp4_source(const std::string& f, const void* k, int64_t k_stride_toke
 // than CUs, or all rows are cut into equal slices for split workers.  Measured
 // (bf16, 32/8 heads unless said, us; equal contexts / drawn from a sixteenth on):
 //  * parts of a row: about a third of the root of its pages, as far as each has a
-//    CU of its own.  One sequence (8 rows) of 2048 keys 11.1 whole, 9.6 in two,
-//    8.6 in four, 9.4 in eight; 32768: 22.3 in eight, 19.2 in 16.  Sixteen of 8192:
-//    33.3 whole, 26.5 in two, 31.1 in four.  1024 keys: 8.1 whole, 8.0 in four;
+//    CU of its own.  One sequence (8 rows) of 2048 keys 11.0 whole, 9.5 in two,
+//    8.4 in four, 9.4 in eight; 32768: 21.7 in eight, 19.0 in 16.  Sixteen of 8192:
+//    32.2 whole, 26.4 in two, 30.8 in four.  1024 keys: 8.0 whole, 7.9 in four;
 //  * waves of a workgroup: eight where there is at most a row per CU (32 sequences
-//    of 2048 keys 14.4, with four 16.9) or rows of 8192 keys and more in a few
-//    rounds (128 of 8192: 173 / 110, with four 182 / 120); else four (128 of 1024:
-//    30.8 / 19.5, with eight 33.0 / 26.8; 256 of 8192: 339 / 203 and 344 / 205);
+//    of 2048 keys 14.4, with four 16.7; of 256 keys 6.3 and 6.2) or rows of 8192
+//    keys and more (128: 171 / 108, with four 180 / 119); else four (128 of 1024:
+//    29.7 / 19.2, with eight 33.1 / 26.8; of 4096 93.7 / 58.1 and 92.1 / 60.8);
 //  * split workers, which do not care how uneven contexts are, but cost a merge
-//    launch: with a row per CU or more past 12288 keys (64 of 16384: 171 / 113, as
-//    rows 169 / 123; 32 of 8192: 51.0 / 37.5, as rows 46.4 / 34.3), with half as
-//    many past 24576 (16 of 32768: 93.3 / 60.4, as rows 88.4 / 67.5; of 16384
-//    51.7 / 37.7 and 47.7 / 37.5).
+//    launch: with a row per CU or more past 12288 keys (64 of 16384: 170 / 112, as
+//    rows 168 / 120; 32 of 8192: 51.3 / 37.4, as rows 45.9 / 33.7), with half as
+//    many past 24576 (16 of 32768: 92.0 / 61.0, as rows 88.1 / 66.3; of 16384
+//    51.2 / 38.0 and 47.6 / 36.6).
 struct Fp4DecodePlan {
     bool split;
     WindowParts rows;
@@ -689,7 +689,7 @@ static WindowParts fp4_rows(int64_t rows, int n_heads, int n_kv_heads, int max_k
     WindowParts w{1, 4};
     if (pages >= 96 && 2 * groups <= cus)
         w.parts = std::min((int)(cus / groups), (int)(0.354 * std::sqrt((double)pages) + 0.5));
-    if ((groups <= cus && pages >= 32) || (groups <= 4 * cus && pages >= 512)) w.waves = 8;
+    if ((groups <= cus && pages >= 32) || pages >= 512) w.waves = 8;
     return w;
 }
 static Fp4DecodePlan fp4_decode_plan(int num_seqs, int n_heads, int n_kv_heads, int max_kv_len, int cus) {
@@ -1440,8 +1440,8 @@ int femto_paged_attention_gemm_fp4(int dtype, const void* q, int64_t q_stride_he
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + femto::prefill_counter_bytes(resident));
     int decode_rows = 0;
     if (p.parts > 0) {
-        // Sequences of one query token run as rows (an MFMA tile would hold one
-        // valid row of 32).
+        // Sequences of one query token run as rows in the tiles' launch (an MFMA
+        // tile would hold one valid row of 32).
         decode_rows = femto::decode_rows_bound(num_seqs, num_tokens, max_q_len);
         femto::DecodePlan plan{};
         plan.nrep_tile = 1;
@@ -1456,8 +1456,11 @@ int femto_paged_attention_gemm_fp4(int dtype, const void* q, int64_t q_stride_he
         d.single_waves = p.waves;
         d.merge_counters = p.parts > 1 ? a.counters + resident : nullptr;
         a.skip_decode_rows = 1;
-        rc = hip_status(femto::launch_fp4_decode(dtype, d, num_seqs, st), (fn + " decode-row launch").c_str());
-        if (rc != FEMTO_OK) return rc;
+        femto::set_mfma_heads(d);
+        const int64_t blocks = (int64_t)num_seqs * d.grid_heads * p.parts;
+        if (blocks > (1 << 30)) return fail(FEMTO_ERR_INVALID, fn + ": too many sequences");
+        a.dec = d;
+        a.decode_blocks = (int)blocks;
     }
     return hip_status(femto::launch_paged_prefill(dtype, a, num_tokens, decode_rows, st), (fn + " launch").c_str());
 }

@@ -71,4 +71,17 @@ __device__ __forceinline__ u32x4 fp4_unpack8(E e, uint32_t w, float scale) {
     return u32x4{fp4_pair<0>(e, w, scale), fp4_pair<1>(e, w, scale), fp4_pair<2>(e, w, scale), fp4_pair<3>(e, w, scale)};
 }
 
+// Global memory said to be such: an address that went through an asm statement
+// has lost it, and its loads would be flat ones (which count as LDS traffic, too).
+typedef const __attribute__((address_space(1))) uint8_t* GlobalBytes;
+__device__ __forceinline__ GlobalBytes as_global(const void* p) { return (GlobalBytes)(uintptr_t)p; }
+template <typename T>
+__device__ __forceinline__ T load_global(GlobalBytes p) {
+    return *reinterpret_cast<const __attribute__((address_space(1))) T*>(p);
+}
+template <typename T>
+__device__ __forceinline__ T load_global_nt(GlobalBytes p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const __attribute__((address_space(1))) T*>(p));
+}
+
 }  // namespace femto

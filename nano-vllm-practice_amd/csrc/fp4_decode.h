@@ -82,15 +82,17 @@ __device__ __forceinline__ Fp4Query fp4_query(const float (&x)[32]) {
     return q;
 }
 
-// The same of dims 32 b .. of a row of 16-bit values; dims from D on are zeros.
+// The same of dims 32 b .. of a row of 16-bit values, times `scale`; dims from D on are zeros.
 template <typename E>
-__device__ __forceinline__ Fp4Query fp4_query_row(const char* row, int b, int D, bool valid) {
+__device__ __forceinline__ Fp4Query fp4_query_row(const char* row, int b, int D, bool valid, float scale) {
     float x[32];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int d = 32 * b + 8 * i;
         const u32x4 w = valid && d < D ? ld16(row + 2 * d) : u32x4{0, 0, 0, 0};
         unpack8(E{}, w, *reinterpret_cast<float(*)[8]>(x + 8 * i));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[8 * i + e] *= scale;
     }
     return fp4_query(x);
 }
@@ -130,12 +132,14 @@ __device__ __forceinline__ void fp4_segment(const DecodeArgs& a, int b, int kv_l
     const int D = FULL ? kDimHead : a.head_dim, N = fp4_blocks(D);
     s.clear();
     const Fp4Query q = fp4_query_row<E>(static_cast<const char*>(a.q) + ((int64_t)(h0 + c) * a.q_stride_head + (int64_t)qrow * a.q_stride_seq) * 2,
-                                        g, D, c < nh);
+                                        g, D, c < nh, 1.0f);
     const int kb = FULL || g < N ? g : 0, vc = FULL || c < 4 * N ? c : 0;
     const uint32_t k_at = 256 * kb + 16 * c, v_at = 256 * N + 64 * N * g + 16 * vc;
     const uint32_t ks_at = 512 * N + 4 * c + kb, vs_at = 512 * N + 64 + 16 * g + 4 * (vc >> 2);
-    const uint8_t* pool = static_cast<const uint8_t*>(a.k_pool) + (int64_t)kvh * a.pool_stride_head;
-    const uint8_t* zero = reinterpret_cast<const uint8_t*>(g_zero_page);
+    const GlobalBytes pool = as_global(a.k_pool) + (int64_t)kvh * a.pool_stride_head;
+    uint64_t zero = (uint64_t)(uintptr_t)g_zero_page;
+    asm volatile("" : "+s"(zero));  // (else its address is loaded, and waited for, for every page)
+    const uint32_t blocks = (uint32_t)min(a.num_blocks, (int64_t)0x7fffffff);
     const int32_t* table = a.tables + (int64_t)b * a.table_stride;
     int tbl = -1;
     // Every page's loads go out, whether it is there or not (past the segment and
@@ -148,14 +152,14 @@ __device__ __forceinline__ void fp4_segment(const DecodeArgs& a, int b, int kv_l
             asm volatile("" : "+v"(tbl));  // waited for here, once per 64 pages
         }
         const int blk = __builtin_amdgcn_readlane(tbl, i & 63);
-        const bool ok = blk >= 0 && (int64_t)blk < a.num_blocks;
-        const uint8_t* page = ok ? pool + (int64_t)blk * a.pool_stride_block : zero;
+        // (an id below 0 is past the pool, too)
+        const GlobalBytes page = (uint32_t)blk < blocks ? pool + (int64_t)blk * a.pool_stride_block : (GlobalBytes)(uintptr_t)zero;
         // Codes are read once (non-temporal: 61 sequences up to 16k 106 -> 92 us);
         // the scales share a line, of which each load takes half.
-        p.k = ld16_nt(page + k_at);
-        p.v = ld16_nt(page + v_at);
+        p.k = load_global_nt<u32x4>(page + k_at);
+        p.v = load_global_nt<u32x4>(page + v_at);
         p.ks = page[ks_at];
-        p.vs = *reinterpret_cast<const uint32_t*>(page + vs_at);
+        p.vs = load_global<uint32_t>(page + vs_at);
     };
     const float scale = a.scale_log2;
     auto consume = [&](int i, Fp4Page (&p)[2]) __attribute__((always_inline)) {

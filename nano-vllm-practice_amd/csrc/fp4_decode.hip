@@ -6,10 +6,9 @@
 
 namespace femto {
 
-// Pairs of pages in registers, one of them computed (three: 0-3 % slower, but 3-8 %
-// faster for calls of four waves a row and equal contexts).
+// Pairs of pages in registers, one of them computed (three: 2 % slower).
 constexpr int kFp4Stages = 2;
-// Split workers: waves per CU (4 or 6: 3-14 % slower, 10 or more 3-8 %).
+// Split workers: waves per CU (6: 4 % slower, 4 18 %, 10 or more 3-8 %).
 constexpr int kFp4SplitWaves = 8;
 
 template <typename E, bool FULL, int W>

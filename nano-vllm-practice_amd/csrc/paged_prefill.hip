@@ -44,7 +44,8 @@ hipError_t launch_paged_prefill(int dtype, PrefillArgs a, int num_tokens, int de
         if (e != hipSuccess) return e;
     }
     if (a.decode_blocks > 0 && !a.skip_decode_rows) return hipErrorInvalidValue;
-    if (a.decode_blocks > 0 && a.window == 0 && a.dec.head_groups * G != a.n_rep) return hipErrorInvalidValue;
+    const bool rows = a.window > 0 || a.fp4;  // what a.decode_blocks run
+    if (a.decode_blocks > 0 && !rows && a.dec.head_groups * G != a.n_rep) return hipErrorInvalidValue;
     a.decode_blocks = (a.decode_blocks + 7) / 8 * 8;
     // Rows under the window in the same launch: the tiles are cut for one slot
     // of every CU, and rows run in the other from the start, half a slot's worth
@@ -61,15 +62,25 @@ hipError_t launch_paged_prefill(int dtype, PrefillArgs a, int num_tokens, int de
     // are a few more (1100 beside 64 rows of 16/8 heads 52 and 72): the host, which
     // knows a lower bound of their number only, cannot tell these apart.
     const int slots = a.resident;
-    if (a.window > 0 && a.decode_blocks > 0) a.resident /= 2;
+    // Over a 4-bit cache a row is short against a chunk's tiles, and as many rows as
+    // CUs run ahead of them (32/8 heads, 1024 tokens behind 4096 beside 127 rows of
+    // 512-8192 keys: 162 us, all first 205, none 168).  Where the rows or
+    // the tiles do not fill the CUs, the tiles stay cut for both slots, behind
+    // all rows: beside 4 rows 81 and 97, beside 31 92 and 107; 512 tokens beside 127
+    // 109 and 123.  Over 100 such shapes this is 3 % at the mean from the best of
+    // nine orders; the host's one view of long and short rows costs most (16/8 heads,
+    // 2048 behind 8192: beside 31 rows 151, with one slot 189, but beside 127 210
+    // with 128 first and 215).
+    const int tile_tokens = a.skip_decode_rows ? std::max(0, num_tokens - decode_rows_max) : num_tokens;
+    const int64_t min_tiles = (int64_t)((tile_tokens + BT - 1) / BT) * a.n_kv_heads * a.head_groups;
+    const bool both_slots = a.fp4 && (2 * a.decode_blocks <= slots || 2 * min_tiles < slots);
+    if (rows && a.decode_blocks > 0 && !both_slots) a.resident /= 2;
     if (a.part) {
         // A split needs all pieces in the resident slots at once, and a call
         // has at least ceil(num_tokens / BT) query tiles per KV head group
         // (not counting sequences of one token when the decode workers take
         // them): when those already fill the slots the call cannot split, and
         // the kernel skips its split estimate.
-        const int tile_tokens = a.skip_decode_rows ? std::max(0, num_tokens - decode_rows_max) : num_tokens;
-        const int64_t min_tiles = (int64_t)((tile_tokens + BT - 1) / BT) * a.n_kv_heads * a.head_groups;
         if (min_tiles >= a.resident) {
             a.part = nullptr;
             a.counters = nullptr;
@@ -78,11 +89,11 @@ hipError_t launch_paged_prefill(int dtype, PrefillArgs a, int num_tokens, int de
             a.total_work = a.total_work > a.resident ? a.total_work : a.resident;
         }
     }
-    if (a.window > 0) {
-        a.rows_first = std::min(a.decode_blocks, slots / 4) / 8 * 8;
-        return launch_window_tiles(dtype, G, a, st);
+    if (rows) {
+        const int first = both_slots ? a.decode_blocks : a.fp4 ? slots / 2 : slots / 4;
+        a.rows_first = std::min(a.decode_blocks, first) / 8 * 8;
+        return a.fp4 ? launch_fp4_tiles(dtype, G, a, st) : launch_window_tiles(dtype, G, a, st);
     }
-    if (a.fp4) return launch_fp4_tiles(dtype, G, a, st);
     hipError_t e = launch_dtype<true, kAllPages>(dtype, G, a, st);
     if (e == hipSuccess && a.decode_blocks > 0 && !a.dec.merge_counters) e = launch_paged_decode_merge(dtype, a.dec, a.num_seqs, st);
     return e;
