@@ -15,10 +15,18 @@
 // and sum of the rotation is rounded by itself; k rounds to 4 bits from there, q
 // to its type.
 //
-// Work: one wave per token, four head rows at a time, 16 lanes of 8 dims each; a
-// block of 32 dims is a quad of lanes, and its largest magnitude two DPP steps.
-// Rows move in batches of loads; the placement is looked up by the whole wave
-// while the first batch is on its way.
+// Work: one wave per token, or two or four where there are few, four head rows at a
+// time, 16 lanes of 8 dims each; a block of 32 dims is a quad of lanes, and its
+// largest magnitude two DPP steps.  Rows move in batches of loads; the placement is
+// looked up by the whole wave while the first batch is on its way.  The other ends
+// of half-split pairs come from their lane (ds_bpermute; loading and norming them
+// twice: 22.6 us for 20.0 below), and the 1 / rms of a batch's 16 rows is one
+// division and root, a row per lane of each quad.
+//
+// Measured (bf16, 32 / 8 heads of 128): prologue of 8 x 512 tokens 20.0 us, 4.4 TB/s,
+// bound by memory; with norms 30.9, bound by their 64-bit operations; of 64 decode
+// tokens 5.1 and 6.1, bound by latency (placement, table, batch).  Write of 8 x 512
+// tokens (16.8 MB read, 4.5 written) 6.5-7, read 4-5; of 64 tokens 3.6 and 3.4.
 #include <type_traits>
 
 #include "fp4.h"
@@ -26,7 +34,7 @@
 
 namespace femto {
 
-constexpr int kFp4Tokens = 4;  // waves (tokens) per workgroup
+constexpr int kFp4Waves = 4;  // per workgroup
 constexpr int kFp4Batch = 4;   // passes of four rows whose loads are in flight
 
 enum Fp4Pairs { kFp4NoPairs, kFp4Interleaved, kFp4HalfChunks, kFp4HalfAny };
@@ -68,9 +76,13 @@ __device__ __forceinline__ double row16_sum_f64(double x) {
     x += dpp_f64<0xB1>(x);   // quad_perm [1,0,3,2]
     return x;
 }
+// That of lane u of the quad (u a constant once unrolled).
+__device__ __forceinline__ double quad_f64(double x, int u) {
+    return u == 0 ? dpp_f64<0x00>(x) : u == 1 ? dpp_f64<0x55>(x) : u == 2 ? dpp_f64<0xAA>(x) : dpp_f64<0xFF>(x);
+}
 
 template <typename E, int PAIRS, bool NORM>
-__global__ __launch_bounds__(64 * kFp4Tokens) void fp4_cache_write_kernel(Fp4CacheArgs a) {
+__global__ __launch_bounds__(64 * kFp4Waves) void fp4_cache_write_kernel(Fp4CacheArgs a) {
 #pragma clang fp contract(off)
     constexpr bool ROPE = PAIRS != kFp4NoPairs;
     const int lane = threadIdx.x & 63, c = lane & 15;
@@ -80,15 +92,16 @@ __global__ __launch_bounds__(64 * kFp4Tokens) void fp4_cache_write_kernel(Fp4Cac
     const int q_end = a.cu_seqlens ? a.cu_seqlens[b + 1] : b + 1;
     const int D = a.head_dim, N = fp4_blocks(D), R = a.rotary_dim, half = R / 2;
     const int H = ROPE ? a.n_heads : 0, KVH = a.n_kv_heads, rows = H + 2 * KVH;
-    const bool has = 8 * c < D;       // dims of the row
+    const bool has = 8 * c < D;        // dims of the row
     const bool held = 8 * c < 32 * N;  // and those that pad its last block
     const bool turned = ROPE && 8 * c < R;
-    // The chunk that holds the other ends of the lane's pairs.
-    const int other = PAIRS == kFp4HalfChunks && turned ? (8 * c < half ? c + half / 8 : c - half / 8) : c;
+    // The lane that has the other ends of this one's pairs.
+    const int other = 4 * ((lane & 48) | (turned ? (8 * c < half ? c + half / 8 : c - half / 8) : c));
     const int32_t* table = a.tables + (int64_t)b * a.table_stride;
+    const int tokens = kFp4Waves >> a.split_shift, first = wave & ((1 << a.split_shift) - 1);
 
     // max_q_len only sizes the grid: longer sequences take more rounds.
-    for (int t = q_begin + (int)blockIdx.x * kFp4Tokens + wave; t < q_end; t += (int)gridDim.x * kFp4Tokens) {
+    for (int t = q_begin + (int)blockIdx.x * tokens + (wave >> a.split_shift); t < q_end; t += (int)gridDim.x * tokens) {
         const char* src[3] = {ROPE ? static_cast<const char*>(a.q) + (int64_t)t * a.q_stride_token * 2 : nullptr,
                               static_cast<const char*>(a.k) + (int64_t)t * a.k_stride_token * 2,
                               static_cast<const char*>(a.v) + (int64_t)t * a.v_stride_token * 2};
@@ -98,28 +111,25 @@ __global__ __launch_bounds__(64 * kFp4Tokens) void fp4_cache_write_kernel(Fp4Cac
             const char* base = s == 0 ? src[0] : s == 1 ? src[1] : src[2];
             return base + (int64_t)(s == 0 ? r : s == 1 ? r - H : r - H - KVH) * hs * 2;
         };
-        u32x4 w0[kFp4Batch], w1[kFp4Batch];
+        u32x4 w[kFp4Batch];
         auto load = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
             for (int u = 0; u < kFp4Batch; ++u) {
                 const int r = base + 4 * u + (lane >> 4);
-                w0[u] = w1[u] = u32x4{0, 0, 0, 0};
-                if (r < rows && has) {
-                    const char* p = row_ptr(r);
-                    w0[u] = ld16(p + 16 * c);
-                    if (PAIRS == kFp4HalfChunks && turned && r < H + KVH) w1[u] = ld16(p + 16 * other);
-                }
+                w[u] = u32x4{0, 0, 0, 0};
+                if (r < rows && has) w[u] = ld16(row_ptr(r) + 16 * c);
             }
         };
-        load(0);
+        const int begin = 4 * kFp4Batch * first;
+        load(begin);
 
         const int p0 = a.positions[q_begin];
         const int blk = fp4_block_of(a, table, p0, t - q_begin);
         const int row = (int)((uint32_t)p0 + (uint32_t)(t - q_begin)) & (kPage - 1);
 
-        // The lane's table fragment and weights.
+        // The lane's table fragment and weights; sn: -sin at a pair's first end.
         float cs[8], sn[8];
-        float wq[8], wk[8], xq[8], xk[8];  // xq, xk: of the other chunk
+        float wq[8], wk[8];
         if constexpr (ROPE) {
             const int pos = a.positions[t];
             const bool in_tables = pos >= 0 && pos < a.rope_rows;
@@ -127,76 +137,80 @@ __global__ __launch_bounds__(64 * kFp4Tokens) void fp4_cache_write_kernel(Fp4Cac
             const float* st = a.sin + (int64_t)(in_tables ? pos : 0) * a.rope_stride;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                // pair of dim 8 c + e
                 const int d = 8 * c + e;
                 const int j = PAIRS == kFp4Interleaved ? d / 2 : d < half ? d : d - half;
                 const bool in = d < R;
+                const bool lead = PAIRS == kFp4Interleaved ? (e & 1) == 0 : d < half;
                 cs[e] = in ? ct[j] : 1.0f;
                 sn[e] = in ? st[j] : 0.0f;
+                if (lead) sn[e] = -sn[e];
                 if (!in_tables) cs[e] = sn[e] = __builtin_nanf("");
             }
             if constexpr (NORM) {
-                auto weights = [&](const void* p, int chunk, float (&f)[8]) __attribute__((always_inline)) {
-                    u32x4 w{0, 0, 0, 0};
-                    if (has) w = ld16(static_cast<const char*>(p) + 16 * chunk);
-                    unpack8(E{}, w, f);
+                auto weights = [&](const void* p, float (&f)[8]) __attribute__((always_inline)) {
+                    u32x4 g{0, 0, 0, 0};
+                    if (has) g = ld16(static_cast<const char*>(p) + 16 * c);
+                    unpack8(E{}, g, f);
                 };
-                weights(a.q_weight, c, wq);
-                weights(a.k_weight, c, wk);
-                if constexpr (PAIRS == kFp4HalfChunks) {
-                    weights(a.q_weight, other, xq);
-                    weights(a.k_weight, other, xk);
-                }
+                weights(a.q_weight, wq);
+                weights(a.k_weight, wk);
             }
         }
 
-        for (int base = 0; base < rows; base += 4 * kFp4Batch) {
-            if (base) load(base);
+        for (int base = begin; base < rows; base += 4 * kFp4Batch << a.split_shift) {
+            if (base != begin) load(base);
+            // 1 / rms of the batch's rows, pass u's by lane u of each quad.
+            double inv = 1.0;
+            if constexpr (NORM) {
+                double mine = 1.0;
+#pragma unroll
+                for (int u = 0; u < kFp4Batch; ++u) {
+                    float x[8];
+                    unpack8(E{}, w[u], x);
+                    double s = 0.0;  // (squares are exact)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s = __builtin_fma((double)x[e], (double)x[e], s);
+                    s = row16_sum_f64(s);
+                    if ((lane & 3) == u) mine = s;
+                }
+                inv = 1.0 / sqrt(mine / (double)D + (double)a.eps);
+            }
 #pragma unroll
             for (int u = 0; u < kFp4Batch; ++u) {
                 const int r = base + 4 * u + (lane >> 4);
                 float x[8];
-                unpack8(E{}, w0[u], x);
+                unpack8(E{}, w[u], x);
                 if constexpr (ROPE) {
-                    double inv = 1.0;
-                    if constexpr (NORM) {
-                        double s = 0.0;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) s += (double)x[e] * (double)x[e];
-                        s = row16_sum_f64(s);
-                        inv = 1.0 / sqrt(s / (double)D + (double)a.eps);
-                    }
                     if (r < H + KVH) {
-                        auto normed = [&](float v, float w) __attribute__((always_inline)) {
-                            return NORM ? (float)((double)v * inv * (double)w) : v;
+                        double by = 1.0;
+                        if constexpr (NORM) by = quad_f64(inv, u);
+                        auto normed = [&](float v, float g) __attribute__((always_inline)) {
+                            return NORM ? (float)((double)v * by * (double)g) : v;
                         };
-                        auto weight = [&](int e) __attribute__((always_inline)) { return NORM ? (r < H ? wq[e] : wk[e]) : 1.0f; };
-                        float y[8];  // the other ends
-                        if constexpr (PAIRS == kFp4HalfChunks) {
-                            unpack8(E{}, w1[u], y);
+                        if constexpr (NORM) {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) y[e] = normed(y[e], NORM ? (r < H ? xq[e] : xk[e]) : 1.0f);
-                        } else if constexpr (PAIRS == kFp4HalfAny) {
-                            const char* p = row_ptr(min(r, rows - 1));
-                            const char* w = static_cast<const char*>(r < H ? a.q_weight : a.k_weight);
+                            for (int e = 0; e < 8; ++e) x[e] = normed(x[e], r < H ? wq[e] : wk[e]);
+                        }
+                        float y[8];  // the other ends
+                        if constexpr (PAIRS == kFp4HalfAny) {
+                            const char* p = row_ptr(r);
+                            const char* g = static_cast<const char*>(r < H ? a.q_weight : a.k_weight);
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
                                 const int d = 8 * c + e, o = d < half ? d + half : d - half;
-                                y[e] = d < R ? normed(elem_at<E>(p + 2 * o), NORM ? elem_at<E>(w + 2 * o) : 1.0f) : 0.0f;
+                                y[e] = d < R ? normed(elem_at<E>(p + 2 * o), NORM ? elem_at<E>(g + 2 * o) : 1.0f) : 0.0f;
                             }
-                        }
+                        } else {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = normed(x[e], weight(e));
-                        if constexpr (PAIRS == kFp4Interleaved) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) y[e] = x[e ^ 1];
+                            for (int e = 0; e < 8; ++e)
+                                y[e] = PAIRS == kFp4Interleaved
+                                           ? x[e ^ 1]
+                                           : __int_as_float(__builtin_amdgcn_ds_bpermute(other, __float_as_int(x[e])));
                         }
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            const int d = 8 * c + e;
-                            const bool first = PAIRS == kFp4Interleaved ? (e & 1) == 0 : d < half;
-                            const float p = x[e] * cs[e], q = y[e] * sn[e];
-                            if (d < R) x[e] = first ? p - q : p + q;
+                            const float z = x[e] * cs[e], o = y[e] * sn[e];
+                            if (PAIRS == kFp4HalfChunks ? turned : 8 * c + e < R) x[e] = z + o;
                         }
                     }
                 }
@@ -227,7 +241,7 @@ __global__ __launch_bounds__(64 * kFp4Tokens) void fp4_cache_write_kernel(Fp4Cac
 
 // Rows of the tokens at positions[q_begin] + 0, 1, .. of each sequence, as E.
 template <typename E>
-__global__ __launch_bounds__(64 * kFp4Tokens) void fp4_cache_read_kernel(Fp4CacheArgs a) {
+__global__ __launch_bounds__(64 * kFp4Waves) void fp4_cache_read_kernel(Fp4CacheArgs a) {
     const int lane = threadIdx.x & 63, c = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.y;
@@ -235,7 +249,7 @@ __global__ __launch_bounds__(64 * kFp4Tokens) void fp4_cache_read_kernel(Fp4Cach
     const int q_end = a.cu_seqlens ? a.cu_seqlens[b + 1] : b + 1;
     const int D = a.head_dim, N = fp4_blocks(D), KVH = a.n_kv_heads;
     const int32_t* table = a.tables + (int64_t)b * a.table_stride;
-    for (int t = q_begin + (int)blockIdx.x * kFp4Tokens + wave; t < q_end; t += (int)gridDim.x * kFp4Tokens) {
+    for (int t = q_begin + (int)blockIdx.x * kFp4Waves + wave; t < q_end; t += (int)gridDim.x * kFp4Waves) {
         const int p0 = a.positions[q_begin];
         const int blk = fp4_block_of(a, table, p0, t - q_begin);
         const int row = (int)((uint32_t)p0 + (uint32_t)(t - q_begin)) & (kPage - 1);
@@ -269,7 +283,7 @@ __global__ __launch_bounds__(64 * kFp4Tokens) void fp4_cache_read_kernel(Fp4Cach
 
 template <typename E, int PAIRS>
 static void launch_write(const Fp4CacheArgs& a, dim3 grid, hipStream_t st) {
-    const dim3 block(64 * kFp4Tokens);
+    const dim3 block(64 * kFp4Waves);
     if constexpr (PAIRS != kFp4NoPairs) {
         if (a.q_weight) {
             hipLaunchKernelGGL((fp4_cache_write_kernel<E, PAIRS, true>), grid, block, 0, st, a);
@@ -281,7 +295,7 @@ static void launch_write(const Fp4CacheArgs& a, dim3 grid, hipStream_t st) {
 
 template <typename E>
 static hipError_t launch_cache(Fp4CacheOp op, const Fp4CacheArgs& a, dim3 grid, hipStream_t st) {
-    if (op == kFp4Read) hipLaunchKernelGGL(fp4_cache_read_kernel<E>, grid, dim3(64 * kFp4Tokens), 0, st, a);
+    if (op == kFp4Read) hipLaunchKernelGGL(fp4_cache_read_kernel<E>, grid, dim3(64 * kFp4Waves), 0, st, a);
     else if (op == kFp4Write) launch_write<E, kFp4NoPairs>(a, grid, st);
     else if (a.interleaved) launch_write<E, kFp4Interleaved>(a, grid, st);
     else if (a.rotary_dim % 16 == 0) launch_write<E, kFp4HalfChunks>(a, grid, st);
@@ -289,9 +303,21 @@ static hipError_t launch_cache(Fp4CacheOp op, const Fp4CacheArgs& a, dim3 grid, 
     return hipGetLastError();
 }
 
-hipError_t launch_fp4_cache(int dtype, Fp4CacheOp op, const Fp4CacheArgs& a, int max_q_len, hipStream_t st) {
+hipError_t launch_fp4_cache(int dtype, Fp4CacheOp op, Fp4CacheArgs a, int max_q_len, hipStream_t st) {
     if (a.num_seqs <= 0 || max_q_len <= 0) return hipSuccess;
-    const dim3 grid((max_q_len - 1) / kFp4Tokens + 1, a.num_seqs);
+    a.split_shift = 0;
+    // A token's batches over several waves, while there are at most two tokens per
+    // CU.  bf16, 32/8 heads of 128 with norms, us by one, two and four waves a token:
+    // 64 sequences of one token 9.6, 7.8, 6.0; a prompt of 512 11.3, 9.3, 8.3, of 1024
+    // 11.8, 11.1, 14.2; 16/2 heads (two batches) 6.7, 5.4, 5.9 and 8.0, 6.4, 7.5.
+    if (op == kFp4Prologue) {
+        int cus = 0;
+        const hipError_t e = device_cu_count(cus);
+        if (e != hipSuccess) return e;
+        const int batches = (a.n_heads + 2 * a.n_kv_heads - 1) / (4 * kFp4Batch) + 1;
+        if ((int64_t)a.num_seqs * max_q_len <= 2 * cus) a.split_shift = batches > 2 ? 2 : batches - 1;
+    }
+    const dim3 grid((((int64_t)max_q_len << a.split_shift) - 1) / kFp4Waves + 1, a.num_seqs);
     switch (dtype) {
         case kDtypeBF16: return launch_cache<BF16>(op, a, grid, st);
         case kDtypeF16: return launch_cache<F16>(op, a, grid, st);

@@ -253,9 +253,10 @@ struct Fp4CacheArgs {
     const float* sin;
     int64_t rope_stride;
     int rope_rows, rotary_dim, interleaved;
+    int split_shift;  // 2^this waves per token share its rows (set by the launch)
 };
 enum Fp4CacheOp { kFp4Write, kFp4Prologue, kFp4Read };
-hipError_t launch_fp4_cache(int dtype, Fp4CacheOp op, const Fp4CacheArgs& a, int max_q_len, hipStream_t st);
+hipError_t launch_fp4_cache(int dtype, Fp4CacheOp op, Fp4CacheArgs a, int max_q_len, hipStream_t st);
 
 // Varlen metadata build (varlen_metadata.hip).
 struct MetadataArgs {
