@@ -642,6 +642,7 @@ static int fp4_cache_args(const std::string& f, int dtype, const void* kv_pool, 
     a.table_stride = table_stride;
     a.num_pages_per_seq = num_pages_per_seq;
     a.num_seqs = num_seqs;
+    a.num_tokens = num_tokens;
     return FEMTO_OK;
 }
 static int fp4_source(const std::string& f, const void* k, int64_t k_stride_token, int64_t k_stride_head, const void* v,
@@ -1252,8 +1253,7 @@ int femto_kv_cache_write_fp4(int dtype, const void* k, int64_t k_stride_token, i
     if (rc != FEMTO_OK || num_seqs == 0 || num_tokens == 0) return rc;
     rc = fp4_source(f, k, k_stride_token, k_stride_head, v, v_stride_token, v_stride_head, a);
     if (rc != FEMTO_OK) return rc;
-    return hip_status(femto::launch_fp4_cache(dtype, femto::kFp4Write, a, cu_seqlens ? std::min(max_q_len, num_tokens) : 1,
-                                              static_cast<hipStream_t>(stream)),
+    return hip_status(femto::launch_fp4_cache(dtype, femto::kFp4Write, a, static_cast<hipStream_t>(stream)),
                       "kv_cache_write_fp4 launch");
 }
 
@@ -1272,8 +1272,7 @@ int femto_kv_cache_read_fp4(int dtype, const void* kv_pool, int64_t num_blocks, 
         return fail(FEMTO_ERR_INVALID, f + ": k_out and v_out must be 16-byte aligned");
     a.k_out = k_out;
     a.v_out = v_out;
-    return hip_status(femto::launch_fp4_cache(dtype, femto::kFp4Read, a, cu_seqlens ? std::min(max_q_len, num_tokens) : 1,
-                                              static_cast<hipStream_t>(stream)),
+    return hip_status(femto::launch_fp4_cache(dtype, femto::kFp4Read, a, static_cast<hipStream_t>(stream)),
                       "kv_cache_read_fp4 launch");
 }
 
@@ -1324,9 +1323,7 @@ int femto_rope_cache_write_fp4(int dtype, const void* q, int64_t q_stride_token,
     a.rope_rows = rope_rows;
     a.rotary_dim = rotary_dim;
     a.interleaved = interleaved != 0;
-    return hip_status(femto::launch_fp4_cache(dtype, femto::kFp4Prologue, a,
-                                              cu_seqlens ? std::min(max_q_len, num_tokens) : 1,
-                                              static_cast<hipStream_t>(stream)),
+    return hip_status(femto::launch_fp4_cache(dtype, femto::kFp4Prologue, a, static_cast<hipStream_t>(stream)),
                       "rope_cache_write_fp4 launch");
 }
 

@@ -23,9 +23,14 @@
 // twice: 22.6 us for 20.0 below), and the 1 / rms of a batch's 16 rows is one
 // division and root, a row per lane of each quad.
 //
+// The grid is by tokens and a wave looks its sequence up, beside its first loads: a
+// grid of sequences by their longest has 32768 workgroups for 1024 new tokens
+// beside 127 rows, 383 of them with a token.
+//
 // Measured (bf16, 32 / 8 heads of 128): prologue of 8 x 512 tokens 20.0 us, 4.4 TB/s,
-// bound by memory; with norms 30.9, bound by their 64-bit operations; of 64 decode
-// tokens 5.1 and 6.1, bound by latency (placement, table, batch).  Write of 8 x 512
+// bound by memory; with norms 29.2, bound by their 64-bit operations; of 64 decode
+// tokens 5.0 and 5.7, bound by latency (placement, table, batch); of 1024 beside 127
+// rows 10.2.  Write of 8 x 512
 // tokens (16.8 MB read, 4.5 written) 6.5-7, read 4-5; of 64 tokens 3.6 and 3.4.
 #include <type_traits>
 
@@ -54,6 +59,28 @@ __device__ __forceinline__ int fp4_block_of(const Fp4CacheArgs& a, const int32_t
         if (c + 64 > col) blk = __builtin_amdgcn_readlane(id, col - c);
     }
     return ends ? -1 : blk;
+}
+
+// Sequence b that token t belongs to and its first token (whole wave, t uniform);
+// false: none.  64 bounds at a time; a sequence without tokens is passed over.
+__device__ __forceinline__ bool fp4_sequence_of(const Fp4CacheArgs& a, int t, int& b, int& q_begin) {
+    b = q_begin = t;
+    if (!a.cu_seqlens) return t < a.num_seqs;
+    const int lane = threadIdx.x & 63;
+    int first = 0, count = a.num_seqs + 1, step;
+    do {  // the last bound that is not past t
+        step = (count + 63) / 64;
+        const bool in = lane * step < count;
+        const int bound = in ? a.cu_seqlens[first + lane * step] : 0;
+        const uint64_t up = __ballot(in && bound <= t);
+        if (!up) return false;
+        const int i = 63 - __builtin_clzll(up);
+        q_begin = __builtin_amdgcn_readlane(bound, i);
+        first += i * step;
+        count = min(step, count - i * step);
+    } while (step > 1);
+    b = first;
+    return b < a.num_seqs && q_begin >= 0;
 }
 
 template <typename E>
@@ -87,9 +114,9 @@ __global__ __launch_bounds__(64 * kFp4Waves) void fp4_cache_write_kernel(Fp4Cach
     constexpr bool ROPE = PAIRS != kFp4NoPairs;
     const int lane = threadIdx.x & 63, c = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int b = blockIdx.y;
-    const int q_begin = a.cu_seqlens ? a.cu_seqlens[b] : b;
-    const int q_end = a.cu_seqlens ? a.cu_seqlens[b + 1] : b + 1;
+    const int first = wave & ((1 << a.split_shift) - 1);
+    const int t = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (kFp4Waves >> a.split_shift)) + (wave >> a.split_shift));
+    if ((uint32_t)t >= (uint32_t)a.num_tokens) return;
     const int D = a.head_dim, N = fp4_blocks(D), R = a.rotary_dim, half = R / 2;
     const int H = ROPE ? a.n_heads : 0, KVH = a.n_kv_heads, rows = H + 2 * KVH;
     const bool has = 8 * c < D;        // dims of the row
@@ -97,144 +124,142 @@ __global__ __launch_bounds__(64 * kFp4Waves) void fp4_cache_write_kernel(Fp4Cach
     const bool turned = ROPE && 8 * c < R;
     // The lane that has the other ends of this one's pairs.
     const int other = 4 * ((lane & 48) | (turned ? (8 * c < half ? c + half / 8 : c - half / 8) : c));
-    const int32_t* table = a.tables + (int64_t)b * a.table_stride;
-    const int tokens = kFp4Waves >> a.split_shift, first = wave & ((1 << a.split_shift) - 1);
 
-    // max_q_len only sizes the grid: longer sequences take more rounds.
-    for (int t = q_begin + (int)blockIdx.x * tokens + (wave >> a.split_shift); t < q_end; t += (int)gridDim.x * tokens) {
-        const char* src[3] = {ROPE ? static_cast<const char*>(a.q) + (int64_t)t * a.q_stride_token * 2 : nullptr,
-                              static_cast<const char*>(a.k) + (int64_t)t * a.k_stride_token * 2,
-                              static_cast<const char*>(a.v) + (int64_t)t * a.v_stride_token * 2};
-        auto row_ptr = [&](int r) __attribute__((always_inline)) {
-            const int s = r < H ? 0 : r < H + KVH ? 1 : 2;
-            const int64_t hs = s == 0 ? a.q_stride_head : s == 1 ? a.k_stride_head : a.v_stride_head;
-            const char* base = s == 0 ? src[0] : s == 1 ? src[1] : src[2];
-            return base + (int64_t)(s == 0 ? r : s == 1 ? r - H : r - H - KVH) * hs * 2;
-        };
-        u32x4 w[kFp4Batch];
-        auto load = [&](int base) __attribute__((always_inline)) {
+    const char* src[3] = {ROPE ? static_cast<const char*>(a.q) + (int64_t)t * a.q_stride_token * 2 : nullptr,
+                          static_cast<const char*>(a.k) + (int64_t)t * a.k_stride_token * 2,
+                          static_cast<const char*>(a.v) + (int64_t)t * a.v_stride_token * 2};
+    auto row_ptr = [&](int r) __attribute__((always_inline)) {
+        const int s = r < H ? 0 : r < H + KVH ? 1 : 2;
+        const int64_t hs = s == 0 ? a.q_stride_head : s == 1 ? a.k_stride_head : a.v_stride_head;
+        const char* base = s == 0 ? src[0] : s == 1 ? src[1] : src[2];
+        return base + (int64_t)(s == 0 ? r : s == 1 ? r - H : r - H - KVH) * hs * 2;
+    };
+    u32x4 w[kFp4Batch];
+    auto load = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < kFp4Batch; ++u) {
-                const int r = base + 4 * u + (lane >> 4);
-                w[u] = u32x4{0, 0, 0, 0};
-                if (r < rows && has) w[u] = ld16(row_ptr(r) + 16 * c);
-            }
-        };
-        const int begin = 4 * kFp4Batch * first;
-        load(begin);
-
-        const int p0 = a.positions[q_begin];
-        const int blk = fp4_block_of(a, table, p0, t - q_begin);
-        const int row = (int)((uint32_t)p0 + (uint32_t)(t - q_begin)) & (kPage - 1);
-
-        // The lane's table fragment and weights; sn: -sin at a pair's first end.
-        float cs[8], sn[8];
-        float wq[8], wk[8];
-        if constexpr (ROPE) {
-            const int pos = a.positions[t];
-            const bool in_tables = pos >= 0 && pos < a.rope_rows;
-            const float* ct = a.cos + (int64_t)(in_tables ? pos : 0) * a.rope_stride;
-            const float* st = a.sin + (int64_t)(in_tables ? pos : 0) * a.rope_stride;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int d = 8 * c + e;
-                const int j = PAIRS == kFp4Interleaved ? d / 2 : d < half ? d : d - half;
-                const bool in = d < R;
-                const bool lead = PAIRS == kFp4Interleaved ? (e & 1) == 0 : d < half;
-                cs[e] = in ? ct[j] : 1.0f;
-                sn[e] = in ? st[j] : 0.0f;
-                if (lead) sn[e] = -sn[e];
-                if (!in_tables) cs[e] = sn[e] = __builtin_nanf("");
-            }
-            if constexpr (NORM) {
-                auto weights = [&](const void* p, float (&f)[8]) __attribute__((always_inline)) {
-                    u32x4 g{0, 0, 0, 0};
-                    if (has) g = ld16(static_cast<const char*>(p) + 16 * c);
-                    unpack8(E{}, g, f);
-                };
-                weights(a.q_weight, wq);
-                weights(a.k_weight, wk);
-            }
+        for (int u = 0; u < kFp4Batch; ++u) {
+            const int r = base + 4 * u + (lane >> 4);
+            w[u] = u32x4{0, 0, 0, 0};
+            if (r < rows && has) w[u] = ld16(row_ptr(r) + 16 * c);
         }
+    };
+    const int begin = 4 * kFp4Batch * first;
+    load(begin);
 
-        for (int base = begin; base < rows; base += 4 * kFp4Batch << a.split_shift) {
-            if (base != begin) load(base);
-            // 1 / rms of the batch's rows, pass u's by lane u of each quad.
-            double inv = 1.0;
-            if constexpr (NORM) {
-                double mine = 1.0;
+    int b, q_begin;
+    if (!fp4_sequence_of(a, t, b, q_begin)) return;
+    const int32_t* table = a.tables + (int64_t)b * a.table_stride;
+    const int p0 = a.positions[q_begin];
+    const int blk = fp4_block_of(a, table, p0, t - q_begin);
+    const int row = (int)((uint32_t)p0 + (uint32_t)(t - q_begin)) & (kPage - 1);
+
+    // The lane's table fragment and weights; sn: -sin at a pair's first end.
+    float cs[8], sn[8];
+    float wq[8], wk[8];
+    if constexpr (ROPE) {
+        const int pos = a.positions[t];
+        const bool in_tables = pos >= 0 && pos < a.rope_rows;
+        const float* ct = a.cos + (int64_t)(in_tables ? pos : 0) * a.rope_stride;
+        const float* st = a.sin + (int64_t)(in_tables ? pos : 0) * a.rope_stride;
 #pragma unroll
-                for (int u = 0; u < kFp4Batch; ++u) {
-                    float x[8];
-                    unpack8(E{}, w[u], x);
-                    double s = 0.0;  // (squares are exact)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s = __builtin_fma((double)x[e], (double)x[e], s);
-                    s = row16_sum_f64(s);
-                    if ((lane & 3) == u) mine = s;
-                }
-                inv = 1.0 / sqrt(mine / (double)D + (double)a.eps);
-            }
+        for (int e = 0; e < 8; ++e) {
+            const int d = 8 * c + e;
+            const int j = PAIRS == kFp4Interleaved ? d / 2 : d < half ? d : d - half;
+            const bool in = d < R;
+            const bool lead = PAIRS == kFp4Interleaved ? (e & 1) == 0 : d < half;
+            cs[e] = in ? ct[j] : 1.0f;
+            sn[e] = in ? st[j] : 0.0f;
+            if (lead) sn[e] = -sn[e];
+            if (!in_tables) cs[e] = sn[e] = __builtin_nanf("");
+        }
+        if constexpr (NORM) {
+            auto weights = [&](const void* p, float (&f)[8]) __attribute__((always_inline)) {
+                u32x4 g{0, 0, 0, 0};
+                if (has) g = ld16(static_cast<const char*>(p) + 16 * c);
+                unpack8(E{}, g, f);
+            };
+            weights(a.q_weight, wq);
+            weights(a.k_weight, wk);
+        }
+    }
+
+    for (int base = begin; base < rows; base += 4 * kFp4Batch << a.split_shift) {
+        if (base != begin) load(base);
+        // 1 / rms of the batch's rows, pass u's by lane u of each quad.
+        double inv = 1.0;
+        if constexpr (NORM) {
+            double mine = 1.0;
 #pragma unroll
             for (int u = 0; u < kFp4Batch; ++u) {
-                const int r = base + 4 * u + (lane >> 4);
                 float x[8];
                 unpack8(E{}, w[u], x);
-                if constexpr (ROPE) {
-                    if (r < H + KVH) {
-                        double by = 1.0;
-                        if constexpr (NORM) by = quad_f64(inv, u);
-                        auto normed = [&](float v, float g) __attribute__((always_inline)) {
-                            return NORM ? (float)((double)v * by * (double)g) : v;
-                        };
-                        if constexpr (NORM) {
+                double s = 0.0;  // (squares are exact)
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) x[e] = normed(x[e], r < H ? wq[e] : wk[e]);
-                        }
-                        float y[8];  // the other ends
-                        if constexpr (PAIRS == kFp4HalfAny) {
-                            const char* p = row_ptr(r);
-                            const char* g = static_cast<const char*>(r < H ? a.q_weight : a.k_weight);
+                for (int e = 0; e < 8; ++e) s = __builtin_fma((double)x[e], (double)x[e], s);
+                s = row16_sum_f64(s);
+                if ((lane & 3) == u) mine = s;
+            }
+            inv = 1.0 / sqrt(mine / (double)D + (double)a.eps);
+        }
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const int d = 8 * c + e, o = d < half ? d + half : d - half;
-                                y[e] = d < R ? normed(elem_at<E>(p + 2 * o), NORM ? elem_at<E>(g + 2 * o) : 1.0f) : 0.0f;
-                            }
-                        } else {
+        for (int u = 0; u < kFp4Batch; ++u) {
+            const int r = base + 4 * u + (lane >> 4);
+            float x[8];
+            unpack8(E{}, w[u], x);
+            if constexpr (ROPE) {
+                if (r < H + KVH) {
+                    double by = 1.0;
+                    if constexpr (NORM) by = quad_f64(inv, u);
+                    auto normed = [&](float v, float g) __attribute__((always_inline)) {
+                        return NORM ? (float)((double)v * by * (double)g) : v;
+                    };
+                    if constexpr (NORM) {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                y[e] = PAIRS == kFp4Interleaved
-                                           ? x[e ^ 1]
-                                           : __int_as_float(__builtin_amdgcn_ds_bpermute(other, __float_as_int(x[e])));
-                        }
+                        for (int e = 0; e < 8; ++e) x[e] = normed(x[e], r < H ? wq[e] : wk[e]);
+                    }
+                    float y[8];  // the other ends
+                    if constexpr (PAIRS == kFp4HalfAny) {
+                        const char* p = row_ptr(r);
+                        const char* g = static_cast<const char*>(r < H ? a.q_weight : a.k_weight);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            const float z = x[e] * cs[e], o = y[e] * sn[e];
-                            if (PAIRS == kFp4HalfChunks ? turned : 8 * c + e < R) x[e] = z + o;
+                            const int d = 8 * c + e, o = d < half ? d + half : d - half;
+                            y[e] = d < R ? normed(elem_at<E>(p + 2 * o), NORM ? elem_at<E>(g + 2 * o) : 1.0f) : 0.0f;
                         }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            y[e] = PAIRS == kFp4Interleaved
+                                       ? x[e ^ 1]
+                                       : __int_as_float(__builtin_amdgcn_ds_bpermute(other, __float_as_int(x[e])));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float z = x[e] * cs[e], o = y[e] * sn[e];
+                        if (PAIRS == kFp4HalfChunks ? turned : 8 * c + e < R) x[e] = z + o;
                     }
                 }
-                if (ROPE && r < H) {
-                    if (has)
-                        st16_nt(static_cast<char*>(a.q_out) + ((int64_t)t * a.q_out_stride_token + (int64_t)r * a.q_out_stride_head) * 2 + 16 * c,
-                                pack8(E{}, x));
-                    continue;
-                }
-                // The block's largest magnitude: this lane's and its quad's.
-                uint32_t top = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-                top = max(top, (uint32_t)dpp_i32<0xB1>((int)top));
-                top = max(top, (uint32_t)dpp_i32<0x4E>((int)top));
-                if (r >= rows || blk < 0 || !held) continue;
-                const int byte = fp4_scale_byte(top);
-                const uint32_t word = byte == kFp4NanScale ? 0u : fp4_pack8(x, fp4_scale(byte));
-                const bool is_k = r < H + KVH;
-                const int h = is_k ? r - H : r - H - KVH;
-                uint8_t* page = a.pool + ((int64_t)blk * KVH + h) * fp4_page_bytes(D);
-                *reinterpret_cast<uint32_t*>(page + (is_k ? fp4_k_at(row, c) : fp4_v_at(N, row, c))) = word;
-                if ((c & 3) == 0) page[is_k ? fp4_k_scale_at(N, row, c >> 2) : fp4_v_scale_at(N, row, c >> 2)] = (uint8_t)byte;
             }
+            if (ROPE && r < H) {
+                if (has)
+                    st16_nt(static_cast<char*>(a.q_out) + ((int64_t)t * a.q_out_stride_token + (int64_t)r * a.q_out_stride_head) * 2 + 16 * c,
+                            pack8(E{}, x));
+                continue;
+            }
+            // The block's largest magnitude: this lane's and its quad's.
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+            top = max(top, (uint32_t)dpp_i32<0xB1>((int)top));
+            top = max(top, (uint32_t)dpp_i32<0x4E>((int)top));
+            if (r >= rows || blk < 0 || !held) continue;
+            const int byte = fp4_scale_byte(top);
+            const uint32_t word = byte == kFp4NanScale ? 0u : fp4_pack8(x, fp4_scale(byte));
+            const bool is_k = r < H + KVH;
+            const int h = is_k ? r - H : r - H - KVH;
+            uint8_t* page = a.pool + ((int64_t)blk * KVH + h) * fp4_page_bytes(D);
+            *reinterpret_cast<uint32_t*>(page + (is_k ? fp4_k_at(row, c) : fp4_v_at(N, row, c))) = word;
+            if ((c & 3) == 0) page[is_k ? fp4_k_scale_at(N, row, c >> 2) : fp4_v_scale_at(N, row, c >> 2)] = (uint8_t)byte;
         }
     }
 }
@@ -244,39 +269,37 @@ template <typename E>
 __global__ __launch_bounds__(64 * kFp4Waves) void fp4_cache_read_kernel(Fp4CacheArgs a) {
     const int lane = threadIdx.x & 63, c = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int b = blockIdx.y;
-    const int q_begin = a.cu_seqlens ? a.cu_seqlens[b] : b;
-    const int q_end = a.cu_seqlens ? a.cu_seqlens[b + 1] : b + 1;
+    const int t = (int)(blockIdx.x * kFp4Waves) + wave;
     const int D = a.head_dim, N = fp4_blocks(D), KVH = a.n_kv_heads;
+    int b, q_begin;
+    if ((uint32_t)t >= (uint32_t)a.num_tokens || !fp4_sequence_of(a, t, b, q_begin)) return;
     const int32_t* table = a.tables + (int64_t)b * a.table_stride;
-    for (int t = q_begin + (int)blockIdx.x * kFp4Waves + wave; t < q_end; t += (int)gridDim.x * kFp4Waves) {
-        const int p0 = a.positions[q_begin];
-        const int blk = fp4_block_of(a, table, p0, t - q_begin);
-        const int row = (int)((uint32_t)p0 + (uint32_t)(t - q_begin)) & (kPage - 1);
-        for (int base = 0; base < 2 * KVH; base += 4 * kFp4Batch) {
-            uint32_t word[kFp4Batch];
-            int byte[kFp4Batch];
+    const int p0 = a.positions[q_begin];
+    const int blk = fp4_block_of(a, table, p0, t - q_begin);
+    const int row = (int)((uint32_t)p0 + (uint32_t)(t - q_begin)) & (kPage - 1);
+    for (int base = 0; base < 2 * KVH; base += 4 * kFp4Batch) {
+        uint32_t word[kFp4Batch];
+        int byte[kFp4Batch];
 #pragma unroll
-            for (int u = 0; u < kFp4Batch; ++u) {
-                const int r = base + 4 * u + (lane >> 4);
-                word[u] = 0;
-                byte[u] = kFp4MinScale;
-                if (r < 2 * KVH && blk >= 0 && 8 * c < D) {
-                    const bool is_k = r < KVH;
-                    const uint8_t* page = a.pool + ((int64_t)blk * KVH + (is_k ? r : r - KVH)) * fp4_page_bytes(D);
-                    word[u] = *reinterpret_cast<const uint32_t*>(page + (is_k ? fp4_k_at(row, c) : fp4_v_at(N, row, c)));
-                    byte[u] = page[is_k ? fp4_k_scale_at(N, row, c >> 2) : fp4_v_scale_at(N, row, c >> 2)];
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < kFp4Batch; ++u) {
-                const int r = base + 4 * u + (lane >> 4);
-                if (r >= 2 * KVH || 8 * c >= D) continue;
+        for (int u = 0; u < kFp4Batch; ++u) {
+            const int r = base + 4 * u + (lane >> 4);
+            word[u] = 0;
+            byte[u] = kFp4MinScale;
+            if (r < 2 * KVH && blk >= 0 && 8 * c < D) {
                 const bool is_k = r < KVH;
-                char* out = static_cast<char*>(is_k ? a.k_out : a.v_out) +
-                            ((int64_t)t * KVH + (is_k ? r : r - KVH)) * D * 2 + 16 * c;
-                st16_nt(out, fp4_unpack8(E{}, word[u], fp4_scale(byte[u])));
+                const uint8_t* page = a.pool + ((int64_t)blk * KVH + (is_k ? r : r - KVH)) * fp4_page_bytes(D);
+                word[u] = *reinterpret_cast<const uint32_t*>(page + (is_k ? fp4_k_at(row, c) : fp4_v_at(N, row, c)));
+                byte[u] = page[is_k ? fp4_k_scale_at(N, row, c >> 2) : fp4_v_scale_at(N, row, c >> 2)];
             }
+        }
+#pragma unroll
+        for (int u = 0; u < kFp4Batch; ++u) {
+            const int r = base + 4 * u + (lane >> 4);
+            if (r >= 2 * KVH || 8 * c >= D) continue;
+            const bool is_k = r < KVH;
+            char* out = static_cast<char*>(is_k ? a.k_out : a.v_out) +
+                        ((int64_t)t * KVH + (is_k ? r : r - KVH)) * D * 2 + 16 * c;
+            st16_nt(out, fp4_unpack8(E{}, word[u], fp4_scale(byte[u])));
         }
     }
 }
@@ -303,21 +326,21 @@ static hipError_t launch_cache(Fp4CacheOp op, const Fp4CacheArgs& a, dim3 grid, 
     return hipGetLastError();
 }
 
-hipError_t launch_fp4_cache(int dtype, Fp4CacheOp op, Fp4CacheArgs a, int max_q_len, hipStream_t st) {
-    if (a.num_seqs <= 0 || max_q_len <= 0) return hipSuccess;
+hipError_t launch_fp4_cache(int dtype, Fp4CacheOp op, Fp4CacheArgs a, hipStream_t st) {
+    if (a.num_seqs <= 0 || a.num_tokens <= 0) return hipSuccess;
     a.split_shift = 0;
     // A token's batches over several waves, while there are at most two tokens per
     // CU.  bf16, 32/8 heads of 128 with norms, us by one, two and four waves a token:
-    // 64 sequences of one token 9.6, 7.8, 6.0; a prompt of 512 11.3, 9.3, 8.3, of 1024
-    // 11.8, 11.1, 14.2; 16/2 heads (two batches) 6.7, 5.4, 5.9 and 8.0, 6.4, 7.5.
+    // 64 tokens 9.6, 7.8, 6.0; 512 11.3, 9.3, 8.3; 1024 11.8, 11.1, 14.2; 16/2 heads (two
+    // batches) 64 tokens 6.7, 5.4, 5.9, 512 8.0, 6.4, 7.5.
     if (op == kFp4Prologue) {
         int cus = 0;
         const hipError_t e = device_cu_count(cus);
         if (e != hipSuccess) return e;
         const int batches = (a.n_heads + 2 * a.n_kv_heads - 1) / (4 * kFp4Batch) + 1;
-        if ((int64_t)a.num_seqs * max_q_len <= 2 * cus) a.split_shift = batches > 2 ? 2 : batches - 1;
+        if (a.num_tokens <= 2 * cus) a.split_shift = batches > 2 ? 2 : batches - 1;
     }
-    const dim3 grid((((int64_t)max_q_len << a.split_shift) - 1) / kFp4Waves + 1, a.num_seqs);
+    const dim3 grid((((int64_t)a.num_tokens << a.split_shift) - 1) / kFp4Waves + 1);
     switch (dtype) {
         case kDtypeBF16: return launch_cache<BF16>(op, a, grid, st);
         case kDtypeF16: return launch_cache<F16>(op, a, grid, st);

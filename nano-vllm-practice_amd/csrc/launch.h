@@ -233,7 +233,7 @@ struct Fp4CacheArgs {
     const int32_t* positions;   // first token of each sequence at positions[q_begin]; rotary positions of all
     const int32_t* tables;
     int64_t table_stride;
-    int num_pages_per_seq, num_seqs;
+    int num_pages_per_seq, num_seqs, num_tokens;
     const void* k;  // writes: (tokens, n_kv_heads, head_dim)
     const void* v;
     int64_t k_stride_token, k_stride_head, v_stride_token, v_stride_head;
@@ -256,7 +256,7 @@ struct Fp4CacheArgs {
     int split_shift;  // 2^this waves per token share its rows (set by the launch)
 };
 enum Fp4CacheOp { kFp4Write, kFp4Prologue, kFp4Read };
-hipError_t launch_fp4_cache(int dtype, Fp4CacheOp op, Fp4CacheArgs a, int max_q_len, hipStream_t st);
+hipError_t launch_fp4_cache(int dtype, Fp4CacheOp op, Fp4CacheArgs a, hipStream_t st);
 
 // Varlen metadata build (varlen_metadata.hip).
 struct MetadataArgs {

@@ -176,3 +176,36 @@ def test_rows_and_tiles_in_every_order(ops, gpu, new, rows):
     assert_close(out, want, BF16, f"{new} beside {rows}", mask=mask)
     again = ops.paged_attention_gemm_fp4(q, pool, cu, new, tables, lens, pos)
     assert torch.equal(again, out)  # partials are merged in order
+
+
+@pytest.mark.parametrize("count", [63, 64, 65, 300, 5000])
+def test_many_sequences(ops, gpu, count):
+    """A wave finds its token's sequence among many, empty ones too (at both ends); rows behind the last sequence and before
+    the first stay as they were."""
+    rng = np.random.default_rng(count)
+    n = rng.choice([0, 1, 2, 17], size=count, p=[0.4, 0.3, 0.2, 0.1])
+    n[0] = n[-1] = n[-2] = 0
+    cu = np.concatenate([[3], 3 + np.cumsum(n)])
+    T, dim = int(cu[-1]) + 4, 16
+    pos = np.concatenate([[0] * 3, *(np.arange(m) + int(rng.integers(0, 14)) for m in n), [0] * 4])
+    tables = rng.permutation(2 * count).reshape(count, 2)
+    g = torch.Generator().manual_seed(count)
+    k, v, q = (torch.randn((T, 1, dim), generator=g).to(F16) for _ in range(3))
+    cos, sin = torch.randn((40, 8), generator=g), torch.randn((40, 8), generator=g)
+    start = rng.integers(0, 100, size=(2 * count, 1, of.page_bytes(dim))).astype(np.uint8)
+    t = lambda x: torch.tensor(np.asarray(x, dtype=np.int32), device=gpu)
+    mine = slice(3, T - 4)
+    dev = torch.tensor(start, device=gpu)
+    ops.kv_cache_write_fp4(k.to(gpu), v.to(gpu), dev, t(pos), t(tables), t(cu), 17)
+    want = of.write(start, np64(k), np64(v), pos, tables, cu, dim)
+    assert np.array_equal(dev.cpu().numpy(), want)
+    rk, rv = ops.kv_cache_read_fp4(dev, dim, F16, t(pos), t(tables), t(cu), 17)
+    wk, wv = of.read(want, pos, tables, cu, dim)
+    assert np.array_equal(np64(rk)[mine], wk[mine]) and np.array_equal(np64(rv)[mine], wv[mine])
+    dev = torch.tensor(start, device=gpu)
+    out = torch.full((T, 1, dim), 7.0, dtype=F16, device=gpu)
+    ops.rope_cache_write_fp4(q.to(gpu), k.to(gpu), v.to(gpu), cos.to(gpu), sin.to(gpu), t(pos), dev, t(tables), t(cu), 17, out=out)
+    turned = lambda x: of.prologue(np64(x), None, 0, cos.numpy(), sin.numpy(), pos, False)
+    assert np.array_equal(np64(out)[mine], np64(torch.tensor(turned(q)).to(F16))[mine])
+    assert (out[:3] == 7).all() and (out[-4:] == 7).all()
+    assert np.array_equal(dev.cpu().numpy(), of.write(start, turned(k), np64(v), pos, tables, cu, dim))
