@@ -173,8 +173,8 @@ __device__ __forceinline__ int serpentine(int k, int n, int cus) {
 // a.k_stride1 bytes from block to block and head to head): K's codes are copied
 // into LDS as they are and multiplied by scaled matrix instructions with q in
 // three terms of 6 bits (fp4_decode.h); V's are loaded into registers a tile
-// ahead, and converted into LDS rows of the storage type after the tile's math,
-// once for all of the tile's query rows.
+// ahead, and converted into LDS rows of the storage type beside the second half of
+// the tile's P . V, once for all of the tile's query rows.
 template <typename E, int G, bool PAGED, bool FUSED, bool FULLD = true, int RULE = kAllPages>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_mfma_kernel(PrefillArgs a) {
     constexpr int EB = 2;
