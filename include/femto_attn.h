@@ -374,8 +374,10 @@ size_t femto_fp4_page_bytes(int head_dim); /* 512 N + 128; 0: head_dim not suppo
  * tokens at positions[cu_seqlens[b]] + 0, 1, .. of each sequence into k_out and
  * v_out (num_tokens, n_kv_heads, head_dim), contiguous; zeros where a write
  * would have stopped (a table column that is -1, past the table or outside the
- * pool).  cu_seqlens == NULL: one token per sequence.  max_q_len only sizes the
- * launch: longer sequences are taken whole.  At most 65535 sequences. */
+ * pool).  cu_seqlens == NULL: one token per sequence.  max_q_len (at least
+ * 1) decides nothing: sequences of any length are taken whole.  Rows of tokens
+ * in no sequence are left as they were.  Tokens of one call want places of their
+ * own: two at one place leave a mix of both.  At most 65535 sequences. */
 int femto_kv_cache_write_fp4(
     int dtype,
     const void* k, int64_t k_stride_token, int64_t k_stride_head,

@@ -348,8 +348,9 @@ def kv_cache_write_fp4(
     ``cu_seqlens`` are those of :func:`kv_cache_write`.  Each 32 dims of a row are
     rounded to the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} times their scale, the
     smallest power of two of which no magnitude is more than 7 (from 2^-119 to 2^125);
-    32 dims that hold an infinity or a NaN become NaN.  ``max_q_len`` only sizes
-    the launch: longer sequences are written whole.
+    32 dims that hold an infinity or a NaN become NaN.  ``max_q_len`` decides nothing
+    here: sequences of any length are written whole.  Tokens of one call want
+    places of their own: two at one place leave a mix of both there.
     """
     for name, t in (("k", k), ("v", v)):
         if not t.is_cuda:
