@@ -356,8 +356,8 @@ static int paged_decode_entry(const char* fn_name, int dtype, const void* q, int
 // keys.  Rows longer than 24 pages are cut where that still leaves each part a CU
 // of its own, into the square root of their pages (each more part shortens the
 // walk, and adds a state to the last part's merge).  One sequence of 8 KV heads
-// (32 query heads, bf16), whole and cut, us: 1024 keys 13.1 and 9.2 (6 parts),
-// 4096 39.2 and 13.1 (8), 8192 74 and 16.4 (12); 256 keys 7.0 whole, 7.3 in two.
+// (32 query heads, bf16), whole and cut, us: 1024 keys 11.2 and 7.6 (6 parts),
+// 4096 39.3 and 9.9 (11), 16384 143 and 16.0 (22); 512 keys 7.4 and 6.8 (5).
 // Sixteen of 4096 keys (128 rows): 48.6, 43.6 in two, 47.4 in three; 24
 // (192 rows): 59.7 and 66.7.  Whole rows take 8 waves where they are long or few.
 struct WindowParts {
@@ -664,10 +664,11 @@ static int fp4_source(const std::string& f, const void* k, int64_t k_stride_toke
 // head, up to kMfmaHeads) is a workgroup, or a few where there are fewer rows
 // than CUs, or all rows are cut into equal slices for split workers.  Measured
 // (bf16, 32/8 heads unless said, us; equal contexts / drawn from a sixteenth on):
-//  * parts of a row: about a third of the root of its pages, as far as each has a
-//    CU of its own.  One sequence (8 rows) of 2048 keys 11.0 whole, 9.5 in two,
-//    8.4 in four, 9.4 in eight; 32768: 21.7 in eight, 19.0 in 16.  Sixteen of 8192:
-//    32.2 whole, 26.4 in two, 30.8 in four.  1024 keys: 8.0 whole, 7.9 in four;
+//  * parts of a row: half the root of its pages, as far as each has a CU of its
+//    own.  One sequence (8 rows) of 1024 keys 7.7 whole, 7.8 in two, 7.2 in four;
+//    2048: 10.5, 9.2, 7.9, in six 8.2, in eight 7.7; 5000: 10.4 in four, 9.0 in
+//    nine, 9.6 in 16; 32768: 19.5 in eight, 14.3 in 16, 14.2 in 24.  Sixteen of
+//    8192: 31.8 whole, 24.7 in two;
 //  * waves of a workgroup: eight where there is at most a row per CU (32 sequences
 //    of 2048 keys 14.4, with four 16.7; of 256 keys 6.3 and 6.2) or rows of 8192
 //    keys and more (128: 171 / 108, with four 180 / 119); else four (128 of 1024:
@@ -688,8 +689,8 @@ static WindowParts fp4_rows(int64_t rows, int n_heads, int n_kv_heads, int max_k
     const int64_t groups = rows * n_kv_heads * ((n_rep + femto::kMfmaHeads - 1) / femto::kMfmaHeads);
     const int pages = max_kv_len > 0 ? (max_kv_len - 1) / femto::kPage + 1 : 0;
     WindowParts w{1, 4};
-    if (pages >= 96 && 2 * groups <= cus)
-        w.parts = std::min((int)(cus / groups), (int)(0.354 * std::sqrt((double)pages) + 0.5));
+    if (pages >= (4 * groups <= cus ? 64 : 96) && 2 * groups <= cus)
+        w.parts = std::min((int)(cus / groups), (int)(0.5 * std::sqrt((double)pages) + 0.5));
     if ((groups <= cus && pages >= 32) || pages >= 512) w.waves = 8;
     return w;
 }

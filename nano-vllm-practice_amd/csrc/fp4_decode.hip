@@ -5,7 +5,7 @@
 // 256-16384 keys, 16/8 heads, 90.8 (556 MB at 6.1 TB/s: split kernel 85, merge 4.6),
 // 256 of 1024-8192, 32/8, 200.6 (1.22 GB at 6.1 TB/s); f16, 16 of 8192-32768, 32/8,
 // 65.4 (5.7 TB/s).  The matrix units are busy 13 % of that.  One sequence of 5000
-// keys 10.7, bound by latency: table, pages, states to memory, count, states back.
+// keys 9.3, bound by latency: table, pages, states to memory, count, states back.
 #include <algorithm>
 
 #include "fp4_decode.h"
