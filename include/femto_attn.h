@@ -436,9 +436,9 @@ size_t femto_paged_attention_gemv_fp4_zero_bytes(void);
 
 /* femto_paged_attention_gemm over a 4-bit cache: token t of sequence b sees the
  * keys j < kv_lens[b] with j <= positions[t]; a token that sees none gives NaN.
- * Sequences of one token are taken as decode rows.  A block of V that is NaN has
- * to be at a position that no token of its sequence's chunk sees past: one in
- * a key j < kv_lens[b] may also reach tokens of the chunk before it.  The
+ * Sequences of one token are taken as decode rows.  A block of V that is NaN in a
+ * key that a token sees also reaches those of its query tile (up to 128 tokens
+ * of the chunk) that do not.  The
  * workspace (256-byte aligned, always needed) has to be zero in its first
  * femto_paged_attention_gemm_split_bytes() bytes before its first use and is
  * left so; calls that may overlap must not share one. */

@@ -592,16 +592,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         lds_dma_one(page4, FULLD || lane < 16 * fp4_n ? 16 * lane : 0,
                     lds_addr(&smem[stage][0][1024 * wave]));
     };
-    // ... and into LDS: V as rows of the storage type, zeros past kv_len (their
-    // weights are 0, and 0 times a NaN would not be); K's scales behind its codes,
-    // those of blocks past the row's 1.
+    // ... and into LDS: V as rows of the storage type, zeros past the last key that
+    // the query tile sees (their weights are 0, and 0 times a NaN would not be);
+    // K's scales behind its codes, those of blocks past the row's 1.
+    int seen4 = kv_len;  // (known before the first use)
     auto mask_fp4 = [&](int it) __attribute__((always_inline)) {
         const int key0 = it * kKvTile + 16 * wave + 4 * lrow;
-        if (it * kKvTile + kKvTile > kv_len) {  // wave-uniform
+        if (it * kKvTile + kKvTile > seen4) {  // wave-uniform
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                v4[j] = key0 + j < kv_len ? v4[j] : 0;
-                v4_scale = key0 + j < kv_len ? v4_scale : v4_scale & ~(0xffu << (8 * j));
+                v4[j] = key0 + j < seen4 ? v4[j] : 0;
+                v4_scale = key0 + j < seen4 ? v4_scale : v4_scale & ~(0xffu << (8 * j));
             }
         }
     };
@@ -783,6 +784,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if (lane == 0) s_kend[wave] = kend_w;
     __syncthreads();
     const int kend = max(max(s_kend[0], s_kend[1]), max(s_kend[2], s_kend[3]));
+    if constexpr (FP4) seen4 = __builtin_amdgcn_readfirstlane(kend);
 
     // Key tiles of this piece: [t_lo, t_hi).  Pieces past the query tile's
     // last visible key have nothing to do (and are not counted); a tile that

@@ -209,3 +209,22 @@ def test_many_sequences(ops, gpu, count):
     assert np.array_equal(np64(out)[mine], np64(torch.tensor(turned(q)).to(F16))[mine])
     assert (out[:3] == 7).all() and (out[-4:] == 7).all()
     assert np.array_equal(dev.cpu().numpy(), of.write(start, turned(k), np64(v), pos, tables, cu, dim))
+
+
+@pytest.mark.parametrize("heads", [(8, 8), (4, 2), (8, 2)])
+def test_nan_values_of_later_tokens(ops, gpu, heads):
+    """V of a later token that is NaN: no token of an earlier query tile (at most 128 tokens) changes, those that see it are
+    NaN in its 32 dims."""
+    w = Batch([(50, 400), (7, 1)], *heads, D, BF16, sum(heads))
+    pool, tables, lens, cu, pos, q = w.on(gpu)
+    run = lambda p: ops.paged_attention_gemm_fp4(q, p, cu, 400, tables, lens, pos)
+    want = run(pool)
+    for token in (390, 399, 200):
+        key = 50 + token
+        bad = w.pool.copy()
+        bad[w.tables[0, key // 16], :, 2 * 1024 + 64 + 16 * (key % 16 // 4) + 4 * 2 + key % 4] = 255  # V's block 2
+        got = run(torch.tensor(bad, device=gpu))
+        first = token // 128 * 128
+        assert torch.equal(got[:, :first], want[:, :first]) and torch.equal(got[:, 400], want[:, 400])
+        assert torch.isnan(got[:, token:400, 64:96]).all()
+        assert torch.equal(got[:, :400, :64], want[:, :400, :64]) and torch.equal(got[:, :400, 96:], want[:, :400, 96:])
