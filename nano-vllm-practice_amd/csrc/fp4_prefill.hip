@@ -5,8 +5,8 @@
 // over the keys j < kv_len, j <= p, p the token's position; k and v are the
 // values that the cache stands for.
 //
-// Measured (bf16 of 128 dims, us): 2048 tokens behind 30720, 32/8 heads, 866-881
-// (1.21-1.23 PFLOP/s; the kernel over a 16-bit cache 947), bound by issue: 6.3 VALU
+// Measured (bf16 of 128 dims, us): 2048 tokens behind 30720, 32/8 heads, 854-881
+// (1.21-1.25 PFLOP/s; the kernel over a 16-bit cache 947), bound by issue: 6.3 VALU
 // instructions per MFMA, the matrix units busy 48 %, and by the clock (inputs of
 // zeros -22 %); 8 x 512 tokens, 16/8, 70, bound by the longest query tile's 40 key
 // tiles in series; 1024 behind 4096 beside 127 rows, 32/8, 164-168, memory (646 MB)
