@@ -374,10 +374,12 @@ size_t femto_fp4_page_bytes(int head_dim); /* 512 N + 128; 0: head_dim not suppo
  * tokens at positions[cu_seqlens[b]] + 0, 1, .. of each sequence into k_out and
  * v_out (num_tokens, n_kv_heads, head_dim), contiguous; zeros where a write
  * would have stopped (a table column that is -1, past the table or outside the
- * pool).  cu_seqlens == NULL: one token per sequence.  max_q_len (at least
- * 1) decides nothing: sequences of any length are taken whole.  Rows of tokens
- * in no sequence are left as they were.  Tokens of one call want places of their
- * own: two at one place leave a mix of both.  At most 65535 sequences. */
+ * pool), and for tokens in no sequence (before cu_seqlens[0], from
+ * cu_seqlens[num_seqs] on).  A call of no sequences (num_seqs == 0) does nothing.
+ * cu_seqlens == NULL: one token per sequence.  max_q_len (at least 1) decides
+ * nothing: sequences of any length are taken whole.  Tokens of one call want
+ * places of their own: two at one place leave a mix of both.  At most 65535
+ * sequences. */
 int femto_kv_cache_write_fp4(
     int dtype,
     const void* k, int64_t k_stride_token, int64_t k_stride_head,
@@ -399,7 +401,8 @@ int femto_kv_cache_read_fp4(
  * k where q_weight and k_weight (head_dim elements each, both or neither) are
  * given: x w / sqrt(mean(x^2) + eps).  The norm is formed in 64 bits and rounded
  * to fp32, the rotation in fp32 with every product and sum rounded by itself;
- * then q rounds to its type and k to 4 bits, v as it is. */
+ * then q rounds to its type and k to 4 bits, v as it is.  Rows of q_out of tokens
+ * in no sequence are left as they were. */
 int femto_rope_cache_write_fp4(
     int dtype,
     const void* q, int64_t q_stride_token, int64_t q_stride_head,

@@ -4,7 +4,7 @@
 // Placement is kv_cache_write.hip's: sequence b's tokens go to positions
 // positions[q_begin] + 0, 1, ..., until the first table column that is -1, past the
 // table or outside the pool.  A read gives zeros where a write would have
-// stopped.
+// stopped, and for tokens of no sequence.
 //
 // The prologue also norms (optional) and rotates q and k on the way:
 //   y = x w / sqrt(mean(x^2) + eps), per head;
@@ -271,12 +271,13 @@ __global__ __launch_bounds__(64 * kFp4Waves) void fp4_cache_read_kernel(Fp4Cache
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = (int)(blockIdx.x * kFp4Waves) + wave;
     const int D = a.head_dim, N = fp4_blocks(D), KVH = a.n_kv_heads;
-    int b, q_begin;
-    if ((uint32_t)t >= (uint32_t)a.num_tokens || !fp4_sequence_of(a, t, b, q_begin)) return;
-    const int32_t* table = a.tables + (int64_t)b * a.table_stride;
-    const int p0 = a.positions[q_begin];
-    const int blk = fp4_block_of(a, table, p0, t - q_begin);
-    const int row = (int)((uint32_t)p0 + (uint32_t)(t - q_begin)) & (kPage - 1);
+    if ((uint32_t)t >= (uint32_t)a.num_tokens) return;
+    int b, q_begin, blk = -1, row = 0;  // (a token of no sequence: zeros)
+    if (fp4_sequence_of(a, t, b, q_begin)) {
+        const int p0 = a.positions[q_begin];
+        blk = fp4_block_of(a, a.tables + (int64_t)b * a.table_stride, p0, t - q_begin);
+        row = (int)((uint32_t)p0 + (uint32_t)(t - q_begin)) & (kPage - 1);
+    }
     for (int base = 0; base < 2 * KVH; base += 4 * kFp4Batch) {
         uint32_t word[kFp4Batch];
         int byte[kFp4Batch];

@@ -857,7 +857,8 @@ def _kv_cache_read_fp4(kv_pool, head_dim, dtype, positions, kv_page_tables, cu_s
     stride, cu_ptr = _check_placement(fn, positions, kv_page_tables, cu_seqlens, tokens, kv_pool.device)
     max_q_len = _int32_arg(fn, "max_q_len", max_q_len)
     with torch.cuda.device(kv_pool.device):
-        k, v = (torch.empty((tokens, kv_pool.size(1), head_dim), dtype=dtype, device=kv_pool.device) for _ in range(2))
+        made = torch.zeros if kv_page_tables.size(0) == 0 else torch.empty  # without sequences nothing is launched
+        k, v = (made((tokens, kv_pool.size(1), head_dim), dtype=dtype, device=kv_pool.device) for _ in range(2))
         if tokens == 0 or kv_page_tables.size(0) == 0:
             return k, v
         rc = _lib.femto_kv_cache_read_fp4(

@@ -373,7 +373,8 @@ def kv_cache_read_fp4(
 
     The tokens are those that :func:`kv_cache_write_fp4` would write with the
     same arguments, e.g. a whole prefix that moves to 16-bit pools; zeros where
-    that would have stopped.  bf16 holds every value exactly; f16 rounds, and
+    that would have stopped, and for tokens that are in no sequence (before
+    ``cu_seqlens[0]``, from ``cu_seqlens[-1]`` on).  bf16 holds every value exactly; f16 rounds, and
     values past its range are infinities.
     """
     if not kv_pool.is_cuda:
@@ -405,7 +406,8 @@ def rope_cache_write_fp4(
     With ``q_norm_weight`` and ``k_norm_weight`` ((head_dim,) of q's dtype, both or
     neither) and ``eps``, q and k first pass the layer's RMSNorms, as in
     :func:`qk_norm_rope_cache_write`.  bf16 or f16.  k is rounded once, from
-    float32.
+    float32.  Rows of ``out`` of tokens in no sequence are left as they were (a
+    new ``out`` holds nothing of meaning there).
     """
     for name, t in (("q", q), ("k", k), ("v", v)):
         if not t.is_cuda:
