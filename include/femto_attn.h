@@ -366,8 +366,11 @@ int femto_rope_cache_write(
  * NaN gets the byte 255, which stands for NaN in all of it.  Scale bytes of
  * other writers are 1 to 254, or 255.
  * q, k, v and outputs are F16 or BF16; the cache does not say which wrote it.
- * Attention and reads take V and values as their own type: those past f16's
- * range are infinities to an f16 call.  No counterpart in the reference. */
+ * Values past f16's range are infinities to an f16 read, 65536 among them, which
+ * f16 values past 57344 are held as (the nearest of the list; a bf16 read
+ * gives it).  f16 attention takes V to twice that range: averages of 65536 are
+ * finite where they are in f16's range, and V from 131072 on is an infinity.
+ * No counterpart in the reference. */
 size_t femto_fp4_page_bytes(int head_dim); /* 512 N + 128; 0: head_dim not supported */
 
 /* femto_kv_cache_write into a 4-bit cache, and the reverse: the rows of the

@@ -608,7 +608,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     };
     auto store_row_fp4 = [&](int j, int stage) __attribute__((always_inline)) {
         const int row = 16 * wave + 4 * lrow + j;
-        const float s = __uint_as_float((j == 3 ? v4_scale >> 1 : v4_scale << (23 - 8 * j)) & 0x7f800000u);
+        const float s = fp4_value_scale<E>(__uint_as_float((j == 3 ? v4_scale >> 1 : v4_scale << (23 - 8 * j)) & 0x7f800000u));
         *reinterpret_cast<u32x4*>(&smem[stage][1][row * kRowBytes + ((lpos ^ swz_v(row)) << 4)]) = fp4_unpack8(E{}, v4[j], s);
     };
     auto store_scales_fp4 = [&](int stage) __attribute__((always_inline)) {
@@ -1184,6 +1184,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     } else {
         tile_loop(std::false_type{});
     }
+    if constexpr (FP4) l_run = fp4_row_sum<E>(l_run);
 
     if constexpr (PREFIX) {
         // The piece's states, for the merge launch (it takes a row's pieces

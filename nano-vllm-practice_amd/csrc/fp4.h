@@ -20,6 +20,8 @@
 // an infinity or a NaN gets the byte 255, which the hardware reads as NaN.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace femto {
@@ -69,6 +71,21 @@ __device__ __forceinline__ uint32_t fp4_pair(F16, uint32_t w, float scale) {
 template <typename E>
 __device__ __forceinline__ u32x4 fp4_unpack8(E e, uint32_t w, float scale) {
     return u32x4{fp4_pair<0>(e, w, scale), fp4_pair<1>(e, w, scale), fp4_pair<2>(e, w, scale), fp4_pair<3>(e, w, scale)};
+}
+
+// The scale at which P . V takes values, from that of the cache: half of it in f16,
+// whose row sums are halved too.  A finite f16 value past 57344 rounds to 65536 in
+// the cache, which f16 has no number for; half of it it has, and an average of such
+// values may well be in its range.  (Halves are as exact: values have two
+// significant bits, and fewer only below 2^-23.  A NaN block's scale stays
+// 2^128.)
+template <typename E>
+__device__ __forceinline__ float fp4_value_scale(float scale) {
+    return std::is_same<E, F16>::value ? 0.5f * scale : scale;
+}
+template <typename E>
+__device__ __forceinline__ float fp4_row_sum(float l) {
+    return std::is_same<E, F16>::value ? 0.5f * l : l;
 }
 
 // Global memory said to be such: an address that went through an asm statement

@@ -18,9 +18,9 @@
 // those dims (fp4_query), a quarter of f16's rounding there; products are exact
 // and sums 32-bit.
 // V is wanted by dims, its values convert to 16 bits two dims at a time
-// (v_cvt_scalef32_pk, exact in bf16), and a permute per two values pairs keys: a
-// 16-byte load holds 8 dims of four keys, so no V passes through LDS.  Row 4 g + i
-// of the O^T tile dt is dim 8 (4 g + i) + dt.
+// (v_cvt_scalef32_pk, exact in bf16; f16: halves of them, fp4_value_scale), and a
+// permute per two values pairs keys: a 16-byte load holds 8 dims of four keys, so
+// no V passes through LDS.  Row 4 g + i of the O^T tile dt is dim 8 (4 g + i) + dt.
 // P rounds to q's type, and the row sum adds the rounded P.
 #pragma once
 
@@ -205,10 +205,10 @@ __device__ __forceinline__ void fp4_segment(const DecodeArgs& a, int b, int kv_l
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t w = p[h].vs;
-            vsc[4 * h] = __uint_as_float((w << 23) & 0x7f800000u);
-            vsc[4 * h + 1] = __uint_as_float((w << 15) & 0x7f800000u);
-            vsc[4 * h + 2] = __uint_as_float((w << 7) & 0x7f800000u);
-            vsc[4 * h + 3] = __uint_as_float((w >> 1) & 0x7f800000u);
+            vsc[4 * h] = fp4_value_scale<E>(__uint_as_float((w << 23) & 0x7f800000u));
+            vsc[4 * h + 1] = fp4_value_scale<E>(__uint_as_float((w << 15) & 0x7f800000u));
+            vsc[4 * h + 2] = fp4_value_scale<E>(__uint_as_float((w << 7) & 0x7f800000u));
+            vsc[4 * h + 3] = fp4_value_scale<E>(__uint_as_float((w >> 1) & 0x7f800000u));
         }
         auto dims = [&](auto pair) __attribute__((always_inline)) {  // 2 pair and 2 pair + 1 of the lane's 8
             constexpr int I = decltype(pair)::value;
@@ -248,7 +248,7 @@ __device__ __forceinline__ void fp4_segment(const DecodeArgs& a, int b, int kv_l
             consume(i, p[x]);
         }
     }
-    s.l = head_sum(s.l);
+    s.l = fp4_row_sum<E>(head_sum(s.l));
 }
 
 // The lane's share of head c's outputs: dims 32 g + 8 i + dt, o[dt][i].

@@ -374,8 +374,9 @@ def kv_cache_read_fp4(
     The tokens are those that :func:`kv_cache_write_fp4` would write with the
     same arguments, e.g. a whole prefix that moves to 16-bit pools; zeros where
     that would have stopped, and for tokens that are in no sequence (before
-    ``cu_seqlens[0]``, from ``cu_seqlens[-1]`` on).  bf16 holds every value exactly; f16 rounds, and
-    values past its range are infinities.
+    ``cu_seqlens[0]``, from ``cu_seqlens[-1]`` on).  bf16 holds every value exactly;
+    f16 rounds, and values past its range are infinities, 65536 among them, which
+    the cache holds for f16 values past 57344.
     """
     if not kv_pool.is_cuda:
         raise ValueError(f"Argument 'kv_pool' must be a CUDA tensor. Got device={kv_pool.device}")
@@ -428,8 +429,8 @@ def paged_attention_gemv_fp4(
     q (n_heads, num_seqs, head_dim) bf16 or f16, head_dim a multiple of 16 up to
     128; ``kv_pool`` (num_blocks, n_kv_heads, page bytes) as written by
     :func:`kv_cache_write_fp4`.  Contexts of any length; an empty one gives zeros.
-    Keys and values are what the cache stands for (f16: V past its range is an
-    infinity); rows behind a context may hold anything.
+    Keys and values are what the cache stands for (f16: V from 131072 on, twice its
+    range, is an infinity); rows behind a context may hold anything.
     """
     return _hip_backend._paged_attention_gemv_fp4(_ensure_valid_tensor(q, "q"), kv_pool, kv_page_tables, kv_lens, max_kv_len)
 
