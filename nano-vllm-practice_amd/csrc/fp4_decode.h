@@ -68,10 +68,15 @@ __device__ __forceinline__ Fp4Query fp4_query(const float (&x)[32]) {
         const int b = byte == kFp4NanScale ? byte : byte - kDown[t];
         const float s = fp4_scale(byte == kFp4NanScale ? 127 : b);
         q.scales |= (uint32_t)b << (8 * t);
-        q.term[t] = __builtin_bit_cast(u32x6, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, s));
+        // These conversions write their first registers before they have read their
+        // last (with the result over registers 2 to 7 of a source: wrong values), and
+        // the compiler takes a source that ends here for free: it is kept.
+        auto w = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, s);
+        asm volatile("" : "+v"(w) : "v"(even), "v"(odd), "v"(s));
+        q.term[t] = __builtin_bit_cast(u32x6, w);
         if (t + 1 < kFp4Terms) {
-            const f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(
-                __builtin_bit_cast(decltype(__builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, s)), q.term[t]), s);
+            f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(w, s);
+            asm volatile("" : "+v"(back) : "v"(w), "v"(s));
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 even[i] -= back[2 * i];
