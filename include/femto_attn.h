@@ -423,7 +423,7 @@ int femto_rope_cache_write_fp4(
  * keys j < kv_lens[b], of any number.  A block id outside the pool, or a column
  * past the table, reads as zeros; kv_len == 0 yields a zero row.  Rows of the last
  * page past kv_len may hold anything.  P rounds to q's type for the second
- * product, everything else is 32-bit or exact but q, which is taken to 2^-14 of
+ * product, everything else is 32-bit or exact but q, which is taken to 2^-18 of
  * the largest magnitude of its 32 dims.  The workspace (256-byte aligned;
  * workspace_size 0: none; it is that of the current device) has to be zero in
  * its first femto_paged_attention_gemv_fp4_zero_bytes() bytes before its first
@@ -444,8 +444,9 @@ size_t femto_paged_attention_gemv_fp4_zero_bytes(void);
  * keys j < kv_lens[b] with j <= positions[t]; a token that sees none gives NaN.
  * Sequences of one token are taken as decode rows.  A block of V that is NaN in a
  * key that a token sees also reaches those of its query tile (up to 128 tokens
- * of the chunk) that do not.  The
- * workspace (256-byte aligned, always needed) has to be zero in its first
+ * of the chunk) that do not.  q is taken to 2^-14 of the largest magnitude of its 32
+ * dims; in a row where 12 dims of a block are under 1/256 of its largest (f16:
+ * 1/32), to 2^-18.  The workspace (256-byte aligned, always needed) has to be zero in its first
  * femto_paged_attention_gemm_split_bytes() bytes before its first use and is
  * left so; calls that may overlap must not share one. */
 int femto_paged_attention_gemm_fp4(

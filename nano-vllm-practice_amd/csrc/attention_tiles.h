@@ -172,7 +172,7 @@ __device__ __forceinline__ int serpentine(int k, int n, int cus) {
 // causal rule over a cache held in 4 bits (fp4.h; a.k the pool, a.k_stride0 and
 // a.k_stride1 bytes from block to block and head to head): K's codes are copied
 // into LDS as they are and multiplied by scaled matrix instructions with q in
-// three terms of 6 bits (fp4_decode.h); V's are loaded into registers a tile
+// three terms of 6 bits, or four (fp4_decode.h); V's are loaded into registers a tile
 // ahead, and converted into LDS rows of the storage type beside the second half of
 // the tile's P . V, once for all of the tile's query rows.
 template <typename E, int G, bool PAGED, bool FUSED, bool FULLD = true, int RULE = kAllPages>
@@ -186,6 +186,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __shared__ int s_kend[4];
     __shared__ int s_kbeg[4];  // kWindowPages
     constexpr bool WINDOW = RULE == kWindowPages, PREFIX = RULE == kTailPages, FP4 = RULE == kFp4Pages;
+    constexpr int kLastTerm = 5 * 1024;  // kFp4Pages, in a stage's K: what is behind a tile's codes and scales
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -813,11 +814,41 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
     // Q rows in registers: the B operand of S^T = K . Q^T.
     u32x4 qreg[8];
-    Fp4Query q4[2];  // kFp4Pages: of dims 32 h2 .. and 64 + 32 h2 ..
+    Fp4Query<kFp4Terms - 1> q4[2];  // kFp4Pages: of dims 32 h2 .. and 64 + 32 h2 ..
+    uint32_t q4_scales[2];
+    bool large = false;  // the wave's scores take q's last terms
     if constexpr (FP4) {
         const char* qrow = reinterpret_cast<const char*>(a.q) + ((int64_t)h * a.q_stride_head + (int64_t)t * a.q_stride_token) * EB;
+        const int D = FULLD ? kDimHead : a.head_dim;
+        Fp4QueryWords qw[2];
+        bool mine = false;
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) q4[kk] = fp4_query_row<E>(qrow, 2 * kk + h2, FULLD ? kDimHead : a.head_dim, qvalid, a.scale_log2);
+        for (int kk = 0; kk < 2; ++kk) qw[kk] = fp4_query_words(qrow, 2 * kk + h2, D, qvalid);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            q4[kk] = fp4_query<E, kFp4Terms - 1>(qw[kk], a.scale_log2);
+            q4_scales[kk] = q4[kk].scales;
+            mine |= fp4_query_large<E>(qw[kk], 2 * kk + h2, D);
+        }
+        // Where a row of the wave wants fourth terms, its scores take them (all
+        // scores: 2048 tokens at 30k 888 -> 989 us); zeros for rows that do not,
+        // whose results so do not depend on the rows beside them.  They wait in LDS,
+        // behind K's codes and scales: there is no register for them.
+        const uint64_t rows = __ballot(mine);
+        large = rows != 0;
+        if (__builtin_expect(large, 0)) {
+            mine = ((rows | rows >> 32) >> l32 & 1) != 0;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                const Fp4Query<kFp4Terms> all = fp4_query<E, kFp4Terms>(fp4_query_words(qrow, 2 * kk + h2, D, qvalid), a.scale_log2);
+                u32x6 w = all.term[kFp4Terms - 1];
+#pragma unroll
+                for (int i = 0; i < 6; ++i) w[i] = mine ? w[i] : 0u;
+                q4_scales[kk] = all.scales;
+                *reinterpret_cast<u32x4*>(&smem[kk][0][kLastTerm + 16 * tid]) = u32x4{w[0], w[1], w[2], w[3]};
+                *reinterpret_cast<u32x2*>(&smem[kk][0][kLastTerm + 4096 + 8 * tid]) = u32x2{w[4], w[5]};
+            }
+        }
     } else {
         const char* qrow = reinterpret_cast<const char*>(a.q) +
                            ((int64_t)b * a.q_stride_batch + (int64_t)h * a.q_stride_head + (int64_t)t * a.q_stride_token) * EB;
@@ -1000,6 +1031,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         auto k4frag = [&](int block, int kk) __attribute__((always_inline)) {
             return *reinterpret_cast<const u32x4*>(ks + 1024 * (l32 >> 4) + 256 * h2 + 16 * (l32 & 15) + 2048 * block + 512 * kk);
         };
+        // q's smallest term of dims 64 kk + 32 h2 ..
+        auto last_term = [&](int kk) __attribute__((always_inline)) {
+            uint32_t id = 0;
+            asm volatile("" : "+v"(id));  // (else its addresses hold registers all the time)
+            id = 64 * wave + __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, id));
+            const u32x4 x = *reinterpret_cast<const u32x4*>(&smem[kk][0][kLastTerm + 16 * id]);
+            const u32x2 y = *reinterpret_cast<const u32x2*>(&smem[kk][0][kLastTerm + 4096 + 8 * id]);
+            return fp4_operand(u32x6{x[0], x[1], x[2], x[3], y[0], y[1]});
+        };
         // (the word's bytes 0 and 2: those of kk = 0 and 1)
         auto k4scale = [&](int block) __attribute__((always_inline)) {
             return *reinterpret_cast<const uint32_t*>(ks + 4 * 1024 + 4 * (32 * block + l32)) >> (8 * h2);
@@ -1021,13 +1061,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 k4[block][1] = k4frag(block, 1);
             }
             __builtin_amdgcn_sched_barrier(0);
-            // MFMA m of a block: term 2 - m / 2 (the smallest first), half m % 2 of the dims.
+            // c + K . (a term of q), half kk of the dims.
+            auto term_of = [&](const f32x16& c, int block, auto kk_c, auto term_c, i32x8 w) __attribute__((always_inline)) {
+                constexpr int kk = decltype(kk_c)::value, term = decltype(term_c)::value;
+                return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(k4[block][kk]), w, c, kFormatFp4, kFormatFp6,
+                                                                       2 * kk, (int)ks4[block], term, (int)q4_scales[kk]);
+            };
+            // MFMA m of a block: term 2 - m / 2 (the smaller first), half m % 2 of the dims.
             auto score = [&](f32x16& s, int block, auto m_c) __attribute__((always_inline)) {
                 constexpr int m = decltype(m_c)::value, kk = m & 1, term = 2 - (m >> 1);
-                s = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(k4[block][kk]), fp4_operand(q4[kk].term[term]),
-                                                                    m == 0 ? neg_m16 : s,
-                                                                    kFormatFp4, kFormatFp6, 2 * kk, (int)ks4[block], term,
-                                                                    (int)q4[kk].scales);
+                s = term_of(m == 0 ? neg_m16 : s, block, std::integral_constant<int, kk>{}, std::integral_constant<int, term>{},
+                            fp4_operand(q4[kk].term[term]));
+            };
+            // The smallest term, where the wave has rows that need it.
+            auto last = [&](f32x16& s, int block) __attribute__((always_inline)) {
+                if (__builtin_expect(!large, 1)) return;
+                constexpr std::integral_constant<int, kFp4Terms - 1> term{};
+                s = term_of(s, block, std::integral_constant<int, 0>{}, term, last_term(0));
+                s = term_of(s, block, std::integral_constant<int, 1>{}, term, last_term(1));
             };
             auto bundle0 = [&](auto m_c) __attribute__((always_inline)) {
                 score(s0, 0, m_c);
@@ -1046,12 +1097,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             };
             bundle0(std::integral_constant<int, 0>{});
             bundle0(std::integral_constant<int, 1>{});
+            last(s0, 0);
             bundle0(std::integral_constant<int, 2>{});
             bundle0(std::integral_constant<int, 3>{});
             bundle0(std::integral_constant<int, 4>{});
             bundle0(std::integral_constant<int, 5>{});
             bundle1(std::integral_constant<int, 0>{});
             bundle1(std::integral_constant<int, 1>{});
+            last(s1, 1);
             bundle1(std::integral_constant<int, 2>{});
             bundle1(std::integral_constant<int, 3>{});
             bundle1(std::integral_constant<int, 4>{});

@@ -13,10 +13,12 @@
 //     which is the operand that the instruction takes.
 //   O^T (128 dims x 16 heads) += V^T . P^T, 8 x v_mfma_f32_16x16x32.
 // The first product reads K without converting it.  Its other operand may have
-// 6 bits at the same rate (8 bits halve it): q is split into three terms of 6 bits,
-// each with a scale for 32 dims, which leave out at most 2^-14 of the largest of
-// those dims (fp4_query), a quarter of f16's rounding there; products are exact
-// and sums 32-bit.
+// 6 bits at the same rate (8 bits halve it): q is split into four terms of 6 bits,
+// each with a scale for 32 dims, which leave out at most 2^-18 of the largest of
+// those dims (fp4_query): nothing of a bf16 dim down to 2^-11 of it, of an f16 one
+// to 2^-8; products are exact and sums 32-bit.  (Three terms, 2^-14, leave a dim of 1
+// beside one of 512 off by 1.6e-2.  The fourth: 61 sequences to 16k 89.9 us either
+// way, one of 5000 keys 9.4 and 9.6.)
 // V is wanted by dims, its values convert to 16 bits two dims at a time
 // (v_cvt_scalef32_pk, exact in bf16; f16: halves of them, fp4_value_scale), and a
 // permute per two values pairs keys: a 16-byte load holds 8 dims of four keys, so
@@ -33,38 +35,69 @@ namespace femto {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
 typedef float f32x32 __attribute__((ext_vector_type(32)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kFp4Terms = 3;
+constexpr int kFp4Terms = 4;
 constexpr int kFormatFp6 = 2, kFormatFp4 = 4;  // operand formats of the scaled matrix instructions
 
-// 32 dims of a query as kFp4Terms terms of 6 bits (a sign, 0 to 7.5); byte i of
+// 32 dims of a query as `TERMS` terms of 6 bits (a sign, 0 to 7.5); byte i of
 // `scales` is the scale byte of term i.
+template <int TERMS>
 struct Fp4Query {
-    u32x6 term[kFp4Terms];
+    u32x6 term[TERMS];
     uint32_t scales;
 };
 
-// x: dims 0 .. 31.  With the first scale s no |x / s| is past 7.75, so the first
-// term leaves at most s / 4; of the second's scale, s / 16, that is at most 4, and at
-// most an eighth of it is left; of the third's, s / 512, again at most 4 and an
-// eighth: 2^-12 s, and the largest magnitude is above 3.875 s.  A block with an
-// infinity or a NaN has NaN scales: its scores are NaN.
-__device__ __forceinline__ Fp4Query fp4_query(const float (&x)[32]) {
-    uint32_t top = 0;
+// Dims 32 b .. of a row of 16-bit values; dims from D on, and rows that are not there: zeros.
+struct Fp4QueryWords {
+    u32x4 w[4];
+};
+__device__ __forceinline__ Fp4QueryWords fp4_query_words(const char* row, int b, int D, bool valid) {
+    Fp4QueryWords q;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    const int byte = top >= 0x7f800000u ? kFp4NanScale : max(10, (int)((top + 0x7ffffu) >> 23) - 2);
-    constexpr int kDown[kFp4Terms] = {0, 4, 9};
-    Fp4Query q;
-    q.scales = 0;
+    for (int i = 0; i < 4; ++i) {
+        const int d = 32 * b + 8 * i;
+        q.w[i] = valid && d < D ? ld16(row + 2 * d) : u32x4{0, 0, 0, 0};
+    }
+    return q;
+}
+// The largest magnitude's bits.
+__device__ __forceinline__ uint32_t fp4_query_top(const Fp4QueryWords& q) {
+    u16x2 top = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, q.w[i >> 2][i & 3] & 0x7fff7fffu));
+    return max(top[0], top[1]);
+}
+
+// The terms of x = (dims) scale.  With the first term's scale s no |x / s| is past
+// 7.75, so it leaves at most s / 4; of the second's scale, s / 16, that is at most
+// 4, and at most an eighth of it is left; of the third's, s / 512, again at most 4
+// and an eighth: 2^-12 s; and of the fourth's, s / 2^14, 2^-17 s, where the largest
+// magnitude is above 3.875 s.  (Of dims below 2 s each leaves half as much.)  A
+// block with an infinity or a NaN has NaN scales: its scores are NaN.
+template <typename E, int TERMS>
+__device__ __forceinline__ Fp4Query<TERMS> fp4_query(const Fp4QueryWords& words, float scale) {
     f32x16 even, odd;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        even[i] = x[2 * i];
-        odd[i] = x[2 * i + 1];
-    }
+    for (int i = 0; i < 4; ++i) {
+        float f[8];
+        unpack8(E{}, words.w[i], f);
 #pragma unroll
-    for (int t = 0; t < kFp4Terms; ++t) {
+        for (int e = 0; e < 4; ++e) {
+            even[4 * i + e] = f[2 * e] * scale;
+            odd[4 * i + e] = f[2 * e + 1] * scale;
+        }
+    }
+    float f[8];
+    unpack8(E{}, u32x4{fp4_query_top(words), 0, 0, 0}, f);
+    const uint32_t top = __float_as_uint(f[0] * scale) & 0x7fffffffu;  // (rounding keeps the order)
+    const int byte = top >= 0x7f800000u ? kFp4NanScale : max(15, (int)((top + 0x7ffffu) >> 23) - 2);
+    constexpr int kDown[kFp4Terms] = {0, 4, 9, 14};
+    Fp4Query<TERMS> q;
+    q.scales = 0;
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t) {
         const int b = byte == kFp4NanScale ? byte : byte - kDown[t];
         const float s = fp4_scale(byte == kFp4NanScale ? 127 : b);
         q.scales |= (uint32_t)b << (8 * t);
@@ -72,11 +105,11 @@ __device__ __forceinline__ Fp4Query fp4_query(const float (&x)[32]) {
         // last (with the result over registers 2 to 7 of a source: wrong values), and
         // the compiler takes a source that ends here for free: it is kept.
         auto w = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, s);
-        asm volatile("" : "+v"(w) : "v"(even), "v"(odd), "v"(s));
+        asm("" : "+v"(w) : "v"(even), "v"(odd), "v"(s));
         q.term[t] = __builtin_bit_cast(u32x6, w);
-        if (t + 1 < kFp4Terms) {
+        if (t + 1 < TERMS) {
             f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(w, s);
-            asm volatile("" : "+v"(back) : "v"(w), "v"(s));
+            asm("" : "+v"(back) : "v"(w), "v"(s));
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 even[i] -= back[2 * i];
@@ -87,19 +120,24 @@ __device__ __forceinline__ Fp4Query fp4_query(const float (&x)[32]) {
     return q;
 }
 
-// The same of dims 32 b .. of a row of 16-bit values, times `scale`; dims from D on are zeros.
+// Whether three terms do not do for the block.  They leave up to 2^-15 of the
+// largest magnitude of small dims, more than half a step of their own in bf16 below
+// 1/256 of it, in f16 below 1/32; with 12 and more such dims of 32 that counts.  (Of
+// 32 normal values 12 that small are one block in 10^9 in bf16, 10^7 in f16.)
+// Zeros among them, which any term holds, are not told apart, but for dims
+// from D on.
 template <typename E>
-__device__ __forceinline__ Fp4Query fp4_query_row(const char* row, int b, int D, bool valid, float scale) {
-    float x[32];
+__device__ __forceinline__ bool fp4_query_large(const Fp4QueryWords& q, int b, int D) {
+    const int below = std::is_same<E, F16>::value ? 5 << 10 : 8 << 7;
+    const uint16_t limit = (uint16_t)max((int)fp4_query_top(q) - below, 0);
+    u16x2 count = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int d = 32 * b + 8 * i;
-        const u32x4 w = valid && d < D ? ld16(row + 2 * d) : u32x4{0, 0, 0, 0};
-        unpack8(E{}, w, *reinterpret_cast<float(*)[8]>(x + 8 * i));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[8 * i + e] *= scale;
+    for (int i = 0; i < 16; ++i) {
+        const u16x2 x = __builtin_bit_cast(u16x2, q.w[i >> 2][i & 3] & 0x7fff7fffu);
+        count += __builtin_elementwise_min(__builtin_elementwise_sub_sat(u16x2{limit, limit}, x), u16x2{1, 1});
     }
-    return fp4_query(x);
+    const int absent = limit > 0 ? max(32 * b + 32 - max(D, 32 * b), 0) : 0;
+    return count[0] + count[1] - absent >= 12;
 }
 
 __device__ __forceinline__ i32x8 fp4_operand(u32x4 w) {
@@ -108,16 +146,11 @@ __device__ __forceinline__ i32x8 fp4_operand(u32x4 w) {
 __device__ __forceinline__ i32x8 fp4_operand(u32x6 w) {
     return i32x8{(int)w[0], (int)w[1], (int)w[2], (int)w[3], (int)w[4], (int)w[5], 0, 0};
 }
-// c + K . q over 128 dims: K's 16 keys x 4 blocks with the scale in byte 0 of ks;
-// the smallest term first.
-__device__ __forceinline__ f32x4 fp4_scores16(u32x4 k, uint32_t ks, const Fp4Query& q) {
-    f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
-    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(k), fp4_operand(q.term[2]), c, kFormatFp4, kFormatFp6,
-                                                         0, (int)ks, 2, (int)q.scales);
-    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(k), fp4_operand(q.term[1]), c, kFormatFp4, kFormatFp6,
-                                                         0, (int)ks, 1, (int)q.scales);
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(k), fp4_operand(q.term[0]), c, kFormatFp4,
-                                                            kFormatFp6, 0, (int)ks, 0, (int)q.scales);
+// c + K . (term T of q) over 128 dims: K's 16 keys x 4 blocks with the scale in byte 0 of ks.
+template <int T>
+__device__ __forceinline__ f32x4 fp4_scores16(u32x4 k, uint32_t ks, const Fp4Query<kFp4Terms>& q, f32x4 c) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(k), fp4_operand(q.term[T]), c, kFormatFp4, kFormatFp6,
+                                                            0, (int)ks, T, (int)q.scales);
 }
 
 // A page in registers: the lane of key (or dims) c = lane % 16 and block (or four
@@ -136,11 +169,11 @@ __device__ __forceinline__ void fp4_segment(const DecodeArgs& a, int b, int kv_l
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int D = FULL ? kDimHead : a.head_dim, N = fp4_blocks(D);
     s.clear();
-    const Fp4Query q = fp4_query_row<E>(static_cast<const char*>(a.q) + ((int64_t)(h0 + c) * a.q_stride_head + (int64_t)qrow * a.q_stride_seq) * 2,
-                                        g, D, c < nh, 1.0f);
+    const Fp4QueryWords qw = fp4_query_words(static_cast<const char*>(a.q) + ((int64_t)(h0 + c) * a.q_stride_head + (int64_t)qrow * a.q_stride_seq) * 2,
+                                             g, D, c < nh);
     const int kb = FULL || g < N ? g : 0, vc = FULL || c < 4 * N ? c : 0;
     const uint32_t k_at = 256 * kb + 16 * c, v_at = 256 * N + 64 * N * g + 16 * vc;
-    const uint32_t ks_at = 512 * N + 4 * c + kb, vs_at = 512 * N + 64 + 16 * g + 4 * (vc >> 2);
+    const uint32_t ks_at = 512 * N + 4 * c, vs_at = 512 * N + 64 + 16 * g + 4 * (vc >> 2);
     const GlobalBytes pool = as_global(a.k_pool) + (int64_t)kvh * a.pool_stride_head;
     uint64_t zero = (uint64_t)(uintptr_t)g_zero_page;
     asm volatile("" : "+s"(zero));  // (else its address is loaded, and waited for, for every page)
@@ -163,17 +196,27 @@ __device__ __forceinline__ void fp4_segment(const DecodeArgs& a, int b, int kv_l
         // the scales share a line, of which each load takes half.
         p.k = load_global_nt<u32x4>(page + k_at);
         p.v = load_global_nt<u32x4>(page + v_at);
-        p.ks = page[ks_at];
+        p.ks = load_global<uint32_t>(page + ks_at);
         p.vs = load_global<uint32_t>(page + vs_at);
     };
     const float scale = a.scale_log2;
+    Fp4Query<kFp4Terms> q;
     auto consume = [&](int i, Fp4Page (&p)[2]) __attribute__((always_inline)) {
         float sc[8];
+        {
+            // The smallest term first; the two pages' products take turns.
+            const uint32_t ks[2] = {p[0].ks >> (8 * kb), p[1].ks >> (8 * kb)};
+            f32x4 x[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const f32x4 x = fp4_scores16(p[h].k, p[h].ks, q);
+            for (int h = 0; h < 2; ++h) x[h] = fp4_scores16<3>(p[h].k, ks[h], q, x[h]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sc[4 * h + j] = x[j];
+            for (int h = 0; h < 2; ++h) x[h] = fp4_scores16<2>(p[h].k, ks[h], q, x[h]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) x[h] = fp4_scores16<1>(p[h].k, ks[h], q, x[h]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) x[h] = fp4_scores16<0>(p[h].k, ks[h], q, x[h]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sc[j] = x[j >> 2][j & 3];
         }
         // Keys past the segment or the context: no weight, and V of zeros (0
         // times a NaN would not be 0).
@@ -242,6 +285,8 @@ __device__ __forceinline__ void fp4_segment(const DecodeArgs& a, int b, int kv_l
         issue(2 * i, p[i][0]);
         issue(2 * i + 1, p[i][1]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    q = fp4_query<E, kFp4Terms>(qw, 1.0f);  // (while they are on their way)
     for (int i0 = 0; i0 < n; i0 += 2 * STAGES) {
 #pragma unroll
         for (int x = 0; x < STAGES; ++x) {

@@ -1,6 +1,12 @@
 """Attention over the 4-bit cache where its values, queries or hidden rows are not the usual ones, against the 64-bit oracle.
 
-f16 values that round to 65536 in the cache.
+* Queries whose blocks of 32 dims hold one large channel: what the other dims hold has to arrive all the same.  The values
+  here need at most 18 bits below a block's largest magnitude's exponent, which a split of q into four terms holds exactly in
+  decode; a prefill query is split after it took the softmax scale, and is off by at most 2^-18 of the largest magnitude of
+  its block.
+* Sharp scores, where one key's weight is near 1 and a score's error moves outputs by as much: bounds per row, from the row's
+  own weights, and far below the spread of its values.
+* f16 values that round to 65536 in the cache.
 """
 
 import numpy as np
@@ -9,7 +15,7 @@ import torch
 
 import oracle.fp4 as of
 from fp4_helpers import Batch, pool_of
-from helpers import half_ulp, np64
+from helpers import assert_close, half_ulp, np64
 
 pytestmark = pytest.mark.gpu
 
@@ -59,14 +65,14 @@ def rows_of(w, decode):
 
 
 def weights(w, decode):
-    """want (H, T, D), sum_j w_j |v_j| and sum_j w_j |v_j - want| (the same shape), and |q| . |k| / sqrt(D) of the row's
-    largest key with q's magnitudes those of its blocks' largest (H, T)."""
+    """want (H, T, D), sum_j w_j |v_j| and sum_j w_j |v_j - want| (the same shape); and of the row's largest key, (H, T) each,
+    the sum over dims of |k| and the root of that of k^2, times the largest |q| of the dim's block, over sqrt(D)."""
     H, T, D = w.q.shape
     K, V = of.rows(w.pool, D)
     rep, q = H // w.pool.shape[1], np64(w.q)
     top = np.abs(q).reshape(H, T, -1, min(32, D)).max(-1).repeat(min(32, D), -1)
     want, size, spread = np.zeros((3, H, T, D))
-    reach = np.zeros((H, T))
+    reach, root = np.zeros((2, H, T))
     for t, length, b in rows_of(w, decode):
         k, v = of.gather(K, w.tables[b], length), of.gather(V, w.tables[b], length)
         for h in range(H):
@@ -77,11 +83,82 @@ def weights(w, decode):
             want[h, t] = p @ x
             size[h, t], spread[h, t] = p @ np.abs(x), p @ np.abs(x - want[h, t])
             reach[h, t] = (np.abs(k[h // rep]) @ top[h, t]).max() / np.sqrt(D)
-    return want, size, spread, reach
+            root[h, t] = np.sqrt((k[h // rep] ** 2 @ top[h, t] ** 2).max() / D)
+    return want, size, spread, reach, root
 
 
 LENS = [1, 17, 64, 100, 333, 1000]
 CHUNKS = [(0, 130), (200, 70), (90, 1), (900, 40), (40, 1)]
+
+
+def large_channels(chunks, heads, dim, dtype, top, seed, decode):
+    """q: N(0, 1) past 1/8, and ``top`` in dims 5, 37, ..; K zero there, else of size 4; V of size 1."""
+    w = Batch(chunks, *heads, dim, dtype, seed, decode=decode)
+    rng = np.random.default_rng(seed)
+    K, V = rng.standard_normal((2, len(w.pool), heads[1], 16, dim))
+    K *= 4
+    K[..., 5::32] = 0
+    refill(w, K, V)
+    q = w.q.float()
+    q = torch.where(q < 0, q.clamp(max=-0.125), q.clamp(min=0.125))
+    q[..., 5::32] = top * torch.sign(q[..., 5::32])
+    w.q = q.to(dtype)
+    return w
+
+
+@pytest.mark.parametrize("dtype,top", [(BF16, 512.0), (F16, 64.0)])
+@pytest.mark.parametrize("dim", [128, 64, 80])
+@pytest.mark.parametrize("heads", [(8, 2), (4, 4)])
+def test_decode_of_queries_with_large_channels(ops, gpu, heads, dim, dtype, top):
+    w = large_channels([(n - 1, 1) for n in LENS], heads, dim, dtype, top, dim + sum(heads), True)
+    assert_close(gemv(ops, gpu, w), of.decode(np64(w.q), w.pool, w.tables, w.kv_lens), dtype, f"channels of {top}")
+
+
+@pytest.mark.parametrize("dtype,top", [(BF16, 512.0), (F16, 64.0)])
+@pytest.mark.parametrize("dim", [128, 64, 80])
+@pytest.mark.parametrize("heads", [(8, 2), (4, 4), (4, 2)])
+def test_prefill_of_queries_with_large_channels(ops, gpu, heads, dim, dtype, top):
+    """The split's error here: at most 2^-18 * 512 of a dim of q, so some 2^-9 / sqrt(3) * 4 of a score, in f16 an eighth."""
+    w = large_channels(CHUNKS, heads, dim, dtype, top, dim + sum(heads), False)
+    assert_close(gemm(ops, gpu, w), of.prefill(np64(w.q), w.pool, w.cu, w.tables, w.kv_lens, w.pos), dtype, f"channels of {top}")
+
+
+@pytest.mark.parametrize("top", [64.0, 1000.0])
+def test_a_query_of_large_channels_beside_others(ops, gpu, top):
+    """Few of a tile's queries have them, in one block each: no other row's result depends on them."""
+    w = Batch([(300, 200), (50, 1), (0, 64)], 8, 2, 128, BF16, 3)
+    pool, tables, lens, cu, pos, q = w.on(gpu)
+    plain = ops.paged_attention_gemm_fp4(q, pool, cu, 200, tables, lens, pos)
+    rows = [3, 70, 199, 200, 230]
+    w.q[:, rows, 40] = top
+    got = gemm(ops, gpu, w)
+    want = of.prefill(np64(w.q), w.pool, w.cu, w.tables, w.kv_lens, w.pos)
+    others = [t for t in range(q.size(1)) if t not in rows]
+    assert_close(got[:, others], want[:, others], BF16, "others")
+    assert_close(got[:, others], np64(plain[:, others]), BF16, "others as before")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("decode,scale", [(d, s) for d in (True, False) for s in (1.0, 4.0, 12.0, 30.0, 200.0) if d or s < 200])
+def test_sharp_scores_row_by_row(ops, gpu, decode, scale, dtype):
+    """K of size ``scale``.  A weight is off by its rounding (eps / 2 of P, and as much of the sum) and by e^(2 ds) - 1, ds
+    a score's error: q's split (decode: none, q's values are held exactly; prefill, three terms: at most 2^-14 of the
+    blocks' largest magnitudes in each dim, six times its random sum) and 32-bit sums of some 130 terms (each at most 2^-24
+    of the sum of magnitudes, ten times their random sum)."""
+    chunks = [(n - 1, 1) for n in LENS] if decode else CHUNKS
+    w = Batch(chunks, 8, 2, 128, dtype, int(10 * scale), decode=decode, scale=scale)
+    hide(w, 255, 255)
+    q = w.q.float()
+    w.q = torch.where(q < 0, q.clamp(max=-2.0**-5), q.clamp(min=2.0**-5)).to(dtype)
+    got = np64(gemv(ops, gpu, w) if decode else gemm(ops, gpu, w))
+    want, size, spread, reach, root = weights(w, decode)
+    ds = ((0 if decode else 6 * 2.0**-14 / np.sqrt(3)) * root + 2.0**-24 * 10 * np.sqrt(130) * reach)[..., None]
+    step = torch.finfo(dtype).eps / 2
+    bound = spread * np.expm1(2 * ds) + size * 2 * step + half_ulp(np.abs(want), dtype) + 2.0**-20
+    K, V = of.rows(w.pool, 128)
+    assert np.median(bound) < 0.02 * np.nanstd(V) and bound.max() < np.nanstd(V), (np.median(bound), bound.max())
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= bound).all(), (np.abs(got - want) / bound).max()
 
 
 @pytest.mark.parametrize("decode", [True, False])
@@ -98,7 +175,7 @@ def test_f16_values_that_round_to_65536(ops, gpu, decode):
     hide(w, 254, 0x77)
     assert (np.abs(of.rows(w.pool, 64)[1]) == 65536.0).any()
     got = np64(gemv(ops, gpu, w) if decode else gemm(ops, gpu, w))
-    want, size, _, _ = weights(w, decode)
+    want, size, _, _, _ = weights(w, decode)
     assert np.isfinite(got).all() and np.abs(want).max() > 10000
     # weights off by 2^-11 each, rounded, their sum's and the query's as much again
     assert (np.abs(got - want) <= size * 2.0**-9 + half_ulp(np.abs(want), F16) + 2.0**-11).all()
