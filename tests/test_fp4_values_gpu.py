@@ -6,7 +6,7 @@
   its block.
 * Sharp scores, where one key's weight is near 1 and a score's error moves outputs by as much: bounds per row, from the row's
   own weights, and far below the spread of its values.
-* f16 values that round to 65536 in the cache.
+* f16 values that round to 65536 in the cache; rows that no sequence holds, with full codes under large scales and NaN.
 """
 
 import numpy as np
@@ -179,3 +179,16 @@ def test_f16_values_that_round_to_65536(ops, gpu, decode):
     assert np.isfinite(got).all() and np.abs(want).max() > 10000
     # weights off by 2^-11 each, rounded, their sum's and the query's as much again
     assert (np.abs(got - want) <= size * 2.0**-9 + half_ulp(np.abs(want), F16) + 2.0**-11).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [128, 48])
+@pytest.mark.parametrize("byte,code", [(254, 0x77), (254, 0xFF), (255, 0x00), (255, 0xFF), (1, 0x99)])
+def test_rows_that_no_sequence_holds(ops, gpu, byte, code, dim, dtype):
+    """Full codes under the largest scale, NaN with any codes: nothing of them arrives."""
+    w = Batch([(n - 1, 1) for n in LENS + [15, 16, 31]], 4, 2, dim, dtype, 7, decode=True)
+    hide(w, byte, code)
+    assert_close(gemv(ops, gpu, w), of.decode(np64(w.q), w.pool, w.tables, w.kv_lens), dtype, "decode")
+    w = Batch(CHUNKS + [(0, 15), (0, 63), (17, 48)], 4, 2, dim, dtype, 8)
+    hide(w, byte, code)
+    assert_close(gemm(ops, gpu, w), of.prefill(np64(w.q), w.pool, w.cu, w.tables, w.kv_lens, w.pos), dtype, "prefill")
