@@ -185,6 +185,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __shared__ int s_seq, s_ltile, s_old;
     __shared__ int s_kend[4];
     __shared__ int s_kbeg[4];  // kWindowPages
+    __shared__ int s_kfull[4], s_nan[4];  // kFp4Pages
     constexpr bool WINDOW = RULE == kWindowPages, PREFIX = RULE == kTailPages, FP4 = RULE == kFp4Pages;
     constexpr int kLastTerm = 5 * 1024;  // kFp4Pages, in a stage's K: what is behind a tile's codes and scales
 
@@ -595,15 +596,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     };
     // ... and into LDS: V as rows of the storage type, zeros past the last key that
     // the query tile sees (their weights are 0, and 0 times a NaN would not be);
-    // K's scales behind its codes, those of blocks past the row's 1.
-    int seen4 = kv_len;  // (known before the first use)
+    // K's scales behind its codes, those of blocks past the row's 1.  From the first
+    // key on that some row does not see, a NaN block of V is zeros too, and its
+    // key, if it is the block's first, in s_nan: the rows that see it are made NaN
+    // in the end.
+    int seen4 = kv_len, full4 = 0;  // (known before the first use)
     auto mask_fp4 = [&](int it) __attribute__((always_inline)) {
         const int key0 = it * kKvTile + 16 * wave + 4 * lrow;
-        if (it * kKvTile + kKvTile > seen4) {  // wave-uniform
+        if (it * kKvTile + kKvTile > full4) {  // wave-uniform
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 v4[j] = key0 + j < seen4 ? v4[j] : 0;
                 v4_scale = key0 + j < seen4 ? v4_scale : v4_scale & ~(0xffu << (8 * j));
+            }
+            const uint32_t nan = ((v4_scale & 0x7f7f7f7fu) + 0x01010101u) & v4_scale & 0x80808080u;  // bytes of 255
+            if (__builtin_expect(__ballot(nan != 0) != 0, 0)) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool is = (nan >> (8 * j + 7) & 1) != 0;
+                    v4[j] = is ? 0 : v4[j];
+                    v4_scale = is ? v4_scale & ~(0xffu << (8 * j)) : v4_scale;
+                }
+                if (nan != 0) atomicMin(&s_nan[lpos >> 2], key0 + (__builtin_ctz(nan) >> 3));
             }
         }
     };
@@ -783,9 +797,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         if (lane == 0) s_kbeg[wave] = lo_min_w;
     }
     if (lane == 0) s_kend[wave] = kend_w;
+    if constexpr (FP4) {
+        if (lane == 0) s_kfull[wave] = kfull_w;
+        if (tid < 4) s_nan[tid] = 0x7fffffff;
+    }
     __syncthreads();
     const int kend = max(max(s_kend[0], s_kend[1]), max(s_kend[2], s_kend[3]));
-    if constexpr (FP4) seen4 = __builtin_amdgcn_readfirstlane(kend);
+    if constexpr (FP4) {
+        seen4 = __builtin_amdgcn_readfirstlane(kend);
+        full4 = __builtin_amdgcn_readfirstlane(min(min(s_kfull[0], s_kfull[1]), min(s_kfull[2], s_kfull[3])));
+    }
 
     // Key tiles of this piece: [t_lo, t_hi).  Pieces past the query tile's
     // last visible key have nothing to do (and are not counted); a tile that
@@ -1237,7 +1258,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     } else {
         tile_loop(std::false_type{});
     }
-    if constexpr (FP4) l_run = fp4_row_sum<E>(l_run);
+    if constexpr (FP4) {
+        l_run = fp4_row_sum<E>(l_run);
+        __syncthreads();
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) {
+            const int key = __builtin_amdgcn_readfirstlane(s_nan[dt]);
+            if (__builtin_expect(key != 0x7fffffff, 0)) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) oacc[dt][e] = key < lim ? __builtin_nanf("") : oacc[dt][e];
+            }
+        }
+    }
 
     if constexpr (PREFIX) {
         // The piece's states, for the merge launch (it takes a row's pieces

@@ -449,8 +449,9 @@ def paged_attention_gemm_fp4(
     Token t of sequence b sees key j iff ``j < kv_lens[b]`` and ``j <=
     positions[t]``; a token that sees no key gives NaN.  Types, dims and the
     pool as :func:`paged_attention_gemv_fp4`; chunks and single tokens may share a
-    call.  V that is NaN or, to f16, infinite in a key that a token sees also
-    reaches those of its query tile (up to 128 tokens of the chunk) that do not.
+    call.  V that is NaN reaches the tokens that see its key and no other; V that is an
+    infinity to f16 (from 131072 on) also reaches, as NaN, those of its query tile
+    (up to 128 tokens of the chunk) that do not.
     """
     return _hip_backend._paged_attention_gemm_fp4(_ensure_valid_tensor(q, "q"), kv_pool, cu_seqlens, max_q_len,
                                                   kv_page_tables, kv_lens, positions)
