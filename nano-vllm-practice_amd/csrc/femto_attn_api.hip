@@ -353,11 +353,12 @@ static int paged_decode_entry(const char* fn_name, int dtype, const void* q, int
 
 // Window rows (window_row in mfma_decode.h): workgroups per (sequence, KV head
 // group) and waves in each, for `rows` sequences whose queries see up to `seen`
-// keys.  Rows longer than 24 pages are cut where that still leaves each part a CU
-// of its own, into the square root of their pages (each more part shortens the
-// walk, and adds a state to the last part's merge).  One sequence of 8 KV heads
-// (32 query heads, bf16), whole and cut, us: 1024 keys 11.2 and 7.6 (6 parts),
-// 4096 39.3 and 9.9 (11), 16384 143 and 16.0 (22); 512 keys 7.4 and 6.8 (5).
+// keys.  Rows of 32 pages and more are cut where that still leaves each part a CU
+// of its own, into 0.7 of the square root of their pages (each more part shortens
+// the walk, and adds a state to the last part's merge).  One sequence of 8 KV heads
+// (32 query heads, bf16), whole and cut, us: 384 keys 6.4 and 6.8 (three parts), 512
+// 7.0 and 6.9 (four), 1024 9.1 and 7.4 (six), 4096 29 and 10.0 (11), 16384 127 and
+// 16.1 (22).
 // Sixteen of 4096 keys (128 rows): 48.6, 43.6 in two, 47.4 in three; 24
 // (192 rows): 59.7 and 66.7.  Whole rows take 8 waves where they are long or few.
 struct WindowParts {
@@ -369,7 +370,7 @@ static WindowParts window_parts(int64_t rows, int n_heads, int n_kv_heads, int s
     const int limit = g_single_max_kv.load(std::memory_order_relaxed);
     const int pages = seen > 0 ? (seen - 1) / femto::kPage + 1 : 0;
     WindowParts w{1, 4};
-    if (limit == kSingleMaxKV && pages >= 24 && 2 * groups <= cus)
+    if (limit == kSingleMaxKV && pages >= 32 && 2 * groups <= cus)
         w.parts = std::min((int)(cus / groups), (int)(0.7 * std::sqrt((double)pages) + 0.5));
     if (limit < 0) w.parts = 2;  // cut wherever there are pages for it
     if (groups > kWindowCounters || pages < 2) w.parts = 1;
