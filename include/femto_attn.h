@@ -382,7 +382,7 @@ size_t femto_fp4_page_bytes(int head_dim); /* 512 N + 128; 0: head_dim not suppo
  * cu_seqlens == NULL: one token per sequence.  max_q_len (at least 1) decides
  * nothing: sequences of any length are taken whole.  Tokens of one call want
  * places of their own: two at one place leave a mix of both.  At most 65535
- * sequences. */
+ * sequences, as femto_kv_cache_write. */
 int femto_kv_cache_write_fp4(
     int dtype,
     const void* k, int64_t k_stride_token, int64_t k_stride_head,

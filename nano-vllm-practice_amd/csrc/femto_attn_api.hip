@@ -624,6 +624,8 @@ static int fp4_cache_args(const std::string& f, int dtype, const void* kv_pool, 
     if (num_seqs == 0 || num_tokens == 0) return FEMTO_OK;
     if (!cu_seqlens && num_tokens != num_seqs)
         return fail(FEMTO_ERR_INVALID, f + ": without cu_seqlens every sequence has one token (num_tokens == num_seqs)");
+    // These two decide nothing in the kernels, whose grid is by tokens: they are the
+    // 16-bit cache's, so that either cache takes the batches that the other does.
     if (max_q_len < 1) return fail(FEMTO_ERR_INVALID, f + ": max_q_len must be >= 1");
     if (num_seqs > 65535) return fail(FEMTO_ERR_INVALID, f + ": at most 65535 sequences per call");
     if (n_kv_heads <= 0) return fail(FEMTO_ERR_INVALID, f + ": head counts must be positive");
