@@ -32,7 +32,7 @@
 // 289 and 222, but 8 x 512 tokens 11.4 us a call for 10.9.)
 //
 // Measured (bf16, 32 / 8 heads of 128): prologue of 8 x 512 tokens 20.0 us, 4.4 TB/s,
-// bound by memory; with norms 29.3: 174 registers leave two waves per SIMD, so the
+// bound by memory; with norms 29.3: 176 registers leave two waves per SIMD, so the
 // 4096 waves run in two rounds, in each of which the VALU is busy 60 % and a wave
 // waits 44 % of its time for loads that nothing else is there to hide.  Of 64 decode
 // tokens 5.0 and 5.7, bound by latency (placement, table, batch); of 1024 beside 127

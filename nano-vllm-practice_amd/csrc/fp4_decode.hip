@@ -2,10 +2,12 @@
 // launches.
 //
 // Measured (bf16 of 128 dims; a call of many, us): bound by memory, 61 sequences of
-// 256-16384 keys, 16/8 heads, 90.8 (556 MB at 6.1 TB/s: split kernel 85, merge 4.6),
-// 256 of 1024-8192, 32/8, 200.6 (1.22 GB at 6.1 TB/s); f16, 16 of 8192-32768, 32/8,
-// 65.4 (5.7 TB/s).  The matrix units are busy 13 % of that.  One sequence of 5000
-// keys 9.3, bound by latency: table, pages, states to memory, count, states back.
+// 256-16384 keys, 16/8 heads, 90.0 (556 MB at 6.2 TB/s: split kernel 84, merge 4.5),
+// 256 of 1024-8192, 32/8, 199.9 (1.22 GB at 6.1 TB/s); f16, 16 of 8192-32768, 32/8,
+// 65.1 (5.7 TB/s).  The matrix units are busy 15 % of that.  One sequence of 5000
+// keys 9.6, bound by latency: table, pages, states to memory, count, states back.
+// Of fewer dims the lanes of absent blocks load block 0 again: the 61 and the 256
+// sequences of 64 dims 71 and 147 (3.9 and 4.1 TB/s), of 80 77 and 162.
 #include <algorithm>
 
 #include "fp4_decode.h"
