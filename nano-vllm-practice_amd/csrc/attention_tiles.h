@@ -837,7 +837,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     u32x4 qreg[8];
     Fp4Query<kFp4Terms - 1> q4[2];  // kFp4Pages: of dims 32 h2 .. and 64 + 32 h2 ..
     uint32_t q4_scales[2];
-    bool large = false;  // the wave's scores take q's last terms
+    int large = 0;  // the wave's scores take q's last terms
     if constexpr (FP4) {
         const char* qrow = reinterpret_cast<const char*>(a.q) + ((int64_t)h * a.q_stride_head + (int64_t)t * a.q_stride_token) * EB;
         const int D = FULLD ? kDimHead : a.head_dim;
@@ -856,8 +856,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         // whose results so do not depend on the rows beside them.  They wait in LDS,
         // behind K's codes and scales: there is no register for them.
         const uint64_t rows = __ballot(mine);
-        large = rows != 0;
-        if (__builtin_expect(large, 0)) {
+        large = __builtin_amdgcn_readfirstlane((int)((uint32_t)rows | (uint32_t)(rows >> 32)));
+        if (__builtin_expect(large != 0, 0)) {
             mine = ((rows | rows >> 32) >> l32 & 1) != 0;
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
@@ -1096,7 +1096,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             };
             // The smallest term, where the wave has rows that need it.
             auto last = [&](f32x16& s, int block) __attribute__((always_inline)) {
-                if (__builtin_expect(!large, 1)) return;
+                int is = large;
+                asm volatile("" : "+s"(is));  // (compared here: else as a lane mask, by two vector instructions)
+                if (__builtin_expect(is == 0, 1)) return;
                 constexpr std::integral_constant<int, kFp4Terms - 1> term{};
                 s = term_of(s, block, std::integral_constant<int, 0>{}, term, last_term(0));
                 s = term_of(s, block, std::integral_constant<int, 1>{}, term, last_term(1));
@@ -1118,19 +1120,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             };
             bundle0(std::integral_constant<int, 0>{});
             bundle0(std::integral_constant<int, 1>{});
-            last(s0, 0);
             bundle0(std::integral_constant<int, 2>{});
             bundle0(std::integral_constant<int, 3>{});
             bundle0(std::integral_constant<int, 4>{});
             bundle0(std::integral_constant<int, 5>{});
+            asm volatile("" : "+v"(s0));  // (keeps its MFMAs from being sunk below the branches, as that of s1)
+            last(s0, 0);
             bundle1(std::integral_constant<int, 0>{});
             bundle1(std::integral_constant<int, 1>{});
-            last(s1, 1);
             bundle1(std::integral_constant<int, 2>{});
             bundle1(std::integral_constant<int, 3>{});
             bundle1(std::integral_constant<int, 4>{});
             bundle1(std::integral_constant<int, 5>{});
-            asm volatile("" ::"v"(s1));  // (keeps its MFMAs from being sunk below settle's branches)
+            // (keeps its MFMAs and the exponentials above from being sunk below the branches)
+            asm volatile("" : "+v"(s1), "+v"(p0[0]), "+v"(p0[1]), "+v"(sum0));
+            last(s1, 1);
         } else {
 #pragma unroll
         for (int n = 0; n < kAhead; ++n) kf[n] = kfrag(n);

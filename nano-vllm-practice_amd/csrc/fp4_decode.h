@@ -129,15 +129,12 @@ __device__ __forceinline__ Fp4Query<TERMS> fp4_query(const Fp4QueryWords& words,
 template <typename E>
 __device__ __forceinline__ bool fp4_query_large(const Fp4QueryWords& q, int b, int D) {
     const int below = std::is_same<E, F16>::value ? 5 << 10 : 8 << 7;
-    const uint16_t limit = (uint16_t)max((int)fp4_query_top(q) - below, 0);
-    u16x2 count = {0, 0};
+    const uint32_t limit = (uint32_t)max((int)fp4_query_top(q) - below, 0) * 0x10001u;
+    int others = 0;  // (bit 15 of a half stays where the subtraction does not borrow it: the magnitude is no smaller)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const u16x2 x = __builtin_bit_cast(u16x2, q.w[i >> 2][i & 3] & 0x7fff7fffu);
-        count += __builtin_elementwise_min(__builtin_elementwise_sub_sat(u16x2{limit, limit}, x), u16x2{1, 1});
-    }
+    for (int i = 0; i < 16; ++i) others += __builtin_popcount(((q.w[i >> 2][i & 3] | 0x80008000u) - limit) & 0x80008000u);
     const int absent = limit > 0 ? max(32 * b + 32 - max(D, 32 * b), 0) : 0;
-    return count[0] + count[1] - absent >= 12;
+    return 32 - others - absent >= 12;
 }
 
 __device__ __forceinline__ i32x8 fp4_operand(u32x4 w) {
