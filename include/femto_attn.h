@@ -446,8 +446,8 @@ size_t femto_paged_attention_gemv_fp4_zero_bytes(void);
  * reaches the tokens that see its key and no other; one that is an infinity to an
  * f16 call (V from 131072 on) also reaches, as NaN, those of its query tile (up to
  * 128 tokens of the chunk) that do not.  q is taken to 2^-14 of the largest magnitude of its 32
- * dims; in a row where 12 dims of a block are under 1/256 of its largest (f16:
- * 1/32), to 2^-18.  The workspace (256-byte aligned, always needed) has to be zero in its first
+ * dims; in a row where 5 dims of a block are under 1/256 of its largest (f16: 12
+ * under 1/32), to 2^-18.  The workspace (256-byte aligned, always needed) has to be zero in its first
  * femto_paged_attention_gemm_split_bytes() bytes before its first use and is
  * left so; calls that may overlap must not share one. */
 int femto_paged_attention_gemm_fp4(

@@ -122,10 +122,11 @@ __device__ __forceinline__ Fp4Query<TERMS> fp4_query(const Fp4QueryWords& words,
 
 // Whether three terms do not do for the block.  They leave up to 2^-15 of the
 // largest magnitude of small dims, more than half a step of their own in bf16 below
-// 1/256 of it, in f16 below 1/32; with 12 and more such dims of 32 that counts.  (Of
-// 32 normal values 12 that small are one block in 10^9 in bf16, 10^7 in f16.)
-// Zeros among them, which any term holds, are not told apart, but for dims
-// from D on.
+// 1/256 of it, in f16 below 1/32.  Five such dims of a block make it so in bf16, 12 of
+// 32 or 6 of 16 in f16 (where fewer are small, the steps of the others count for
+// more).  Of normal values that is one block of 32 in 200 000, in f16 one in a
+// million.  Zeros among them, which any term holds, are not told apart, but for
+// dims from D on.
 template <typename E>
 __device__ __forceinline__ bool fp4_query_large(const Fp4QueryWords& q, int b, int D) {
     const int below = std::is_same<E, F16>::value ? 5 << 10 : 8 << 7;
@@ -133,8 +134,9 @@ __device__ __forceinline__ bool fp4_query_large(const Fp4QueryWords& q, int b, i
     int others = 0;  // (bit 15 of a half stays where the subtraction does not borrow it: the magnitude is no smaller)
 #pragma unroll
     for (int i = 0; i < 16; ++i) others += __builtin_popcount(((q.w[i >> 2][i & 3] | 0x80008000u) - limit) & 0x80008000u);
-    const int absent = limit > 0 ? max(32 * b + 32 - max(D, 32 * b), 0) : 0;
-    return 32 - others - absent >= 12;
+    const int absent = max(32 * b + 32 - max(D, 32 * b), 0);  // zeros, small where the limit is not 0
+    const int enough = std::is_same<E, F16>::value ? 3 * (32 - absent) / 8 : 5;
+    return limit > 0 && 32 - others - absent >= enough;
 }
 
 __device__ __forceinline__ i32x8 fp4_operand(u32x4 w) {

@@ -192,3 +192,29 @@ def test_rows_that_no_sequence_holds(ops, gpu, byte, code, dim, dtype):
     w = Batch(CHUNKS + [(0, 15), (0, 63), (17, 48)], 4, 2, dim, dtype, 8)
     hide(w, byte, code)
     assert_close(gemm(ops, gpu, w), of.prefill(np64(w.q), w.pool, w.cu, w.tables, w.kv_lens, w.pos), dtype, "prefill")
+
+
+@pytest.mark.parametrize("dtype,top", [(BF16, 512.0), (F16, 64.0)])
+@pytest.mark.parametrize("dim", [128, 112, 48, 16])
+def test_large_channels_of_a_split_tile_and_beside_rows(ops, gpu, dim, dtype, top):
+    """A long context's tile in pieces, which split q each for themselves, and decode rows in the same launch."""
+    w = large_channels([(6000, 64), (100, 20)] + [(n, 1) for n in (0, 40, 700)], (8, 2), dim, dtype, top, dim, False)
+    want = of.prefill(np64(w.q), w.pool, w.cu, w.tables, w.kv_lens, w.pos)
+    first = gemm(ops, gpu, w)
+    assert_close(first, want, dtype, f"channels of {top}, dim {dim}")
+    assert torch.equal(gemm(ops, gpu, w), first)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_zeros_infinities_and_nan_in_queries(ops, gpu, dtype):
+    """Rows of zeros (plain averages), rows with most dims zero, and an infinity or a NaN in one row, which stays its own."""
+    w = Batch([(100, 70), (0, 33), (64, 1)], 4, 2, 128, dtype, 11)
+    w.q[:, 3] = 0
+    w.q[:, 7, 1:] = 0
+    w.q[:, 40, 33:] = 0
+    w.q[1, 10, 70], w.q[2, 75, 0], w.q[3, 103, 127] = float("inf"), float("nan"), float("-inf")
+    got = gemm(ops, gpu, w)
+    want = of.prefill(np64(w.q), w.pool, w.cu, w.tables, w.kv_lens, w.pos)
+    for h, t in ((1, 10), (2, 75), (3, 103)):
+        want[h, t] = np.nan  # (infinite scores of both signs, or of one and NaN for those of zero: the row is NaN)
+    assert_close(got, want, dtype, "zeros and infinities")
